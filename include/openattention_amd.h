@@ -542,6 +542,79 @@ typedef struct oa_step_args {
 } oa_step_args;
 int oa_step(const oa_step_args* args, void* stream);
 
+/*
+ * A layer's query and key rows (tokens x q_heads / kv_heads rows of head_dim values; strides per token and
+ * per head in elements), each head normalised and turned to its token's position in one pass:
+ *   y = x / sqrt(mean(x^2) + eps) * w   (wq / wk: head_dim weights of the rows' type; NULL: y = x)
+ *   out_i = y_i cos_i - y_(i + D/2) sin_i,   out_(i + D/2) = y_(i + D/2) cos_i + y_i sin_i
+ * in fp32, rounded once.  dtype 0 / 1 / 2: bf16 / fp16 / fp32 rows; head_dim 64, 128 or 256; pos int32 or,
+ * pos_is_64, int64; cos_t, sin_t: (positions, head_dim / 2) fp32 rows of table_stride.  A token of negative
+ * position (padding) gives zeros, one past the tables NaN.  Bases 16-byte aligned, strides multiples of 16
+ * bytes; outputs may be the inputs.
+ */
+int oa_qk_norm_rope(const void* q, long q_st, long q_sh, const void* k, long k_st, long k_sh, int tokens,
+                    int q_heads, int kv_heads, int head_dim, int dtype, const void* pos, int pos_is_64,
+                    const float* cos_t, const float* sin_t, long table_stride, int positions, const void* wq,
+                    const void* wk, float eps, void* q_out, long qo_st, long qo_sh, void* k_out, long ko_st,
+                    long ko_sh, void* stream);
+
+/*
+ * Page tables of a paged cache, on the device.  table (requests, width) int32 rows of table_stride: page ids,
+ * -1 for none; lens (requests): tokens held, in ceil(lens / page) pages; free (pages): a stack of the ids
+ * nobody holds, its height in *nfree (top: free[nfree - 1]); page: a power of two, 32 .. 1024.
+ *
+ * extend: request i adds add[i] >= 0 tokens.  Pages are popped in the order of requests and of their pages;
+ * slots[t] = page id * page + offset and pos[t] of the new tokens, request after request, cu (requests + 1)
+ * their starts; slots and pos from cu[requests] to total are -1.  truncate: request i keeps the first
+ * min(keep[i], lens[i]) tokens (keep[i] < 0: all); its other pages go back so that a truncation to the old
+ * lengths restores the stack that an extension changed.
+ *
+ * Either takes effect for all requests or for none; then nothing changes (an extension's slots, pos are -1,
+ * its cu 0) and *status |= 1 (a negative count, a length outside of the table's row), 2 (too few free pages,
+ * or more than the stack holds), 4 (more than total tokens).  ws: 3 requests + 1 ints of scratch.
+ */
+int oa_kv_pages_extend(const int* add, int* lens, int* table, long table_stride, int* free, int* nfree, int* status,
+                       int requests, int width, int pages, int page, int total, int* slots, int* pos, int* cu, int* ws,
+                       void* stream);
+int oa_kv_pages_truncate(const int* keep, int* lens, int* table, long table_stride, int* free, int* nfree, int* status,
+                         int requests, int width, int pages, int page, int* ws, void* stream);
+
+/*
+ * The 4-bit cache: codes kc, vc (pages, kv_heads, page, head_dim / 2) and scales ks, vs (pages, kv_heads, page,
+ * head_dim / 32) bytes, pages code_stride and scale_stride bytes apart; head_dim 64 or 128.  A block of 32
+ * values of a row is a 4-bit code for each (sign, two bits of exponent, one of mantissa: 0, .5, 1, 1.5, 2, 3,
+ * 4, 6; the even value of a row in the low half of a byte) and a byte s, scaling by 2^(s - 127): the smallest
+ * 2^e with max |x| < 7 * 2^e, -125 <= e <= 125; rounding to nearest, ties to the even code, at most 6.  A
+ * block with a value that is not finite is held as s = 255, NaN.
+ *
+ * write: rows of tokens (strides per token and head in elements; dtype 0 / 1 / 2: bf16 / fp16 / fp32) into
+ * their slots.  A slot outside of the cache (-1: padding) is passed over; slots of one call are distinct, a
+ * slot given twice holds some mixture of its rows.  read: the values at slots (dtype 0 or 2: bf16, exact, or
+ * fp32); a slot outside of the cache gives zeros.
+ */
+int oa_kv4_write(const void* k, long k_st, long k_sh, const void* v, long v_st, long v_sh, int tokens, int kv_heads,
+                 int head_dim, int dtype, const int* slots, void* kc, void* ks, void* vc, void* vs, long code_stride,
+                 long scale_stride, int pages, int page, void* stream);
+int oa_kv4_read(const int* slots, const void* kc, const void* ks, const void* vc, const void* vs, long code_stride,
+                long scale_stride, int pages, int page, void* k, long k_st, long k_sh, void* v, long v_st, long v_sh,
+                int tokens, int kv_heads, int head_dim, int dtype, void* stream);
+
+/*
+ * Causal attention over the 4-bit cache.  Sequence b holds lens[b] keys in the pages of its table row; its
+ * query tokens are rows cu[b] .. cu[b + 1] - 1 of q (tokens, q_heads, head_dim) bf16 (cu NULL: row b alone),
+ * the last of them its newest key's, so that token j of R sees keys 0 .. lens - R + j.  out as q.  fp32 scores,
+ * softmax and sums; weights in 16 bits.  A row that sees no key gives 0; rows behind cu[sequences], and tokens
+ * of a sequence from max_q on, are left as they were.  NaN: rows that need a page id outside of the cache, and
+ * those of sequences longer than their table row or than nchunk * chunk keys.  Keys are split into nchunk pieces
+ * of `chunk` (a multiple of 128); with more than one, ws_o (tokens * q_heads * nchunk * head_dim) and ws_ml (* 2)
+ * floats hold the pieces' sums.
+ */
+int oa_kv4_attn(const void* q, long q_st, long q_sh, const void* kc, const void* ks, const void* vc, const void* vs,
+                long code_stride, long scale_stride, int pages, int page, const int* table, long table_stride, int width,
+                const int* lens, const int* cu, int sequences, int tokens, int max_q, int q_heads, int kv_heads,
+                int head_dim, float sm_scale, int chunk, int nchunk, float* ws_o, float* ws_ml, void* out, long o_st,
+                long o_sh, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,437 @@
+// Causal attention of the newest tokens of every sequence over a 4-bit paged cache (layout and codes:
+// oa_kv4.hip):  out = sum_t p_t v_t / sum_t p_t,  p_t = exp(scale q . k_t - max),  t up to the row's own
+// position, in one pass over the keys with a running maximum and sum.
+//
+// One workgroup of four waves takes 16 NQ query rows of a KV head (row = token * G + head, so that any
+// number of query heads fills the tiles) and a chunk of keys; each wave walks its own tiles of 32 keys
+// and the waves join at the end.  With several chunks a second kernel joins them.
+//   scores   S^T = K Q^T by v_mfma_f32_16x16x32_bf16: a lane of the K operand holds 32 dims of one key,
+//            a block of the cache, whose codes become bf16 with one conversion per pair, scale included
+//            (the contraction takes the dims in that order on both sides).  All products are exact.
+//   values   O^T = V^T P^T: the weights are the B operand as the scores left them; V goes to bf16 the
+//            same way, through the wave's own LDS tile, and comes back by the LDS transpose reads.
+// Weights go into the product as two bf16 terms, so that the sum keeps 16 bits of each: up to 8 rows
+// the second term sits in the tile's other 8 columns, otherwise it takes a second product.
+#include <cfloat>
+
+#include "oa_common.h"
+
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef unsigned int uint4v __attribute__((ext_vector_type(4)));
+typedef unsigned int uint2v __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) short4v lds_short4v;
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * 64;
+constexpr int kTile = 32;                // keys per tile
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct AttnArgs {
+  const uint16_t* q; long q_st, q_sh;
+  const uint8_t* kc; const uint8_t* ks; const uint8_t* vc; const uint8_t* vs;
+  long c_sp, s_sp;                       // bytes between pages
+  const int* table; long t_st;
+  const int* lens; const int* cu;
+  uint16_t* out; long o_st, o_sh;
+  float* ws_o; float* ws_ml;             // partial sums, (maximum, sum) by (row, chunk)
+  int B, HKV, G, tokens, max_q, width, NP, lp, chunk, nchunk;
+  float c;                               // scale * log2 e
+};
+
+// what a sequence asks: its rows and how many keys they see
+struct Seq {
+  int n, r0, R;
+  bool bad;                              // more keys than the table or the call covers
+};
+
+__device__ __forceinline__ Seq seq_of(const AttnArgs& a, int b) {
+  Seq s;
+  s.n = max(a.lens[b], 0);
+  s.r0 = a.cu ? a.cu[b] : b;
+  const int r1 = a.cu ? a.cu[b + 1] : b + 1;
+  s.R = s.r0 < 0 || r1 < s.r0 || r1 > a.tokens ? 0 : r1 - s.r0;         // (starts that do not fit the rows: none)
+  s.bad = (long)s.n > min((long)a.width << a.lp, (long)a.nchunk * a.chunk);
+  return s;
+}
+
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  const f32x2 x = {a, b};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2));
+}
+__device__ __forceinline__ float scale_of(unsigned s) {
+  return s == 255 ? __builtin_nanf("") : __uint_as_float(s << 23);
+}
+// 8 codes to bf16, scaled
+__device__ __forceinline__ bf16x8 from4(unsigned w, float f) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 0);
+  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 1);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 2);
+  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 3);
+  const uint4v x = {__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, c),
+                    __builtin_bit_cast(uint32_t, d)};
+  return __builtin_bit_cast(bf16x8, x);
+}
+__device__ __forceinline__ float max_groups(float v) {     // over the four 16-lane groups
+  const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+  const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+}
+__device__ __forceinline__ float sum_groups(float v) {
+  const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+  const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(y[0]) + __uint_as_float(y[1]);
+}
+
+// what the lanes of a wave exchange through its LDS tile stays in program order (the LDS keeps it)
+__device__ __forceinline__ void lane_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local"); }
+
+// one tile's codes and scales of this lane: keys lane % 16 and 16 + lane % 16, a quarter of the dims
+template <int D>
+struct Tile {
+  unsigned k[2][D / 32], v[2][D / 32];
+  unsigned ks[2], vs[2];
+  bool bad;
+};
+
+template <int N>
+__device__ __forceinline__ void load_words(unsigned (&w)[N], const uint8_t* p) {
+  if constexpr (N == 4) {
+    const uint4v x = *reinterpret_cast<const uint4v*>(p);
+    w[0] = x[0]; w[1] = x[1]; w[2] = x[2]; w[3] = x[3];
+  } else {
+    const uint2v x = *reinterpret_cast<const uint2v*>(p);
+    w[0] = x[0]; w[1] = x[1];
+  }
+}
+
+// NQ tiles of 16 query rows; DUP: at most 8 rows, columns 8.. repeat them for the weights' second terms
+template <int D, int NQ, bool DUP>
+__global__ void __launch_bounds__(kThreads) kv4_attn_kernel(AttnArgs a) {
+  constexpr int kSteps = D / 32;         // products of a 16 x 16 score tile; words of a lane's codes
+  constexpr int kDims = D / 16;          // tiles of 16 dims
+  constexpr int kRowB = D * 2;           // bytes of a value row in LDS
+  constexpr int kStage = kTile * kRowB;
+  constexpr int kCols = DUP ? 8 : 16;
+  // value tiles of the waves; at the end their sums, 16 rows of D floats each
+  __shared__ __align__(16) char s_v[kWaves * (kStage > 64 * D ? kStage : 64 * D)];
+  __shared__ float s_m[kWaves][NQ * 16], s_l[kWaves][NQ * 16];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, g = lane >> 4;
+  const int units = a.B * a.HKV;
+  const int ch = blockIdx.x % a.nchunk, rest = blockIdx.x / a.nchunk;
+  const int bh = rest % units, row0 = rest / units * (NQ * kCols);
+  const int b = bh / a.HKV, h = bh - b * a.HKV;
+  const Seq sq = seq_of(a, b);
+  const int rows = min(sq.R, a.max_q) * a.G;
+  if (row0 >= rows) return;
+  const int first = sq.n - sq.R;         // position of the sequence's first query token
+  const int hi = sq.bad ? 0 : first + (min(row0 + NQ * kCols, rows) - 1) / a.G + 1;    // keys any row sees
+  const int all = first + row0 / a.G + 1;                                              // keys every row sees
+  const int k0 = ch * a.chunk, k1 = min(k0 + a.chunk, hi);
+  if (k0 >= k1 && a.nchunk > 1) return;
+
+  // this lane's columns: rows of q and how many keys they see (0: none such)
+  bf16x8 Q[NQ][kSteps];
+  int lim[NQ];
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    const int r = row0 + x * kCols + (DUP ? col & 7 : col);
+    const int rr = min(r, rows - 1), j = rr / a.G, hd = h * a.G + rr - j * a.G;
+    lim[x] = r < rows ? first + j + 1 : 0;
+    const uint16_t* p = a.q + (long)(sq.r0 + j) * a.q_st + (long)hd * a.q_sh + g * (D / 4);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) Q[x][s] = *reinterpret_cast<const bf16x8*>(p + 8 * s);
+  }
+
+  const int* trow = a.table + (long)b * a.t_st;
+  const int pmask = (1 << a.lp) - 1;
+  const long headc = ((long)h << a.lp) * (D / 2), heads = ((long)h << a.lp) * (D / 32);
+  const int last = (k1 - 1) >> a.lp;     // the chunk's last page
+  auto page_at = [&](int t0) { return trow[min(t0 >> a.lp, last)]; };
+  auto load = [&](Tile<D>& t, int t0, int page) {
+    t.bad = (unsigned)page >= (unsigned)a.NP;
+    const long pg = t.bad ? 0 : page;
+    const int off = (t0 & pmask) + col;
+    const uint8_t* kc = a.kc + pg * a.c_sp + headc;
+    const uint8_t* vc = a.vc + pg * a.c_sp + headc;
+    const uint8_t* ks = a.ks + pg * a.s_sp + heads;
+    const uint8_t* vs = a.vs + pg * a.s_sp + heads;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      load_words<kSteps>(t.k[c], kc + (off + 16 * c) * (D / 2) + g * (D / 8));
+      load_words<kSteps>(t.v[c], vc + (off + 16 * c) * (D / 2) + g * (D / 8));
+      t.ks[c] = ks[(off + 16 * c) * (D / 32) + g * D / 128];
+      t.vs[c] = vs[(off + 16 * c) * (D / 32) + g * D / 128];
+    }
+  };
+
+  // LDS tile of 32 value rows; 16-byte chunk x of row r lies at x ^ f(r): 16 rows written at one chunk
+  // and 16 rows read at two both spread over all banks
+  char* const sv = s_v + wave * kStage;
+  auto fsw = [](int r) { return D == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : ((r >> 1) & 3) << 1; };
+  const int wbase = col * kRowB, wf = fsw(col);
+  const int lr = 4 * g + ((lane & 15) >> 2), rf = fsw(lr), lc = lane & 3;
+  auto val_op = [&](int d) {
+    const int ad = lr * kRowB + (((2 * d + (lc >> 1)) ^ rf) << 4) + (lc & 1) * 8;
+    const short4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v*)(sv + ad));
+    const short4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v*)(sv + ad + 16 * kRowB));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+
+  f32x4 O[NQ][kDims];
+  float m[NQ], l[NQ];
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    m[x] = -FLT_MAX;
+    l[x] = 0.f;
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) O[x][d] = f32x4(0.f);
+  }
+
+  constexpr int kStride = kWaves * kTile;
+  int t0 = k0 + wave * kTile;
+  Tile<D> nx;
+  int page = 0;
+  if (t0 < k1) {
+    load(nx, t0, page_at(t0));
+    page = page_at(t0 + kStride);
+  }
+  for (; t0 < k1; t0 += kStride) {
+    const Tile<D> t = nx;
+    if (t0 + kStride < k1) {
+      load(nx, t0 + kStride, page);
+      page = page_at(t0 + 2 * kStride);
+    }
+    const bool mask = t0 + kTile > all;  // some row does not see some key
+
+    f32x4 S[NQ][2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const float f = t.bad ? __builtin_nanf("") : scale_of(t.ks[c]);
+#pragma unroll
+      for (int x = 0; x < NQ; ++x) S[x][c] = f32x4(0.f);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const bf16x8 kop = from4(t.k[c][s], f);
+#pragma unroll
+        for (int x = 0; x < NQ; ++x) S[x][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop, Q[x][s], S[x][c], 0, 0, 0);
+      }
+    }
+    // values into the LDS tile; keys past the last one any row sees count as zeros (their weights are 0,
+    // but what lies there may be anything), and so do NaN blocks of keys that only some rows see
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int key = t0 + 16 * c + col;
+      float f = scale_of(t.vs[c]);
+      if (mask && (key >= hi || t.vs[c] == 255)) f = 0.f;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+        *reinterpret_cast<bf16x8*>(sv + wbase + 16 * c * kRowB + (((g * (D / 32) + s) ^ wf) << 4)) = from4(t.v[c][s], f);
+    }
+
+    lane_order();
+    uint4v P[NQ], Plo[NQ];
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
+      float v[8];
+      float mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] = S[x][i >> 2][i & 3] * a.c;
+        if (mask && t0 + 16 * (i >> 2) + 4 * g + (i & 3) >= lim[x]) v[i] = -INFINITY;
+        mx = fmaxf(mx, v[i]);
+      }
+      if (__any(mx > m[x])) {
+        const float mn = fmaxf(m[x], max_groups(mx)), alpha = __builtin_amdgcn_exp2f(m[x] - mn);
+        m[x] = mn;
+        l[x] *= alpha;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) O[x][d] *= alpha;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] = __builtin_amdgcn_exp2f(v[i] - m[x]);
+        l[x] += v[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t u = pack2(v[2 * i], v[2 * i + 1]);
+        const uint32_t lo = pack2(v[2 * i] - __uint_as_float(u << 16), v[2 * i + 1] - __uint_as_float(u & 0xffff0000u));
+        P[x][i] = DUP && (lane & 8) ? lo : u;
+        Plo[x][i] = lo;
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) {
+      const bf16x8 vop = val_op(d);
+#pragma unroll
+      for (int x = 0; x < NQ; ++x) {
+        O[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vop, __builtin_bit_cast(bf16x8, P[x]), O[x][d], 0, 0, 0);
+        if (!DUP) O[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vop, __builtin_bit_cast(bf16x8, Plo[x]), O[x][d], 0, 0, 0);
+      }
+    }
+    lane_order();
+    if (mask) {                          // NaN blocks, into the rows that see them (rare)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        unsigned long nan = __ballot(t.vs[c] == 255 && t0 + 16 * c + col < hi);
+        while (nan) {
+          const int at = __builtin_ctzl(nan), key = t0 + 16 * c + (at & 15), blk = (at >> 4) * D / 128;
+          nan &= nan - 1;
+#pragma unroll
+          for (int x = 0; x < NQ; ++x)
+#pragma unroll
+            for (int d = 0; d < kDims; ++d)
+              if (d / 2 == blk && key < lim[x]) O[x][d] = f32x4(__builtin_nanf(""));
+        }
+      }
+    }
+  }
+
+  // the four waves' sums, with a common maximum
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    const float lt = sum_groups(l[x]);
+    if (g == 0) {
+      s_m[wave][x * 16 + col] = m[x];
+      s_l[wave][x * 16 + col] = lt;
+    }
+  }
+  float* const so = reinterpret_cast<float*>(s_v);
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    __syncthreads();                     // (every wave is done with its tile, or with the previous sums)
+    const int sc = x * 16 + col;
+    const float M = fmaxf(fmaxf(s_m[0][sc], s_m[1][sc]), fmaxf(s_m[2][sc], s_m[3][sc]));
+    const float e = __builtin_amdgcn_exp2f(m[x] - M);
+#pragma unroll
+    for (int d = 0; d < kDims; ++d)      // 16-byte chunk y of column col at y ^ col
+      *reinterpret_cast<f32x4*>(so + (wave * 16 + col) * D + (((4 * d + g) ^ col) << 2)) = O[x][d] * e;
+    __syncthreads();
+    constexpr int kChunks = D / 4;
+    for (int i = threadIdx.x; i < kCols * kChunks; i += kThreads) {
+      const int cl = i / kChunks, y = i % kChunks, r = row0 + x * kCols + cl;
+      if (r >= rows) continue;
+      const int c16 = x * 16 + cl;
+      const float Mr = fmaxf(fmaxf(s_m[0][c16], s_m[1][c16]), fmaxf(s_m[2][c16], s_m[3][c16]));
+      float L = 0.f;
+      f32x4 o = f32x4(0.f);
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        L += s_l[w][c16] * __builtin_amdgcn_exp2f(s_m[w][c16] - Mr);
+        o += *reinterpret_cast<const f32x4*>(so + (w * 16 + cl) * D + ((y ^ cl) << 2));
+        if (DUP) o += *reinterpret_cast<const f32x4*>(so + (w * 16 + 8 + cl) * D + ((y ^ (8 + cl)) << 2));
+      }
+      const int j = r / a.G, hd = h * a.G + r - j * a.G;
+      if (a.nchunk == 1) {
+        const int seen = first + j + 1;
+        o = sq.bad ? f32x4(__builtin_nanf("")) : seen > 0 ? o / L : f32x4(0.f);
+        *reinterpret_cast<uint2v*>(a.out + (long)(sq.r0 + j) * a.o_st + (long)hd * a.o_sh + 4 * y) =
+            uint2v{pack2(o[0], o[1]), pack2(o[2], o[3])};
+      } else {
+        const long at = ((long)(sq.r0 + j) * (a.HKV * a.G) + hd) * a.nchunk + ch;
+        *reinterpret_cast<f32x4*>(a.ws_o + at * D + 4 * y) = o;
+        if (y == 0) *reinterpret_cast<f32x2*>(a.ws_ml + at * 2) = f32x2{Mr, L};
+      }
+    }
+  }
+}
+
+// joins a row's chunks: weights exp2(m_i - max m), by groups of D / 4 lanes
+template <int D>
+__global__ void __launch_bounds__(kThreads) kv4_join_kernel(AttnArgs a) {
+  constexpr int kLanes = D / 4, kGroups = kThreads / kLanes;
+  __shared__ float s_r[kWaves];
+  __shared__ __align__(16) float s_o[kGroups][D];
+  __shared__ float s_l[kGroups];
+  const int heads = a.HKV * a.G;
+  const int hd = blockIdx.x % heads, rest = blockIdx.x / heads, j = rest % a.max_q, b = rest / a.max_q;
+  const Seq sq = seq_of(a, b);
+  if (j >= sq.R) return;
+  const int seen = sq.n - sq.R + j + 1, tid = threadIdx.x;
+  const int nv = sq.bad || seen <= 0 ? 0 : (seen + a.chunk - 1) / a.chunk;
+  const long row = ((long)(sq.r0 + j) * heads + hd) * a.nchunk;
+  const float* ml = a.ws_ml + row * 2;
+  float M = -FLT_MAX;
+  for (int i = tid; i < nv; i += kThreads) M = fmaxf(M, ml[2 * i]);
+  M = oa::wave_max(M);
+  if ((tid & 63) == 0) s_r[tid >> 6] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(s_r[0], s_r[1]), fmaxf(s_r[2], s_r[3]));
+  const int grp = tid / kLanes, y = tid % kLanes;
+  f32x4 o = f32x4(0.f);
+  float L = 0.f;
+  for (int i = grp; i < nv; i += kGroups) {
+    const float w = __builtin_amdgcn_exp2f(ml[2 * i] - M);
+    L += w * ml[2 * i + 1];
+    o += *reinterpret_cast<const f32x4*>(a.ws_o + (row + i) * D + 4 * y) * w;
+  }
+  *reinterpret_cast<f32x4*>(&s_o[grp][4 * y]) = o;
+  if (y == 0) s_l[grp] = L;
+  __syncthreads();
+  if (grp) return;
+#pragma unroll
+  for (int k = 1; k < kGroups; ++k) {
+    o += *reinterpret_cast<const f32x4*>(&s_o[k][4 * y]);
+    L += s_l[k];
+  }
+  o = sq.bad ? f32x4(__builtin_nanf("")) : nv ? o / L : f32x4(0.f);
+  *reinterpret_cast<uint2v*>(a.out + (long)(sq.r0 + j) * a.o_st + (long)hd * a.o_sh + 4 * y) =
+      uint2v{pack2(o[0], o[1]), pack2(o[2], o[3])};
+}
+
+template <int D>
+int launch(const AttnArgs& a, hipStream_t st) {
+  const long rows = (long)a.max_q * a.G;
+  const int cols = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
+  const long blocks = (rows + cols - 1) / cols * a.B * a.HKV * a.nchunk, joins = (long)a.B * a.max_q * a.HKV * a.G;
+  if (blocks > 0x7fffffffL || joins > 0x7fffffffL) return OA_EINVAL;
+  const dim3 grid((unsigned)blocks), blk(kThreads);
+  if (cols == 8) hipLaunchKernelGGL((kv4_attn_kernel<D, 1, true>), grid, blk, 0, st, a);
+  else if (cols == 16) hipLaunchKernelGGL((kv4_attn_kernel<D, 1, false>), grid, blk, 0, st, a);
+  else hipLaunchKernelGGL((kv4_attn_kernel<D, 2, false>), grid, blk, 0, st, a);
+  if (a.nchunk > 1) hipLaunchKernelGGL((kv4_join_kernel<D>), dim3((unsigned)joins), blk, 0, st, a);
+  return OA_LAUNCH_STATUS();
+}
+
+}  // namespace
+
+extern "C" int oa_kv4_attn(const void* q, long q_st, long q_sh, const void* kc, const void* ks, const void* vc,
+                           const void* vs, long code_stride, long scale_stride, int pages, int page, const int* table,
+                           long table_stride, int width, const int* lens, const int* cu, int sequences, int tokens,
+                           int max_q, int q_heads, int kv_heads, int head_dim, float sm_scale, int chunk, int nchunk,
+                           float* ws_o, float* ws_ml, void* out, long o_st, long o_sh, void* stream) {
+  auto odd = [](const void* p, uintptr_t n) { return !p || (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0; };
+  if ((head_dim != 64 && head_dim != 128) || sequences < 0 || tokens < 0 || max_q <= 0 || kv_heads <= 0 || q_heads <= 0 ||
+      q_heads % kv_heads || (long)max_q * (q_heads / kv_heads) > (1L << 30) || pages <= 0 || page < 32 || page > 1024 ||
+      (page & (page - 1)) || (long)pages * page > 0x7fffffffL || width <= 0 || (long)width * page > 0x7fffffffL ||
+      table_stride < width || chunk < 128 || chunk % 128 || nchunk <= 0 || (long)nchunk * chunk > 0x7ffffff0L)
+    return OA_EINVAL;
+  if (!cu && (max_q != 1 || sequences != tokens)) return OA_EINVAL;
+  if (!sequences || !tokens) return 0;
+  if (odd(q, 16) || q_st % 8 || q_sh % 8 || odd(out, 8) || o_st % 4 || o_sh % 4 || odd(kc, 16) || odd(ks, 16) || odd(vc, 16) ||
+      odd(vs, 16) || !table || !lens || code_stride < (long)kv_heads * page * (head_dim / 2) ||
+      scale_stride < (long)kv_heads * page * (head_dim / 32) || code_stride % 16 || scale_stride % 16 || !(sm_scale == sm_scale))
+    return OA_EINVAL;
+  if (nchunk > 1 && (odd(ws_o, 16) || odd(ws_ml, 8))) return OA_EINVAL;
+  AttnArgs a;
+  a.q = (const uint16_t*)q; a.q_st = q_st; a.q_sh = q_sh;
+  a.kc = (const uint8_t*)kc; a.ks = (const uint8_t*)ks; a.vc = (const uint8_t*)vc; a.vs = (const uint8_t*)vs;
+  a.c_sp = code_stride; a.s_sp = scale_stride;
+  a.table = table; a.t_st = table_stride; a.lens = lens; a.cu = cu;
+  a.out = (uint16_t*)out; a.o_st = o_st; a.o_sh = o_sh;
+  a.ws_o = ws_o; a.ws_ml = ws_ml;
+  a.B = sequences; a.HKV = kv_heads; a.G = q_heads / kv_heads; a.tokens = tokens; a.max_q = max_q;
+  a.width = width; a.NP = pages; a.lp = __builtin_ctz(page); a.chunk = chunk; a.nchunk = nchunk;
+  a.c = sm_scale * kLog2e;
+  return head_dim == 64 ? launch<64>(a, (hipStream_t)stream) : launch<128>(a, (hipStream_t)stream);
+}

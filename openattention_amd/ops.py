@@ -6,8 +6,9 @@ Operator surface kept from the reference:
                           sm_scale=None, block_n=64, block_b=64, num_warps=4)
                                                                         triton_expand_decode.py:139-165
 plus one function per decode stage (index_update, qgs_prep, qgs_scan, topk_select, errorgate,
-waterfill, topq, residual, residual_flash, dense_decode), each a thin checked call of the C ABI
-(include/openattention_amd.h) on torch's current HIP stream.  Shape, dtype, device, alignment
+waterfill, topq, residual, residual_flash, dense_decode) and the operators of the 4-bit paged cache
+(qk_norm_rope, kv_pages_extend, kv_pages_truncate, kv4_write, kv4_read, kv4_attn), each a thin checked
+call of the C ABI (include/openattention_amd.h) on torch's current HIP stream.  Shape, dtype, device, alignment
 and stride checks happen here; the kernels trust them.  There is no CPU path: tensors must live
 on a HIP device and the kernel library must be built.
 """
@@ -659,6 +660,267 @@ def prefill_attn(q, k, v, sm_scale: float) -> torch.Tensor:
              v.stride(1), v.stride(2), HQ, k.shape[1], T, HEAD_DIM, float(sm_scale), _ptr(out), out.stride(2),
              out.stride(1), _stream(dev))
     return out.transpose(1, 2)
+
+
+# ================================================================== 4-bit paged cache
+_DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+KV4_BLOCK = 32             # values that share a scale
+
+
+def _run(dev: torch.device, name: str, *args) -> None:
+    """lib.call on dev's current stream, with dev the current device for the launch."""
+    if dev.index == torch.cuda.current_device():
+        lib.call(name, *args, _stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            lib.call(name, *args, _stream(dev))
+
+
+def _plain(*named) -> None:
+    """Tensors whose data a kernel may take as it stands, with no gradient to be formed: these
+    operators have no backward pass, and would cut a graph in silence."""
+    grad = torch.is_grad_enabled()
+    for t, name in named:
+        if t is None:
+            continue
+        _need(not (grad and t.requires_grad), f"{name} requires a gradient, and this operator has no backward pass "
+              "(call it under torch.no_grad())")
+        _need(not t.is_neg(), f"{name}: a lazily negated view (call resolve_neg())")
+
+
+def _rows(t: torch.Tensor, name: str, out: bool = False) -> None:
+    """(tokens, heads, D) rows that are loaded 16 bytes at a time; of an output, rows that do not overlap."""
+    n = 4 if t.dtype == torch.float32 else 8
+    s0, s1, s2 = t.stride()
+    if t.numel() == 0:
+        return
+    _need(s2 == 1, f"{name}: last dimension must be contiguous")
+    _need((s0 % n == 0 or t.shape[0] == 1) and (s1 % n == 0 or t.shape[1] == 1) and t.data_ptr() % 16 == 0,
+          f"{name}: rows must start at multiples of 16 bytes")
+    if out:
+        T, H, Dh = t.shape
+        _need((H == 1 or s1 >= Dh) and (T == 1 or s0 >= (Dh if H == 1 else s1 * (H - 1) + Dh))
+              or (T == 1 or s0 >= Dh) and (H == 1 or s1 >= (Dh if T == 1 else s0 * (T - 1) + Dh)),
+              f"{name}: rows overlap")
+
+
+def _strides(t: torch.Tensor) -> tuple:
+    """token and head strides; of a single token or head, whose stride is free, that of a contiguous row"""
+    s0, s1 = t.stride(0), t.stride(1)
+    return (s0 if t.shape[0] > 1 else 0), (s1 if t.shape[1] > 1 else 0)
+
+
+def qk_norm_rope(q, k, pos, cos, sin, wq=None, wk=None, eps: float = 1e-6, q_out=None, k_out=None):
+    """Query and key rows of a layer, each head normalised (x / sqrt(mean(x^2) + eps) * w) and turned to
+    its token's position (halves of the head dimension as pairs) in one pass, fp32 inside.
+    q (T, HQ, D), k (T, HKV, D) bf16, fp16 or fp32, D 64, 128 or 256, any token and head strides of whole
+    16 bytes (views of one product, say); pos (T,) int32 or int64; cos, sin (P, D / 2) fp32; wq, wk (D,)
+    of q's type, None for a rotation alone.  A token of negative position (padding) gives zeros, one of P
+    or more NaN.  Returns (q_out, k_out), contiguous unless given; either may be its input."""
+    dev = _dev(q, k, pos, cos, sin, wq, wk, q_out, k_out)
+    _need(q.dim() == 3 and k.dim() == 3 and q.shape[0] == k.shape[0] and q.shape[2] == k.shape[2],
+          "q, k: (T, HQ, D) and (T, HKV, D)")
+    T, HQ, Dh = q.shape
+    HKV = k.shape[1]
+    _need(q.dtype in _DT and k.dtype == q.dtype, "q, k: bf16, fp16 or fp32, both of one type")
+    _need(Dh in (64, 128, 256), "head dimension: 64, 128 or 256")
+    _need(T * (HQ + HKV) <= 1 << 27, "T * (HQ + HKV): at most 2^27 rows")
+    _need(pos.dtype in (torch.int32, torch.int64) and pos.shape == (T,) and pos.is_contiguous(),
+          "pos: (T,) int32 or int64, contiguous")
+    for t, name in ((cos, "cos"), (sin, "sin")):
+        _chk(t, name, torch.float32, (cos.shape[0], Dh // 2))
+        _need(t.shape[0] >= 1 and (t.stride(0) % 4 == 0 or t.shape[0] == 1) and t.stride(0) == cos.stride(0)
+              and t.data_ptr() % 16 == 0, "cos, sin: rows of one stride, starting at multiples of 16 bytes")
+    for t, name in ((wq, "wq"), (wk, "wk")):
+        if t is not None:
+            _chk(t, name, q.dtype, (Dh,), contiguous=True)
+            _need(t.data_ptr() % 16 == 0, f"{name}: base pointer misaligned")
+    _need(eps >= 0, "eps: not negative")
+    _plain((q, "q"), (k, "k"), (wq, "wq"), (wk, "wk"), (cos, "cos"), (sin, "sin"), (q_out, "q_out"), (k_out, "k_out"))
+    if q_out is None:
+        q_out = torch.empty(q.shape, device=dev, dtype=q.dtype)
+    if k_out is None:
+        k_out = torch.empty(k.shape, device=dev, dtype=k.dtype)
+    _need(q_out.shape == q.shape and k_out.shape == k.shape and q_out.dtype == q.dtype and k_out.dtype == q.dtype,
+          "q_out, k_out: as q, k")
+    for t, name, o in ((q, "q", False), (k, "k", False), (q_out, "q_out", True), (k_out, "k_out", True)):
+        _rows(t, name, o)
+    _run(dev, "oa_qk_norm_rope", _ptr(q), *_strides(q), _ptr(k), *_strides(k), T, HQ, HKV, Dh, _DT[q.dtype], _ptr(pos),
+         int(pos.dtype == torch.int64), _ptr(cos), _ptr(sin), cos.stride(0) if cos.shape[0] > 1 else 0, cos.shape[0],
+         _ptr(wq), _ptr(wk), float(eps), _ptr(q_out), *_strides(q_out), _ptr(k_out), *_strides(k_out))
+    return q_out, k_out
+
+
+def _page(page: int) -> None:
+    _need(32 <= page <= 1024 and page & (page - 1) == 0, f"page: a power of two, 32 to 1024 (got {page})")
+
+
+def _pages_state(count, lens, table, free, nfree, status, page: int, what: str) -> torch.device:
+    dev = _dev(count, lens, table, free, nfree, status)
+    _page(page)
+    _need(table.dim() == 2 and table.dtype == torch.int32 and table.shape[0] >= 1 and table.shape[1] >= 1
+          and (table.stride(1) == 1 or table.shape[1] == 1)
+          and (table.stride(0) >= table.shape[1] or table.shape[0] == 1), "table: (requests, width) int32 rows")
+    B, width = table.shape
+    for t, name, shape in ((count, what, (B,)), (lens, "lens", (B,)), (free, "free", (None,)), (nfree, "nfree", (1,)),
+                           (status, "status", (1,))):
+        _chk(t, name, torch.int32, shape, contiguous=True)
+    _need(free.numel() >= 1 and free.numel() * page < 1 << 31 and width * page < 1 << 31 and B <= 1 << 24,
+          "pool and table: fewer than 2^31 tokens, at most 2^24 requests")
+    return dev
+
+
+def kv_pages_extend(add, lens, table, free, nfree, status, page: int, total: int):
+    """Requests add tokens (add (B,) int32, lens (B,) what they hold): pages popped off the stack of free
+    ids (free, height nfree (1,)) into their rows of table (B, width), lens grown.  Returns int32 (slots
+    (total,), pos (total,), cu (B + 1,)): page id * page + offset and position of the new tokens, request
+    after request, from cu[i] on; -1 behind cu[B].  All on the device, so that a captured step can cross
+    into new pages.  For all requests or for none: where a count is negative, a request outgrows its row
+    (status |= 1), free pages do not reach (2) or there are more than `total` new tokens (4), nothing
+    changes, slots and pos are -1 and cu is 0; status (1,) is the caller's to look at and to clear."""
+    dev = _pages_state(add, lens, table, free, nfree, status, page, "add")
+    B, width = table.shape
+    _need(0 <= total <= 1 << 30, "total: 0 to 2^30")
+    buf = torch.empty(2 * total + 4 * B + 2, device=dev, dtype=torch.int32)
+    slots, pos, cu, ws = buf[:total], buf[total:2 * total], buf[2 * total:2 * total + B + 1], buf[2 * total + B + 1:]
+    _run(dev, "oa_kv_pages_extend", _ptr(add), _ptr(lens), _ptr(table), max(table.stride(0), width), _ptr(free),
+         _ptr(nfree), _ptr(status), B, width, free.numel(), page, total, _ptr(slots) or None, _ptr(pos) or None, _ptr(cu),
+         _ptr(ws))
+    return slots, pos, cu
+
+
+def kv_pages_truncate(keep, lens, table, free, nfree, status, page: int) -> None:
+    """Request i keeps its first min(keep[i], lens[i]) tokens (keep[i] < 0: all; 0: the request ends); pages
+    it no longer needs go back to the stack and leave the table (-1).  A truncation to the lengths before
+    an extension undoes it.  Nothing changes where the stack would outgrow `free` (status |= 2)."""
+    dev = _pages_state(keep, lens, table, free, nfree, status, page, "keep")
+    B, width = table.shape
+    ws = torch.empty(3 * B + 1, device=dev, dtype=torch.int32)
+    _run(dev, "oa_kv_pages_truncate", _ptr(keep), _ptr(lens), _ptr(table), max(table.stride(0), width), _ptr(free),
+         _ptr(nfree), _ptr(status), B, width, free.numel(), page, _ptr(ws))
+
+
+def _kv4_cache(kc, ks, vc, vs) -> tuple:
+    """(pages, heads, page, D) of a 4-bit cache's tensors; pages may lie apart (a layer of a larger tensor)."""
+    _need(kc.dim() == 4 and kc.dtype == torch.uint8 and kc.shape[0] >= 1 and kc.shape[1] >= 1,
+          "kc: (pages, heads, page, D / 2) uint8")
+    NP, HKV, page, half = kc.shape
+    Dh = 2 * half
+    _page(page)
+    _need(Dh in (64, 128), "head dimension: 64 or 128")
+    _need(NP * page < 1 << 31, "cache: fewer than 2^31 slots")
+    for t, name, w in ((kc, "kc", half), (vc, "vc", half), (ks, "ks", Dh // KV4_BLOCK), (vs, "vs", Dh // KV4_BLOCK)):
+        _need(t.dtype == torch.uint8 and t.shape == (NP, HKV, page, w), f"{name}: ({NP}, {HKV}, {page}, {w}) uint8")
+        _need(t.stride()[1:] == (page * w, w, 1) and (NP == 1 or t.stride(0) % 16 == 0 and t.stride(0) >= HKV * page * w)
+              and t.data_ptr() % 16 == 0, f"{name}: contiguous pages that start at multiples of 16 bytes")
+    _need(NP == 1 or kc.stride(0) == vc.stride(0) and ks.stride(0) == vs.stride(0),
+          "kc, vc and ks, vs: pages at the same distance")
+    return NP, HKV, page, Dh
+
+
+def _page_strides(kc, ks) -> tuple:
+    NP, HKV, page, half = kc.shape
+    return (kc.stride(0), ks.stride(0)) if NP > 1 else (HKV * page * half, HKV * page * ks.shape[3])
+
+
+def _slots(slots, T: int) -> None:
+    _chk(slots, "slots", torch.int32, (T,), contiguous=True)
+
+
+def kv4_write(k, v, slots, kc, ks, vc, vs) -> None:
+    """Key and value rows (T, HKV, D) bf16, fp16 or fp32 rounded to 4 bits (blocks of 32 with a power-of-two
+    scale) and put at slots (T,) int32 = page id * page + offset of the cache kc, vc (pages, HKV, page,
+    D / 2), ks, vs (pages, HKV, page, D / 32) uint8.  Rows of a slot outside of the cache (-1) are passed
+    over.  The slots of one call are distinct (a slot given twice ends with blocks of either row)."""
+    dev = _dev(k, v, slots, kc, ks, vc, vs)
+    NP, HKV, page, Dh = _kv4_cache(kc, ks, vc, vs)
+    T = k.shape[0]
+    _need(k.dim() == 3 and k.shape == (T, HKV, Dh) and v.shape == k.shape, f"k, v: (T, {HKV}, {Dh})")
+    _need(k.dtype in _DT and v.dtype == k.dtype, "k, v: bf16, fp16 or fp32, both of one type")
+    _need(T * HKV <= 1 << 26, "T * HKV: at most 2^26 rows")
+    _slots(slots, T)
+    _plain((k, "k"), (v, "v"))
+    _rows(k, "k")
+    _rows(v, "v")
+    _run(dev, "oa_kv4_write", _ptr(k), *_strides(k), _ptr(v), *_strides(v), T, HKV, Dh, _DT[k.dtype], _ptr(slots),
+         _ptr(kc), _ptr(ks), _ptr(vc), _ptr(vs), *_page_strides(kc, ks), NP, page)
+
+
+def kv4_read(slots, kc, ks, vc, vs, dtype: torch.dtype = torch.bfloat16):
+    """The values (k, v), each (T, HKV, D) bf16 (which holds them exactly) or fp32, at slots (T,) int32 of a
+    4-bit cache; zeros for a slot outside of it."""
+    dev = _dev(slots, kc, ks, vc, vs)
+    NP, HKV, page, Dh = _kv4_cache(kc, ks, vc, vs)
+    _need(slots.dim() == 1, "slots: (T,) int32")
+    T = slots.shape[0]
+    _slots(slots, T)
+    _need(dtype in (torch.bfloat16, torch.float32), "dtype: bf16 or fp32")
+    _need(T * HKV <= 1 << 26, "T * HKV: at most 2^26 rows")
+    k = torch.empty(T, HKV, Dh, device=dev, dtype=dtype)
+    v = torch.empty_like(k)
+    _run(dev, "oa_kv4_read", _ptr(slots), _ptr(kc), _ptr(ks), _ptr(vc), _ptr(vs), *_page_strides(kc, ks), NP, page,
+         _ptr(k), *_strides(k), _ptr(v), *_strides(v), T, HKV, Dh, _DT[dtype])
+    return k, v
+
+
+def kv4_chunk(cap: int, units: int) -> int:
+    """Keys per workgroup of kv4_attn: `units` (sequence, KV head, query tile) triples with up to `cap` keys
+    are cut until about 2048 workgroups are there, but into pieces of at least 256 keys."""
+    n = max(1, 2048 // max(units, 1))
+    return max(256, -(-cap // (n * 128)) * 128)
+
+
+def kv4_attn(q, kc, ks, vc, vs, table, lens, sm_scale: float | None = None, cu_q=None, max_q: int = 1, out=None,
+             max_len: int | None = None) -> torch.Tensor:
+    """Causal attention of the newest tokens of every sequence over a 4-bit paged cache.
+    q (T, HQ, D) bf16, HQ any multiple of the cache's heads; table (B, width) int32 page ids; lens (B,)
+    int32 keys that the sequences hold, these tokens among them.  Tokens cu_q[b] .. cu_q[b + 1] - 1
+    (cu_q (B + 1,) int32) are the last of sequence b, at most max_q of them; cu_q None: one token each.
+    Token j of R sees keys 0 .. lens[b] - R + j; one that sees none gives 0.  max_len: a bound on lens
+    that the caller knows (the table's width otherwise).  NaN: rows that need a page id outside of the
+    cache, and those of sequences longer than their table row or than max_len (rounded up to whole pieces,
+    kv4_chunk).  Rows of `out` behind
+    cu_q[B] are left as they were (0 where the call makes it)."""
+    dev = _dev(q, kc, ks, vc, vs, table, lens, cu_q, out)
+    NP, HKV, page, Dh = _kv4_cache(kc, ks, vc, vs)
+    _need(q.dim() == 3 and q.dtype == torch.bfloat16 and q.shape[2] == Dh and q.shape[1] >= 1 and q.shape[1] % HKV == 0,
+          f"q: (T, a multiple of {HKV}, {Dh}) bf16")
+    T, HQ, _ = q.shape
+    _need(table.dim() == 2 and table.dtype == torch.int32 and table.shape[1] >= 1
+          and (table.stride(1) == 1 or table.shape[1] == 1)
+          and (table.stride(0) >= table.shape[1] or table.shape[0] <= 1), "table: (B, width) int32 rows")
+    B, width = table.shape
+    _need(width * page < 1 << 31, "table: fewer than 2^31 keys to a row")
+    _chk(lens, "lens", torch.int32, (B,), contiguous=True)
+    if cu_q is None:
+        _need(T == B and max_q == 1, "without cu_q every sequence has one row of q")
+    else:
+        _chk(cu_q, "cu_q", torch.int32, (B + 1,), contiguous=True)
+    _need(max_q >= 1 and max_q * (HQ // HKV) <= 1 << 30, "max_q: at least 1")
+    scale = Dh ** -0.5 if sm_scale is None else float(sm_scale)
+    _need(scale == scale, "sm_scale is NaN")
+    _need(max_len is None or max_len >= 0, "max_len: not negative")
+    _plain((q, "q"), (out, "out"))
+    _rows(q, "q")
+    if out is None:
+        out = (torch.empty if cu_q is None else torch.zeros)(q.shape, device=dev, dtype=q.dtype)
+    _need(out.shape == q.shape and out.dtype == q.dtype, "out: as q")
+    _rows(out, "out", True)
+    if T == 0 or B == 0:
+        return out
+    rows = max_q * (HQ // HKV)
+    cap = max(1, width * page if max_len is None else min(max_len, width * page))
+    chunk = kv4_chunk(cap, B * HKV * -(-rows // (8 if rows <= 8 else 16 if rows <= 16 else 32)))
+    nchunk = -(-cap // chunk)
+    ml = ws = None
+    if nchunk > 1:
+        n = T * HQ * nchunk
+        ws = torch.empty(n * (Dh + 2), device=dev, dtype=torch.float32)
+        ml = ws[n * Dh:]
+    _run(dev, "oa_kv4_attn", _ptr(q), *_strides(q), _ptr(kc), _ptr(ks), _ptr(vc), _ptr(vs), *_page_strides(kc, ks), NP,
+         page, _ptr(table), max(table.stride(0), width), width, _ptr(lens), _ptr(cu_q), B, T, max_q, HQ, HKV, Dh, scale,
+         chunk, nchunk, _ptr(ws), _ptr(ml), _ptr(out), *_strides(out))
+    return out
 
 
 # ================================================================== prefill index build

@@ -1,0 +1,537 @@
+"""The 4-bit paged cache on the GPU: head norms with rotation, page tables, cache rows and attention
+against 64-bit references (tests/kv4_ref.py), alone and as a decode loop runs them."""
+import math
+import random
+
+import pytest
+import torch
+
+from openattention_amd import ops
+from tests import kv4_ref as ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def randn(g, *shape, dtype=torch.float32):
+    return torch.randn(*shape, generator=g, device=DEV).to(dtype)
+
+
+def i32(x):
+    return torch.tensor(x, device=DEV, dtype=torch.int32)
+
+
+def tables(P, D, half=None):
+    inv = 500000.0 ** (-torch.arange(0, D, 2, dtype=torch.float64) / D)
+    a = torch.arange(P, dtype=torch.float64)[:, None] * inv
+    return a.cos().float().to(DEV), a.sin().float().to(DEV)
+
+
+# ================================================================== head norms with rotation
+def check_rope(out, x, pos, cos, sin, w, eps):
+    want, size = ref.rope(x, pos, cos, sin, w, eps)
+    # fp32: 16 squares a lane and four joins, halved by the root (10), mean, root, quotient, two products
+    # (5), a product and a sum of the rotation (2): under 20 steps of 2^-24; then the type's own rounding
+    half = torch.finfo(x.dtype).eps / 2
+    tol = 20 * 2.0 ** -24 * size
+    tol = tol + half * (want.abs() + tol) + (2.0 ** -24 if x.dtype == torch.float16 else 0)
+    bad = ~((out.double() - want).abs() <= tol)
+    assert torch.equal(torch.isnan(want), torch.isnan(out))
+    assert not (bad & ~torch.isnan(want)).any()
+
+
+@pytest.mark.parametrize("T,HQ,HKV,D,dtype,norm,pos64", [
+    (1, 32, 8, 128, torch.bfloat16, True, False), (33, 32, 8, 128, torch.bfloat16, True, True),
+    (257, 14, 2, 64, torch.float16, False, False), (5, 3, 1, 256, torch.float32, True, True),
+    (70, 7, 7, 128, torch.float16, True, False), (1001, 5, 1, 64, torch.bfloat16, False, True),
+    (9, 1, 0, 128, torch.bfloat16, True, False), (3, 40, 8, 128, torch.float32, False, False)])
+def test_rope(T, HQ, HKV, D, dtype, norm, pos64):
+    print(f"[case] rope {T} {HQ} {HKV} {D} {dtype} norm={norm}", flush=True)
+    g = gen(T)
+    qkv = randn(g, T, (HQ + 2 * HKV) * D, dtype=dtype)
+    q = qkv[:, :HQ * D].view(T, HQ, D)
+    k = qkv[:, HQ * D:(HQ + HKV) * D].view(T, HKV, D)
+    cos, sin = tables(5000, D)
+    pos = torch.randint(0, 5000, (T,), generator=g, device=DEV)
+    pos = pos if pos64 else pos.int()
+    wq, wk = (randn(g, D, dtype=dtype), randn(g, D, dtype=dtype)) if norm else (None, None)
+    keep = qkv.clone()
+    qo, ko = ops.qk_norm_rope(q, k, pos, cos, sin, wq, wk, 1e-5)
+    assert torch.equal(qkv, keep)
+    check_rope(qo, q, pos, cos, sin, wq, 1e-5)
+    check_rope(ko, k, pos, cos, sin, wk, 1e-5)
+
+
+def test_rope_layouts_padding_and_in_place():
+    """Head-major rows, wider tables, one norm only, zero rows, padding, positions past the tables, outputs
+    that are the inputs; what the call does not own stays as it was."""
+    g = gen(7)
+    T, HQ, HKV, D = 13, 4, 2, 128
+    q = randn(g, HQ, T, D, dtype=torch.bfloat16).transpose(0, 1)
+    k = randn(g, HKV, T, D + 8, dtype=torch.bfloat16).transpose(0, 1)[..., :D]
+    q[4] = 0
+    cos, sin = tables(100, 2 * D)
+    cos, sin = cos[:, :D // 2], sin[:, :D // 2]
+    pos = torch.randint(0, 100, (T,), generator=g, device=DEV)
+    pos[2], pos[5], pos[7], pos[9] = -1, 100, -(1 << 40), 1 << 40
+    wk = randn(g, D, dtype=torch.bfloat16)
+    for wq in (None, randn(g, D, dtype=torch.bfloat16)):
+        qo = torch.full((T + 1, HQ, D), 7.0, device=DEV, dtype=torch.bfloat16)
+        a, b = ops.qk_norm_rope(q, k, pos, cos, sin, wq, wk, 1e-5, q_out=qo[:T])
+        assert a.data_ptr() == qo.data_ptr() and (qo[T] == 7).all()
+        check_rope(a, q, pos, cos, sin, wq, 1e-5)
+        check_rope(b, k, pos, cos, sin, wk, 1e-5)
+    q2, k2 = q.clone(memory_format=torch.preserve_format), k.clone()
+    ops.qk_norm_rope(q2, k2, pos, cos, sin, wq, wk, 1e-5, q_out=q2, k_out=k2)
+    assert torch.equal(q2.isnan(), a.isnan()) and torch.equal(q2.nan_to_num(), a.nan_to_num())
+    assert torch.equal(k2.nan_to_num(), b.nan_to_num())
+    e = ops.qk_norm_rope(q[:0], k[:0], pos[:0], cos, sin, wq, wk)
+    assert e[0].shape == (0, HQ, D)
+
+
+# ================================================================== pages
+def pool_state(seed, B, width, page, spare):
+    r = random.Random(seed)
+    lens = [r.choice((0, 1, page - 1, page, page + 1, r.randrange(width * page // 2))) for _ in range(B)]
+    lens = [min(n, width * page) for n in lens]
+    held = [-(-n // page) for n in lens]
+    NP = sum(held) + spare
+    ids = list(range(NP))
+    r.shuffle(ids)
+    table, at = [], 0
+    for h in held:
+        table.append(ids[at:at + h] + [-1] * (width - h))
+        at += h
+    free = ids[at:] + [0] * at
+    return lens, table, free, spare
+
+
+def same(pool, lens, table, free, nfree, status):
+    assert lens.tolist() == pool.lens and table.tolist() == pool.table and int(nfree) == pool.nfree
+    assert free.tolist() == pool.free and int(status) == pool.status
+
+
+@pytest.mark.parametrize("B,width,page,most", [(1, 4, 32, 40), (5, 9, 64, 100), (64, 12, 32, 60), (300, 5, 128, 30),
+                                               (1500, 6, 32, 9)])
+def test_pages_follow_the_pool(B, width, page, most):
+    print(f"[case] pages {B} {width} {page} {most}", flush=True)
+    lens, table, free, spare = pool_state(B, B, width, page, 4 * B)
+    pool = ref.Pool(lens, table, free, spare, page)
+    st = [i32(lens), i32(table), i32(free), i32([spare]), i32([0])]
+    r = random.Random(B + 1)
+    for it in range(8):
+        add = [r.choice((0, 1, 1, r.randint(0, most))) for _ in range(B)]
+        if it == 3:
+            add[r.randrange(B)] = -1
+        total = sum(max(a, 0) for a in add) + r.choice((0, 0, 3))
+        if it == 5:
+            total = max(0, sum(add) - 1)
+        want = pool.extend(add, total)
+        got = ops.kv_pages_extend(i32(add), *st, page, total)
+        for w, x in zip(want, got):
+            assert x.dtype == torch.int32 and x.tolist() == w
+        same(pool, *st)
+        keep = [r.choice((-1, n, max(0, n - 1), r.randint(0, n + 2), 0)) for n in pool.lens]
+        pool.truncate(keep)
+        ops.kv_pages_truncate(i32(keep), *st, page)
+        same(pool, *st)
+
+
+def test_pages_refusals_change_nothing():
+    page = 32
+    # (30 and 32 tokens in a page each, one page free, rows of 128 tokens: 30 + 3 and 32 + 3 take a page each,
+    # 30 + 97 three more)
+    for add, total, why in (([1, -1], 9, 1), ([1, 97], 99, 1), ([40, 40], 80, 2), ([3, 3], 5, 2 | 4), ([97, 60], 9, 2 | 4),
+                            ([1, 0], 0, 4), ([2, 3], 4, 4), ([99, 1], 0, 1 | 4)):
+        lens, table, free = i32([30, 32]), i32([[3, -1, -1, -1], [0, -1, -1, -1]]), i32([1, 2, 9, 9])
+        st = [lens, table, free, i32([1]), i32([0])]
+        keep = [t.clone() for t in st]
+        slots, pos, cu = ops.kv_pages_extend(i32(add), *st, page, total)
+        assert int(st[4]) == why
+        assert (slots == -1).all() and (pos == -1).all() and (cu == 0).all() and cu.numel() == 3
+        assert all(torch.equal(a, b) for a, b in zip(st[:4], keep[:4]))
+        st[4] |= 8                                        # the word is added to, never cleared
+        ops.kv_pages_extend(i32([1, 0]), *st, page, 4)
+        assert int(st[4]) == why | 8 and st[0].tolist() == [31, 32]
+    # more pages than the stack can hold go back to nothing
+    st = [i32([64, 64]), i32([[0, 1], [2, 3]]), i32([5, 6, 7, 8]), i32([2]), i32([0])]
+    ops.kv_pages_truncate(i32([0, 0]), *st, 32)
+    assert int(st[4]) == 2 and st[0].tolist() == [64, 64] and st[1].tolist() == [[0, 1], [2, 3]] and int(st[3]) == 2
+    # lengths outside of a row, ids outside of the pool: no slot is given
+    st = [i32([-5, 0]), i32([[0, 1], [2, 3]]), i32([5, 6, 7, 8]), i32([2]), i32([0])]
+    assert (ops.kv_pages_extend(i32([1, 1]), *st, 32, 2)[0] == -1).all() and int(st[4]) == 1
+    st = [i32([0, 3]), i32([[0, 1], [1 << 27, 3]]), i32([5, -7, 7, 8]), i32([2]), i32([0])]
+    assert ops.kv_pages_extend(i32([1, 1]), *st, 32, 2)[0].tolist() == [-1, -1]
+
+
+def test_pages_rows_of_a_wider_table():
+    wide = torch.full((3, 10), 77, device=DEV, dtype=torch.int32)
+    table = wide[:, 2:6]
+    table.fill_(-1)
+    st = [i32([0, 0, 0]), table, i32(range(9)), i32([9]), i32([0])]
+    slots, pos, cu = ops.kv_pages_extend(i32([33, 0, 5]), *st, 32, 38)
+    assert table.tolist() == [[8, 7, -1, -1], [-1] * 4, [6, -1, -1, -1]] and cu.tolist() == [0, 33, 33, 38]
+    assert (wide[:, :2] == 77).all() and (wide[:, 6:] == 77).all()
+
+
+# ================================================================== cache rows
+def new_cache(NP, HKV, page, D, fill=None, g=None):
+    out = []
+    for w in (D // 2, D // 32, D // 2, D // 32):
+        if fill is None:
+            out.append(torch.randint(0, 256, (NP, HKV, page, w), generator=g, device=DEV, dtype=torch.uint8))
+        else:
+            out.append(torch.full((NP, HKV, page, w), fill, device=DEV, dtype=torch.uint8))
+    return out
+
+
+def hard_rows(T, HKV, D, dtype, g):
+    """Rows whose blocks meet every rule: borders between codes and their neighbours, all magnitudes,
+    zeros of both signs, values that are not finite."""
+    x = randn(g, T, HKV, D)
+    e = torch.randint(-40 if dtype != torch.float16 else -12, 40 if dtype != torch.float16 else 12, (T, HKV, D // 32, 1),
+                      generator=g, device=DEV).float()
+    x = (x.unflatten(-1, (-1, 32)) * torch.exp2(e)).flatten(-2)
+    edge = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 6.99, 7.0, 0.0, -0.0, -0.25, -5.0, 3.0, 0.5], device=DEV)
+    b = x.view(T, HKV, -1, 32)
+    b[0::3, :, 0, :16] = edge * torch.exp2(e[0::3, :, 0])
+    b[0::3, :, 0, 16:] = b[0::3, :, 0, :16] * (1 + 2.0 ** -8)
+    b[1::3, :, 0] = 7.0 * torch.exp2(e[1::3, :, 0]) * torch.where(torch.arange(32, device=DEV) == 9, 1.0, 2.0 ** -6)
+    b[2::7, :, 1] = 0
+    x = x.to(dtype)
+    flat = x.view(T, HKV, -1, 32)
+    if T > 8:
+        flat[3, 0, 0, 5], flat[4, 0, 0, 31], flat[5, 0, 1, 0] = math.nan, math.inf, -math.inf
+        if dtype != torch.float16:
+            flat[6, 0, 0] = torch.tensor([2.0 ** -126, -2.0 ** -127, 2.0 ** -128, 3 * 2.0 ** -128] * 8).to(dtype)
+            flat[7, 0, 0, 3] = torch.finfo(dtype).max
+            flat[8, 0, 1, :2] = torch.tensor([1.75 * 2.0 ** 127, 1.7 * 2.0 ** 127]).to(dtype)
+    return x
+
+
+@pytest.mark.parametrize("T,HKV,D,page,dtype", [(1, 8, 128, 64, torch.bfloat16), (50, 3, 128, 32, torch.bfloat16),
+                                                (301, 2, 64, 128, torch.float16), (77, 5, 64, 32, torch.float32),
+                                                (40, 1, 128, 64, torch.float32), (33, 8, 128, 64, torch.float16)])
+def test_cache_rows_are_the_nearest_codes(T, HKV, D, page, dtype):
+    print(f"[case] cache rows {T} {HKV} {D} {page} {dtype}", flush=True)
+    g = gen(T + D)
+    NP = -(-T // page) + 2
+    cache = new_cache(NP, HKV, page, D, g=g)
+    before = [t.clone() for t in cache]
+    kv = torch.cat([hard_rows(T, HKV, D, dtype, g), hard_rows(T, HKV, D, dtype, g)], 1)       # side by side, as in a product
+    k, v = kv[:, :HKV], kv[:, HKV:]
+    slots = torch.randperm(NP * page, generator=g, device=DEV)[:T].int()
+    ops.kv4_write(k, v, slots, *cache)
+    p, o = slots.long() // page, slots.long() % page
+    for x, c, s in ((k, 0, 1), (v, 2, 3)):
+        qc, qs = ref.quantise(x)
+        before[c][p, :, o], before[s][p, :, o] = qc, qs
+        assert torch.equal(cache[s], before[s])
+        assert torch.equal(cache[c], before[c])
+    for dt in (torch.bfloat16, torch.float32):
+        for x, c, s in zip(ops.kv4_read(slots, *cache, dtype=dt), (0, 2), (1, 3)):
+            want = ref.rows_at(cache[c], cache[s], slots)
+            assert x.dtype == dt and torch.equal(x.isnan(), want.isnan())
+            assert torch.equal(x.double().nan_to_num(7.0), want.nan_to_num(7.0))
+
+
+def test_cache_every_bf16_value():
+    """Each of the 65536 bf16 patterns, in blocks with a larger neighbour and alone."""
+    bits = torch.arange(65536, device=DEV, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    alone = torch.zeros(65536, 32, device=DEV, dtype=torch.bfloat16)
+    alone[:, 11] = bits
+    beside = alone.clone()
+    beside[:, 3] = (bits.float().abs() * 5.3).clamp(max=3e38).to(torch.bfloat16)
+    x = torch.cat([alone, beside]).view(1024, 32, 2, 64)
+    k, v = x[:, :, 0], x[:, :, 1]
+    cache = new_cache(32, 32, 32, 64, fill=0)
+    slots = torch.arange(1024, device=DEV, dtype=torch.int32)
+    ops.kv4_write(k, v, slots, *cache)
+    for y, c, s in ((k, 0, 1), (v, 2, 3)):
+        qc, qs = ref.quantise(y)
+        assert torch.equal(cache[s].transpose(1, 2).reshape(1024, 32, 2), qs)
+        assert torch.equal(cache[c].transpose(1, 2).reshape(1024, 32, 32), qc)
+
+
+def test_cache_padding_and_layers_of_one_tensor():
+    """Slots outside of the cache are passed over and read as zeros; the caches of several layers lie in one
+    tensor, page by page; the neighbours keep what they hold."""
+    g = gen(3)
+    NP, HKV, page, D, T = 5, 2, 32, 128, 20
+    big = [torch.randint(0, 256, (NP, 3, HKV, page, w), generator=g, device=DEV, dtype=torch.uint8) for w in (64, 4, 64, 4)]
+    keep = [t.clone() for t in big]
+    cache = [t[:, 1] for t in big]
+    k, v = randn(g, T, HKV, D, dtype=torch.bfloat16), randn(g, T, HKV, D, dtype=torch.bfloat16)
+    slots = torch.randperm(NP * page, generator=g, device=DEV)[:T].int()
+    slots[3], slots[8], slots[19] = -1, NP * page, -(1 << 31)
+    ops.kv4_write(k, v, slots, *cache)
+    ok = (slots >= 0) & (slots < NP * page)
+    p, o = slots[ok].long() // page, slots[ok].long() % page
+    for x, c in ((k, 0), (v, 2)):
+        qc, qs = ref.quantise(x[ok])
+        keep[c][p, 1, :, o], keep[c + 1][p, 1, :, o] = qc, qs
+    assert all(torch.equal(a, b) for a, b in zip(big, keep))
+    kr, vr = ops.kv4_read(slots, *cache)
+    assert (kr[~ok] == 0).all() and (vr[~ok] == 0).all()
+    assert torch.equal(kr[ok].double(), ref.rows_at(cache[0], cache[1], slots[ok]))
+    ops.kv4_write(k[:0], v[:0], slots[:0], *cache)
+    assert ops.kv4_read(slots[:0], *cache)[0].shape == (0, HKV, D)
+
+
+# ================================================================== attention
+def paged(lens, HKV, D, page, g, spare=2, extra_width=0):
+    """A cache of garbage with the sequences' rows put into shuffled pages of it."""
+    held = [-(-n // page) for n in lens]
+    NP = sum(held) + spare
+    cache = new_cache(NP, HKV, page, D, g=g)
+    for s in (1, 3):                                      # garbage scales, NaN among them
+        cache[s].copy_(torch.where(cache[s] % 3 == 0, 255, cache[s] % 252 + 2))
+    perm = torch.randperm(NP, generator=g, device=DEV).tolist()
+    width = max(max(held), 1) + extra_width
+    table, at = [], 0
+    for h in held:
+        table.append(perm[at:at + h] + [-1] * (width - h))
+        at += h
+    table = i32(table)
+    for slots in ref.held(table, lens, page):
+        if slots.numel():
+            k, v = randn(g, slots.numel(), HKV, D) * 1.5, randn(g, slots.numel(), HKV, D)
+            ops.kv4_write(k, v, slots.int().to(DEV), *cache)
+    return cache, table
+
+
+def want_attn(q, cache, table, lens, cu, scale, page):
+    out = torch.zeros(q.shape, dtype=torch.float64, device=DEV)
+    err = torch.zeros_like(out)
+    for b, slots in enumerate(ref.held(table, lens, page)):
+        r = slice(cu[b], cu[b + 1])
+        slots = slots.to(DEV)
+        k, v = ref.rows_at(cache[0], cache[1], slots), ref.rows_at(cache[2], cache[3], slots)
+        out[r], err[r] = ref.attn(q[r], k, v, lens[b], scale)
+    return out, err
+
+
+def check_attn(out, want, err):
+    half = torch.finfo(torch.bfloat16).eps / 2
+    assert torch.equal(out.isnan(), want.isnan())
+    bad = ~((out.double() - want).abs() <= err + half * (want.abs() + err)) & ~want.isnan()
+    assert not bad.any(), ((out.double() - want).abs() - err - half * want.abs()).nan_to_num(0).max()
+
+
+def starts(rows):
+    cu = [0]
+    for r in rows:
+        cu.append(cu[-1] + r)
+    return cu
+
+
+CASES = [  # lens, rows (None: one each), HQ, HKV, D, page
+    ([1], None, 4, 1, 128, 32), ([31], None, 32, 8, 128, 64), ([33, 0, 1, 64, 65, 32, 700], None, 32, 8, 128, 32),
+    ([129, 127, 128], None, 8, 8, 128, 64), ([300, 5], None, 14, 2, 64, 128), ([1025], None, 40, 8, 128, 1024),
+    ([97], None, 48, 2, 64, 32), ([515, 1, 40], [2, 1, 2], 32, 8, 128, 64), ([100, 33, 7, 0], [4, 0, 4, 0], 16, 4, 128, 32),
+    ([260, 90], [33, 65], 8, 2, 128, 64), ([130], [130], 6, 2, 64, 32), ([400, 3, 77], [5, 3, 1], 14, 2, 64, 64),
+    ([4000], None, 4, 1, 128, 64), ([2, 5], [4, 9], 4, 2, 128, 32), ([2500, 800], [20, 3], 7, 1, 128, 32)]
+
+
+@pytest.mark.parametrize("case", range(len(CASES)))
+@pytest.mark.parametrize("chunk", [None, 128, 100000])
+def test_attention(case, chunk, monkeypatch):
+    lens, rows, HQ, HKV, D, page = CASES[case]
+    print(f"[case] attn {CASES[case]} chunk={chunk}", flush=True)
+    if chunk:
+        monkeypatch.setattr(ops, "kv4_chunk", lambda cap, units: min(chunk, -(-cap // 128) * 128))
+    g = gen(case)
+    cache, table = paged(lens, HKV, D, page, g, extra_width=case % 3)
+    cu = starts(rows or [1] * len(lens))
+    # the rows of a product, every second token's
+    q = randn(g, 2 * cu[-1], HQ + 2, D, dtype=torch.bfloat16)[::2, 1:-1] * 1.3
+    scale = D ** -0.5 if case % 2 else 0.11
+    out = ops.kv4_attn(q, *cache, table, i32(lens), scale, cu_q=i32(cu) if rows else None, max_q=max(rows) if rows else 1)
+    check_attn(out, *want_attn(q, cache, table, lens, cu, scale, page))
+
+
+def test_attention_scales():
+    """A negative scale, one of zero, large scores (one key takes all), and equal keys."""
+    g = gen(5)
+    lens = [150, 70]
+    cache, table = paged(lens, 2, 128, 32, g)
+    q = randn(g, 2, 8, 128, dtype=torch.bfloat16)
+    for scale in (-0.09, 0.0, 30.0):
+        out = ops.kv4_attn(q, *cache, table, i32(lens), scale)
+        check_attn(out, *want_attn(q, cache, table, lens, [0, 1, 2], scale, 32))
+    k = torch.ones(150, 2, 128, device=DEV)
+    slots = ref.held(table, lens, 32)[0].int().to(DEV)
+    v = randn(g, 150, 2, 128)
+    ops.kv4_write(k * 2.0 ** 90, v, slots, *cache)
+    q = torch.full_like(q, 2.0 ** 30)
+    out = ops.kv4_attn(q, *cache, table, i32(lens), 1e-6)
+    check_attn(out[:1], *want_attn(q[:1], cache, table[:1], lens[:1], [0, 1], 1e-6, 32))
+
+
+@pytest.mark.parametrize("rows", [1, 3, 40])
+def test_attention_nan_stays_with_who_sees_it(rows):
+    """A key or a value that is not finite makes NaN of the rows that see it (a value: of its block of
+    dims), and of no others: not of earlier tokens, other heads or other sequences."""
+    g = gen(rows)
+    lens, page = [70, 70, 70], 32
+    cache, table = paged(lens, 2, 128, page, g)
+    held = ref.held(table, lens, page)
+    for b, key in ((0, 69 - rows // 2), (1, 50), (2, 69)):
+        k, v = randn(g, 1, 2, 128), randn(g, 1, 2, 128)
+        v[0, 1, 40] = math.nan
+        if b == 1:
+            k[0, 0, 3] = math.inf
+        ops.kv4_write(k, v, held[b][key:key + 1].int().to(DEV), *cache)
+    cu = starts([rows] * 3)
+    q = randn(g, cu[-1], 8, 128, dtype=torch.bfloat16)
+    out = ops.kv4_attn(q, *cache, table, i32(lens), cu_q=i32(cu), max_q=rows)
+    want, err = want_attn(q, cache, table, lens, cu, 128 ** -0.5, page)
+    # a row that does not see the key is formed without it; matmul's 0 * NaN of the reference is not
+    assert want.isnan().any() and not want.isnan().all()
+    check_attn(out, want, err)
+
+
+def test_attention_bad_pages_lengths_and_starts():
+    """Page ids outside of the cache, lengths past the table, starts that do not fit: NaN, or rows left as
+    they were, and no access outside of the cache."""
+    g = gen(11)
+    lens, page = [100, 100, 100, 40], 32
+    cache, table = paged(lens, 2, 128, page, g)
+    q = randn(g, 4, 8, 128, dtype=torch.bfloat16)
+    table[0, 1], table[1, 3], table[3, 3] = -1, 1 << 30, 12345
+    out = ops.kv4_attn(q, *cache, table, i32([100, 100, 100, 40]))
+    assert out[:2].isnan().all() and not out[2:].isnan().any()
+    out = ops.kv4_attn(q, *cache, table, i32([100, 1 << 30, 100, -3]), max_len=128)
+    assert out[1].isnan().all() and (out[3] == 0).all() and not out[2].isnan().any()
+    own = torch.full_like(q, 5.0)
+    ops.kv4_attn(q, *cache, table, i32(lens), cu_q=i32([0, 0, 0, 1, 2]), max_q=1, out=own)
+    assert not own[0].isnan().any() and (own[2:] == 5).all()
+    own.fill_(5.0)
+    ops.kv4_attn(q, *cache, table, i32(lens), cu_q=i32([9, 3, -4, 1 << 30, -(1 << 31)]), max_q=2, out=own)
+    assert (own == 5).all()
+    new = ops.kv4_attn(q, *cache, table, i32(lens), cu_q=i32([0, 0, 0, 1, 1]), max_q=1)
+    assert (new[1:] == 0).all()
+    assert ops.kv4_attn(q[:0], *cache, table[:0], i32([])).shape == (0, 8, 128)
+
+
+def test_pages_far_apart():
+    """Offsets past 32 bits: pages of codes 2^31 + 4096 bytes apart."""
+    step = (1 << 31) + 4096
+    base = [torch.empty(2 * step + 8192, device=DEV, dtype=torch.uint8) for _ in range(2)]
+    sc = [torch.empty(3, 1, 32, 4, device=DEV, dtype=torch.uint8) for _ in range(2)]
+    cache = [base[0].as_strided((3, 1, 32, 64), (step, 2048, 64, 1)), sc[0],
+             base[1].as_strided((3, 1, 32, 64), (step, 2048, 64, 1)), sc[1]]
+    g = gen(2)
+    table, lens = i32([[2, 0, 1]]), [90]
+    slots = ref.held(table, lens, 32)[0].int().to(DEV)
+    k, v = randn(g, 90, 1, 128), randn(g, 90, 1, 128)
+    ops.kv4_write(k, v, slots, *cache)
+    kr, _ = ops.kv4_read(slots, *cache, dtype=torch.float32)
+    qc, qs = ref.quantise(k)
+    assert torch.equal(kr.double(), ref.values(qc, qs))
+    q = randn(g, 1, 4, 128, dtype=torch.bfloat16)
+    out = ops.kv4_attn(q, *cache, table, i32(lens))
+    check_attn(out, *want_attn(q, cache, table, lens, [0, 1], 128 ** -0.5, 32))
+
+
+# ================================================================== together
+def decode_loop(steps, graph, B=3, HQ=8, HKV=2, D=128, page=32, seed=0):
+    """Tokens of B sequences through extension, norm and rotation, cache and attention, one step after the
+    other, eagerly or as one captured step that is replayed; returns outputs of every step and the state."""
+    g = gen(seed)
+    width, NP = 4, 14
+    cache = new_cache(NP, HKV, page, D, fill=255)
+    lens, table = i32([29, 0, 63][:B]), torch.full((B, width), -1, device=DEV, dtype=torch.int32)
+    free, nfree, status = torch.arange(NP, device=DEV, dtype=torch.int32), i32([NP]), i32([0])
+    cos, sin = tables(width * page, D)
+    wq, wk = randn(g, D, dtype=torch.bfloat16), randn(g, D, dtype=torch.bfloat16)
+    # the prompts
+    start = lens.clone()
+    lens.zero_()
+    total = int(start.sum())
+    slots, pos, cu = ops.kv_pages_extend(start, lens, table, free, nfree, status, page, total)
+    prompt = randn(g, total, (HQ + 2 * HKV) * D, dtype=torch.bfloat16)
+    xs = randn(g, steps, B, (HQ + 2 * HKV) * D, dtype=torch.bfloat16)
+    one = torch.ones(B, device=DEV, dtype=torch.int32)
+    x = torch.empty_like(xs[0])
+
+    def layer(x, slots, pos, **kw):
+        n = x.shape[0]
+        q, k = ops.qk_norm_rope(x[:, :HQ * D].view(n, HQ, D), x[:, HQ * D:(HQ + HKV) * D].view(n, HKV, D), pos, cos, sin,
+                                wq, wk)
+        ops.kv4_write(k, x[:, (HQ + HKV) * D:].view(n, HKV, D), slots, *cache)
+        return ops.kv4_attn(q, *cache, table, lens, **kw), q, k
+
+    def step():
+        slots, pos, _ = ops.kv_pages_extend(one, lens, table, free, nfree, status, page, B)
+        return layer(x, slots, pos)
+
+    outs = [layer(prompt, slots, pos, cu_q=cu, max_q=63)[0].clone()]
+    if graph:
+        x.copy_(xs[0])
+        state = [t.clone() for t in (lens, table, free, nfree, status, *cache)]
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            step()
+        torch.cuda.current_stream().wait_stream(s)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            res = step()
+        for t, u in zip((lens, table, free, nfree, status, *cache), state):
+            t.copy_(u)
+    for i in range(steps):
+        x.copy_(xs[i])
+        if graph:
+            gr.replay()
+        else:
+            res = step()
+        outs.append(res[0].clone())
+        if i % 3 == 0:
+            torch.cuda.synchronize()
+    return outs, [lens, table, free, nfree, status, *cache], (prompt, xs, start, cos, sin, wq, wk)
+
+
+def test_decode_loop_eager_and_captured():
+    """40 steps that cross pages: a captured step replayed gives what the eager loop gives, bit for bit, and
+    both what the sequences' own rows give in 64 bits."""
+    steps, HQ, HKV, D, page = 40, 8, 2, 128, 32
+    eager, st, (prompt, xs, start, cos, sin, wq, wk) = decode_loop(steps, False)
+    captured, st2, _ = decode_loop(steps, True)
+    assert all(torch.equal(a, b) for a, b in zip(eager, captured))
+    assert all(torch.equal(a, b) for a, b in zip(st, st2))
+    assert int(st[4]) == 0
+    lens, first = start.tolist(), starts(start.tolist())
+    for b in range(3):
+        rows = torch.cat([prompt[first[b]:first[b + 1]], xs[:, b]])
+        n = rows.shape[0]
+        q, k = ops.qk_norm_rope(rows[:, :HQ * D].view(n, HQ, D), rows[:, HQ * D:(HQ + HKV) * D].view(n, HKV, D),
+                                torch.arange(n, device=DEV), cos, sin, wq, wk)
+        kk = ref.values(*ref.quantise(k))
+        vv = ref.values(*ref.quantise(rows[:, (HQ + HKV) * D:].view(n, HKV, D)))
+        want, err = ref.attn(q, kk, vv, n, D ** -0.5)
+        check_attn(eager[0][first[b]:first[b + 1]], want[:lens[b]], err[:lens[b]])
+        check_attn(torch.stack([eager[1 + i][b] for i in range(steps)]), want[lens[b]:], err[lens[b]:])
+
+
+def test_two_streams_at_once():
+    """Two attentions and two extensions over different states on two streams give what each gives alone."""
+    g = gen(9)
+    sets = []
+    for n in (3000, 2000):
+        cache, table = paged([n], 8, 128, 64, g)
+        sets.append((randn(g, 1, 32, 128, dtype=torch.bfloat16), cache, table, i32([n])))
+    alone = [ops.kv4_attn(q, *c, t, n) for q, c, t, n in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, ((q, c, t, n), s) in enumerate(zip(sets, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(ops.kv4_attn(q, *c, t, n))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, a) for xs, a in zip(got, alone) for x in xs)
