@@ -13,6 +13,7 @@
 // Weights go into the product as two bf16 terms, so that the sum keeps 16 bits of each: up to 8 rows
 // the second term sits in the tile's other 8 columns, otherwise it takes a second product.
 #include <cfloat>
+#include <type_traits>
 
 #include "oa_common.h"
 
@@ -40,7 +41,7 @@ struct AttnArgs {
   const int* lens; const int* cu;
   uint16_t* out; long o_st, o_sh;
   float* ws_o; float* ws_ml;             // partial sums, (maximum, sum) by (row, chunk)
-  int B, HKV, G, tokens, max_q, width, NP, lp, chunk, nchunk;
+  int B, HKV, G, tokens, max_q, width, NP, lp, chunk, nchunk, ntile;
   float c;                               // scale * log2 e
 };
 
@@ -64,10 +65,7 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   const f32x2 x = {a, b};
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2));
 }
-__device__ __forceinline__ float scale_of(unsigned s) {
-  return s == 255 ? __builtin_nanf("") : __uint_as_float(s << 23);
-}
-// 8 codes to bf16, scaled
+// 8 codes to bf16, scaled by a power of two (all exponent bits set, a scale byte of 255: NaN)
 __device__ __forceinline__ bf16x8 from4(unsigned w, float f) {
   const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 0);
   const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 1);
@@ -98,7 +96,7 @@ template <int D>
 struct Tile {
   unsigned k[2][D / 32], v[2][D / 32];
   unsigned ks[2], vs[2];
-  bool bad;
+  unsigned bad;                          // the exponent of NaN where the page is outside of the cache
 };
 
 template <int N>
@@ -114,7 +112,7 @@ __device__ __forceinline__ void load_words(unsigned (&w)[N], const uint8_t* p) {
 
 // NQ tiles of 16 query rows; DUP: at most 8 rows, columns 8.. repeat them for the weights' second terms
 template <int D, int NQ, bool DUP>
-__global__ void __launch_bounds__(kThreads) kv4_attn_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, NQ > 1 ? 2 : 3) kv4_attn_kernel(AttnArgs a) {
   constexpr int kSteps = D / 32;         // products of a 16 x 16 score tile; words of a lane's codes
   constexpr int kDims = D / 16;          // tiles of 16 dims
   constexpr int kRowB = D * 2;           // bytes of a value row in LDS
@@ -127,8 +125,10 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(AttnArgs a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
   const int units = a.B * a.HKV;
-  const int ch = blockIdx.x % a.nchunk, rest = blockIdx.x / a.nchunk;
-  const int bh = rest % units, row0 = rest / units * (NQ * kCols);
+  // (sequence, head) fastest: workgroups go to the XCDs in turn, so that a long sequence's pieces and a
+  // batch's short sequences spread over all of them, and the query tiles of a piece meet in one L2
+  const int bh = blockIdx.x % units, rest = blockIdx.x / units;
+  const int ch = rest / a.ntile, row0 = (rest - ch * a.ntile) * (NQ * kCols);
   const int b = bh / a.HKV, h = bh - b * a.HKV;
   const Seq sq = seq_of(a, b);
   const int rows = min(sq.R, a.max_q) * a.G;
@@ -139,7 +139,10 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(AttnArgs a) {
   const int k0 = ch * a.chunk, k1 = min(k0 + a.chunk, hi);
   if (k0 >= k1 && a.nchunk > 1) return;
 
-  // this lane's columns: rows of q and how many keys they see (0: none such)
+  // this lane's columns: rows of q (negated under a negative scale: the maximum is taken before scaling)
+  // and how many keys they see (0: no such row)
+  const float c = fabsf(a.c);
+  const unsigned flip = a.c < 0.f ? 0x80008000u : 0u;
   bf16x8 Q[NQ][kSteps];
   int lim[NQ];
 #pragma unroll
@@ -149,28 +152,37 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(AttnArgs a) {
     lim[x] = r < rows ? first + j + 1 : 0;
     const uint16_t* p = a.q + (long)(sq.r0 + j) * a.q_st + (long)hd * a.q_sh + g * (D / 4);
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) Q[x][s] = *reinterpret_cast<const bf16x8*>(p + 8 * s);
+    for (int s = 0; s < kSteps; ++s) {
+      const uint4v w = *reinterpret_cast<const uint4v*>(p + 8 * s);
+      Q[x][s] = __builtin_bit_cast(bf16x8, w ^ uint4v(flip));
+    }
   }
 
+  // a tile's addresses: a scalar base and fixed lane offsets
   const int* trow = a.table + (long)b * a.t_st;
   const int pmask = (1 << a.lp) - 1;
   const long headc = ((long)h << a.lp) * (D / 2), heads = ((long)h << a.lp) * (D / 32);
-  const int last = (k1 - 1) >> a.lp;     // the chunk's last page
+  const unsigned oc = col * (D / 2) + g * (D / 8), os = col * (D / 32) + g * D / 128;
+  const int last = (k1 - 1) >> a.lp;     // the piece's last page
   auto page_at = [&](int t0) { return trow[min(t0 >> a.lp, last)]; };
   auto load = [&](Tile<D>& t, int t0, int page) {
-    t.bad = (unsigned)page >= (unsigned)a.NP;
-    const long pg = t.bad ? 0 : page;
-    const int off = (t0 & pmask) + col;
-    const uint8_t* kc = a.kc + pg * a.c_sp + headc;
-    const uint8_t* vc = a.vc + pg * a.c_sp + headc;
-    const uint8_t* ks = a.ks + pg * a.s_sp + heads;
-    const uint8_t* vs = a.vs + pg * a.s_sp + heads;
+    const bool bad = (unsigned)page >= (unsigned)a.NP;
+    t.bad = bad ? 0x7f800000u : 0u;
+    const long pg = bad ? 0 : page, off = t0 & pmask;
+    const long bc = pg * a.c_sp + headc + off * (D / 2), bs = pg * a.s_sp + heads + off * (D / 32);
+    const uint8_t* kc = a.kc + bc;
+    const uint8_t* vc = a.vc + bc;
+    const uint8_t* ks = a.ks + bs;
+    const uint8_t* vs = a.vs + bs;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      load_words<kSteps>(t.k[c], kc + (off + 16 * c) * (D / 2) + g * (D / 8));
-      load_words<kSteps>(t.v[c], vc + (off + 16 * c) * (D / 2) + g * (D / 8));
-      t.ks[c] = ks[(off + 16 * c) * (D / 32) + g * D / 128];
-      t.vs[c] = vs[(off + 16 * c) * (D / 32) + g * D / 128];
+      load_words<kSteps>(t.k[c], kc + oc + 16 * c * (D / 2));
+      t.ks[c] = ks[os + 16 * c * (D / 32)];
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      load_words<kSteps>(t.v[c], vc + oc + 16 * c * (D / 2));
+      t.vs[c] = vs[os + 16 * c * (D / 32)];
     }
   };
 
@@ -188,35 +200,35 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(AttnArgs a) {
   };
 
   f32x4 O[NQ][kDims];
-  float m[NQ], l[NQ];
+  float m[NQ], l[NQ];                    // running maximum, scaled, and sum of the lane's keys
+  bool big[NQ];                          // a maximum is past 2^24 (uniform)
 #pragma unroll
   for (int x = 0; x < NQ; ++x) {
     m[x] = -FLT_MAX;
     l[x] = 0.f;
+    big[x] = false;
 #pragma unroll
     for (int d = 0; d < kDims; ++d) O[x][d] = f32x4(0.f);
   }
 
   constexpr int kStride = kWaves * kTile;
-  int t0 = k0 + wave * kTile;
-  Tile<D> nx;
+  const int tb = k0 + wave * kTile;
+  const int nt = max(0, (k1 - tb + kStride - 1) / kStride);                  // this wave's tiles
+  const int nfull = min(nt, max(0, (all - tb - kTile + kStride) / kStride));  // those that every row sees whole
   int page = 0;
-  if (t0 < k1) {
-    load(nx, t0, page_at(t0));
-    page = page_at(t0 + kStride);
-  }
-  for (; t0 < k1; t0 += kStride) {
-    const Tile<D> t = nx;
-    if (t0 + kStride < k1) {
-      load(nx, t0 + kStride, page);
+
+  // tile i from t; tile i + 1 is fetched into n
+  auto body = [&](auto mask_c, int i, const Tile<D>& t, Tile<D>& n) {
+    constexpr bool MASK = decltype(mask_c)::value;
+    const int t0 = tb + i * kStride;
+    if (i + 1 < nt) {
+      load(n, t0 + kStride, page);
       page = page_at(t0 + 2 * kStride);
     }
-    const bool mask = t0 + kTile > all;  // some row does not see some key
-
     f32x4 S[NQ][2];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const float f = t.bad ? __builtin_nanf("") : scale_of(t.ks[c]);
+      const float f = __uint_as_float(t.ks[c] << 23 | t.bad);
 #pragma unroll
       for (int x = 0; x < NQ; ++x) S[x][c] = f32x4(0.f);
 #pragma unroll
@@ -226,19 +238,19 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(AttnArgs a) {
         for (int x = 0; x < NQ; ++x) S[x][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop, Q[x][s], S[x][c], 0, 0, 0);
       }
     }
-    // values into the LDS tile; keys past the last one any row sees count as zeros (their weights are 0,
-    // but what lies there may be anything), and so do NaN blocks of keys that only some rows see
+    // values into the LDS tile.  In a masked tile keys past the last one any row sees count as zeros (their
+    // weights are 0, but what lies there may be anything), and so do NaN blocks of keys that some rows see
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const int key = t0 + 16 * c + col;
-      float f = scale_of(t.vs[c]);
-      if (mask && (key >= hi || t.vs[c] == 255)) f = 0.f;
+      unsigned e = t.vs[c];
+      if (MASK && (t0 + 16 * c + col >= hi || e == 255)) e = 0;
+      const float f = __uint_as_float(e << 23);
 #pragma unroll
       for (int s = 0; s < kSteps; ++s)
         *reinterpret_cast<bf16x8*>(sv + wbase + 16 * c * kRowB + (((g * (D / 32) + s) ^ wf) << 4)) = from4(t.v[c][s], f);
     }
-
     lane_order();
+
     uint4v P[NQ], Plo[NQ];
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
@@ -246,20 +258,29 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(AttnArgs a) {
       float mx = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        v[i] = S[x][i >> 2][i & 3] * a.c;
-        if (mask && t0 + 16 * (i >> 2) + 4 * g + (i & 3) >= lim[x]) v[i] = -INFINITY;
+        v[i] = S[x][i >> 2][i & 3];
+        if (MASK) v[i] = t0 + 16 * (i >> 2) + 4 * g + (i & 3) < lim[x] ? v[i] * c : -INFINITY;
         mx = fmaxf(mx, v[i]);
       }
+      if (!MASK) mx *= c;
       if (__any(mx > m[x])) {
         const float mn = fmaxf(m[x], max_groups(mx)), alpha = __builtin_amdgcn_exp2f(m[x] - mn);
         m[x] = mn;
         l[x] *= alpha;
 #pragma unroll
         for (int d = 0; d < kDims; ++d) O[x][d] *= alpha;
+        // the maximum rounds S c, so that the fma below leaves up to half its last place: past 2^24 more than
+        // the exponential should see, and an infinity in time.  There S c is rounded first, as the maximum is
+        big[x] = __any(fabsf(mn) >= 16777216.f);
       }
+      if (!MASK && big[x]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= c;
+      }
+      const float cc = MASK || big[x] ? 1.f : c;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        v[i] = __builtin_amdgcn_exp2f(v[i] - m[x]);
+        v[i] = __builtin_amdgcn_exp2f(MASK ? v[i] - m[x] : fmaf(v[i], cc, -m[x]));
         l[x] += v[i];
       }
 #pragma unroll
@@ -280,7 +301,7 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(AttnArgs a) {
       }
     }
     lane_order();
-    if (mask) {                          // NaN blocks, into the rows that see them (rare)
+    if (MASK) {                          // NaN blocks, into the rows that see them (rare)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         unsigned long nan = __ballot(t.vs[c] == 255 && t0 + 16 * c + col < hi);
@@ -294,6 +315,31 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(AttnArgs a) {
               if (d / 2 == blk && key < lim[x]) O[x][d] = f32x4(__builtin_nanf(""));
         }
       }
+    }
+  };
+  {
+    typedef std::integral_constant<bool, false> whole;
+    typedef std::integral_constant<bool, true> masked;
+    Tile<D> ta, tc;
+    if (nt > 0) {
+      load(ta, tb, page_at(tb));
+      page = page_at(tb + kStride);
+    }
+    int i = 0;
+#pragma unroll 1
+    for (; i + 2 <= nfull; i += 2) {
+      body(whole(), i, ta, tc);
+      body(whole(), i + 1, tc, ta);
+    }
+    if (i < nfull) {
+      body(whole(), i, ta, tc);
+      ta = tc;
+      ++i;
+    }
+#pragma unroll 1
+    for (; i < nt; ++i) {
+      body(masked(), i, ta, tc);
+      ta = tc;
     }
   }
 
@@ -390,10 +436,11 @@ __global__ void __launch_bounds__(kThreads) kv4_join_kernel(AttnArgs a) {
 }
 
 template <int D>
-int launch(const AttnArgs& a, hipStream_t st) {
+int launch(AttnArgs a, hipStream_t st) {
   const long rows = (long)a.max_q * a.G;
   const int cols = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
-  const long blocks = (rows + cols - 1) / cols * a.B * a.HKV * a.nchunk, joins = (long)a.B * a.max_q * a.HKV * a.G;
+  a.ntile = (int)((rows + cols - 1) / cols);
+  const long blocks = (long)a.ntile * a.nchunk * a.B * a.HKV, joins = (long)a.B * a.max_q * a.HKV * a.G;
   if (blocks > 0x7fffffffL || joins > 0x7fffffffL) return OA_EINVAL;
   const dim3 grid((unsigned)blocks), blk(kThreads);
   if (cols == 8) hipLaunchKernelGGL((kv4_attn_kernel<D, 1, true>), grid, blk, 0, st, a);

@@ -663,51 +663,64 @@ def prefill_attn(q, k, v, sm_scale: float) -> torch.Tensor:
 
 
 # ================================================================== 4-bit paged cache
+# (eager decode steps call these once per layer: a call's checks are most of its time on the host, so
+# they run on sizes and strides fetched once, and format nothing unless they fail)
 _DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 KV4_BLOCK = 32             # values that share a scale
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _run(dev: torch.device, name: str, *args) -> None:
-    """lib.call on dev's current stream, with dev the current device for the launch."""
-    if dev.index == torch.cuda.current_device():
-        lib.call(name, *args, _stream(dev))
+def _where(*ts) -> int:
+    """The index of the device that all these tensors are on."""
+    i = ts[0].get_device()
+    for t in ts:
+        if t is not None and (t.get_device() != i or i < 0):
+            _dev(*ts)
+            raise RuntimeError(f"tensors on different devices: {[u.device for u in ts if u is not None]}")
+    return i
+
+
+def _run(i: int, name: str, *args) -> None:
+    """lib.call on device i's current stream, with i the current device for the launch."""
+    if i == torch.cuda.current_device():
+        lib.call(name, *args, _raw_stream(i))
     else:
-        with torch.cuda.device(dev):
-            lib.call(name, *args, _stream(dev))
+        with torch.cuda.device(i):
+            lib.call(name, *args, _raw_stream(i))
 
 
-def _plain(*named) -> None:
+def _plain(*ts) -> None:
     """Tensors whose data a kernel may take as it stands, with no gradient to be formed: these
     operators have no backward pass, and would cut a graph in silence."""
     grad = torch.is_grad_enabled()
-    for t, name in named:
-        if t is None:
-            continue
-        _need(not (grad and t.requires_grad), f"{name} requires a gradient, and this operator has no backward pass "
-              "(call it under torch.no_grad())")
-        _need(not t.is_neg(), f"{name}: a lazily negated view (call resolve_neg())")
+    for t in ts:
+        if t is not None and (grad and t.requires_grad or t.is_neg()):
+            raise ValueError("a lazily negated view (call resolve_neg())" if t.is_neg() else
+                             "a tensor requires a gradient, and this operator has no backward pass (call it under "
+                             "torch.no_grad())")
 
 
-def _rows(t: torch.Tensor, name: str, out: bool = False) -> None:
-    """(tokens, heads, D) rows that are loaded 16 bytes at a time; of an output, rows that do not overlap."""
-    n = 4 if t.dtype == torch.float32 else 8
+def _rows(t: torch.Tensor, T: int, H: int, Dh: int, name: str, out: bool = False) -> tuple:
+    """(pointer, token stride, head stride) of rows (T, H, Dh) that are loaded 16 bytes at a time; of an
+    output, rows that do not overlap.  The stride of a single token or head, which is free, counts as 0."""
     s0, s1, s2 = t.stride()
-    if t.numel() == 0:
-        return
-    _need(s2 == 1, f"{name}: last dimension must be contiguous")
-    _need((s0 % n == 0 or t.shape[0] == 1) and (s1 % n == 0 or t.shape[1] == 1) and t.data_ptr() % 16 == 0,
-          f"{name}: rows must start at multiples of 16 bytes")
-    if out:
-        T, H, Dh = t.shape
-        _need((H == 1 or s1 >= Dh) and (T == 1 or s0 >= (Dh if H == 1 else s1 * (H - 1) + Dh))
-              or (T == 1 or s0 >= Dh) and (H == 1 or s1 >= (Dh if T == 1 else s0 * (T - 1) + Dh)),
-              f"{name}: rows overlap")
+    if T <= 1:
+        s0 = 0
+    if H <= 1:
+        s1 = 0
+    p = t.data_ptr()
+    if p % 16 or (s0 | s1) % (4 if t.dtype is torch.float32 else 8) or s2 != 1:
+        _need(T * H == 0, f"{name}: contiguous rows that start at multiples of 16 bytes (strides {t.stride()})")
+    if out and not (H <= 1 or s1 >= Dh) & (T <= 1 or s0 >= s1 * (H - 1) + Dh):
+        _need(T * H == 0 or (T <= 1 or s0 >= Dh) and (H <= 1 or s1 >= s0 * (T - 1) + Dh), f"{name}: rows overlap")
+    return p, s0, s1
 
 
-def _strides(t: torch.Tensor) -> tuple:
-    """token and head strides; of a single token or head, whose stride is free, that of a contiguous row"""
-    s0, s1 = t.stride(0), t.stride(1)
-    return (s0 if t.shape[0] > 1 else 0), (s1 if t.shape[1] > 1 else 0)
+def _ints(t: torch.Tensor, n: int, name: str) -> int:
+    """pointer of n contiguous int32"""
+    if t.dtype is not torch.int32 or t.shape != (n,) or n > 1 and t.stride(0) != 1:
+        raise ValueError(f"{name}: ({n},) int32, contiguous (got {tuple(t.shape)} {t.dtype})")
+    return t.data_ptr()
 
 
 def qk_norm_rope(q, k, pos, cos, sin, wq=None, wk=None, eps: float = 1e-6, q_out=None, k_out=None):
@@ -717,57 +730,72 @@ def qk_norm_rope(q, k, pos, cos, sin, wq=None, wk=None, eps: float = 1e-6, q_out
     16 bytes (views of one product, say); pos (T,) int32 or int64; cos, sin (P, D / 2) fp32; wq, wk (D,)
     of q's type, None for a rotation alone.  A token of negative position (padding) gives zeros, one of P
     or more NaN.  Returns (q_out, k_out), contiguous unless given; either may be its input."""
-    dev = _dev(q, k, pos, cos, sin, wq, wk, q_out, k_out)
-    _need(q.dim() == 3 and k.dim() == 3 and q.shape[0] == k.shape[0] and q.shape[2] == k.shape[2],
-          "q, k: (T, HQ, D) and (T, HKV, D)")
+    i = _where(q, k, pos, cos, sin, wq, wk, q_out, k_out)
+    dt = q.dtype
+    if q.dim() != 3 or k.dim() != 3 or k.shape[::2] != q.shape[::2] or dt not in _DT or k.dtype is not dt:
+        raise ValueError("q, k: (T, HQ, D) and (T, HKV, D), both bf16, fp16 or fp32")
     T, HQ, Dh = q.shape
     HKV = k.shape[1]
-    _need(q.dtype in _DT and k.dtype == q.dtype, "q, k: bf16, fp16 or fp32, both of one type")
-    _need(Dh in (64, 128, 256), "head dimension: 64, 128 or 256")
-    _need(T * (HQ + HKV) <= 1 << 27, "T * (HQ + HKV): at most 2^27 rows")
-    _need(pos.dtype in (torch.int32, torch.int64) and pos.shape == (T,) and pos.is_contiguous(),
-          "pos: (T,) int32 or int64, contiguous")
-    for t, name in ((cos, "cos"), (sin, "sin")):
-        _chk(t, name, torch.float32, (cos.shape[0], Dh // 2))
-        _need(t.shape[0] >= 1 and (t.stride(0) % 4 == 0 or t.shape[0] == 1) and t.stride(0) == cos.stride(0)
-              and t.data_ptr() % 16 == 0, "cos, sin: rows of one stride, starting at multiples of 16 bytes")
-    for t, name in ((wq, "wq"), (wk, "wk")):
-        if t is not None:
-            _chk(t, name, q.dtype, (Dh,), contiguous=True)
-            _need(t.data_ptr() % 16 == 0, f"{name}: base pointer misaligned")
-    _need(eps >= 0, "eps: not negative")
-    _plain((q, "q"), (k, "k"), (wq, "wq"), (wk, "wk"), (cos, "cos"), (sin, "sin"), (q_out, "q_out"), (k_out, "k_out"))
+    if Dh not in (64, 128, 256) or T * (HQ + HKV) > 1 << 27:
+        raise ValueError(f"head dimension 64, 128 or 256 (got {Dh}), at most 2^27 rows")
+    pt = pos.dtype
+    if pt not in (torch.int32, torch.int64) or pos.shape != (T,) or T > 1 and pos.stride(0) != 1:
+        raise ValueError(f"pos: ({T},) int32 or int64, contiguous")
+    P = cos.shape[0]
+    cst, sst, cp, sp = cos.stride(), sin.stride(), cos.data_ptr(), sin.data_ptr()
+    if (cos.shape != (P, Dh // 2) or sin.shape != cos.shape or cos.dtype is not torch.float32
+            or sin.dtype is not torch.float32 or P < 1 or cst != sst or cst[1] != 1 or P > 1 and cst[0] % 4
+            or (cp | sp) % 16):
+        raise ValueError(f"cos, sin: (positions, {Dh // 2}) fp32 rows of one stride, starting at multiples of 16 bytes")
+    wqp = wkp = None
+    if wq is not None:
+        wqp = wq.data_ptr()
+        if wq.shape != (Dh,) or wq.dtype is not dt or wq.stride(0) != 1 or wqp % 16:
+            raise ValueError(f"wq: ({Dh},) of q's type, contiguous, 16-byte aligned")
+    if wk is not None:
+        wkp = wk.data_ptr()
+        if wk.shape != (Dh,) or wk.dtype is not dt or wk.stride(0) != 1 or wkp % 16:
+            raise ValueError(f"wk: ({Dh},) of q's type, contiguous, 16-byte aligned")
+    if not eps >= 0:
+        raise ValueError("eps: not negative")
+    _plain(q, k, cos, sin, wq, wk, q_out, k_out)
     if q_out is None:
-        q_out = torch.empty(q.shape, device=dev, dtype=q.dtype)
+        q_out = q.new_empty((T, HQ, Dh))
     if k_out is None:
-        k_out = torch.empty(k.shape, device=dev, dtype=k.dtype)
-    _need(q_out.shape == q.shape and k_out.shape == k.shape and q_out.dtype == q.dtype and k_out.dtype == q.dtype,
-          "q_out, k_out: as q, k")
-    for t, name, o in ((q, "q", False), (k, "k", False), (q_out, "q_out", True), (k_out, "k_out", True)):
-        _rows(t, name, o)
-    _run(dev, "oa_qk_norm_rope", _ptr(q), *_strides(q), _ptr(k), *_strides(k), T, HQ, HKV, Dh, _DT[q.dtype], _ptr(pos),
-         int(pos.dtype == torch.int64), _ptr(cos), _ptr(sin), cos.stride(0) if cos.shape[0] > 1 else 0, cos.shape[0],
-         _ptr(wq), _ptr(wk), float(eps), _ptr(q_out), *_strides(q_out), _ptr(k_out), *_strides(k_out))
+        k_out = k.new_empty((T, HKV, Dh))
+    if q_out.shape != q.shape or k_out.shape != k.shape or q_out.dtype is not dt or k_out.dtype is not dt:
+        raise ValueError("q_out, k_out: as q, k")
+    _run(i, "oa_qk_norm_rope", *_rows(q, T, HQ, Dh, "q"), *_rows(k, T, HKV, Dh, "k"), T, HQ, HKV, Dh, _DT[dt],
+         pos.data_ptr(), pt is torch.int64, cp, sp, cst[0] if P > 1 else 0, P, wqp, wkp, eps,
+         *_rows(q_out, T, HQ, Dh, "q_out", True), *_rows(k_out, T, HKV, Dh, "k_out", True))
     return q_out, k_out
 
 
 def _page(page: int) -> None:
-    _need(32 <= page <= 1024 and page & (page - 1) == 0, f"page: a power of two, 32 to 1024 (got {page})")
+    if not 32 <= page <= 1024 or page & (page - 1):
+        raise ValueError(f"page: a power of two, 32 to 1024 (got {page})")
 
 
-def _pages_state(count, lens, table, free, nfree, status, page: int, what: str) -> torch.device:
-    dev = _dev(count, lens, table, free, nfree, status)
-    _page(page)
-    _need(table.dim() == 2 and table.dtype == torch.int32 and table.shape[0] >= 1 and table.shape[1] >= 1
-          and (table.stride(1) == 1 or table.shape[1] == 1)
-          and (table.stride(0) >= table.shape[1] or table.shape[0] == 1), "table: (requests, width) int32 rows")
+def _table(table: torch.Tensor, page: int) -> tuple:
+    """(pointer, row stride, rows, width) of a table of page ids"""
+    if table.dim() != 2 or table.dtype is not torch.int32:
+        raise ValueError("table: (requests, width) int32")
     B, width = table.shape
-    for t, name, shape in ((count, what, (B,)), (lens, "lens", (B,)), (free, "free", (None,)), (nfree, "nfree", (1,)),
-                           (status, "status", (1,))):
-        _chk(t, name, torch.int32, shape, contiguous=True)
-    _need(free.numel() >= 1 and free.numel() * page < 1 << 31 and width * page < 1 << 31 and B <= 1 << 24,
-          "pool and table: fewer than 2^31 tokens, at most 2^24 requests")
-    return dev
+    s0, s1 = table.stride()
+    if width < 1 or width * page >= 1 << 31 or width > 1 and s1 != 1 or B > 1 and s0 < width or B > 1 << 24:
+        raise ValueError("table: contiguous rows of fewer than 2^31 tokens, at most 2^24 requests")
+    return table.data_ptr(), max(s0, width), B, width
+
+
+def _pages_state(count, lens, table, free, nfree, status, page: int, what: str) -> tuple:
+    """The arguments that both calls of the page tables begin with."""
+    _page(page)
+    tp, ts, B, width = _table(table, page)
+    NP = free.shape[0] if free.dim() == 1 else 0
+    if B < 1 or NP < 1 or NP * page >= 1 << 31:
+        raise ValueError("at least one request; free: (pages,) int32, a pool of fewer than 2^31 tokens")
+    return (_ints(count, B, what), _ints(lens, B, "lens"), tp, ts, _ints(free, NP, "free"), _ints(nfree, 1, "nfree"),
+            _ints(status, 1, "status"), B, width, NP, page)
 
 
 def kv_pages_extend(add, lens, table, free, nfree, status, page: int, total: int):
@@ -778,14 +806,14 @@ def kv_pages_extend(add, lens, table, free, nfree, status, page: int, total: int
     into new pages.  For all requests or for none: where a count is negative, a request outgrows its row
     (status |= 1), free pages do not reach (2) or there are more than `total` new tokens (4), nothing
     changes, slots and pos are -1 and cu is 0; status (1,) is the caller's to look at and to clear."""
-    dev = _pages_state(add, lens, table, free, nfree, status, page, "add")
-    B, width = table.shape
-    _need(0 <= total <= 1 << 30, "total: 0 to 2^30")
-    buf = torch.empty(2 * total + 4 * B + 2, device=dev, dtype=torch.int32)
-    slots, pos, cu, ws = buf[:total], buf[total:2 * total], buf[2 * total:2 * total + B + 1], buf[2 * total + B + 1:]
-    _run(dev, "oa_kv_pages_extend", _ptr(add), _ptr(lens), _ptr(table), max(table.stride(0), width), _ptr(free),
-         _ptr(nfree), _ptr(status), B, width, free.numel(), page, total, _ptr(slots) or None, _ptr(pos) or None, _ptr(cu),
-         _ptr(ws))
+    i = _where(add, lens, table, free, nfree, status)
+    st = _pages_state(add, lens, table, free, nfree, status, page, "add")
+    if not 0 <= total <= 1 << 30:
+        raise ValueError("total: 0 to 2^30")
+    B = st[7]
+    slots, pos, cu, ws = add.new_empty(2 * total + 4 * B + 2).split((total, total, B + 1, 3 * B + 1))
+    p = cu.data_ptr()
+    _run(i, "oa_kv_pages_extend", *st, total, p - 8 * total, p - 4 * total, p, p + 4 * B + 4)
     return slots, pos, cu
 
 
@@ -793,38 +821,33 @@ def kv_pages_truncate(keep, lens, table, free, nfree, status, page: int) -> None
     """Request i keeps its first min(keep[i], lens[i]) tokens (keep[i] < 0: all; 0: the request ends); pages
     it no longer needs go back to the stack and leave the table (-1).  A truncation to the lengths before
     an extension undoes it.  Nothing changes where the stack would outgrow `free` (status |= 2)."""
-    dev = _pages_state(keep, lens, table, free, nfree, status, page, "keep")
-    B, width = table.shape
-    ws = torch.empty(3 * B + 1, device=dev, dtype=torch.int32)
-    _run(dev, "oa_kv_pages_truncate", _ptr(keep), _ptr(lens), _ptr(table), max(table.stride(0), width), _ptr(free),
-         _ptr(nfree), _ptr(status), B, width, free.numel(), page, _ptr(ws))
+    i = _where(keep, lens, table, free, nfree, status)
+    st = _pages_state(keep, lens, table, free, nfree, status, page, "keep")
+    ws = keep.new_empty(3 * st[7] + 1)
+    _run(i, "oa_kv_pages_truncate", *st, ws.data_ptr())
 
 
 def _kv4_cache(kc, ks, vc, vs) -> tuple:
-    """(pages, heads, page, D) of a 4-bit cache's tensors; pages may lie apart (a layer of a larger tensor)."""
-    _need(kc.dim() == 4 and kc.dtype == torch.uint8 and kc.shape[0] >= 1 and kc.shape[1] >= 1,
-          "kc: (pages, heads, page, D / 2) uint8")
+    """(pointers, page strides, pages, page) of a 4-bit cache's tensors, its heads and head dimension; pages may
+    lie apart (a layer of a larger tensor)."""
+    if kc.dim() != 4:
+        raise ValueError("kc: (pages, heads, page, D / 2) uint8")
     NP, HKV, page, half = kc.shape
-    Dh = 2 * half
+    blocks = half // (KV4_BLOCK // 2)
     _page(page)
-    _need(Dh in (64, 128), "head dimension: 64 or 128")
-    _need(NP * page < 1 << 31, "cache: fewer than 2^31 slots")
-    for t, name, w in ((kc, "kc", half), (vc, "vc", half), (ks, "ks", Dh // KV4_BLOCK), (vs, "vs", Dh // KV4_BLOCK)):
-        _need(t.dtype == torch.uint8 and t.shape == (NP, HKV, page, w), f"{name}: ({NP}, {HKV}, {page}, {w}) uint8")
-        _need(t.stride()[1:] == (page * w, w, 1) and (NP == 1 or t.stride(0) % 16 == 0 and t.stride(0) >= HKV * page * w)
-              and t.data_ptr() % 16 == 0, f"{name}: contiguous pages that start at multiples of 16 bytes")
-    _need(NP == 1 or kc.stride(0) == vc.stride(0) and ks.stride(0) == vs.stride(0),
-          "kc, vc and ks, vs: pages at the same distance")
-    return NP, HKV, page, Dh
-
-
-def _page_strides(kc, ks) -> tuple:
-    NP, HKV, page, half = kc.shape
-    return (kc.stride(0), ks.stride(0)) if NP > 1 else (HKV * page * half, HKV * page * ks.shape[3])
-
-
-def _slots(slots, T: int) -> None:
-    _chk(slots, "slots", torch.int32, (T,), contiguous=True)
+    if half not in (32, 64) or NP < 1 or HKV < 1 or NP * page >= 1 << 31:
+        raise ValueError(f"cache: head dimension 64 or 128 (got {2 * half}), at least one page and head, fewer than 2^31 slots")
+    u8 = torch.uint8
+    if (vc.shape != kc.shape or ks.shape != (NP, HKV, page, blocks) or vs.shape != ks.shape
+            or kc.dtype is not u8 or ks.dtype is not u8 or vc.dtype is not u8 or vs.dtype is not u8):
+        raise ValueError(f"cache: codes ({NP}, {HKV}, {page}, {half}), scales ({NP}, {HKV}, {page}, {blocks}), uint8")
+    c, s = kc.stride(), ks.stride()
+    ps = kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr()
+    c0, s0 = (c[0], s[0]) if NP > 1 else (HKV * page * half, HKV * page * blocks)
+    if (vc.stride() != c or vs.stride() != s or c[1:] != (page * half, half, 1) or s[1:] != (page * blocks, blocks, 1)
+            or c0 < HKV * page * half or s0 < HKV * page * blocks or (c0 | s0 | ps[0] | ps[1] | ps[2] | ps[3]) % 16):
+        raise ValueError("cache: contiguous pages that start at multiples of 16 bytes, those of k and v at one distance")
+    return ps, (c0, s0, NP, page), HKV, 2 * half
 
 
 def kv4_write(k, v, slots, kc, ks, vc, vs) -> None:
@@ -832,34 +855,28 @@ def kv4_write(k, v, slots, kc, ks, vc, vs) -> None:
     scale) and put at slots (T,) int32 = page id * page + offset of the cache kc, vc (pages, HKV, page,
     D / 2), ks, vs (pages, HKV, page, D / 32) uint8.  Rows of a slot outside of the cache (-1) are passed
     over.  The slots of one call are distinct (a slot given twice ends with blocks of either row)."""
-    dev = _dev(k, v, slots, kc, ks, vc, vs)
-    NP, HKV, page, Dh = _kv4_cache(kc, ks, vc, vs)
-    T = k.shape[0]
-    _need(k.dim() == 3 and k.shape == (T, HKV, Dh) and v.shape == k.shape, f"k, v: (T, {HKV}, {Dh})")
-    _need(k.dtype in _DT and v.dtype == k.dtype, "k, v: bf16, fp16 or fp32, both of one type")
-    _need(T * HKV <= 1 << 26, "T * HKV: at most 2^26 rows")
-    _slots(slots, T)
-    _plain((k, "k"), (v, "v"))
-    _rows(k, "k")
-    _rows(v, "v")
-    _run(dev, "oa_kv4_write", _ptr(k), *_strides(k), _ptr(v), *_strides(v), T, HKV, Dh, _DT[k.dtype], _ptr(slots),
-         _ptr(kc), _ptr(ks), _ptr(vc), _ptr(vs), *_page_strides(kc, ks), NP, page)
+    i = _where(k, v, slots, kc, ks, vc, vs)
+    ps, where, HKV, Dh = _kv4_cache(kc, ks, vc, vs)
+    T, dt = k.shape[0], k.dtype
+    if k.shape != (T, HKV, Dh) or v.shape != k.shape or dt not in _DT or v.dtype is not dt or T * HKV > 1 << 26:
+        raise ValueError(f"k, v: (T, {HKV}, {Dh}), both bf16, fp16 or fp32, at most 2^26 rows")
+    _plain(k, v)
+    _run(i, "oa_kv4_write", *_rows(k, T, HKV, Dh, "k"), *_rows(v, T, HKV, Dh, "v"), T, HKV, Dh, _DT[dt],
+         _ints(slots, T, "slots"), *ps, *where)
 
 
 def kv4_read(slots, kc, ks, vc, vs, dtype: torch.dtype = torch.bfloat16):
     """The values (k, v), each (T, HKV, D) bf16 (which holds them exactly) or fp32, at slots (T,) int32 of a
     4-bit cache; zeros for a slot outside of it."""
-    dev = _dev(slots, kc, ks, vc, vs)
-    NP, HKV, page, Dh = _kv4_cache(kc, ks, vc, vs)
-    _need(slots.dim() == 1, "slots: (T,) int32")
-    T = slots.shape[0]
-    _slots(slots, T)
-    _need(dtype in (torch.bfloat16, torch.float32), "dtype: bf16 or fp32")
-    _need(T * HKV <= 1 << 26, "T * HKV: at most 2^26 rows")
-    k = torch.empty(T, HKV, Dh, device=dev, dtype=dtype)
-    v = torch.empty_like(k)
-    _run(dev, "oa_kv4_read", _ptr(slots), _ptr(kc), _ptr(ks), _ptr(vc), _ptr(vs), *_page_strides(kc, ks), NP, page,
-         _ptr(k), *_strides(k), _ptr(v), *_strides(v), T, HKV, Dh, _DT[dtype])
+    i = _where(slots, kc, ks, vc, vs)
+    ps, where, HKV, Dh = _kv4_cache(kc, ks, vc, vs)
+    T = slots.shape[0] if slots.dim() == 1 else 0
+    sp = _ints(slots, T, "slots")
+    if dtype not in (torch.bfloat16, torch.float32) or T * HKV > 1 << 26:
+        raise ValueError("dtype: bf16 or fp32; at most 2^26 rows")
+    k = kc.new_empty((T, HKV, Dh), dtype=dtype)
+    v = kc.new_empty((T, HKV, Dh), dtype=dtype)
+    _run(i, "oa_kv4_read", sp, *ps, *where, k.data_ptr(), HKV * Dh, Dh, v.data_ptr(), HKV * Dh, Dh, T, HKV, Dh, _DT[dtype])
     return k, v
 
 
@@ -879,47 +896,44 @@ def kv4_attn(q, kc, ks, vc, vs, table, lens, sm_scale: float | None = None, cu_q
     Token j of R sees keys 0 .. lens[b] - R + j; one that sees none gives 0.  max_len: a bound on lens
     that the caller knows (the table's width otherwise).  NaN: rows that need a page id outside of the
     cache, and those of sequences longer than their table row or than max_len (rounded up to whole pieces,
-    kv4_chunk).  Rows of `out` behind
-    cu_q[B] are left as they were (0 where the call makes it)."""
-    dev = _dev(q, kc, ks, vc, vs, table, lens, cu_q, out)
-    NP, HKV, page, Dh = _kv4_cache(kc, ks, vc, vs)
-    _need(q.dim() == 3 and q.dtype == torch.bfloat16 and q.shape[2] == Dh and q.shape[1] >= 1 and q.shape[1] % HKV == 0,
-          f"q: (T, a multiple of {HKV}, {Dh}) bf16")
-    T, HQ, _ = q.shape
-    _need(table.dim() == 2 and table.dtype == torch.int32 and table.shape[1] >= 1
-          and (table.stride(1) == 1 or table.shape[1] == 1)
-          and (table.stride(0) >= table.shape[1] or table.shape[0] <= 1), "table: (B, width) int32 rows")
-    B, width = table.shape
-    _need(width * page < 1 << 31, "table: fewer than 2^31 keys to a row")
-    _chk(lens, "lens", torch.int32, (B,), contiguous=True)
-    if cu_q is None:
-        _need(T == B and max_q == 1, "without cu_q every sequence has one row of q")
-    else:
-        _chk(cu_q, "cu_q", torch.int32, (B + 1,), contiguous=True)
-    _need(max_q >= 1 and max_q * (HQ // HKV) <= 1 << 30, "max_q: at least 1")
-    scale = Dh ** -0.5 if sm_scale is None else float(sm_scale)
-    _need(scale == scale, "sm_scale is NaN")
-    _need(max_len is None or max_len >= 0, "max_len: not negative")
-    _plain((q, "q"), (out, "out"))
-    _rows(q, "q")
+    kv4_chunk).  Rows of `out` behind cu_q[B] are left as they were (0 where the call makes it)."""
+    i = _where(q, kc, ks, vc, vs, table, lens, cu_q, out)
+    ps, where, HKV, Dh = _kv4_cache(kc, ks, vc, vs)
+    tp, ts, B, width = _table(table, where[3])
+    T, HQ = q.shape[:2] if q.dim() == 3 else (0, 0)
+    if q.shape != (T, HQ, Dh) or q.dtype is not torch.bfloat16 or HQ < 1 or HQ % HKV:
+        raise ValueError(f"q: (T, a multiple of {HKV}, {Dh}) bf16")
+    G = HQ // HKV
+    lp = _ints(lens, B, "lens")
+    cp = None
+    if cu_q is not None:
+        cp = _ints(cu_q, B + 1, "cu_q")
+    elif T != B or max_q != 1:
+        raise ValueError("without cu_q every sequence has one row of q")
+    scale = Dh ** -0.5 if sm_scale is None else sm_scale
+    if not 1 <= max_q <= (1 << 30) // G or scale != scale or max_len is not None and max_len < 0:
+        raise ValueError("max_q: at least 1; sm_scale: not NaN; max_len: not negative")
+    _plain(q, out)
+    qa = _rows(q, T, HQ, Dh, "q")
     if out is None:
-        out = (torch.empty if cu_q is None else torch.zeros)(q.shape, device=dev, dtype=q.dtype)
-    _need(out.shape == q.shape and out.dtype == q.dtype, "out: as q")
-    _rows(out, "out", True)
+        out = q.new_empty((T, HQ, Dh)) if cp is None else q.new_zeros((T, HQ, Dh))
+    elif out.shape != q.shape or out.dtype is not torch.bfloat16:
+        raise ValueError("out: as q")
+    oa = _rows(out, T, HQ, Dh, "out", True)
     if T == 0 or B == 0:
         return out
-    rows = max_q * (HQ // HKV)
-    cap = max(1, width * page if max_len is None else min(max_len, width * page))
+    rows = max_q * G
+    cap = max(1, width * where[3] if max_len is None else min(max_len, width * where[3]))
     chunk = kv4_chunk(cap, B * HKV * -(-rows // (8 if rows <= 8 else 16 if rows <= 16 else 32)))
     nchunk = -(-cap // chunk)
-    ml = ws = None
+    wp = mp = None
     if nchunk > 1:
         n = T * HQ * nchunk
-        ws = torch.empty(n * (Dh + 2), device=dev, dtype=torch.float32)
-        ml = ws[n * Dh:]
-    _run(dev, "oa_kv4_attn", _ptr(q), *_strides(q), _ptr(kc), _ptr(ks), _ptr(vc), _ptr(vs), *_page_strides(kc, ks), NP,
-         page, _ptr(table), max(table.stride(0), width), width, _ptr(lens), _ptr(cu_q), B, T, max_q, HQ, HKV, Dh, scale,
-         chunk, nchunk, _ptr(ws), _ptr(ml), _ptr(out), *_strides(out))
+        ws = q.new_empty(n * (Dh + 2), dtype=torch.float32)
+        wp = ws.data_ptr()
+        mp = wp + 4 * n * Dh
+    _run(i, "oa_kv4_attn", *qa, *ps, *where, tp, ts, width, lp, cp, B, T, max_q, HQ, HKV, Dh, scale, chunk, nchunk, wp, mp,
+         *oa)
     return out
 
 
