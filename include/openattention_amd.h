@@ -561,7 +561,8 @@ int oa_qk_norm_rope(const void* q, long q_st, long q_sh, const void* k, long k_s
 /*
  * Page tables of a paged cache, on the device.  table (requests, width) int32 rows of table_stride: page ids,
  * -1 for none; lens (requests): tokens held, in ceil(lens / page) pages; free (pages): a stack of the ids
- * nobody holds, its height in *nfree (top: free[nfree - 1]); page: a power of two, 32 .. 1024.
+ * nobody holds, its height in *nfree (top: free[nfree - 1]); page: a power of two, 32 .. 1024;
+ * a row of the table holds at most 2^30 tokens.
  *
  * extend: request i adds add[i] >= 0 tokens.  Pages are popped in the order of requests and of their pages;
  * slots[t] = page id * page + offset and pos[t] of the new tokens, request after request, cu (requests + 1)

@@ -130,41 +130,26 @@ __global__ void __launch_bounds__(kThreads, NQ > 1 ? 2 : 3) kv4_attn_kernel(Attn
   const int bh = blockIdx.x % units, rest = blockIdx.x / units;
   const int ch = rest / a.ntile, row0 = (rest - ch * a.ntile) * (NQ * kCols);
   const int b = bh / a.HKV, h = bh - b * a.HKV;
+  // (the table's entries are requested beside the length: what lies past it is not used)
+  constexpr int kStride = kWaves * kTile;
+  const int k0 = ch * a.chunk, tb = k0 + wave * kTile;
+  const int* trow = a.table + (long)b * a.t_st;
+  auto page_at = [&](int t0) { return trow[min(t0 >> a.lp, a.width - 1)]; };
+  const int page0 = page_at(tb);
+  int page = page_at(tb + kStride);
   const Seq sq = seq_of(a, b);
   const int rows = min(sq.R, a.max_q) * a.G;
   if (row0 >= rows) return;
   const int first = sq.n - sq.R;         // position of the sequence's first query token
   const int hi = sq.bad ? 0 : first + (min(row0 + NQ * kCols, rows) - 1) / a.G + 1;    // keys any row sees
   const int all = first + row0 / a.G + 1;                                              // keys every row sees
-  const int k0 = ch * a.chunk, k1 = min(k0 + a.chunk, hi);
+  const int k1 = min(k0 + a.chunk, hi);
   if (k0 >= k1 && a.nchunk > 1) return;
 
-  // this lane's columns: rows of q (negated under a negative scale: the maximum is taken before scaling)
-  // and how many keys they see (0: no such row)
-  const float c = fabsf(a.c);
-  const unsigned flip = a.c < 0.f ? 0x80008000u : 0u;
-  bf16x8 Q[NQ][kSteps];
-  int lim[NQ];
-#pragma unroll
-  for (int x = 0; x < NQ; ++x) {
-    const int r = row0 + x * kCols + (DUP ? col & 7 : col);
-    const int rr = min(r, rows - 1), j = rr / a.G, hd = h * a.G + rr - j * a.G;
-    lim[x] = r < rows ? first + j + 1 : 0;
-    const uint16_t* p = a.q + (long)(sq.r0 + j) * a.q_st + (long)hd * a.q_sh + g * (D / 4);
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const uint4v w = *reinterpret_cast<const uint4v*>(p + 8 * s);
-      Q[x][s] = __builtin_bit_cast(bf16x8, w ^ uint4v(flip));
-    }
-  }
-
   // a tile's addresses: a scalar base and fixed lane offsets
-  const int* trow = a.table + (long)b * a.t_st;
   const int pmask = (1 << a.lp) - 1;
   const long headc = ((long)h << a.lp) * (D / 2), heads = ((long)h << a.lp) * (D / 32);
   const unsigned oc = col * (D / 2) + g * (D / 8), os = col * (D / 32) + g * D / 128;
-  const int last = (k1 - 1) >> a.lp;     // the piece's last page
-  auto page_at = [&](int t0) { return trow[min(t0 >> a.lp, last)]; };
   auto load = [&](Tile<D>& t, int t0, int page) {
     const bool bad = (unsigned)page >= (unsigned)a.NP;
     t.bad = bad ? 0x7f800000u : 0u;
@@ -185,6 +170,29 @@ __global__ void __launch_bounds__(kThreads, NQ > 1 ? 2 : 3) kv4_attn_kernel(Attn
       t.vs[c] = vs[os + 16 * c * (D / 32)];
     }
   };
+  const int nt = max(0, (k1 - tb + kStride - 1) / kStride);                  // this wave's tiles
+  const int nfull = min(nt, max(0, (all - tb - kTile + kStride) / kStride));  // those that every row sees whole
+  Tile<D> ta, tc;
+  if (nt > 0) load(ta, tb, page0);
+
+  // this lane's columns: rows of q (negated under a negative scale: the maximum is taken before scaling)
+  // and how many keys they see (0: no such row)
+  const float c = fabsf(a.c);
+  const unsigned flip = a.c < 0.f ? 0x80008000u : 0u;
+  bf16x8 Q[NQ][kSteps];
+  int lim[NQ];
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    const int r = row0 + x * kCols + (DUP ? col & 7 : col);
+    const int rr = min(r, rows - 1), j = rr / a.G, hd = h * a.G + rr - j * a.G;
+    lim[x] = r < rows ? first + j + 1 : 0;
+    const uint16_t* p = a.q + (long)(sq.r0 + j) * a.q_st + (long)hd * a.q_sh + g * (D / 4);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const uint4v w = *reinterpret_cast<const uint4v*>(p + 8 * s);
+      Q[x][s] = __builtin_bit_cast(bf16x8, w ^ uint4v(flip));
+    }
+  }
 
   // LDS tile of 32 value rows; 16-byte chunk x of row r lies at x ^ f(r): 16 rows written at one chunk
   // and 16 rows read at two both spread over all banks
@@ -211,11 +219,6 @@ __global__ void __launch_bounds__(kThreads, NQ > 1 ? 2 : 3) kv4_attn_kernel(Attn
     for (int d = 0; d < kDims; ++d) O[x][d] = f32x4(0.f);
   }
 
-  constexpr int kStride = kWaves * kTile;
-  const int tb = k0 + wave * kTile;
-  const int nt = max(0, (k1 - tb + kStride - 1) / kStride);                  // this wave's tiles
-  const int nfull = min(nt, max(0, (all - tb - kTile + kStride) / kStride));  // those that every row sees whole
-  int page = 0;
 
   // tile i from t; tile i + 1 is fetched into n
   auto body = [&](auto mask_c, int i, const Tile<D>& t, Tile<D>& n) {
@@ -320,11 +323,6 @@ __global__ void __launch_bounds__(kThreads, NQ > 1 ? 2 : 3) kv4_attn_kernel(Attn
   {
     typedef std::integral_constant<bool, false> whole;
     typedef std::integral_constant<bool, true> masked;
-    Tile<D> ta, tc;
-    if (nt > 0) {
-      load(ta, tb, page_at(tb));
-      page = page_at(tb + kStride);
-    }
     int i = 0;
 #pragma unroll 1
     for (; i + 2 <= nfull; i += 2) {
@@ -416,10 +414,23 @@ __global__ void __launch_bounds__(kThreads) kv4_join_kernel(AttnArgs a) {
   const int grp = tid / kLanes, y = tid % kLanes;
   f32x4 o = f32x4(0.f);
   float L = 0.f;
-  for (int i = grp; i < nv; i += kGroups) {
-    const float w = __builtin_amdgcn_exp2f(ml[2 * i] - M);
-    L += w * ml[2 * i + 1];
-    o += *reinterpret_cast<const f32x4*>(a.ws_o + (row + i) * D + 4 * y) * w;
+  constexpr int kAtOnce = 4;             // pieces whose loads are in flight together
+  for (int i = grp; i < nv; i += kAtOnce * kGroups) {
+    f32x4 x[kAtOnce];
+    f32x2 w[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int at = min(i + k * kGroups, nv - 1);
+      x[k] = *reinterpret_cast<const f32x4*>(a.ws_o + (row + at) * D + 4 * y);
+      w[k] = *reinterpret_cast<const f32x2*>(ml + 2 * at);
+    }
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      if (i + k * kGroups >= nv) break;
+      const float e = __builtin_amdgcn_exp2f(w[k][0] - M);
+      L += e * w[k][1];
+      o += x[k] * e;
+    }
   }
   *reinterpret_cast<f32x4*>(&s_o[grp][4 * y]) = o;
   if (y == 0) s_l[grp] = L;
@@ -460,8 +471,8 @@ extern "C" int oa_kv4_attn(const void* q, long q_st, long q_sh, const void* kc, 
   auto odd = [](const void* p, uintptr_t n) { return !p || (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0; };
   if ((head_dim != 64 && head_dim != 128) || sequences < 0 || tokens < 0 || max_q <= 0 || kv_heads <= 0 || q_heads <= 0 ||
       q_heads % kv_heads || (long)max_q * (q_heads / kv_heads) > (1L << 30) || pages <= 0 || page < 32 || page > 1024 ||
-      (page & (page - 1)) || (long)pages * page > 0x7fffffffL || width <= 0 || (long)width * page > 0x7fffffffL ||
-      table_stride < width || chunk < 128 || chunk % 128 || nchunk <= 0 || (long)nchunk * chunk > 0x7ffffff0L)
+      (page & (page - 1)) || (long)pages * page > 0x7fffffffL || width <= 0 || (long)width * page > (1L << 30) ||
+      table_stride < width || chunk < 128 || chunk % 128 || nchunk <= 0 || (long)nchunk * chunk > (1L << 30) + (1L << 29))
     return OA_EINVAL;
   if (!cu && (max_q != 1 || sequences != tokens)) return OA_EINVAL;
   if (!sequences || !tokens) return 0;

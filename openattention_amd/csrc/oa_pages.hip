@@ -230,7 +230,7 @@ constexpr int kAloneRows = 256;
 int take(PagesArgs& a, const int* count, int* lens, int* table, long t_st, int* free, int* nfree, int* status, int B,
          int width, int NP, int page, int* ws) {
   if (!count || !lens || !table || !free || !nfree || !status || !ws || B <= 0 || width <= 0 || t_st < width || NP <= 0 ||
-      page < 32 || page > 1024 || (page & (page - 1)) || (long)NP * page > 0x7fffffffL || (long)width * page > 0x7fffffffL ||
+      page < 32 || page > 1024 || (page & (page - 1)) || (long)NP * page > 0x7fffffffL || (long)width * page > (1L << 30) ||
       B > (1 << 24))
     return OA_EINVAL;
   a = PagesArgs{};

@@ -782,8 +782,8 @@ def _table(table: torch.Tensor, page: int) -> tuple:
         raise ValueError("table: (requests, width) int32")
     B, width = table.shape
     s0, s1 = table.stride()
-    if width < 1 or width * page >= 1 << 31 or width > 1 and s1 != 1 or B > 1 and s0 < width or B > 1 << 24:
-        raise ValueError("table: contiguous rows of fewer than 2^31 tokens, at most 2^24 requests")
+    if width < 1 or width * page > 1 << 30 or width > 1 and s1 != 1 or B > 1 and s0 < width or B > 1 << 24:
+        raise ValueError("table: contiguous rows of at most 2^30 tokens, at most 2^24 requests")
     return table.data_ptr(), max(s0, width), B, width
 
 
@@ -881,10 +881,12 @@ def kv4_read(slots, kc, ks, vc, vs, dtype: torch.dtype = torch.bfloat16):
 
 
 def kv4_chunk(cap: int, units: int) -> int:
-    """Keys per workgroup of kv4_attn: `units` (sequence, KV head, query tile) triples with up to `cap` keys
-    are cut until about 2048 workgroups are there, but into pieces of at least 256 keys."""
-    n = max(1, 2048 // max(units, 1))
-    return max(256, -(-cap // (n * 128)) * 128)
+    """Keys per workgroup of kv4_attn, for `units` (sequence, KV head, query tile) triples of up to `cap` keys:
+    two workgroups to a compute unit, but pieces of at least 384 keys (their start and end cost as much
+    as some 300 keys) and at most an eighth of the longest sequence (or 1024), so that a batch does not
+    wait for one piece of it."""
+    n = max(min(max(cap * units // 512, 384), max(cap // 8, 1024)), 384)
+    return min(-(-n // 128), -(-cap // 128)) * 128
 
 
 def kv4_attn(q, kc, ks, vc, vs, table, lens, sm_scale: float | None = None, cu_q=None, max_q: int = 1, out=None,

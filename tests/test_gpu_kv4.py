@@ -338,12 +338,13 @@ CASES = [  # lens, rows (None: one each), HQ, HKV, D, page
 
 
 @pytest.mark.parametrize("case", range(len(CASES)))
-@pytest.mark.parametrize("chunk", [None, 128, 100000])
-def test_attention(case, chunk, monkeypatch):
+@pytest.mark.parametrize("chunk,copies", [(None, 1), (128, 1), (1 << 20, 1), (256, 5)])
+def test_attention(case, chunk, copies, monkeypatch):
+    print(f"[case] attn {CASES[case]} chunk={chunk} copies={copies}", flush=True)
     lens, rows, HQ, HKV, D, page = CASES[case]
-    print(f"[case] attn {CASES[case]} chunk={chunk}", flush=True)
     if chunk:
         monkeypatch.setattr(ops, "kv4_chunk", lambda cap, units: min(chunk, -(-cap // 128) * 128))
+    lens, rows = lens * copies, rows and rows * copies
     g = gen(case)
     cache, table = paged(lens, HKV, D, page, g, extra_width=case % 3)
     cu = starts(rows or [1] * len(lens))
@@ -352,6 +353,23 @@ def test_attention(case, chunk, monkeypatch):
     scale = D ** -0.5 if case % 2 else 0.11
     out = ops.kv4_attn(q, *cache, table, i32(lens), scale, cu_q=i32(cu) if rows else None, max_q=max(rows) if rows else 1)
     check_attn(out, *want_attn(q, cache, table, lens, cu, scale, page))
+
+
+def test_attention_of_many_sequences():
+    """More sequences than a workgroup has threads, most of them short or empty."""
+    g = gen(77)
+    r = random.Random(4)
+    lens = [r.choice((0, 0, 1, 2, 33, 100, 200)) for _ in range(700)]
+    lens[650] = 1500
+    rows = [min(n, r.choice((0, 1, 2, 3))) if n else r.choice((0, 1)) for n in lens]
+    cache, table = paged(lens, 1, 64, 32, g)
+    cu = starts(rows)
+    q = randn(g, cu[-1], 4, 64, dtype=torch.bfloat16)
+    out = ops.kv4_attn(q, *cache, table, i32(lens), cu_q=i32(cu), max_q=3)
+    check_attn(out, *want_attn(q, cache, table, lens, cu, 0.125, 32))
+    q = randn(g, 700, 2, 64, dtype=torch.bfloat16)
+    out = ops.kv4_attn(q, *cache, table, i32(lens))
+    check_attn(out, *want_attn(q, cache, table, lens, list(range(701)), 0.125, 32))
 
 
 def test_attention_scales():
