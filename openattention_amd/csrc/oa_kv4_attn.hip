@@ -99,15 +99,14 @@ struct Tile {
   unsigned bad;                          // the exponent of NaN where the page is outside of the cache
 };
 
-template <int N>
+// ONCE: codes that no other workgroup reads pass by the caches (32 x 32768 keys: 206 us through them, 187)
+template <bool ONCE, int N>
 __device__ __forceinline__ void load_words(unsigned (&w)[N], const uint8_t* p) {
-  if constexpr (N == 4) {
-    const uint4v x = *reinterpret_cast<const uint4v*>(p);
-    w[0] = x[0]; w[1] = x[1]; w[2] = x[2]; w[3] = x[3];
-  } else {
-    const uint2v x = *reinterpret_cast<const uint2v*>(p);
-    w[0] = x[0]; w[1] = x[1];
-  }
+  typedef unsigned vec __attribute__((ext_vector_type(N)));
+  const vec* q = reinterpret_cast<const vec*>(p);
+  const vec x = ONCE ? __builtin_nontemporal_load(q) : *q;
+#pragma unroll
+  for (int i = 0; i < N; ++i) w[i] = x[i];
 }
 
 // NQ tiles of 16 query rows; DUP: at most 8 rows, columns 8.. repeat them for the weights' second terms
@@ -161,12 +160,12 @@ __global__ void __launch_bounds__(kThreads, NQ > 1 ? 2 : 3) kv4_attn_kernel(Attn
     const uint8_t* vs = a.vs + bs;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      load_words<kSteps>(t.k[c], kc + oc + 16 * c * (D / 2));
+      load_words<NQ == 1>(t.k[c], kc + oc + 16 * c * (D / 2));
       t.ks[c] = ks[os + 16 * c * (D / 32)];
     }
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      load_words<kSteps>(t.v[c], vc + oc + 16 * c * (D / 2));
+      load_words<NQ == 1>(t.v[c], vc + oc + 16 * c * (D / 2));
       t.vs[c] = vs[os + 16 * c * (D / 32)];
     }
   };
@@ -325,14 +324,9 @@ __global__ void __launch_bounds__(kThreads, NQ > 1 ? 2 : 3) kv4_attn_kernel(Attn
     typedef std::integral_constant<bool, true> masked;
     int i = 0;
 #pragma unroll 1
-    for (; i + 2 <= nfull; i += 2) {
-      body(whole(), i, ta, tc);
-      body(whole(), i + 1, tc, ta);
-    }
-    if (i < nfull) {
+    for (; i < nfull; ++i) {             // (two tiles to a turn, without the copies: 186 us for 182)
       body(whole(), i, ta, tc);
       ta = tc;
-      ++i;
     }
 #pragma unroll 1
     for (; i < nt; ++i) {
