@@ -10,7 +10,9 @@
 // Layout: codes (pages, heads, page, D / 2), scales (pages, heads, page, D / 32), bytes; slot = page id
 // * page + offset.
 //
-// A lane takes 8 values of a row (16 bytes of bf16, 4 of codes), four lanes a block.
+// A lane takes 8 values of a row (16 bytes of bf16, 4 of codes), four lanes a block, a workgroup one head
+// of K or V for 16 or 32 successive tokens: where their slots follow each other, as a prompt's do, codes
+// and scales are whole lines.
 #include "oa_common.h"
 
 namespace {
@@ -34,30 +36,43 @@ struct Kv4Args {
   const int* slots;
   uint8_t* kc; uint8_t* ks; uint8_t* vc; uint8_t* vs;
   long c_sp, s_sp;                       // bytes between pages of codes and of scales
-  unsigned units, kv_heads;              // (token, K or V, head)
+  int tokens, kv_heads;
   int lp;                                // log2 of the page
   unsigned nslots;
 };
 
+// a lane's row: its token, whether it is there, and where its values and codes lie
 struct Row {
-  unsigned tok, head;
-  bool isv;
+  int tok;
+  unsigned slot;
+  bool live;
   uint8_t* codes;
   uint8_t* scales;
 };
 
 template <int D>
-__device__ __forceinline__ Row row_of(const Kv4Args& a, unsigned u, unsigned slot) {
+__device__ __forceinline__ Row row_of(const Kv4Args& a, int blk, bool isv, int head) {
+  constexpr int kLanes = D / 8;          // lanes of a row
   Row r;
-  r.tok = u / (2 * a.kv_heads);
-  const unsigned w = u - r.tok * 2 * a.kv_heads;
-  r.isv = w >= a.kv_heads;
-  r.head = w - (r.isv ? a.kv_heads : 0);
-  const unsigned page = slot >> a.lp, off = slot & ((1u << a.lp) - 1);
-  const long in = ((long)r.head << a.lp) + off;
-  r.codes = (r.isv ? a.vc : a.kc) + (long)page * a.c_sp + in * (D / 2);
-  r.scales = (r.isv ? a.vs : a.ks) + (long)page * a.s_sp + in * (D / 32);
+  r.tok = blk * (kThreads / kLanes) + (int)threadIdx.x / kLanes;
+  r.live = r.tok < a.tokens;
+  r.slot = r.live ? (unsigned)a.slots[r.tok] : ~0u;
+  const unsigned s = r.slot < a.nslots ? r.slot : 0, page = s >> a.lp, off = s & ((1u << a.lp) - 1);
+  const long in = ((long)head << a.lp) + off;
+  r.codes = (isv ? a.vc : a.kc) + (long)page * a.c_sp + in * (D / 2);
+  r.scales = (isv ? a.vs : a.ks) + (long)page * a.s_sp + in * (D / 32);
   return r;
+}
+
+// the lowest byte of each block's first lane, in the row's first lane
+template <int D>
+__device__ __forceinline__ unsigned scales_of_row(unsigned s) {
+  unsigned w = s | (unsigned)__builtin_amdgcn_update_dpp(0, (int)s, 0x104, 0xf, 0xf, true) << 8;      // row_shl 4, 8, 12
+  if (D == 128) {
+    w |= (unsigned)__builtin_amdgcn_update_dpp(0, (int)s, 0x108, 0xf, 0xf, true) << 16;
+    w |= (unsigned)__builtin_amdgcn_update_dpp(0, (int)s, 0x10c, 0xf, 0xf, true) << 24;
+  }
+  return w;
 }
 
 __device__ __forceinline__ unsigned max4(unsigned v) {     // over the lanes of a block
@@ -67,17 +82,14 @@ __device__ __forceinline__ unsigned max4(unsigned v) {     // over the lanes of 
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) kv4_write_kernel(Kv4Args a) {
-  constexpr int kLanes = D / 8;          // lanes of a row
   typedef typename Vec8<T>::type vec;
-  const unsigned idx = blockIdx.x * kThreads + threadIdx.x;
-  const unsigned u = idx / kLanes, l = idx % kLanes;
-  if (u >= a.units) return;              // (whole rows of lanes)
-  const unsigned slot = (unsigned)a.slots[u / (2 * a.kv_heads)];
-  if (slot >= a.nslots) return;          // padding
-  const Row r = row_of<D>(a, u, slot);
-  const T* x = r.isv ? (const T*)a.v + (long)r.tok * a.v_st + (long)r.head * a.v_sh
-                     : (const T*)a.k + (long)r.tok * a.k_st + (long)r.head * a.k_sh;
-  const f32x8 f = __builtin_convertvector(*reinterpret_cast<const vec*>(x + 8 * l), f32x8);
+  const int head = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, l = threadIdx.x % (D / 8);
+  const bool isv = rest & 1;
+  const Row r = row_of<D>(a, rest >> 1, isv, head);
+  const int tok = min(r.tok, a.tokens - 1);          // (lanes past the end repeat the last row, unstored)
+  const T* x = isv ? (const T*)a.v + (long)tok * a.v_st + (long)head * a.v_sh
+                   : (const T*)a.k + (long)tok * a.k_st + (long)head * a.k_sh;
+  const f32x8 f = __builtin_convertvector(__builtin_nontemporal_load(reinterpret_cast<const vec*>(x + 8 * l)), f32x8);
   unsigned top = 0;                      // of |x| as bits: NaN above infinity above all else
 #pragma unroll
   for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
@@ -91,20 +103,21 @@ __global__ void __launch_bounds__(kThreads) kv4_write_kernel(Kv4Args a) {
   c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[2] * inv, f[3] * inv, 1.f, 1);
   c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[4] * inv, f[5] * inv, 1.f, 2);
   c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[6] * inv, f[7] * inv, 1.f, 3);
+  const unsigned w = scales_of_row<D>(fine ? e + 127 : 255);
+  if (r.slot >= a.nslots) return;        // padding
   *reinterpret_cast<unsigned*>(r.codes + 4 * l) = fine ? c : 0u;
-  if (l % 4 == 0) r.scales[l / 4] = (uint8_t)(fine ? e + 127 : 255);
+  if (l) return;
+  if (D == 128) *reinterpret_cast<unsigned*>(r.scales) = w;
+  else *reinterpret_cast<uint16_t*>(r.scales) = (uint16_t)w;
 }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) kv4_read_kernel(Kv4Args a) {
-  constexpr int kLanes = D / 8;
   typedef typename Vec8<T>::type vec;
-  const unsigned idx = blockIdx.x * kThreads + threadIdx.x;
-  const unsigned u = idx / kLanes, l = idx % kLanes;
-  if (u >= a.units) return;
-  const unsigned slot = (unsigned)a.slots[u / (2 * a.kv_heads)];
-  const bool held = slot < a.nslots;     // (padding reads slot 0 and gives zeros)
-  const Row r = row_of<D>(a, u, held ? slot : 0);
+  const int head = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, l = threadIdx.x % (D / 8);
+  const bool isv = rest & 1;
+  const Row r = row_of<D>(a, rest >> 1, isv, head);
+  const bool held = r.slot < a.nslots;   // (padding reads slot 0 and gives zeros)
   const unsigned c = *reinterpret_cast<const unsigned*>(r.codes + 4 * l);
   const unsigned s = r.scales[l / 4];
   const float f = s == 255 ? __builtin_nanf("") : __uint_as_float(s << 23);
@@ -115,9 +128,9 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(Kv4Args a) {
   f32x8 y;
 #pragma unroll
   for (int i = 0; i < 8; ++i) y[i] = held ? (float)b[i / 2][i % 2] * f : 0.f;
-  T* o = r.isv ? (T*)a.v + (long)r.tok * a.v_st + (long)r.head * a.v_sh
-               : (T*)a.k + (long)r.tok * a.k_st + (long)r.head * a.k_sh;
-  *reinterpret_cast<vec*>(o + 8 * l) = __builtin_convertvector(y, vec);
+  if (!r.live) return;
+  T* o = isv ? (T*)a.v + (long)r.tok * a.v_st + (long)head * a.v_sh : (T*)a.k + (long)r.tok * a.k_st + (long)head * a.k_sh;
+  __builtin_nontemporal_store(__builtin_convertvector(y, vec), reinterpret_cast<vec*>(o + 8 * l));
 }
 
 // the checks that both directions share
@@ -131,7 +144,7 @@ int take(Kv4Args& a, const void* k, long k_st, long k_sh, const void* v, long v_
   if ((D != 64 && D != 128) || tokens < 0 || kv_heads <= 0 || pages <= 0 || page < 32 || page > 1024 || (page & (page - 1)) ||
       (long)pages * page > 0x7fffffffL || (long)tokens * kv_heads > (1L << 26))
     return OA_EINVAL;
-  a.units = 2u * tokens * kv_heads;
+  a.tokens = tokens;
   if (!tokens) return 0;
   if (bad(k, k_st, k_sh) || bad(v, v_st, v_sh) || odd(kc) || odd(ks) || odd(vc) ||
       odd(vs) || !slots || code_stride < (long)kv_heads * page * (D / 2) || scale_stride < (long)kv_heads * page * (D / 32) ||
@@ -148,7 +161,10 @@ int take(Kv4Args& a, const void* k, long k_st, long k_sh, const void* v, long v_
   return 0;
 }
 
-dim3 grid_of(const Kv4Args& a, int D) { return dim3((unsigned)(((long)a.units * (D / 8) + kThreads - 1) / kThreads)); }
+dim3 grid_of(const Kv4Args& a, int D) {
+  const int rows = kThreads / (D / 8);
+  return dim3((unsigned)((long)((a.tokens + rows - 1) / rows) * 2 * a.kv_heads));
+}
 
 template <typename T>
 void write_rows(const Kv4Args& a, int D, hipStream_t st) {
@@ -171,7 +187,7 @@ extern "C" int oa_kv4_write(const void* k, long k_st, long k_sh, const void* v, 
   if (const int e = take(a, k, k_st, k_sh, v, v_st, v_sh, tokens, kv_heads, head_dim, dtype == 2 ? 4 : 8, slots, kc, ks,
                          vc, vs, code_stride, scale_stride, pages, page))
     return e;
-  if (!a.units) return 0;
+  if (!tokens) return 0;
   const hipStream_t st = (hipStream_t)stream;
   if (dtype == 0) write_rows<__bf16>(a, head_dim, st);
   else if (dtype == 1) write_rows<_Float16>(a, head_dim, st);
@@ -189,7 +205,7 @@ extern "C" int oa_kv4_read(const int* slots, const void* kc, const void* ks, con
                          const_cast<void*>(kc), const_cast<void*>(ks), const_cast<void*>(vc), const_cast<void*>(vs),
                          code_stride, scale_stride, pages, page))
     return e;
-  if (!a.units) return 0;
+  if (!tokens) return 0;
   const hipStream_t st = (hipStream_t)stream;
   if (dtype == 0) read_rows<__bf16>(a, head_dim, st);
   else read_rows<float>(a, head_dim, st);

@@ -85,8 +85,8 @@ __global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(RopeArgs a) {
   if (!live) return;
   T* o = isq ? (T*)a.qo + (long)tok * a.qo_st + (long)hd * a.qo_sh
              : (T*)a.ko + (long)tok * a.ko_st + (long)(hd - a.q_heads) * a.ko_sh;
-  *reinterpret_cast<vec*>(o + 8 * lh) = __builtin_convertvector(o0, vec);
-  *reinterpret_cast<vec*>(o + D / 2 + 8 * lh) = __builtin_convertvector(o1, vec);
+  __builtin_nontemporal_store(__builtin_convertvector(o0, vec), reinterpret_cast<vec*>(o + 8 * lh));
+  __builtin_nontemporal_store(__builtin_convertvector(o1, vec), reinterpret_cast<vec*>(o + D / 2 + 8 * lh));
 }
 
 template <typename T>
