@@ -10,18 +10,22 @@
 // *status (1: a negative count or a request longer than its row of the table; 2: too few free pages, or
 // more than a stack can hold; 4: more tokens than the caller has slots for).
 //
-// One workgroup adds up what every request needs (a scan over the requests), decides, and writes
-// lengths, starts and the stack's height; with few tokens it also writes slots and pages.  For many,
-// a second launch does: a lane per token finds its request by bisection of the starts.
+// One workgroup adds up what every request needs (a scan over the requests, as many threads as there are up
+// to 1024), decides, and writes lengths, starts and the stack's height; with few tokens or requests it also
+// writes slots and pages.  For many, a second launch does: a lane per token finds its request by bisection
+// of the starts, a wave per request moves its returned pages.  Bound by the latency of its few dependent
+// accesses: 32 requests that add a token and take it
+// back 5.5 us, 1000 that add 360000 tokens and give them back 13.4 (captured calls).
 #include "oa_common.h"
 
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kWaves = kThreads / 64;
+constexpr int kMost = 1024;              // threads of the planning workgroup
 constexpr int kFill = 256;
+constexpr int kStarts = 4096;            // starts that a workgroup of the second launch holds in LDS
 // tokens up to which the planning workgroup writes the slots itself
 constexpr int kAlone = 2048;
+constexpr unsigned kFull = 0x7fffffffu;  // what sums stop at
 
 struct PagesArgs {
   const int* count;                      // tokens to add, or to keep
@@ -33,198 +37,252 @@ struct PagesArgs {
   int* ws;                               // length, first new page of each request (2 B), stack height
 };
 
-// inclusive sum over the lanes of a wave
-__device__ __forceinline__ long wave_scan(long v, int lane) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const long o = __shfl_up(v, d);
-    if (lane >= d) v += o;
-  }
-  return v;
+__device__ __forceinline__ unsigned add_to(unsigned a, unsigned b) { return min(a + b, kFull); }   // (both at most kFull)
+
+// inclusive sum over the lanes of a wave, stopping at kFull
+__device__ __forceinline__ unsigned wave_scan(unsigned v) {
+  v = add_to(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false));     // row_shr 1, 2, 4, 8
+  v = add_to(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false));
+  v = add_to(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false));
+  v = add_to(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false));
+  v = add_to(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false));     // rows 0 to 1, 2 to 3
+  return add_to(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false));  // rows 1 to 2, 3
 }
 
+template <int THREADS>
 struct Scan {
-  long part[2][kWaves];
+  unsigned part[2][THREADS / 64];
 };
 
-// exclusive sums of two values over the workgroup and their totals (two barriers)
-__device__ __forceinline__ void block_scan(Scan& s, long a, long b, long& ea, long& eb, long& ta, long& tb) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long ia = wave_scan(a, lane), ib = wave_scan(b, lane);
+// inclusive sums of two values over the workgroup and their totals
+template <int THREADS>
+__device__ __forceinline__ void block_scan(Scan<THREADS>& s, unsigned& a, unsigned& b, unsigned& ta, unsigned& tb) {
+  a = wave_scan(a);
+  b = wave_scan(b);
+  if (THREADS == 64) {
+    ta = (unsigned)__builtin_amdgcn_readlane((int)a, 63);
+    tb = (unsigned)__builtin_amdgcn_readlane((int)b, 63);
+    return;
+  }
+  const int wave = threadIdx.x >> 6;
   __syncthreads();
-  if (lane == 63) {
-    s.part[0][wave] = ia;
-    s.part[1][wave] = ib;
+  if ((threadIdx.x & 63) == 63) {
+    s.part[0][wave] = a;
+    s.part[1][wave] = b;
   }
   __syncthreads();
-  ea = ia - a;
-  eb = ib - b;
+  unsigned oa = 0, ob = 0;
   ta = tb = 0;
-  for (int w = 0; w < kWaves; ++w) {
-    const long x = s.part[0][w], y = s.part[1][w];
-    if (w < wave) {
-      ea += x;
-      eb += y;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
+    if (w == wave) {
+      oa = ta;
+      ob = tb;
     }
-    ta += x;
-    tb += y;
+    ta = add_to(ta, s.part[0][w]);
+    tb = add_to(tb, s.part[1][w]);
   }
+  a = add_to(a, oa);
+  b = add_to(b, ob);
 }
 
-__device__ __forceinline__ long pages_of(long tokens, int lp) { return (tokens + (1L << lp) - 1) >> lp; }
+__device__ __forceinline__ int pages_of(int tokens, int lp) { return (tokens + (1 << lp) - 1) >> lp; }   // (at most 2^30 + page)
 
 // lengths outside of what a row of the table can hold count as its nearest end
-__device__ __forceinline__ long held_len(const PagesArgs& a, int i) {
-  return min(max((long)a.lens[i], 0l), (long)a.width << a.lp);
-}
+__device__ __forceinline__ int held_len(const PagesArgs& a, int i) { return min(max(a.lens[i], 0), a.width << a.lp); }
 
-// slot and position of token t, and, from the first token on a new page, the table's entry
-__device__ __forceinline__ void fill_token(const PagesArgs& a, int t, int nfree) {
-  int lo = 0, hi = a.B - 1;              // the last request that starts at or before t
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.cu[mid] <= t) lo = mid;
-    else hi = mid - 1;
+// slot and position of token t, and, from the first token on a new page, the table's entry.  cu: the starts
+__device__ __forceinline__ void fill_token(const PagesArgs& a, const int* cu, const int* len_of, const int* new_of, int t,
+                                           int nfree) {
+  int lo = 0, n = a.B;                   // the last request that starts at or before t
+  while (n > 1) {
+    const int half = n >> 1;
+    if (cu[lo + half] <= t) lo += half;
+    n -= half;
   }
-  const int len = a.ws[lo], p = len + t - a.cu[lo], at = p >> a.lp, held = (int)pages_of(len, a.lp);
+  const int len = len_of[lo], p = len + t - cu[lo], at = p >> a.lp, held = pages_of(len, a.lp);
   int* row = a.table + (long)lo * a.t_st;
-  const int id = at >= held ? a.free[nfree - 1 - (a.ws[a.B + lo] + at - held)] : row[at];
+  const int id = at >= held ? a.free[nfree - 1 - (new_of[lo] + at - held)] : row[at];
   if (at >= held && (p & ((1 << a.lp) - 1)) == 0) row[at] = id;
   a.slots[t] = (unsigned)id < (unsigned)a.NP ? (id << a.lp) + (p & ((1 << a.lp) - 1)) : -1;
   a.pos[t] = p;
 }
 
-__global__ void __launch_bounds__(kThreads) pages_extend_kernel(PagesArgs a, int alone) {
-  __shared__ Scan s;
+// a request's tokens and pages to add; what cannot be is noted in *bad
+__device__ __forceinline__ void wanted(const PagesArgs& a, int i, int& len, int& n, int& need, int* bad) {
+  n = a.count[i];
+  const int have = a.lens[i];
+  len = held_len(a, i);
+  if (n < 0 || len != have || n > (a.width << a.lp) - len) {
+    atomicOr(bad, 1);
+    n = 0;
+  }
+  need = pages_of(len + n, a.lp) - pages_of(len, a.lp);
+}
+
+// THREADS: 64 (the requests fit a wave), 256, 1024 (any number of requests)
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) pages_extend_kernel(PagesArgs a, int alone) {
+  __shared__ Scan<THREADS> s;
   __shared__ int s_bad;
+  __shared__ int s_cu[THREADS], s_len[THREADS], s_new[THREADS];
   const int tid = threadIdx.x;
+  const bool once = a.B <= THREADS;
   if (tid == 0) s_bad = 0;
-  __syncthreads();
   const int nfree = min(max(*a.nfree, 0), a.NP);
+  __syncthreads();
   // what all requests need
-  long tokens = 0, pages = 0;
-  for (int i0 = 0; i0 < a.B; i0 += kThreads) {
+  unsigned tokens = 0, pages = 0, e0 = 0, e1 = 0;
+  int len = 0, n = 0, need = 0;
+  for (int i0 = 0; i0 < a.B; i0 += THREADS) {
     const int i = i0 + tid;
-    long n = 0, need = 0;
-    if (i < a.B) {
-      n = a.count[i];
-      const long len = held_len(a, i);
-      if (n < 0 || len != a.lens[i] || len + n > (long)a.width << a.lp) {
-        atomicOr(&s_bad, 1);
-        n = 0;
-      }
-      need = pages_of(len + n, a.lp) - pages_of(len, a.lp);
-    }
-    long e0, e1, t0, t1;
-    block_scan(s, n, need, e0, e1, t0, t1);
-    tokens += t0;
-    pages += t1;
+    len = n = need = 0;
+    if (i < a.B) wanted(a, i, len, n, need, &s_bad);
+    unsigned t0, t1;
+    e0 = n;
+    e1 = need;
+    block_scan<THREADS>(s, e0, e1, t0, t1);
+    tokens = add_to(tokens, t0);
+    pages = add_to(pages, t1);
   }
   __syncthreads();
-  const int bad = s_bad | (pages > nfree ? 2 : 0) | (tokens > a.total ? 4 : 0);
+  const int bad = s_bad | (pages > (unsigned)nfree ? 2 : 0) | (tokens > (unsigned)a.total ? 4 : 0);
   if (bad && tid == 0) *a.status |= bad;
-  // starts, lengths
-  long tok0 = 0, page0 = 0;
-  for (int i0 = 0; i0 < a.B; i0 += kThreads) {
+  // starts, lengths (sums that a refused call may have cut short are not used)
+  unsigned tok0 = 0, page0 = 0;
+  for (int i0 = 0; i0 < a.B; i0 += THREADS) {
     const int i = i0 + tid;
-    long n = 0, need = 0, len = 0;
-    if (i < a.B && !bad) {
-      n = a.count[i];
-      len = a.lens[i];
-      need = pages_of(len + n, a.lp) - pages_of(len, a.lp);
+    unsigned t0 = tokens, t1 = pages;
+    if (!once) {
+      len = n = need = 0;
+      if (i < a.B && !bad) wanted(a, i, len, n, need, &s_bad);
+      e0 = n;
+      e1 = need;
+      block_scan<THREADS>(s, e0, e1, t0, t1);
     }
-    long e0, e1, t0, t1;
-    block_scan(s, n, need, e0, e1, t0, t1);
     if (i < a.B) {
-      a.cu[i + 1] = (int)(tok0 + e0 + n);
+      const int end = bad ? 0 : (int)(tok0 + e0), at = bad ? 0 : end - n, page = (int)(page0 + e1) - need;
+      a.cu[i + 1] = end;
       if (i == 0) a.cu[0] = 0;
-      a.ws[i] = (int)len;
-      a.ws[a.B + i] = (int)(page0 + e1);
-      if (!bad) a.lens[i] = (int)(len + n);
+      if (once) {
+        s_cu[tid] = at;
+        s_len[tid] = len;
+        s_new[tid] = page;
+      }
+      if (!once || !alone) {
+        a.ws[i] = len;
+        a.ws[a.B + i] = page;
+      }
+      if (!bad) a.lens[i] = len + n;
     }
     tok0 += t0;
     page0 += t1;
   }
   if (tid == 0) {
     a.ws[2 * a.B] = nfree;
-    if (!bad) *a.nfree = nfree - (int)page0;
+    if (!bad) *a.nfree = nfree - (int)pages;
   }
   if (!alone) return;
-  __syncthreads();                       // (starts and lengths of the whole workgroup, through memory)
-  for (int t = tid; t < a.total; t += kThreads) {
-    if (t < tok0) fill_token(a, t, nfree);
-    else a.slots[t] = a.pos[t] = -1;
+  __syncthreads();                       // (starts and lengths of the whole workgroup)
+  for (int t = tid; t < a.total; t += THREADS) {
+    if (bad || t >= (int)tokens) a.slots[t] = a.pos[t] = -1;
+    else if (once) fill_token(a, s_cu, s_len, s_new, t, nfree);
+    else fill_token(a, a.cu, a.ws, a.ws + a.B, t, nfree);
   }
 }
 
 __global__ void __launch_bounds__(kFill) pages_fill_kernel(PagesArgs a) {
-  const int t = blockIdx.x * kFill + threadIdx.x;
+  __shared__ int s_cu[kStarts];
+  const int t = blockIdx.x * kFill + threadIdx.x, end = a.cu[a.B], nfree = a.ws[2 * a.B];
+  const bool near = a.B <= kStarts;
+  if (near) {
+    for (int i = threadIdx.x; i < a.B; i += kFill) s_cu[i] = a.cu[i];
+    __syncthreads();
+  }
   if (t >= a.total) return;
-  if (t < a.cu[a.B]) fill_token(a, t, a.ws[2 * a.B]);
-  else a.slots[t] = a.pos[t] = -1;
+  if (t >= end) a.slots[t] = a.pos[t] = -1;
+  else if (near) fill_token(a, s_cu, a.ws, a.ws + a.B, t, nfree);
+  else fill_token(a, a.cu, a.ws, a.ws + a.B, t, nfree);
 }
 
-// the returned pages of request i, by the lanes of one wave
-__device__ __forceinline__ void give_back(const PagesArgs& a, int i, long left, long held, long first, int top, int lane) {
-  int* row = a.table + (long)i * a.t_st;
-  for (long c = left + lane; c < held; c += 64) {
-    a.free[top - 1 - (first + c - left)] = row[c];
+// the returned pages of a request, by the lanes of one wave
+__device__ __forceinline__ void give_back(const PagesArgs& a, int i, int left, int gone, int first, int top, int lane) {
+  int* row = a.table + (long)i * a.t_st + left;
+  for (int c = lane; c < gone; c += 64) {
+    a.free[top - 1 - (first + c)] = row[c];
     row[c] = -1;
   }
 }
 
-__global__ void __launch_bounds__(kThreads) pages_truncate_kernel(PagesArgs a, int alone) {
-  __shared__ Scan s;
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) pages_truncate_kernel(PagesArgs a, int alone) {
+  __shared__ Scan<THREADS> s;
+  __shared__ int s_left[THREADS], s_gone[THREADS], s_first[THREADS];
   const int tid = threadIdx.x;
+  const bool once = a.B <= THREADS;
   const int nfree = min(max(*a.nfree, 0), a.NP);
-  long pages = 0;
-  for (int i0 = 0; i0 < a.B; i0 += kThreads) {
-    const int i = i0 + tid;
-    long gone = 0, e0, e1, t0, t1;
+  unsigned pages = 0, e0 = 0, e1 = 0, t1;
+  int gone = 0, keep = 0;
+  auto returned = [&](int i) {
+    gone = keep = 0;
     if (i < a.B) {
-      const long len = held_len(a, i), keep = a.count[i] < 0 ? len : min((long)a.count[i], len);
+      const int len = held_len(a, i), k = a.count[i];
+      keep = k < 0 ? len : min(k, len);
       gone = pages_of(len, a.lp) - pages_of(keep, a.lp);
     }
-    block_scan(s, gone, 0, e0, e1, t0, t1);
-    pages += t0;
+  };
+  for (int i0 = 0; i0 < a.B; i0 += THREADS) {
+    unsigned t0;
+    returned(i0 + tid);
+    e0 = gone;
+    e1 = 0;
+    block_scan<THREADS>(s, e0, e1, t0, t1);
+    pages = add_to(pages, t0);
   }
-  const bool bad = nfree + pages > a.NP;
-  if (bad && tid == 0) *a.status |= 2;
-  long page0 = 0;
-  for (int i0 = 0; i0 < a.B; i0 += kThreads) {
+  const bool bad = pages > (unsigned)(a.NP - nfree);
+  const int top = nfree + (bad ? 0 : (int)pages);
+  unsigned page0 = 0;
+  for (int i0 = 0; i0 < a.B; i0 += THREADS) {
     const int i = i0 + tid;
-    long gone = 0, len = 0, keep = 0, e0, e1, t0, t1;
-    if (i < a.B) {
-      len = held_len(a, i);
-      keep = bad || a.count[i] < 0 ? len : min((long)a.count[i], len);
-      gone = pages_of(len, a.lp) - pages_of(keep, a.lp);
+    unsigned t0 = pages;
+    if (!once) {
+      returned(i);
+      e0 = gone;
+      e1 = 0;
+      block_scan<THREADS>(s, e0, e1, t0, t1);
     }
-    block_scan(s, gone, 0, e0, e1, t0, t1);
     if (i < a.B) {
-      a.ws[i] = (int)pages_of(keep, a.lp);
-      a.ws[a.B + i] = (int)(page0 + e0);
-      a.ws[2 * a.B + 1 + i] = (int)gone;
-      if (!bad) a.lens[i] = (int)keep;
+      const int left = pages_of(keep, a.lp), first = (int)(page0 + e0) - gone, g = bad ? 0 : gone;
+      if (alone) {                       // (then all requests have a thread)
+        s_left[tid] = left;
+        s_gone[tid] = g;
+        s_first[tid] = first;
+      } else {
+        a.ws[i] = left;
+        a.ws[a.B + i] = first;
+        a.ws[2 * a.B + 1 + i] = g;
+      }
+      if (!bad) a.lens[i] = keep;
     }
-    page0 += t0;
+    page0 = add_to(page0, t0);
   }
   if (tid == 0) {
-    a.ws[2 * a.B] = nfree + (int)page0;
-    if (!bad) *a.nfree = nfree + (int)page0;
+    a.ws[2 * a.B] = top;
+    if (bad) *a.status |= 2;
+    else *a.nfree = top;
   }
   if (!alone) return;
   __syncthreads();
-  for (int i = tid >> 6; i < a.B; i += kWaves)
-    give_back(a, i, a.ws[i], (long)a.ws[i] + a.ws[2 * a.B + 1 + i], a.ws[a.B + i], nfree + (int)page0, tid & 63);
+  for (int i = tid >> 6; i < a.B; i += THREADS / 64) give_back(a, i, s_left[i], s_gone[i], s_first[i], top, tid & 63);
 }
 
 __global__ void __launch_bounds__(kFill) pages_back_kernel(PagesArgs a) {
   const int i = blockIdx.x * (kFill / 64) + (threadIdx.x >> 6);
   if (i >= a.B) return;
-  give_back(a, i, a.ws[i], (long)a.ws[i] + a.ws[2 * a.B + 1 + i], a.ws[a.B + i], a.ws[2 * a.B], threadIdx.x & 63);
+  give_back(a, i, a.ws[i], a.ws[2 * a.B + 1 + i], a.ws[a.B + i], a.ws[2 * a.B], threadIdx.x & 63);
 }
 
-// requests up to which the planning workgroup moves the returned pages itself
+// requests up to which the planning workgroup moves the returned pages itself (at most its threads)
 constexpr int kAloneRows = 256;
 
 int take(PagesArgs& a, const int* count, int* lens, int* table, long t_st, int* free, int* nfree, int* status, int B,
@@ -250,7 +308,9 @@ extern "C" int oa_kv_pages_extend(const int* add, int* lens, int* table, long ta
   a.total = total; a.slots = slots; a.pos = pos; a.cu = cu;
   const hipStream_t st = (hipStream_t)stream;
   const int alone = total <= kAlone;
-  hipLaunchKernelGGL(pages_extend_kernel, dim3(1), dim3(kThreads), 0, st, a, alone);
+  if (requests <= 64 && total <= 256) hipLaunchKernelGGL(pages_extend_kernel<64>, dim3(1), dim3(64), 0, st, a, alone);
+  else if (requests <= 256 && total <= 512) hipLaunchKernelGGL(pages_extend_kernel<256>, dim3(1), dim3(256), 0, st, a, alone);
+  else hipLaunchKernelGGL(pages_extend_kernel<kMost>, dim3(1), dim3(kMost), 0, st, a, alone);
   if (!alone) hipLaunchKernelGGL(pages_fill_kernel, dim3((total + kFill - 1) / kFill), dim3(kFill), 0, st, a);
   return OA_LAUNCH_STATUS();
 }
@@ -261,7 +321,9 @@ extern "C" int oa_kv_pages_truncate(const int* keep, int* lens, int* table, long
   if (const int e = take(a, keep, lens, table, table_stride, free, nfree, status, requests, width, pages, page, ws)) return e;
   const hipStream_t st = (hipStream_t)stream;
   const int alone = requests <= kAloneRows;
-  hipLaunchKernelGGL(pages_truncate_kernel, dim3(1), dim3(kThreads), 0, st, a, alone);
+  if (requests <= 16) hipLaunchKernelGGL(pages_truncate_kernel<64>, dim3(1), dim3(64), 0, st, a, alone);
+  else if (requests <= 64) hipLaunchKernelGGL(pages_truncate_kernel<256>, dim3(1), dim3(256), 0, st, a, alone);
+  else hipLaunchKernelGGL(pages_truncate_kernel<kMost>, dim3(1), dim3(kMost), 0, st, a, alone);
   if (!alone)
     hipLaunchKernelGGL(pages_back_kernel, dim3((requests + kFill / 64 - 1) / (kFill / 64)), dim3(kFill), 0, st, a);
   return OA_LAUNCH_STATUS();

@@ -124,7 +124,7 @@ def load() -> ct.CDLL:
 
 def call(name: str, *args) -> None:
     """Call one C entry point; a nonzero status raises RuntimeError with the HIP error text."""
-    lib = load()
+    lib = _LIB or load()
     st = getattr(lib, name)(*args)
     if st != 0:
         msg = lib.oa_error_string(st).decode()

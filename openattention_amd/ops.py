@@ -668,13 +668,14 @@ def prefill_attn(q, k, v, sm_scale: float) -> torch.Tensor:
 _DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 KV4_BLOCK = 32             # values that share a scale
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_get_device = torch._C._cuda_getDevice
 
 
 def _where(*ts) -> int:
     """The index of the device that all these tensors are on."""
     i = ts[0].get_device()
     for t in ts:
-        if t is not None and (t.get_device() != i or i < 0):
+        if t is not None and t.get_device() != i or i < 0:
             _dev(*ts)
             raise RuntimeError(f"tensors on different devices: {[u.device for u in ts if u is not None]}")
     return i
@@ -682,7 +683,7 @@ def _where(*ts) -> int:
 
 def _run(i: int, name: str, *args) -> None:
     """lib.call on device i's current stream, with i the current device for the launch."""
-    if i == torch.cuda.current_device():
+    if i == _get_device():
         lib.call(name, *args, _raw_stream(i))
     else:
         with torch.cuda.device(i):
@@ -694,10 +695,12 @@ def _plain(*ts) -> None:
     operators have no backward pass, and would cut a graph in silence."""
     grad = torch.is_grad_enabled()
     for t in ts:
-        if t is not None and (grad and t.requires_grad or t.is_neg()):
-            raise ValueError("a lazily negated view (call resolve_neg())" if t.is_neg() else
-                             "a tensor requires a gradient, and this operator has no backward pass (call it under "
-                             "torch.no_grad())")
+        if t is not None:
+            if grad and t.requires_grad:
+                raise ValueError("a tensor requires a gradient, and this operator has no backward pass (call it under "
+                                 "torch.no_grad())")
+            if t.is_neg():
+                raise ValueError("a lazily negated view (call resolve_neg())")
 
 
 def _rows(t: torch.Tensor, T: int, H: int, Dh: int, name: str, out: bool = False) -> tuple:

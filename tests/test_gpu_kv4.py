@@ -115,8 +115,8 @@ def same(pool, lens, table, free, nfree, status):
     assert free.tolist() == pool.free and int(status) == pool.status
 
 
-@pytest.mark.parametrize("B,width,page,most", [(1, 4, 32, 40), (5, 9, 64, 100), (64, 12, 32, 60), (300, 5, 128, 30),
-                                               (1500, 6, 32, 9)])
+@pytest.mark.parametrize("B,width,page,most", [(1, 4, 32, 40), (5, 9, 64, 100), (64, 12, 32, 60), (300, 5, 128, 30), (40, 6, 32, 4), (200, 6, 64, 3),
+                                               (1500, 6, 32, 9), (1500, 6, 32, 1), (4500, 4, 32, 3)])
 def test_pages_follow_the_pool(B, width, page, most):
     print(f"[case] pages {B} {width} {page} {most}", flush=True)
     lens, table, free, spare = pool_state(B, B, width, page, 4 * B)
