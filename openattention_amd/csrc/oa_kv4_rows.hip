@@ -1,0 +1,309 @@
+// Causal attention over the 4-bit paged cache for many query rows of a KV head (a question, a piece of a
+// prompt): the same sums as in oa_kv4_attn.hip, with the keys' codes turned to bf16 once for 128 rows.
+//
+// One workgroup of four waves takes 128 query rows of a KV head, 32 to a wave, and a chunk of keys.  Of a tile of
+// 32 keys, waves 0 and 1 turn K to bf16 and waves 2 and 3 V, a block of 32 values to a lane, into LDS tiles
+// that all four read.  Products are v_mfma_f32_32x32x16_bf16: S^T = K Q^T, whose lanes hold 16 keys' scores of
+// one row, and O^T = V^T P^T twice, for the weights' two bf16 terms, with V^T by the LDS transpose reads
+// (the contraction takes keys in the order the scores left them).
+// The loop is a pipeline: iteration i issues the products of S(i + 1) and of O += V(i - 1) P(i - 1) between
+// the steps of the softmax of S(i), puts K(i + 2) and V(i) into LDS and requests the codes after them.
+// Tiles: rows of 2 D bytes whose 16-byte chunks c lie at c ^ f(row), so that 16 rows read at one chunk (K) and
+// the transpose reads (V) spread over all banks.
+#include "oa_kv4_attn.h"
+
+namespace {
+
+using namespace kv4;
+
+typedef float float16v __attribute__((ext_vector_type(16)));
+
+constexpr int kWaveRows = 32;
+constexpr int kRows = kWaves * kWaveRows;
+constexpr int kAhead = 2;                // steps whose LDS operands are requested ahead
+
+__device__ __forceinline__ float16v mfma(bf16x8 a, bf16x8 b, float16v c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+struct Weights {                         // P^T of a 32-key tile, 16 keys per operand, in two terms
+  uint4v hi[2], lo[2];
+};
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
+  constexpr int kSteps = D / 16;         // products of a score tile, and of a value tile for each term
+  constexpr int kDims = D / 32;          // tiles of 32 dims
+  constexpr int kRowB = D * 2, kTileB = kTile * kRowB;
+  constexpr int kWords = D / 32;         // words of codes that a staging lane turns to bf16
+  __shared__ __align__(16) char s_t[4 * kTileB];          // K even, K odd, V even, V odd tiles
+  __shared__ unsigned long s_nan[2][2];                    // NaN blocks of a masked V tile, by parity and half
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n32 = lane & 31, h = lane >> 5;
+  const int units = a.B * a.HKV;
+  const int bh = blockIdx.x % units, rest = blockIdx.x / units;
+  const int ch = rest / a.ntile, row0 = (rest - ch * a.ntile) * kRows;
+  const int b = bh / a.HKV, head = bh - b * a.HKV;
+  const Seq sq = seq_of(a, b);
+  const int rows = min(sq.R, a.max_q) * a.G;
+  if (row0 >= rows) return;
+  const int first = sq.n - sq.R;         // position of the sequence's first query token
+  const int hi = sq.bad ? 0 : first + (min(row0 + kRows, rows) - 1) / a.G + 1;         // keys any row sees
+  const int all = first + row0 / a.G + 1;                                              // keys every row sees
+  const int k0 = ch * a.chunk, k1 = min(k0 + a.chunk, hi);
+  if (k0 >= k1 && a.nchunk > 1) return;
+  const int n = max(0, (k1 - k0 + kTile - 1) / kTile);     // tiles
+  const int nfull = min(n, max(0, (all - k0) / kTile));    // those that every row sees whole
+
+  char* const s_k = s_t;
+  char* const s_v = s_t + 2 * kTileB;
+  auto fsw = [](int r) { return D == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : ((r >> 1) & 1) << 2 | ((r >> 2) & 3); };
+
+  // staging: lanes 0..127 of the workgroup K, the others V; key lane / 4 of the tile, a quarter of its dims
+  const bool isv = wave >= 2;
+  const int skey = (tid & 127) >> 2, sg = tid & 3;
+  const int* trow = a.table + (long)b * a.t_st;
+  const int pmask = (1 << a.lp) - 1;
+  const uint8_t* const cbase = (isv ? a.vc : a.kc) + ((long)head << a.lp) * (D / 2);
+  const uint8_t* const sbase = (isv ? a.vs : a.ks) + ((long)head << a.lp) * (D / 32);
+  const unsigned oc = skey * (D / 2) + sg * (D / 8), os = skey * (D / 32) + sg * D / 128;
+  unsigned cw[kWords], sw = 0, sbad = 0;
+  auto page_at = [&](int tile) { return trow[min((k0 + tile * kTile) >> a.lp, a.width - 1)]; };
+  auto fetch = [&](int tile, int page) {                   // (past the last tile: read, never used)
+    const bool bad = (unsigned)page >= (unsigned)a.NP;
+    sbad = bad && !isv ? 0x7f800000u : 0u;
+    const long pg = bad ? 0 : page, off = (k0 + tile * kTile) & pmask;
+    const uint8_t* p = cbase + pg * a.c_sp + off * (D / 2) + oc;
+    typedef unsigned vec __attribute__((ext_vector_type(kWords)));
+    const vec x = *reinterpret_cast<const vec*>(p);
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) cw[i] = x[i];
+    sw = (sbase + pg * a.s_sp + off * (D / 32))[os];
+  };
+  const int sdst = skey * kRowB, sf = fsw(skey);
+  // values of keys past the last one any row sees count as zeros (their weights are 0, but what lies there may
+  // be anything), and so do NaN blocks of a masked tile, which s_nan remembers
+  auto put = [&](int tile, int parity) {
+    unsigned e = sw;
+    if (isv && tile >= nfull) {
+      const bool nan = e == 255 && k0 + tile * kTile + skey < hi;
+      const unsigned long at = __ballot(nan);
+      if (lane == 0) s_nan[parity][wave & 1] = at;
+      if (nan || k0 + tile * kTile + skey >= hi) e = 0;
+    }
+    const float f = __uint_as_float(e << 23 | sbad);
+    char* const t = (isv ? s_v : s_k) + parity * kTileB + sdst;
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) *reinterpret_cast<bf16x8*>(t + (((sg * kWords + i) ^ sf) << 4)) = from4(cw[i], f);
+  };
+
+  // operand addresses (bytes in a tile)
+  const int kad = n32 * kRowB + ((h ^ fsw(n32)) << 4);                     // ^ (step << 5)
+  const int lr = (lane & 15) >> 2, lc = lane & 3, dsub = (lane >> 4) & 1;
+  const int vad = (4 * h + lr) * kRowB + (((dsub * 2 + (lc >> 1)) ^ fsw(4 * h + lr)) << 4) + ((lc & 1) << 3);
+  auto key_op = [&](const char* tile, int step) { return *reinterpret_cast<const bf16x8*>(tile + (kad ^ (step << 5))); };
+  // V^T of dims 32 db .. and keys 16 kk ..: two transposed reads of 4 keys, 8 apart
+  auto val_op = [&](char* tile, int db, int kk) {
+    const int ad = vad ^ (db << 6);
+    const short4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v*)(tile + ad + kk * 16 * kRowB));
+    const short4v y =
+        __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v*)(tile + (ad ^ 32) + kk * 16 * kRowB + 8 * kRowB));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+
+  // this lane's row (negated under a negative scale: the maximum is taken before scaling) and how many keys it
+  // sees (0: no such row)
+  const float c = fabsf(a.c);
+  const int r = row0 + wave * kWaveRows + n32;
+  const int rr = min(r, rows - 1), j = rr / a.G, hd = head * a.G + rr - j * a.G;
+  const int lim = r < rows ? first + j + 1 : 0;
+  bf16x8 Q[kSteps];
+  {
+    const unsigned flip = a.c < 0.f ? 0x80008000u : 0u;
+    const uint16_t* p = a.q + (long)(sq.r0 + j) * a.q_st + (long)hd * a.q_sh + 8 * h;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+      Q[s] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4v*>(p + 16 * s) ^ uint4v(flip));
+  }
+
+  float16v O[kDims], S0 = float16v(0.f), S1;
+  Weights P0, P1;
+#pragma unroll
+  for (int d = 0; d < kDims; ++d) O[d] = float16v(0.f);
+  float m = -FLT_MAX, l = 0.f;           // running maximum, scaled, and sum of the lane's keys
+  bool big = false;                      // a maximum is past 2^24 (uniform)
+
+  if (n > 0) {
+    // K(0), K(1) and zeros for V(-1), whose weights are 0; then K(2) and V(0) requested
+    const int lead = isv ? 0 : 2;        // tiles that this lane's staging is ahead of the loop
+    if (!isv) {
+      fetch(0, page_at(0));
+      put(0, 0);
+      fetch(1, page_at(1));
+      put(1, 1);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) *reinterpret_cast<uint4v*>(s_v + kTileB + sdst + ((sg * kWords + i) << 4)) = uint4v(0u);
+    }
+    P1.hi[0] = P1.hi[1] = P1.lo[0] = P1.lo[1] = uint4v(0u);
+    fetch(lead, page_at(lead));
+    int page = page_at(lead + 1);
+    oa::lds_barrier();
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) S0 = mfma(key_op(s_k, s), Q[s], S0);
+    oa::lds_barrier();                   // K(0) has been read: its place takes K(2)
+
+    // O += V(tile) P(tile)'s NaN blocks, into the rows that see them (rare)
+    auto nan_blocks = [&](int tile, int parity) {
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
+        unsigned long at = s_nan[parity][half];
+        while (at) {
+          const int bit = __builtin_ctzl(at), key = k0 + tile * kTile + 16 * half + (bit >> 2), blk = (bit & 3) * D / 128;
+          at &= at - 1;
+#pragma unroll
+          for (int d = 0; d < kDims; ++d)
+            if (d == blk && key < lim) O[d] = float16v(__builtin_nanf(""));
+        }
+      }
+    };
+    // iteration i (parity odd = i & 1): K(i + 1), V(i - 1) are in the other parity's tiles
+    auto body = [&](auto mask_c, auto odd_c, int i, float16v& S, float16v& Sn, const Weights& Pp, Weights& Pn) {
+      constexpr bool MASK = decltype(mask_c)::value;
+      constexpr int kOdd = decltype(odd_c)::value;
+      char* const kt = s_k + (1 - kOdd) * kTileB;
+      char* const vt = s_v + (1 - kOdd) * kTileB;
+      put(i + lead, kOdd);
+      fetch(i + lead + 1, page);
+      page = page_at(i + lead + 2);
+      float mx = -INFINITY, alpha = 1.f, p0 = 0.f;
+      bool moved = false;
+      Sn = float16v(0.f);
+      bf16x8 kop[kSteps], vop[kSteps];
+#pragma unroll
+      for (int s = 0; s < kAhead; ++s) {
+        kop[s] = key_op(kt, s);
+        vop[s] = val_op(vt, s >> 1, s & 1);
+      }
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        if (s + kAhead < kSteps) {
+          kop[s + kAhead] = key_op(kt, s + kAhead);
+          vop[s + kAhead] = val_op(vt, (s + kAhead) >> 1, (s + kAhead) & 1);
+        }
+        Sn = mfma(kop[s], Q[s], Sn);
+        O[s >> 1] = mfma(vop[s], __builtin_bit_cast(bf16x8, Pp.hi[s & 1]), O[s >> 1]);
+        O[s >> 1] = mfma(vop[s], __builtin_bit_cast(bf16x8, Pp.lo[s & 1]), O[s >> 1]);
+        if (s == 0) {                    // the tile's maximum
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            if (MASK) S[r] = k0 + i * kTile + 8 * (r >> 2) + 4 * h + (r & 3) < lim ? S[r] * c : -INFINITY;
+            mx = fmaxf(mx, S[r]);
+          }
+        } else if (s == 1) {
+          const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+          mx = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * (MASK ? 1.f : c);
+          moved = __any(mx > m);
+          if (moved) {
+            const float mn = fmaxf(m, mx);
+            alpha = __builtin_amdgcn_exp2f(m - mn);
+            l *= alpha;
+            m = mn;
+            // (as in oa_kv4_attn.hip: past 2^24 the product is rounded before the maximum is taken off)
+            big = __any(fabsf(m) >= 16777216.f);
+          }
+          if (!MASK && big) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) S[r] *= c;
+          }
+        } else {
+#pragma unroll
+          for (int r = (s - 2) * 16 / (kSteps - 2); r < (s - 1) * 16 / (kSteps - 2); ++r) {
+            const float p1 = __builtin_amdgcn_exp2f(MASK ? S[r] - m : fmaf(S[r], big ? 1.f : c, -m));
+            l += p1;
+            if (r & 1) {
+              const uint32_t u = pack2(p0, p1);
+              uint32_t w = pack2(p0 - __uint_as_float(u << 16), p1 - __uint_as_float(u & 0xffff0000u));
+              asm volatile("" : "+v"(w));          // (pinned here: left alone they all sink below the products)
+              Pn.hi[r >> 3][(r & 7) >> 1] = u;
+              Pn.lo[r >> 3][(r & 7) >> 1] = w;
+            }
+            p0 = p1;
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (MASK && i > nfull) nan_blocks(i - 1, 1 - kOdd);
+      if (moved) {                       // (after O += V(i - 1) P(i - 1), whose weights had the old maximum)
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) O[d] *= alpha;
+      }
+      oa::lds_barrier();
+    };
+    typedef std::integral_constant<int, 0> even_t;
+    typedef std::integral_constant<int, 1> odd_t;
+    typedef std::integral_constant<bool, false> whole;
+    typedef std::integral_constant<bool, true> masked;
+    auto finish = [&](int parity, const Weights& P) {        // V(n - 1) P(n - 1)
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const bf16x8 vop = val_op(s_v + parity * kTileB, s >> 1, s & 1);
+        O[s >> 1] = mfma(vop, __builtin_bit_cast(bf16x8, P.hi[s & 1]), O[s >> 1]);
+        O[s >> 1] = mfma(vop, __builtin_bit_cast(bf16x8, P.lo[s & 1]), O[s >> 1]);
+      }
+      if (n > nfull) nan_blocks(n - 1, parity);
+    };
+    int i = 0;
+#pragma unroll 1
+    for (; i + 2 <= nfull; i += 2) {
+      body(whole(), even_t(), i, S0, S1, P1, P0);
+      body(whole(), odd_t(), i + 1, S1, S0, P0, P1);
+    }
+#pragma unroll 1
+    for (; i < n; i += 2) {              // (a tile or two more than need it run masked, which changes nothing)
+      body(masked(), even_t(), i, S0, S1, P1, P0);
+      if (i + 1 < n) body(masked(), odd_t(), i + 1, S1, S0, P0, P1);
+    }
+    if (n & 1) finish(0, P0);
+    else finish(1, P1);
+  }
+
+  const auto lx = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+  const float L = __uint_as_float(lx[0]) + __uint_as_float(lx[1]);
+  if (r >= rows) return;
+  if (a.nchunk == 1) {
+    const float inv = 1.f / L;
+    const bool none = lim <= 0;
+    uint16_t* o = a.out + (long)(sq.r0 + j) * a.o_st + (long)hd * a.o_sh + 4 * h;
+#pragma unroll
+    for (int d = 0; d < kDims; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        f32x4 x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = sq.bad ? __builtin_nanf("") : none ? 0.f : O[d][4 * g + e] * inv;
+        *reinterpret_cast<uint2v*>(o + 32 * d + 8 * g) = uint2v{pack2(x[0], x[1]), pack2(x[2], x[3])};
+      }
+  } else {
+    const long at = ((long)(sq.r0 + j) * (a.HKV * a.G) + hd) * a.nchunk + ch;
+#pragma unroll
+    for (int d = 0; d < kDims; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(a.ws_o + at * D + 32 * d + 8 * g + 4 * h) =
+            f32x4{O[d][4 * g], O[d][4 * g + 1], O[d][4 * g + 2], O[d][4 * g + 3]};
+    if (h == 0) *reinterpret_cast<f32x2*>(a.ws_ml + at * 2) = f32x2{m, L};
+  }
+}
+
+}  // namespace
+
+namespace kv4 {
+
+void launch_rows(const AttnArgs& a, int head_dim, dim3 grid, hipStream_t st) {
+  if (head_dim == 64) hipLaunchKernelGGL(kv4_rows_kernel<64>, grid, dim3(kThreads), 0, st, a);
+  else hipLaunchKernelGGL(kv4_rows_kernel<128>, grid, dim3(kThreads), 0, st, a);
+}
+
+}  // namespace kv4

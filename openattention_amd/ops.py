@@ -929,7 +929,7 @@ def kv4_attn(q, kc, ks, vc, vs, table, lens, sm_scale: float | None = None, cu_q
         return out
     rows = max_q * G
     cap = max(1, width * where[3] if max_len is None else min(max_len, width * where[3]))
-    chunk = kv4_chunk(cap, B * HKV * -(-rows // (8 if rows <= 8 else 16 if rows <= 16 else 32)))
+    chunk = kv4_chunk(cap, B * HKV * -(-rows // (8 if rows <= 8 else 16 if rows <= 16 else 32 if rows <= 64 else 128)))
     nchunk = -(-cap // chunk)
     wp = mp = None
     if nchunk > 1:
