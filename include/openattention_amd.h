@@ -608,13 +608,14 @@ int oa_kv4_read(const int* slots, const void* kc, const void* ks, const void* vc
  * of a sequence from max_q on, are left as they were.  NaN: rows that need a page id outside of the cache, and
  * those of sequences longer than their table row or than nchunk * chunk keys.  Keys are split into nchunk pieces
  * of `chunk` (a multiple of 128); with more than one, ws_o (tokens * q_heads * nchunk * head_dim) and ws_ml (* 2)
- * floats hold the pieces' sums.
+ * floats hold the pieces' sums; with more than 64 rows of a KV head (max_q * q_heads / kv_heads), ws_flag holds
+ * sequences * kv_heads * nchunk * ceil(rows / 128) ints.
  */
 int oa_kv4_attn(const void* q, long q_st, long q_sh, const void* kc, const void* ks, const void* vc, const void* vs,
                 long code_stride, long scale_stride, int pages, int page, const int* table, long table_stride, int width,
                 const int* lens, const int* cu, int sequences, int tokens, int max_q, int q_heads, int kv_heads,
-                int head_dim, float sm_scale, int chunk, int nchunk, float* ws_o, float* ws_ml, void* out, long o_st,
-                long o_sh, void* stream);
+                int head_dim, float sm_scale, int chunk, int nchunk, float* ws_o, float* ws_ml, int* ws_flag, void* out,
+                long o_st, long o_sh, void* stream);
 
 #ifdef __cplusplus
 }

@@ -30,6 +30,7 @@ struct AttnArgs {
   const int* lens; const int* cu;
   uint16_t* out; long o_st, o_sh;
   float* ws_o; float* ws_ml;             // partial sums, (maximum, sum) by (row, chunk)
+  int* ws_flag;                          // by workgroup of oa_kv4_rows.hip
   int B, HKV, G, tokens, max_q, width, NP, lp, chunk, nchunk, ntile;
   float c;                               // scale * log2 e
 };

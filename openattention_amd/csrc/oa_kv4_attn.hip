@@ -408,7 +408,7 @@ extern "C" int oa_kv4_attn(const void* q, long q_st, long q_sh, const void* kc, 
                            const void* vs, long code_stride, long scale_stride, int pages, int page, const int* table,
                            long table_stride, int width, const int* lens, const int* cu, int sequences, int tokens,
                            int max_q, int q_heads, int kv_heads, int head_dim, float sm_scale, int chunk, int nchunk,
-                           float* ws_o, float* ws_ml, void* out, long o_st, long o_sh, void* stream) {
+                           float* ws_o, float* ws_ml, int* ws_flag, void* out, long o_st, long o_sh, void* stream) {
   auto odd = [](const void* p, uintptr_t n) { return !p || (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0; };
   if ((head_dim != 64 && head_dim != 128) || sequences < 0 || tokens < 0 || max_q <= 0 || kv_heads <= 0 || q_heads <= 0 ||
       q_heads % kv_heads || (long)max_q * (q_heads / kv_heads) > (1L << 30) || pages <= 0 || page < 32 || page > 1024 ||
@@ -421,14 +421,15 @@ extern "C" int oa_kv4_attn(const void* q, long q_st, long q_sh, const void* kc, 
       odd(vs, 16) || !table || !lens || code_stride < (long)kv_heads * page * (head_dim / 2) ||
       scale_stride < (long)kv_heads * page * (head_dim / 32) || code_stride % 16 || scale_stride % 16 || !(sm_scale == sm_scale))
     return OA_EINVAL;
-  if (nchunk > 1 && (odd(ws_o, 16) || odd(ws_ml, 8))) return OA_EINVAL;
+  if ((nchunk > 1 && (odd(ws_o, 16) || odd(ws_ml, 8))) || ((long)max_q * (q_heads / kv_heads) > kFewRows && odd(ws_flag, 4)))
+    return OA_EINVAL;
   AttnArgs a;
   a.q = (const uint16_t*)q; a.q_st = q_st; a.q_sh = q_sh;
   a.kc = (const uint8_t*)kc; a.ks = (const uint8_t*)ks; a.vc = (const uint8_t*)vc; a.vs = (const uint8_t*)vs;
   a.c_sp = code_stride; a.s_sp = scale_stride;
   a.table = table; a.t_st = table_stride; a.lens = lens; a.cu = cu;
   a.out = (uint16_t*)out; a.o_st = o_st; a.o_sh = o_sh;
-  a.ws_o = ws_o; a.ws_ml = ws_ml;
+  a.ws_o = ws_o; a.ws_ml = ws_ml; a.ws_flag = ws_flag;
   a.B = sequences; a.HKV = kv_heads; a.G = q_heads / kv_heads; a.tokens = tokens; a.max_q = max_q;
   a.width = width; a.NP = pages; a.lp = __builtin_ctz(page); a.chunk = chunk; a.nchunk = nchunk;
   a.c = sm_scale * kLog2e;

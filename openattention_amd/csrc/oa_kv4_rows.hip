@@ -4,12 +4,18 @@
 // One workgroup of four waves takes 128 query rows of a KV head, 32 to a wave, and a chunk of keys.  Of a tile of
 // 32 keys, waves 0 and 1 turn K to bf16 and waves 2 and 3 V, a block of 32 values to a lane, into LDS tiles
 // that all four read.  Products are v_mfma_f32_32x32x16_bf16: S^T = K Q^T, whose lanes hold 16 keys' scores of
-// one row, and O^T = V^T P^T twice, for the weights' two bf16 terms, with V^T by the LDS transpose reads
-// (the contraction takes keys in the order the scores left them).
+// one row, and O^T = V^T P^T with V^T by the LDS transpose reads (the contraction takes keys in the order the
+// scores left them).
+// Weights and values go into the second product in fp16: weights times 2^15 (11 bits of each, down to 2^-29),
+// and values, codes of two bits times 2^(s - ref), exactly, where ref is the largest scale of the block of
+// dims in the chunk's first tile.  That holds scales from 2^-13 to 2^13 of ref; a workgroup that meets
+// another one leaves a flag, and a second launch does its part again with values in bf16, which holds all, and
+// weights in two bf16 terms (both in one kernel spill registers).
 // The loop is a pipeline: iteration i issues the products of S(i + 1) and of O += V(i - 1) P(i - 1) between
 // the steps of the softmax of S(i), puts K(i + 2) and V(i) into LDS and requests the codes after them.
-// Tiles: rows of 2 D bytes whose 16-byte chunks c lie at c ^ f(row), so that 16 rows read at one chunk (K) and
-// the transpose reads (V) spread over all banks.
+// Tiles: rows of 2 D bytes, 5 (D = 64: 1) 16-byte places apart, so that 16 rows read or written at one place and
+// the transpose reads spread over the banks and every address is one register and a constant (exchanged
+// places instead, as in the prompt's kernel, take 16 more registers and spill).
 #include "oa_kv4_attn.h"
 
 namespace {
@@ -26,18 +32,52 @@ __device__ __forceinline__ float16v mfma(bf16x8 a, bf16x8 b, float16v c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-struct Weights {                         // P^T of a 32-key tile, 16 keys per operand, in two terms
-  uint4v hi[2], lo[2];
-};
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
-template <int D>
+__device__ __forceinline__ float16v mfma16(bf16x8 a, uint4v b, float16v c) {     // both hold fp16
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ uint32_t pack2h(float a, float b) {
+  const f32x2 x = {a, b};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, f16x2));
+}
+// 8 codes to fp16, scaled by a power of two (all exponent bits set: NaN)
+__device__ __forceinline__ bf16x8 from4h(unsigned w, float f) {
+  const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 0);
+  const f16x2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 1);
+  const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 2);
+  const f16x2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, f, 3);
+  const uint4v x = {__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, c),
+                    __builtin_bit_cast(uint32_t, d)};
+  return __builtin_bit_cast(bf16x8, x);
+}
+
+constexpr int kSpan = 13;                // largest |log2| of a scale over the reference's that fp16 takes
+constexpr float kLift = 15.f;            // log2 of what weights are multiplied by
+
+template <bool TWO> struct Weights;      // P^T of a 32-key tile, 16 keys per operand
+template <> struct Weights<false> { uint4v hi[2]; };
+template <> struct Weights<true> { uint4v hi[2], lo[2]; };       // two bf16 terms
+
+__device__ __forceinline__ float16v value_product(bf16x8 v, const Weights<false>& p, int kk, float16v o) {
+  return mfma16(v, p.hi[kk], o);
+}
+__device__ __forceinline__ float16v value_product(bf16x8 v, const Weights<true>& p, int kk, float16v o) {
+  o = mfma(v, __builtin_bit_cast(bf16x8, p.hi[kk]), o);
+  return mfma(v, __builtin_bit_cast(bf16x8, p.lo[kk]), o);
+}
+
+template <int D, bool TWO>
 __global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
   constexpr int kSteps = D / 16;         // products of a score tile, and of a value tile for each term
   constexpr int kDims = D / 32;          // tiles of 32 dims
-  constexpr int kRowB = D * 2, kTileB = kTile * kRowB;
+  constexpr int kRowB = D * 2 + (D == 128 ? 80 : 16), kTileB = kTile * kRowB;
   constexpr int kWords = D / 32;         // words of codes that a staging lane turns to bf16
   __shared__ __align__(16) char s_t[4 * kTileB];          // K even, K odd, V even, V odd tiles
   __shared__ unsigned long s_nan[2][2];                    // NaN blocks of a masked V tile, by parity and half
+  __shared__ unsigned s_ref[2][4];                         // largest scales of the first V tile, by half and quarter
+  __shared__ unsigned s_wide;                              // a scale is out of fp16's span
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n32 = lane & 31, h = lane >> 5;
@@ -53,13 +93,12 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
   const int all = first + row0 / a.G + 1;                                              // keys every row sees
   const int k0 = ch * a.chunk, k1 = min(k0 + a.chunk, hi);
   if (k0 >= k1 && a.nchunk > 1) return;
+  if (TWO && !a.ws_flag[blockIdx.x]) return;
   const int n = max(0, (k1 - k0 + kTile - 1) / kTile);     // tiles
   const int nfull = min(n, max(0, (all - k0) / kTile));    // those that every row sees whole
 
   char* const s_k = s_t;
   char* const s_v = s_t + 2 * kTileB;
-  auto fsw = [](int r) { return D == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : ((r >> 1) & 1) << 2 | ((r >> 2) & 3); };
-
   // staging: lanes 0..127 of the workgroup K, the others V; key lane / 4 of the tile, a quarter of its dims
   const bool isv = wave >= 2;
   const int skey = (tid & 127) >> 2, sg = tid & 3;
@@ -81,58 +120,73 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
     for (int i = 0; i < kWords; ++i) cw[i] = x[i];
     sw = (sbase + pg * a.s_sp + off * (D / 32))[os];
   };
-  const int sdst = skey * kRowB, sf = fsw(skey);
+  const int sdst = skey * kRowB + (sg * kWords << 4);
   // values of keys past the last one any row sees count as zeros (their weights are 0, but what lies there may
   // be anything), and so do NaN blocks of a masked tile, which s_nan remembers
+  unsigned ref = 0, wide = 0;            // (a lane of V: its block's reference; it met a scale out of span)
   auto put = [&](int tile, int parity) {
     unsigned e = sw;
+    bool out = false;
     if (isv && tile >= nfull) {
       const bool nan = e == 255 && k0 + tile * kTile + skey < hi;
       const unsigned long at = __ballot(nan);
       if (lane == 0) s_nan[parity][wave & 1] = at;
-      if (nan || k0 + tile * kTile + skey >= hi) e = 0;
+      out = nan || k0 + tile * kTile + skey >= hi;
     }
-    const float f = __uint_as_float(e << 23 | sbad);
     char* const t = (isv ? s_v : s_k) + parity * kTileB + sdst;
+    if (isv && !TWO) {
+      unsigned any = 0;
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) *reinterpret_cast<bf16x8*>(t + (((sg * kWords + i) ^ sf) << 4)) = from4(cw[i], f);
+      for (int i = 0; i < kWords; ++i) any |= cw[i];
+      const bool zero = out || !(any & 0x77777777u);
+      const int x = (int)e - (int)ref;
+      if (!zero && e != 255 && (x < -kSpan || x > kSpan)) wide = 1;
+      const float f = __uint_as_float(zero ? 0x3f800000u : e == 255 ? 0x7f800000u : (unsigned)(127 + x) << 23);
+#pragma unroll
+      for (int i = 0; i < kWords; ++i)
+        *reinterpret_cast<bf16x8*>(t + (i << 4)) = from4h(out ? 0u : cw[i], f);
+    } else {
+      const float f = __uint_as_float((out ? 0u : e) << 23 | sbad);
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) *reinterpret_cast<bf16x8*>(t + (i << 4)) = from4(cw[i], f);
+    }
   };
 
   // operand addresses (bytes in a tile)
-  const int kad = n32 * kRowB + ((h ^ fsw(n32)) << 4);                     // ^ (step << 5)
+  const int kad = n32 * kRowB + (h << 4);
   const int lr = (lane & 15) >> 2, lc = lane & 3, dsub = (lane >> 4) & 1;
-  const int vad = (4 * h + lr) * kRowB + (((dsub * 2 + (lc >> 1)) ^ fsw(4 * h + lr)) << 4) + ((lc & 1) << 3);
-  auto key_op = [&](const char* tile, int step) { return *reinterpret_cast<const bf16x8*>(tile + (kad ^ (step << 5))); };
+  const int vad = (4 * h + lr) * kRowB + (dsub << 5) + (lc << 3);
+  auto key_op = [&](const char* tile, int step) { return *reinterpret_cast<const bf16x8*>(tile + kad + (step << 5)); };
   // V^T of dims 32 db .. and keys 16 kk ..: two transposed reads of 4 keys, 8 apart
   auto val_op = [&](char* tile, int db, int kk) {
-    const int ad = vad ^ (db << 6);
-    const short4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v*)(tile + ad + kk * 16 * kRowB));
-    const short4v y =
-        __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v*)(tile + (ad ^ 32) + kk * 16 * kRowB + 8 * kRowB));
+    char* const p = tile + vad + (db << 6) + kk * 16 * kRowB;
+    const short4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v*)p);
+    const short4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v*)(p + 8 * kRowB));
     return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
   };
 
-  // this lane's row (negated under a negative scale: the maximum is taken before scaling) and how many keys it
-  // sees (0: no such row)
-  const float c = fabsf(a.c);
+  // this lane's row (negated under a negative scale, as the maximum is taken before scaling, and zeros under one of
+  // 0, so that masked scores stay -inf) and how many keys it sees (0: no such row)
+  const float c = a.c == 0.f ? 1.f : fabsf(a.c);
   const int r = row0 + wave * kWaveRows + n32;
   const int rr = min(r, rows - 1), j = rr / a.G, hd = head * a.G + rr - j * a.G;
   const int lim = r < rows ? first + j + 1 : 0;
   bf16x8 Q[kSteps];
   {
-    const unsigned flip = a.c < 0.f ? 0x80008000u : 0u;
+    const unsigned flip = a.c < 0.f ? 0x80008000u : 0u, keep = a.c == 0.f ? 0u : ~0u;
     const uint16_t* p = a.q + (long)(sq.r0 + j) * a.q_st + (long)hd * a.q_sh + 8 * h;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s)
-      Q[s] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4v*>(p + 16 * s) ^ uint4v(flip));
+      Q[s] = __builtin_bit_cast(bf16x8, (*reinterpret_cast<const uint4v*>(p + 16 * s) ^ uint4v(flip)) & uint4v(keep));
   }
 
   float16v O[kDims], S0 = float16v(0.f), S1;
-  Weights P0, P1;
+  Weights<TWO> P0, P1;
 #pragma unroll
   for (int d = 0; d < kDims; ++d) O[d] = float16v(0.f);
-  float m = -FLT_MAX, l = 0.f;           // running maximum, scaled, and sum of the lane's keys
+  float m = -FLT_MAX, l = 0.f;           // running maximum, scaled, and sum of the lane's keys, times 2^kLift
   bool big = false;                      // a maximum is past 2^24 (uniform)
+  if (tid == 0) s_wide = 0;
 
   if (n > 0) {
     // K(0), K(1) and zeros for V(-1), whose weights are 0; then K(2) and V(0) requested
@@ -144,12 +198,21 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
       put(1, 1);
     } else {
 #pragma unroll
-      for (int i = 0; i < kWords; ++i) *reinterpret_cast<uint4v*>(s_v + kTileB + sdst + ((sg * kWords + i) << 4)) = uint4v(0u);
+      for (int i = 0; i < kWords; ++i) *reinterpret_cast<uint4v*>(s_v + kTileB + sdst + (i << 4)) = uint4v(0u);
     }
-    P1.hi[0] = P1.hi[1] = P1.lo[0] = P1.lo[1] = uint4v(0u);
+    P1.hi[0] = P1.hi[1] = uint4v(0u);
+    if constexpr (TWO) P1.lo[0] = P1.lo[1] = uint4v(0u);
     fetch(lead, page_at(lead));
     int page = page_at(lead + 1);
+    if (!TWO && isv) {                   // the largest scale of each quarter (of each block where D is 128) in V(0)
+      unsigned e = sw == 255 || k0 + skey >= hi ? 0 : sw;
+#pragma unroll
+      for (int x = 4; x < 64; x <<= 1) e = max(e, (unsigned)__shfl_xor((int)e, x));
+      if (D == 64) e = max(e, (unsigned)__shfl_xor((int)e, 1));
+      if (lane < 4) s_ref[wave & 1][lane] = e;
+    }
     oa::lds_barrier();
+    if (!TWO) ref = max(s_ref[0][sg], s_ref[1][sg]);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) S0 = mfma(key_op(s_k, s), Q[s], S0);
     oa::lds_barrier();                   // K(0) has been read: its place takes K(2)
@@ -169,8 +232,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
       }
     };
     // iteration i (parity odd = i & 1): K(i + 1), V(i - 1) are in the other parity's tiles
-    auto body = [&](auto mask_c, auto odd_c, int i, float16v& S, float16v& Sn, const Weights& Pp, Weights& Pn) {
-      constexpr bool MASK = decltype(mask_c)::value;
+    auto body = [&](auto odd_c, int i, float16v& S, float16v& Sn, const Weights<TWO>& Pp, Weights<TWO>& Pn) {
       constexpr int kOdd = decltype(odd_c)::value;
       char* const kt = s_k + (1 - kOdd) * kTileB;
       char* const vt = s_v + (1 - kOdd) * kTileB;
@@ -193,17 +255,18 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
           vop[s + kAhead] = val_op(vt, (s + kAhead) >> 1, (s + kAhead) & 1);
         }
         Sn = mfma(kop[s], Q[s], Sn);
-        O[s >> 1] = mfma(vop[s], __builtin_bit_cast(bf16x8, Pp.hi[s & 1]), O[s >> 1]);
-        O[s >> 1] = mfma(vop[s], __builtin_bit_cast(bf16x8, Pp.lo[s & 1]), O[s >> 1]);
+        O[s >> 1] = value_product(vop[s], Pp, s & 1, O[s >> 1]);
         if (s == 0) {                    // the tile's maximum
+          if (i >= nfull) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            if (MASK) S[r] = k0 + i * kTile + 8 * (r >> 2) + 4 * h + (r & 3) < lim ? S[r] * c : -INFINITY;
-            mx = fmaxf(mx, S[r]);
+            for (int r = 0; r < 16; ++r)
+              if (k0 + i * kTile + 8 * (r >> 2) + 4 * h + (r & 3) >= lim) S[r] = -INFINITY;
           }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) mx = fmaxf(mx, S[r]);
         } else if (s == 1) {
           const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-          mx = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * (MASK ? 1.f : c);
+          mx = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * c;
           moved = __any(mx > m);
           if (moved) {
             const float mn = fmaxf(m, mx);
@@ -213,28 +276,28 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
             // (as in oa_kv4_attn.hip: past 2^24 the product is rounded before the maximum is taken off)
             big = __any(fabsf(m) >= 16777216.f);
           }
-          if (!MASK && big) {
+          if (big) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) S[r] *= c;
           }
         } else {
 #pragma unroll
           for (int r = (s - 2) * 16 / (kSteps - 2); r < (s - 1) * 16 / (kSteps - 2); ++r) {
-            const float p1 = __builtin_amdgcn_exp2f(MASK ? S[r] - m : fmaf(S[r], big ? 1.f : c, -m));
+            const float p1 = __builtin_amdgcn_exp2f(fmaf(S[r], big ? 1.f : c, kLift - m));
             l += p1;
             if (r & 1) {
-              const uint32_t u = pack2(p0, p1);
-              uint32_t w = pack2(p0 - __uint_as_float(u << 16), p1 - __uint_as_float(u & 0xffff0000u));
-              asm volatile("" : "+v"(w));          // (pinned here: left alone they all sink below the products)
+              uint32_t u = TWO ? pack2(p0, p1) : pack2h(p0, p1);
+              asm volatile("" : "+v"(u));          // (pinned here: left alone they all sink below the products)
               Pn.hi[r >> 3][(r & 7) >> 1] = u;
-              Pn.lo[r >> 3][(r & 7) >> 1] = w;
+              if constexpr (TWO)
+                Pn.lo[r >> 3][(r & 7) >> 1] = pack2(p0 - __uint_as_float(u << 16), p1 - __uint_as_float(u & 0xffff0000u));
             }
             p0 = p1;
           }
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-      if (MASK && i > nfull) nan_blocks(i - 1, 1 - kOdd);
+      if (i > nfull) nan_blocks(i - 1, 1 - kOdd);
       if (moved) {                       // (after O += V(i - 1) P(i - 1), whose weights had the old maximum)
 #pragma unroll
         for (int d = 0; d < kDims; ++d) O[d] *= alpha;
@@ -243,30 +306,31 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
     };
     typedef std::integral_constant<int, 0> even_t;
     typedef std::integral_constant<int, 1> odd_t;
-    typedef std::integral_constant<bool, false> whole;
-    typedef std::integral_constant<bool, true> masked;
-    auto finish = [&](int parity, const Weights& P) {        // V(n - 1) P(n - 1)
+    auto finish = [&](int parity, const Weights<TWO>& P) {        // V(n - 1) P(n - 1)
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         const bf16x8 vop = val_op(s_v + parity * kTileB, s >> 1, s & 1);
-        O[s >> 1] = mfma(vop, __builtin_bit_cast(bf16x8, P.hi[s & 1]), O[s >> 1]);
-        O[s >> 1] = mfma(vop, __builtin_bit_cast(bf16x8, P.lo[s & 1]), O[s >> 1]);
+        O[s >> 1] = value_product(vop, P, s & 1, O[s >> 1]);
       }
       if (n > nfull) nan_blocks(n - 1, parity);
     };
-    int i = 0;
 #pragma unroll 1
-    for (; i + 2 <= nfull; i += 2) {
-      body(whole(), even_t(), i, S0, S1, P1, P0);
-      body(whole(), odd_t(), i + 1, S1, S0, P0, P1);
-    }
-#pragma unroll 1
-    for (; i < n; i += 2) {              // (a tile or two more than need it run masked, which changes nothing)
-      body(masked(), even_t(), i, S0, S1, P1, P0);
-      if (i + 1 < n) body(masked(), odd_t(), i + 1, S1, S0, P0, P1);
+    for (int i = 0; i < n; i += 2) {
+      body(even_t(), i, S0, S1, P1, P0);
+      if (i + 1 < n) body(odd_t(), i + 1, S1, S0, P0, P1);
     }
     if (n & 1) finish(0, P0);
     else finish(1, P1);
+    if (!TWO) {
+      if (wide) s_wide = 1;
+#pragma unroll
+      for (int d = 0; d < kDims; ++d)    // (a reference of 0: all values were)
+        O[d] *= __uint_as_float(max(s_ref[0][d * 128 / D], s_ref[1][d * 128 / D]) << 23);
+    }
+  }
+  if (!TWO) {
+    oa::lds_barrier();
+    if (tid == 0) a.ws_flag[blockIdx.x] = (int)s_wide;
   }
 
   const auto lx = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
@@ -302,8 +366,13 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
 namespace kv4 {
 
 void launch_rows(const AttnArgs& a, int head_dim, dim3 grid, hipStream_t st) {
-  if (head_dim == 64) hipLaunchKernelGGL(kv4_rows_kernel<64>, grid, dim3(kThreads), 0, st, a);
-  else hipLaunchKernelGGL(kv4_rows_kernel<128>, grid, dim3(kThreads), 0, st, a);
+  if (head_dim == 64) {
+    hipLaunchKernelGGL((kv4_rows_kernel<64, false>), grid, dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((kv4_rows_kernel<64, true>), grid, dim3(kThreads), 0, st, a);
+  } else {
+    hipLaunchKernelGGL((kv4_rows_kernel<128, false>), grid, dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((kv4_rows_kernel<128, true>), grid, dim3(kThreads), 0, st, a);
+  }
 }
 
 }  // namespace kv4

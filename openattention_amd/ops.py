@@ -929,16 +929,19 @@ def kv4_attn(q, kc, ks, vc, vs, table, lens, sm_scale: float | None = None, cu_q
         return out
     rows = max_q * G
     cap = max(1, width * where[3] if max_len is None else min(max_len, width * where[3]))
-    chunk = kv4_chunk(cap, B * HKV * -(-rows // (8 if rows <= 8 else 16 if rows <= 16 else 32 if rows <= 64 else 128)))
+    units = B * HKV * -(-rows // (8 if rows <= 8 else 16 if rows <= 16 else 32 if rows <= 64 else 128))
+    chunk = kv4_chunk(cap, units)
     nchunk = -(-cap // chunk)
-    wp = mp = None
-    if nchunk > 1:
-        n = T * HQ * nchunk
-        ws = q.new_empty(n * (Dh + 2), dtype=torch.float32)
+    wp = mp = fp = None
+    parts = T * HQ * nchunk if nchunk > 1 else 0
+    flags = units * nchunk if rows > 64 else 0
+    if parts or flags:
+        ws = q.new_empty(parts * (Dh + 2) + flags, dtype=torch.float32)
         wp = ws.data_ptr()
-        mp = wp + 4 * n * Dh
+        mp = wp + 4 * parts * Dh
+        fp = mp + 8 * parts
     _run(i, "oa_kv4_attn", *qa, *ps, *where, tp, ts, width, lp, cp, B, T, max_q, HQ, HKV, Dh, scale, chunk, nchunk, wp, mp,
-         *oa)
+         fp, *oa)
     return out
 
 

@@ -55,11 +55,11 @@ def rows_at(codes, scales, slots):
     return values(codes[p, :, o], scales[p, :, o])
 
 
-def attn(q, k, v, n, scale):
+def attn(q, k, v, n, scale, weight=2.0 ** -16):
     """One sequence: q (R, HQ, D) the newest tokens of k, v (n, HKV, D) fp64.  Returns the fp64 output
     and the fp32 kernel's error bound beside the output's own rounding: sums of D exact products (each
-    sum off by D 2^-24 of its terms' sizes, as a score and once more in the maximum), weights in two
-    bf16 terms (2^-16), exponentials and sums over n keys ((n + 64) 2^-24); and what fp32 does not hold:
+    sum off by D 2^-24 of its terms' sizes, as a score and once more in the maximum), weights rounded
+    to `weight` of themselves (two bf16 terms 2^-16; fp16, for more than 64 rows of a KV head, 2^-11), exponentials and sums over n keys ((n + 64) 2^-24); and what fp32 does not hold:
     a weight, or its second term, under 2^-126 counts as 0, so that each key may be off by 2^-125 |v|."""
     R, HQ, D = q.shape
     HKV = k.shape[1]
@@ -76,7 +76,7 @@ def attn(q, k, v, n, scale):
         size = (x.abs()[:, :, None] * kk.abs()[:, None]).sum(-1).amax(-1) * abs(scale)
         out[j] = torch.matmul(w, vv).reshape(HQ, D)
         a = torch.matmul(w, vv.abs()).reshape(HQ, D)
-        err[j] = a * (2 * size.reshape(HQ, 1) * (D + 4) * 2.0 ** -24 + 2.0 ** -16 + (m + 64) * 2.0 ** -24)
+        err[j] = a * (2 * size.reshape(HQ, 1) * (D + 4) * 2.0 ** -24 + weight + (m + 64) * 2.0 ** -24)
         err[j] += 2.0 ** -125 * vv.abs().sum(1).repeat_interleave(G, 0)
     return out, err
 

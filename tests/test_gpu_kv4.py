@@ -307,11 +307,12 @@ def paged(lens, HKV, D, page, g, spare=2, extra_width=0):
 def want_attn(q, cache, table, lens, cu, scale, page):
     out = torch.zeros(q.shape, dtype=torch.float64, device=DEV)
     err = torch.zeros_like(out)
+    most = max(b - a for a, b in zip(cu, cu[1:])) * q.shape[1] // cache[0].shape[1]
     for b, slots in enumerate(ref.held(table, lens, page)):
         r = slice(cu[b], cu[b + 1])
         slots = slots.to(DEV)
         k, v = ref.rows_at(cache[0], cache[1], slots), ref.rows_at(cache[2], cache[3], slots)
-        out[r], err[r] = ref.attn(q[r], k, v, lens[b], scale)
+        out[r], err[r] = ref.attn(q[r], k, v, lens[b], scale, 2.0 ** -11 if most > 64 else 2.0 ** -16)
     return out, err
 
 
@@ -353,6 +354,48 @@ def test_attention(case, chunk, copies, monkeypatch):
     scale = D ** -0.5 if case % 2 else 0.11
     out = ops.kv4_attn(q, *cache, table, i32(lens), scale, cu_q=i32(cu) if rows else None, max_q=max(rows) if rows else 1)
     check_attn(out, *want_attn(q, cache, table, lens, cu, scale, page))
+
+
+@pytest.mark.parametrize("rows", [17, 40])
+def test_attention_values_of_all_sizes(rows):
+    """Values whose scales lie up to 2^24 apart from key to key and block to block, a first tile of zeros, of
+    NaN in masked places: what fp16 does not hold is done in bf16."""
+    g = gen(rows + 1)
+    page, lens = 32, [300, 200, 150, 70]
+    cache, table = paged(lens, 2, 128, page, g)
+    for b, slots in enumerate(ref.held(table, lens, page)):
+        n = lens[b]
+        k, v = randn(g, n, 2, 128), randn(g, n, 2, 128).view(n, 2, 4, 32)
+        if b == 0:
+            v *= torch.exp2(torch.randint(-12, 13, (n, 2, 4, 1), generator=g, device=DEV).float())
+        elif b == 1:
+            v[:64] = 0                                    # nothing to go by in the first tile
+            v[100:] *= 2.0 ** 60
+        elif b == 2:
+            v *= 2.0 ** -100
+            v[:, :, 2] *= torch.exp2(torch.arange(n, device=DEV).float() / 12)[:, None, None]
+        ops.kv4_write(k, v.view(n, 2, 128), slots.int().to(DEV), *cache)
+    cu = starts([rows] * 4)
+    q = randn(g, cu[-1], 8, 128, dtype=torch.bfloat16)
+    out = ops.kv4_attn(q, *cache, table, i32(lens), cu_q=i32(cu), max_q=rows)
+    check_attn(out, *want_attn(q, cache, table, lens, cu, 128 ** -0.5, page))
+
+
+def test_attention_of_small_weights():
+    """One key takes a weight of 1 and 20000 others about 2^-16 each, half of the sum together."""
+    g = gen(8)
+    n, rows, page = 20001, 40, 64
+    cache, table = paged([n], 1, 64, page, g)
+    k = torch.zeros(n, 1, 64, device=DEV)
+    k[0, 0, :8] = 1.0
+    v = torch.ones(n, 1, 64, device=DEV)
+    v[0] = -1.0
+    ops.kv4_write(k, v, ref.held(table, [n], page)[0].int().to(DEV), *cache)
+    q = torch.zeros(rows, 4, 64, device=DEV, dtype=torch.bfloat16)
+    q[..., :8] = 11.0 / 8
+    for R in (1, rows):
+        out = ops.kv4_attn(q[:R], *cache, table, i32([n]), 1.0, cu_q=i32([0, R]), max_q=R)
+        check_attn(out, *want_attn(q[:R], cache, table, [n], [0, R], 1.0, page))
 
 
 def test_attention_of_many_sequences():
@@ -532,6 +575,7 @@ def test_decode_loop_eager_and_captured():
         kk = ref.values(*ref.quantise(k))
         vv = ref.values(*ref.quantise(rows[:, (HQ + HKV) * D:].view(n, HKV, D)))
         want, err = ref.attn(q, kk, vv, n, D ** -0.5)
+        err[:lens[b]] = ref.attn(q[:lens[b]], kk[:lens[b]], vv[:lens[b]], lens[b], D ** -0.5, 2.0 ** -11)[1]
         check_attn(eager[0][first[b]:first[b + 1]], want[:lens[b]], err[:lens[b]])
         check_attn(torch.stack([eager[1 + i][b] for i in range(steps)]), want[lens[b]:], err[lens[b]:])
 
