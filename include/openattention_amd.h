@@ -582,8 +582,8 @@ int oa_kv_pages_truncate(const int* keep, int* lens, int* table, long table_stri
 
 /*
  * The 4-bit cache: codes kc, vc (pages, kv_heads, page, head_dim / 2) and scales ks, vs (pages, kv_heads, page,
- * head_dim / 32) bytes, pages code_stride and scale_stride bytes apart; head_dim 64 or 128.  A block of 32
- * values of a row is a 4-bit code for each (sign, two bits of exponent, one of mantissa: 0, .5, 1, 1.5, 2, 3,
+ * head_dim / 32) bytes, pages code_stride and scale_stride (under 2^32) bytes apart; head_dim 64 or 128.  A block
+ * of 32 values of a row is a 4-bit code for each (sign, two bits of exponent, one of mantissa: 0, .5, 1, 1.5, 2, 3,
  * 4, 6; the even value of a row in the low half of a byte) and a byte s, scaling by 2^(s - 127): the smallest
  * 2^e with max |x| < 7 * 2^e, -125 <= e <= 125; rounding to nearest, ties to the even code, at most 6.  A
  * block with a value that is not finite is held as s = 255, NaN.

@@ -65,6 +65,14 @@ __device__ __forceinline__ bf16x8 from4(unsigned w, float f) {
                     __builtin_bit_cast(uint32_t, d)};
   return __builtin_bit_cast(bf16x8, x);
 }
+// An entry of a table's row, the same for all lanes, by a vector load: scalar loads come back in no order, and
+// beside one in flight every wait for LDS waits for all of it.
+__device__ __forceinline__ int table_entry(const int* row, int i) {
+  int zero;
+  asm("v_mov_b32 %0, 0" : "=v"(zero));
+  return row[i + zero];
+}
+
 // NQ tiles of 16 rows for each workgroup, the waves on keys of their own (oa_kv4_attn.hip), or 128 rows, 32 to a
 // wave, over shared keys (oa_kv4_rows.hip)
 void launch_rows(const AttnArgs& a, int head_dim, dim3 grid, hipStream_t st);

@@ -419,7 +419,8 @@ extern "C" int oa_kv4_attn(const void* q, long q_st, long q_sh, const void* kc, 
   if (!sequences || !tokens) return 0;
   if (odd(q, 16) || q_st % 8 || q_sh % 8 || odd(out, 8) || o_st % 4 || o_sh % 4 || odd(kc, 16) || odd(ks, 16) || odd(vc, 16) ||
       odd(vs, 16) || !table || !lens || code_stride < (long)kv_heads * page * (head_dim / 2) ||
-      scale_stride < (long)kv_heads * page * (head_dim / 32) || code_stride % 16 || scale_stride % 16 || !(sm_scale == sm_scale))
+      scale_stride < (long)kv_heads * page * (head_dim / 32) || code_stride % 16 || scale_stride % 16 ||
+      code_stride > 0xffffffffL || scale_stride > 0xffffffffL || !(sm_scale == sm_scale))
     return OA_EINVAL;
   if ((nchunk > 1 && (odd(ws_o, 16) || odd(ws_ml, 8))) || ((long)max_q * (q_heads / kv_heads) > kFewRows && odd(ws_flag, 4)))
     return OA_EINVAL;

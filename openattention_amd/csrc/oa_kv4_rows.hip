@@ -6,7 +6,8 @@
 // that all four read.  Products are v_mfma_f32_32x32x16_bf16: S^T = K Q^T, whose lanes hold 16 keys' scores of
 // one row, and O^T = V^T P^T with V^T by the LDS transpose reads (the contraction takes keys in the order the
 // scores left them).
-// Weights and values go into the second product in fp16: weights times 2^15 (11 bits of each, down to 2^-29),
+// Weights and values go into the second product in fp16: weights times 2^7 (11 bits of each, down to 2^-21
+// of the maximum; up to 2^8 past it, so that the sums are rescaled in few tiles),
 // and values, codes of two bits times 2^(s - ref), exactly, where ref is the largest scale of the block of
 // dims in the chunk's first tile.  That holds scales from 2^-13 to 2^13 of ref; a workgroup that meets
 // another one leaves a flag, and a second launch does its part again with values in bf16, which holds all, and
@@ -54,7 +55,8 @@ __device__ __forceinline__ bf16x8 from4h(unsigned w, float f) {
 }
 
 constexpr int kSpan = 13;                // largest |log2| of a scale over the reference's that fp16 takes
-constexpr float kLift = 15.f;            // log2 of what weights are multiplied by
+constexpr float kLift = 7.f;             // log2 of what weights are multiplied by
+constexpr float kLazy = 8.f;             // log2 of how far a weight may pass 1 before the sums are rescaled
 
 template <bool TWO> struct Weights;      // P^T of a 32-key tile, 16 keys per operand
 template <> struct Weights<false> { uint4v hi[2]; };
@@ -107,49 +109,65 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
   const uint8_t* const cbase = (isv ? a.vc : a.kc) + ((long)head << a.lp) * (D / 2);
   const uint8_t* const sbase = (isv ? a.vs : a.ks) + ((long)head << a.lp) * (D / 32);
   const unsigned oc = skey * (D / 2) + sg * (D / 8), os = skey * (D / 32) + sg * D / 128;
-  unsigned cw[kWords], sw = 0, sbad = 0;
-  auto page_at = [&](int tile) { return trow[min((k0 + tile * kTile) >> a.lp, a.width - 1)]; };
-  auto fetch = [&](int tile, int page) {                   // (past the last tile: read, never used)
+  // two tiles' codes are on their way, by parity (one: 104 us for 88, as each is read from HBM by few)
+  struct Staged {
+    unsigned w[kWords], s, bad;
+    int next;                            // the table's entry for the tile after the next
+  } st[2];
+  auto page_at = [&](int tile) { return table_entry(trow, min((k0 + tile * kTile) >> a.lp, a.width - 1)); };
+  auto fetch = [&](Staged& x, int tile, int entry) {       // (past the last tile: read, never used)
+    const int page = __builtin_amdgcn_readfirstlane(entry);
     const bool bad = (unsigned)page >= (unsigned)a.NP;
-    sbad = bad && !isv ? 0x7f800000u : 0u;
-    const long pg = bad ? 0 : page, off = (k0 + tile * kTile) & pmask;
-    const uint8_t* p = cbase + pg * a.c_sp + off * (D / 2) + oc;
+    x.bad = bad && !isv ? 0x7f800000u : 0u;
+    const unsigned pg = bad ? 0 : page, off = (k0 + tile * kTile) & pmask;
+    const uint8_t* p = cbase + ((unsigned long)pg * (unsigned)a.c_sp + off * (D / 2)) + oc;
     typedef unsigned vec __attribute__((ext_vector_type(kWords)));
-    const vec x = *reinterpret_cast<const vec*>(p);
+    const vec c = *reinterpret_cast<const vec*>(p);
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) cw[i] = x[i];
-    sw = (sbase + pg * a.s_sp + off * (D / 32))[os];
+    for (int i = 0; i < kWords; ++i) x.w[i] = c[i];
+    x.s = (sbase + ((unsigned long)pg * (unsigned)a.s_sp + off * (D / 32)))[os];
+    x.next = page_at(tile + 2);
   };
   const int sdst = skey * kRowB + (sg * kWords << 4);
   // values of keys past the last one any row sees count as zeros (their weights are 0, but what lies there may
   // be anything), and so do NaN blocks of a masked tile, which s_nan remembers
   unsigned ref = 0, wide = 0;            // (a lane of V: its block's reference; it met a scale out of span)
-  auto put = [&](int tile, int parity) {
-    unsigned e = sw;
-    bool out = false;
+  struct Put {
+    char* to;
+    float f;                             // the block's scale
+    bool out;                            // zeros instead
+  };
+  auto put_begin = [&](const Staged& y, int tile, int parity) {
+    Put t;
+    t.to = (isv ? s_v : s_k) + parity * kTileB + sdst;
+    t.out = false;
     if (isv && tile >= nfull) {
-      const bool nan = e == 255 && k0 + tile * kTile + skey < hi;
+      const bool nan = y.s == 255 && k0 + tile * kTile + skey < hi;
       const unsigned long at = __ballot(nan);
       if (lane == 0) s_nan[parity][wave & 1] = at;
-      out = nan || k0 + tile * kTile + skey >= hi;
+      t.out = nan || k0 + tile * kTile + skey >= hi;
     }
-    char* const t = (isv ? s_v : s_k) + parity * kTileB + sdst;
     if (isv && !TWO) {
       unsigned any = 0;
 #pragma unroll
-      for (int i = 0; i < kWords; ++i) any |= cw[i];
-      const bool zero = out || !(any & 0x77777777u);
-      const int x = (int)e - (int)ref;
-      if (!zero && e != 255 && (x < -kSpan || x > kSpan)) wide = 1;
-      const float f = __uint_as_float(zero ? 0x3f800000u : e == 255 ? 0x7f800000u : (unsigned)(127 + x) << 23);
-#pragma unroll
-      for (int i = 0; i < kWords; ++i)
-        *reinterpret_cast<bf16x8*>(t + (i << 4)) = from4h(out ? 0u : cw[i], f);
+      for (int i = 0; i < kWords; ++i) any |= y.w[i];
+      const bool zero = t.out || !(any & 0x77777777u);
+      const int x = (int)y.s - (int)ref;
+      if (!zero && y.s != 255 && (x < -kSpan || x > kSpan)) wide = 1;
+      t.f = __uint_as_float(zero ? 0x3f800000u : y.s == 255 ? 0x7f800000u : (unsigned)(127 + x) << 23);
     } else {
-      const float f = __uint_as_float((out ? 0u : e) << 23 | sbad);
-#pragma unroll
-      for (int i = 0; i < kWords; ++i) *reinterpret_cast<bf16x8*>(t + (i << 4)) = from4(cw[i], f);
+      t.f = __uint_as_float(t.out ? 0x3f800000u : y.s << 23 | y.bad);
     }
+    return t;
+  };
+  auto put_word = [&](const Put& t, const Staged& y, int i) {
+    const unsigned w = t.out ? 0u : y.w[i];
+    *reinterpret_cast<bf16x8*>(t.to + (i << 4)) = isv && !TWO ? from4h(w, t.f) : from4(w, t.f);
+  };
+  auto put = [&](const Staged& y, int tile, int parity) {
+    const Put t = put_begin(y, tile, parity);
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) put_word(t, y, i);
   };
 
   // operand addresses (bytes in a tile)
@@ -189,23 +207,23 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
   if (tid == 0) s_wide = 0;
 
   if (n > 0) {
-    // K(0), K(1) and zeros for V(-1), whose weights are 0; then K(2) and V(0) requested
+    // K(0), K(1) and zeros for V(-1), whose weights are 0; then K(2), K(3), V(0) and V(1) requested
     const int lead = isv ? 0 : 2;        // tiles that this lane's staging is ahead of the loop
     if (!isv) {
-      fetch(0, page_at(0));
-      put(0, 0);
-      fetch(1, page_at(1));
-      put(1, 1);
+      fetch(st[0], 0, page_at(0));
+      fetch(st[1], 1, page_at(1));
+      put(st[0], 0, 0);
+      put(st[1], 1, 1);
     } else {
 #pragma unroll
       for (int i = 0; i < kWords; ++i) *reinterpret_cast<uint4v*>(s_v + kTileB + sdst + (i << 4)) = uint4v(0u);
     }
     P1.hi[0] = P1.hi[1] = uint4v(0u);
     if constexpr (TWO) P1.lo[0] = P1.lo[1] = uint4v(0u);
-    fetch(lead, page_at(lead));
-    int page = page_at(lead + 1);
+    fetch(st[0], lead, page_at(lead));
+    fetch(st[1], lead + 1, page_at(lead + 1));
     if (!TWO && isv) {                   // the largest scale of each quarter (of each block where D is 128) in V(0)
-      unsigned e = sw == 255 || k0 + skey >= hi ? 0 : sw;
+      unsigned e = st[0].s == 255 || k0 + skey >= hi ? 0 : st[0].s;
 #pragma unroll
       for (int x = 4; x < 64; x <<= 1) e = max(e, (unsigned)__shfl_xor((int)e, x));
       if (D == 64) e = max(e, (unsigned)__shfl_xor((int)e, 1));
@@ -236,9 +254,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
       constexpr int kOdd = decltype(odd_c)::value;
       char* const kt = s_k + (1 - kOdd) * kTileB;
       char* const vt = s_v + (1 - kOdd) * kTileB;
-      put(i + lead, kOdd);
-      fetch(i + lead + 1, page);
-      page = page_at(i + lead + 2);
+      const Put to = put_begin(st[kOdd], i + lead, kOdd);
       float mx = -INFINITY, alpha = 1.f, p0 = 0.f;
       bool moved = false;
       Sn = float16v(0.f);
@@ -267,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
         } else if (s == 1) {
           const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
           mx = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * c;
-          moved = __any(mx > m);
+          moved = __any(mx > m + kLazy);
           if (moved) {
             const float mn = fmaxf(m, mx);
             alpha = __builtin_amdgcn_exp2f(m - mn);
@@ -295,6 +311,8 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
             p0 = p1;
           }
         }
+        if (s >= kSteps - kWords) put_word(to, st[kOdd], s - (kSteps - kWords));
+        if (s == kSteps - 1) fetch(st[kOdd], i + lead + 2, st[kOdd].next);
         __builtin_amdgcn_sched_barrier(0);
       }
       if (i > nfull) nan_blocks(i - 1, 1 - kOdd);

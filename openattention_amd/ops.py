@@ -848,8 +848,9 @@ def _kv4_cache(kc, ks, vc, vs) -> tuple:
     ps = kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr()
     c0, s0 = (c[0], s[0]) if NP > 1 else (HKV * page * half, HKV * page * blocks)
     if (vc.stride() != c or vs.stride() != s or c[1:] != (page * half, half, 1) or s[1:] != (page * blocks, blocks, 1)
-            or c0 < HKV * page * half or s0 < HKV * page * blocks or (c0 | s0 | ps[0] | ps[1] | ps[2] | ps[3]) % 16):
-        raise ValueError("cache: contiguous pages that start at multiples of 16 bytes, those of k and v at one distance")
+            or c0 < HKV * page * half or s0 < HKV * page * blocks or c0 >> 32 or (c0 | s0 | ps[0] | ps[1] | ps[2] | ps[3]) % 16):
+        raise ValueError("cache: contiguous pages that start at multiples of 16 bytes, those of k and v at one distance "
+                         "under 2^32 bytes")
     return ps, (c0, s0, NP, page), HKV, 2 * half
 
 
