@@ -1,9 +1,9 @@
 // Causal attention over the 4-bit paged cache for many query rows of a KV head (a question, a piece of a
 // prompt): the same sums as in oa_kv4_attn.hip, with the keys' codes turned to bf16 once for 128 rows.
 //
-// One workgroup of four waves takes 128 query rows of a KV head, 32 to a wave, and a chunk of keys.  Of a tile of
-// 32 keys, waves 0 and 1 turn K to bf16 and waves 2 and 3 V, a block of 32 values to a lane, into LDS tiles
-// that all four read.  Products are v_mfma_f32_32x32x16_bf16: S^T = K Q^T, whose lanes hold 16 keys' scores of
+// One workgroup of four waves takes 128 query rows of a KV head, 32 to a wave, and a chunk of keys.  A tile of 32
+// keys is turned to bf16 (V: fp16) by all of them, 16 values of K and of V to a lane (8 where D is 64), into LDS
+// tiles that all four read.  Products are v_mfma_f32_32x32x16: S^T = K Q^T, whose lanes hold 16 keys' scores of
 // one row, and O^T = V^T P^T with V^T by the LDS transpose reads (the contraction takes keys in the order the
 // scores left them).
 // Weights and values go into the second product in fp16: weights times 2^7 (11 bits of each, down to 2^-21
@@ -13,8 +13,8 @@
 // another one leaves a flag, and a second launch does its part again with values in bf16, which holds all, and
 // weights in two bf16 terms (both in one kernel spill registers).
 // The loop is a pipeline: iteration i issues the products of S(i + 1) and of O += V(i - 1) P(i - 1) between
-// the steps of the softmax of S(i), puts K(i + 2) and V(i) into LDS and requests the codes after them.
-// Tiles: rows of 2 D bytes, 5 (D = 64: 1) 16-byte places apart, so that 16 rows read or written at one place and
+// the steps of the softmax of S(i), puts tile i + 2 into LDS and requests the codes of tile i + 4.
+// Tiles: rows of 2 D bytes, 5 (D = 64: 1) 16-byte places apart, so that rows read or written at one place and
 // the transpose reads spread over the banks and every address is one register and a constant (exchanged
 // places instead, as in the prompt's kernel, take 16 more registers and spill).
 #include "oa_kv4_attn.h"
@@ -75,10 +75,10 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
   constexpr int kSteps = D / 16;         // products of a score tile, and of a value tile for each term
   constexpr int kDims = D / 32;          // tiles of 32 dims
   constexpr int kRowB = D * 2 + (D == 128 ? 80 : 16), kTileB = kTile * kRowB;
-  constexpr int kWords = D / 32;         // words of codes that a staging lane turns to bf16
-  __shared__ __align__(16) char s_t[4 * kTileB];          // K even, K odd, V even, V odd tiles
-  __shared__ unsigned long s_nan[2][2];                    // NaN blocks of a masked V tile, by parity and half
-  __shared__ unsigned s_ref[2][4];                         // largest scales of the first V tile, by half and quarter
+  constexpr int kWords = D / 64;         // words of codes of K and of V that a lane turns to floats
+  __shared__ __align__(16) char s_t[6 * kTileB];          // K even, K odd, V of tiles i % 4
+  __shared__ unsigned long s_nan[4][kWaves];               // NaN blocks of a masked V tile, by the lanes of each wave
+  __shared__ unsigned s_ref[kWaves][8];                    // largest scales of the first V tile, by wave and part
   __shared__ unsigned s_wide;                              // a scale is out of fp16's span
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -99,75 +99,70 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
   const int n = max(0, (k1 - k0 + kTile - 1) / kTile);     // tiles
   const int nfull = min(n, max(0, (all - k0) / kTile));    // those that every row sees whole
 
-  char* const s_k = s_t;
   char* const s_v = s_t + 2 * kTileB;
-  // staging: lanes 0..127 of the workgroup K, the others V; key lane / 4 of the tile, a quarter of its dims
-  const bool isv = wave >= 2;
-  const int skey = (tid & 127) >> 2, sg = tid & 3;
+  // staging: key lane / 8 of the tile, an eighth of its dims
+  const int skey = tid >> 3, sg = tid & 7;
   const int* trow = a.table + (long)b * a.t_st;
   const int pmask = (1 << a.lp) - 1;
-  const uint8_t* const cbase = (isv ? a.vc : a.kc) + ((long)head << a.lp) * (D / 2);
-  const uint8_t* const sbase = (isv ? a.vs : a.ks) + ((long)head << a.lp) * (D / 32);
-  const unsigned oc = skey * (D / 2) + sg * (D / 8), os = skey * (D / 32) + sg * D / 128;
-  // two tiles' codes are on their way, by parity (one: 104 us for 88, as each is read from HBM by few)
+  const unsigned long headc = ((unsigned long)head << a.lp) * (D / 2), heads = ((unsigned long)head << a.lp) * (D / 32);
+  const unsigned oc = skey * (D / 2) + sg * (D / 16), os = skey * (D / 32) + sg * D / 256;
+  typedef unsigned words __attribute__((ext_vector_type(kWords)));
+  // two tiles' codes are on their way, by parity
   struct Staged {
-    unsigned w[kWords], s, bad;
+    words k, v;
+    unsigned ks, vs, bad;
     int next;                            // the table's entry for the tile after the next
   } st[2];
   auto page_at = [&](int tile) { return table_entry(trow, min((k0 + tile * kTile) >> a.lp, a.width - 1)); };
   auto fetch = [&](Staged& x, int tile, int entry) {       // (past the last tile: read, never used)
-    const int page = __builtin_amdgcn_readfirstlane(entry);
-    const bool bad = (unsigned)page >= (unsigned)a.NP;
-    x.bad = bad && !isv ? 0x7f800000u : 0u;
+    const unsigned page = __builtin_amdgcn_readfirstlane(entry);
+    const bool bad = page >= (unsigned)a.NP;
+    x.bad = bad ? 0x7f800000u : 0u;
     const unsigned pg = bad ? 0 : page, off = (k0 + tile * kTile) & pmask;
-    const uint8_t* p = cbase + ((unsigned long)pg * (unsigned)a.c_sp + off * (D / 2)) + oc;
-    typedef unsigned vec __attribute__((ext_vector_type(kWords)));
-    const vec c = *reinterpret_cast<const vec*>(p);
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) x.w[i] = c[i];
-    x.s = (sbase + ((unsigned long)pg * (unsigned)a.s_sp + off * (D / 32)))[os];
+    const unsigned long bc = (unsigned long)pg * (unsigned)a.c_sp + headc + off * (D / 2);
+    const unsigned long bs = (unsigned long)pg * (unsigned)a.s_sp + heads + off * (D / 32);
+    x.k = *reinterpret_cast<const words*>(a.kc + bc + oc);
+    x.ks = (a.ks + bs)[os];
+    x.v = *reinterpret_cast<const words*>(a.vc + bc + oc);
+    x.vs = (a.vs + bs)[os];
     x.next = page_at(tile + 2);
   };
-  const int sdst = skey * kRowB + (sg * kWords << 4);
-  // values of keys past the last one any row sees count as zeros (their weights are 0, but what lies there may
-  // be anything), and so do NaN blocks of a masked tile, which s_nan remembers
-  unsigned ref = 0, wide = 0;            // (a lane of V: its block's reference; it met a scale out of span)
+  char* const sdst = s_t + skey * kRowB + sg * (D / 4);
+  unsigned ref = 0, wide = 0;            // this lane's block's reference; it met a scale out of span
+  // A lane's V block in a tile: its scale as a float, or zeros instead of its values: those of keys past the last
+  // one any row sees (their weights are 0, but what lies there may be anything), and of NaN blocks of a masked
+  // tile, which s_nan remembers
   struct Put {
-    char* to;
-    float f;                             // the block's scale
-    bool out;                            // zeros instead
+    float f;
+    bool out;
   };
-  auto put_begin = [&](const Staged& y, int tile, int parity) {
+  auto put_begin = [&](const Staged& y, int tile) {
     Put t;
-    t.to = (isv ? s_v : s_k) + parity * kTileB + sdst;
     t.out = false;
-    if (isv && tile >= nfull) {
-      const bool nan = y.s == 255 && k0 + tile * kTile + skey < hi;
+    if (tile >= nfull) {
+      const bool past = k0 + tile * kTile + skey >= hi, nan = y.vs == 255 && !past;
       const unsigned long at = __ballot(nan);
-      if (lane == 0) s_nan[parity][wave & 1] = at;
-      t.out = nan || k0 + tile * kTile + skey >= hi;
+      if (lane == 0) s_nan[tile & 3][wave] = at;
+      t.out = nan || past;
     }
-    if (isv && !TWO) {
-      unsigned any = 0;
-#pragma unroll
-      for (int i = 0; i < kWords; ++i) any |= y.w[i];
-      const bool zero = t.out || !(any & 0x77777777u);
-      const int x = (int)y.s - (int)ref;
-      if (!zero && y.s != 255 && (x < -kSpan || x > kSpan)) wide = 1;
-      t.f = __uint_as_float(zero ? 0x3f800000u : y.s == 255 ? 0x7f800000u : (unsigned)(127 + x) << 23);
+    if (TWO) {
+      t.f = __uint_as_float(t.out ? 0x3f800000u : y.vs << 23);
     } else {
-      t.f = __uint_as_float(t.out ? 0x3f800000u : y.s << 23 | y.bad);
+      unsigned any = y.v[0];
+      if constexpr (kWords > 1) any |= y.v[1];
+      const bool zero = t.out || !(any & 0x77777777u);
+      const int x = (int)y.vs - (int)ref;
+      if (!zero && y.vs != 255 && (x < -kSpan || x > kSpan)) wide = 1;
+      t.f = __uint_as_float(zero ? 0x3f800000u : y.vs == 255 ? 0x7f800000u : (unsigned)(127 + x) << 23);
     }
     return t;
   };
-  auto put_word = [&](const Put& t, const Staged& y, int i) {
-    const unsigned w = t.out ? 0u : y.w[i];
-    *reinterpret_cast<bf16x8*>(t.to + (i << 4)) = isv && !TWO ? from4h(w, t.f) : from4(w, t.f);
+  auto put_k = [&](const Staged& y, int parity, int i) {
+    *reinterpret_cast<bf16x8*>(sdst + parity * kTileB + (i << 4)) = from4(y.k[i], __uint_as_float(y.ks << 23 | y.bad));
   };
-  auto put = [&](const Staged& y, int tile, int parity) {
-    const Put t = put_begin(y, tile, parity);
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) put_word(t, y, i);
+  auto put_v = [&](const Put& t, const Staged& y, int tile, int i) {
+    const unsigned w = t.out ? 0u : y.v[i];
+    *reinterpret_cast<bf16x8*>(sdst + (2 + (tile & 3)) * kTileB + (i << 4)) = TWO ? from4(w, t.f) : from4h(w, t.f);
   };
 
   // operand addresses (bytes in a tile)
@@ -207,41 +202,45 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
   if (tid == 0) s_wide = 0;
 
   if (n > 0) {
-    // K(0), K(1) and zeros for V(-1), whose weights are 0; then K(2), K(3), V(0) and V(1) requested
-    const int lead = isv ? 0 : 2;        // tiles that this lane's staging is ahead of the loop
-    if (!isv) {
-      fetch(st[0], 0, page_at(0));
-      fetch(st[1], 1, page_at(1));
-      put(st[0], 0, 0);
-      put(st[1], 1, 1);
-    } else {
+    // tiles 0 and 1 and zeros for V(-1), whose weights are 0; then tiles 2 and 3 requested
+    fetch(st[0], 0, page_at(0));
+    fetch(st[1], 1, page_at(1));
+    if (!TWO) {                          // the largest scale of each block of dims in V(0)
+      unsigned e = st[0].vs == 255 || k0 + skey >= hi ? 0 : st[0].vs;
 #pragma unroll
-      for (int i = 0; i < kWords; ++i) *reinterpret_cast<uint4v*>(s_v + kTileB + sdst + (i << 4)) = uint4v(0u);
+      for (int x = 1; x < 64; x <<= 1)
+        if (x >= 8 || x < 256 / D) e = max(e, (unsigned)__shfl_xor((int)e, x));
+      if (lane < 8) s_ref[wave][lane] = e;
+      oa::lds_barrier();
+      ref = max(max(s_ref[0][sg], s_ref[1][sg]), max(s_ref[2][sg], s_ref[3][sg]));
     }
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const Put t = put_begin(st[x], x);
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) {
+        put_k(st[x], x, i);
+        put_v(t, st[x], x, i);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) *reinterpret_cast<uint4v*>(sdst + 5 * kTileB + (i << 4)) = uint4v(0u);
     P1.hi[0] = P1.hi[1] = uint4v(0u);
     if constexpr (TWO) P1.lo[0] = P1.lo[1] = uint4v(0u);
-    fetch(st[0], lead, page_at(lead));
-    fetch(st[1], lead + 1, page_at(lead + 1));
-    if (!TWO && isv) {                   // the largest scale of each quarter (of each block where D is 128) in V(0)
-      unsigned e = st[0].s == 255 || k0 + skey >= hi ? 0 : st[0].s;
-#pragma unroll
-      for (int x = 4; x < 64; x <<= 1) e = max(e, (unsigned)__shfl_xor((int)e, x));
-      if (D == 64) e = max(e, (unsigned)__shfl_xor((int)e, 1));
-      if (lane < 4) s_ref[wave & 1][lane] = e;
-    }
+    fetch(st[0], 2, st[0].next);
+    fetch(st[1], 3, st[1].next);
     oa::lds_barrier();
-    if (!TWO) ref = max(s_ref[0][sg], s_ref[1][sg]);
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) S0 = mfma(key_op(s_k, s), Q[s], S0);
+    for (int s = 0; s < kSteps; ++s) S0 = mfma(key_op(s_t, s), Q[s], S0);
     oa::lds_barrier();                   // K(0) has been read: its place takes K(2)
 
     // O += V(tile) P(tile)'s NaN blocks, into the rows that see them (rare)
-    auto nan_blocks = [&](int tile, int parity) {
+    auto nan_blocks = [&](int tile) {
 #pragma unroll 1
-      for (int half = 0; half < 2; ++half) {
-        unsigned long at = s_nan[parity][half];
+      for (int w = 0; w < kWaves; ++w) {
+        unsigned long at = s_nan[tile & 3][w];
         while (at) {
-          const int bit = __builtin_ctzl(at), key = k0 + tile * kTile + 16 * half + (bit >> 2), blk = (bit & 3) * D / 128;
+          const int bit = __builtin_ctzl(at), key = k0 + tile * kTile + 8 * w + (bit >> 3), blk = (bit & 7) * D / 256;
           at &= at - 1;
 #pragma unroll
           for (int d = 0; d < kDims; ++d)
@@ -249,12 +248,12 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
         }
       }
     };
-    // iteration i (parity odd = i & 1): K(i + 1), V(i - 1) are in the other parity's tiles
+    // iteration i (parity odd = i & 1): K(i + 1) is in the other parity's tile
     auto body = [&](auto odd_c, int i, float16v& S, float16v& Sn, const Weights<TWO>& Pp, Weights<TWO>& Pn) {
       constexpr int kOdd = decltype(odd_c)::value;
-      char* const kt = s_k + (1 - kOdd) * kTileB;
-      char* const vt = s_v + (1 - kOdd) * kTileB;
-      const Put to = put_begin(st[kOdd], i + lead, kOdd);
+      char* const kt = s_t + (1 - kOdd) * kTileB;
+      char* const vt = s_v + ((i - 1) & 3) * kTileB;
+      const Put to = put_begin(st[kOdd], i + 2);
       float mx = -INFINITY, alpha = 1.f, p0 = 0.f;
       bool moved = false;
       Sn = float16v(0.f);
@@ -311,11 +310,15 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
             p0 = p1;
           }
         }
-        if (s >= kSteps - kWords) put_word(to, st[kOdd], s - (kSteps - kWords));
-        if (s == kSteps - 1) fetch(st[kOdd], i + lead + 2, st[kOdd].next);
+        if (s >= kSteps - 2 * kWords) {
+          const int x = s - (kSteps - 2 * kWords);
+          if (x < kWords) put_k(st[kOdd], kOdd, x);
+          else put_v(to, st[kOdd], i + 2, x - kWords);
+        }
+        if (s == kSteps - 1) fetch(st[kOdd], i + 4, st[kOdd].next);
         __builtin_amdgcn_sched_barrier(0);
       }
-      if (i > nfull) nan_blocks(i - 1, 1 - kOdd);
+      if (i > nfull) nan_blocks(i - 1);
       if (moved) {                       // (after O += V(i - 1) P(i - 1), whose weights had the old maximum)
 #pragma unroll
         for (int d = 0; d < kDims; ++d) O[d] *= alpha;
@@ -324,26 +327,27 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
     };
     typedef std::integral_constant<int, 0> even_t;
     typedef std::integral_constant<int, 1> odd_t;
-    auto finish = [&](int parity, const Weights<TWO>& P) {        // V(n - 1) P(n - 1)
+    auto finish = [&](const Weights<TWO>& P) {               // V(n - 1) P(n - 1)
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
-        const bf16x8 vop = val_op(s_v + parity * kTileB, s >> 1, s & 1);
+        const bf16x8 vop = val_op(s_v + ((n - 1) & 3) * kTileB, s >> 1, s & 1);
         O[s >> 1] = value_product(vop, P, s & 1, O[s >> 1]);
       }
-      if (n > nfull) nan_blocks(n - 1, parity);
+      if (n > nfull) nan_blocks(n - 1);
     };
 #pragma unroll 1
     for (int i = 0; i < n; i += 2) {
       body(even_t(), i, S0, S1, P1, P0);
       if (i + 1 < n) body(odd_t(), i + 1, S1, S0, P0, P1);
     }
-    if (n & 1) finish(0, P0);
-    else finish(1, P1);
+    if (n & 1) finish(P0);
+    else finish(P1);
     if (!TWO) {
       if (wide) s_wide = 1;
 #pragma unroll
       for (int d = 0; d < kDims; ++d)    // (a reference of 0: all values were)
-        O[d] *= __uint_as_float(max(s_ref[0][d * 128 / D], s_ref[1][d * 128 / D]) << 23);
+        O[d] *= __uint_as_float(max(max(s_ref[0][d * 256 / D], s_ref[1][d * 256 / D]),
+                                    max(s_ref[2][d * 256 / D], s_ref[3][d * 256 / D])) << 23);
     }
   }
   if (!TWO) {
