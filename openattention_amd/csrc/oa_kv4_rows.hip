@@ -104,7 +104,10 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
   const int skey = tid >> 3, sg = tid & 7;
   const int* trow = a.table + (long)b * a.t_st;
   const int pmask = (1 << a.lp) - 1;
-  const unsigned long headc = ((unsigned long)head << a.lp) * (D / 2), heads = ((unsigned long)head << a.lp) * (D / 32);
+  const uint8_t* const kc = a.kc + ((long)head << a.lp) * (D / 2);
+  const uint8_t* const vc = a.vc + ((long)head << a.lp) * (D / 2);
+  const uint8_t* const ks = a.ks + ((long)head << a.lp) * (D / 32);
+  const uint8_t* const vs = a.vs + ((long)head << a.lp) * (D / 32);
   const unsigned oc = skey * (D / 2) + sg * (D / 16), os = skey * (D / 32) + sg * D / 256;
   typedef unsigned words __attribute__((ext_vector_type(kWords)));
   // two tiles' codes are on their way, by parity
@@ -114,17 +117,17 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
     int next;                            // the table's entry for the tile after the next
   } st[2];
   auto page_at = [&](int tile) { return table_entry(trow, min((k0 + tile * kTile) >> a.lp, a.width - 1)); };
-  auto fetch = [&](Staged& x, int tile, int entry) {       // (past the last tile: read, never used)
-    const unsigned page = __builtin_amdgcn_readfirstlane(entry);
+  auto fetch = [&](Staged& x, int tile, unsigned page) {   // (past the last tile: read, never used)
+    // (by lane, though all have the same page: one multiply-add to an address instead of some 20 scalar steps)
     const bool bad = page >= (unsigned)a.NP;
     x.bad = bad ? 0x7f800000u : 0u;
-    const unsigned pg = bad ? 0 : page, off = (k0 + tile * kTile) & pmask;
-    const unsigned long bc = (unsigned long)pg * (unsigned)a.c_sp + headc + off * (D / 2);
-    const unsigned long bs = (unsigned long)pg * (unsigned)a.s_sp + heads + off * (D / 32);
-    x.k = *reinterpret_cast<const words*>(a.kc + bc + oc);
-    x.ks = (a.ks + bs)[os];
-    x.v = *reinterpret_cast<const words*>(a.vc + bc + oc);
-    x.vs = (a.vs + bs)[os];
+    const unsigned pg = bad ? 0u : page, off = (k0 + tile * kTile) & pmask;
+    const unsigned long rc = (unsigned long)pg * (unsigned)a.c_sp + (oc + off * (D / 2));
+    const unsigned long rs = (unsigned long)pg * (unsigned)a.s_sp + (os + off * (D / 32));
+    x.k = *reinterpret_cast<const words*>(kc + rc);
+    x.ks = ks[rs];
+    x.v = *reinterpret_cast<const words*>(vc + rc);
+    x.vs = vs[rs];
     x.next = page_at(tile + 2);
   };
   char* const sdst = s_t + skey * kRowB + sg * (D / 4);
