@@ -10,7 +10,10 @@ n - 1 of the cache C.K[l], C.V[l] before the attention runs, and n lives on the 
 token -- is captured once in a hipGraph and replayed with n advancing on the device.
 
 With `method` an OursHIP the attention is its decode (the gfx950 sparse stage); with
-method = None it is the dense split-K decode kernel over [0, n) on the same cache.
+method = None it is the dense split-K decode kernel over [0, n) on the same cache.  With `cache` a
+KV4Cache keys and values are held in 4 bits in its pages instead: the step extends every sequence by
+its token, and positions and lengths are the cache's, one for each sequence.  `qk_norm` gives every
+layer norms of the query and key heads.
 
 `prefill` runs a prompt through the model one batch row at a time, as the reference's runner
 does (graph_runner.py:615-622): every layer's attention goes through the hook's prefill branch
@@ -26,7 +29,7 @@ import torch
 import types
 
 from openattention_amd import ops
-from openattention_amd.method import C as CTX, Method, attn_hook
+from openattention_amd.method import C as CTX, Method, attn_hook, prefill_attention
 from openattention_amd.synth import llama31_inv_freq
 
 HID, NLAYER, HQ, HKV, D, FFN, VOCAB = 4096, 32, 32, 8, 128, 14336, 128256
@@ -48,11 +51,15 @@ def rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
 
 
 class LlamaShaped:
-    def __init__(self, B: int, Lmax: int, dev, layers: int = NLAYER, seed: int = 0, method=None):
+    def __init__(self, B: int, Lmax: int, dev, layers: int = NLAYER, seed: int = 0, method=None, cache=None,
+                 qk_norm: bool = False):
         """method: an OursHIP over these layers (sparse attention) or None (dense attention).
-        The KV cache is C.K / C.V (set by the caller), (B, 8, Lmax, 128) bf16 per layer."""
+        The KV cache is C.K / C.V (set by the caller), (B, 8, Lmax, 128) bf16 per layer, or `cache`, a
+        KV4Cache of B requests and these layers (method None)."""
+        if cache is not None and (method is not None or cache.B != B or cache.layers != layers):
+            raise ValueError("cache: for B requests and these layers, without a method")
         self.B, self.Lmax, self.dev, self.L = B, Lmax, dev, layers
-        self.method = method
+        self.method, self.cache, self.qk_norm = method, cache, qk_norm
         g = torch.Generator(device=dev).manual_seed(seed)
 
         def w(*shape):
@@ -73,6 +80,8 @@ class LlamaShaped:
         fr = torch.outer(t, inv)
         emb = torch.cat([fr, fr], -1)
         self.cos, self.sin = emb.cos(), emb.sin()                       # (Lmax, D) fp32
+        self.half = self.cos[:, :D // 2], self.sin[:, :D // 2]           # (a head's halves turn by the same angles)
+        self.qn, self.kn = ([1 + w(D) * 5 for _ in range(layers)] if qk_norm else [None] * layers for _ in range(2))
         self.tok = torch.zeros(B, device=dev, dtype=torch.long)         # token at position n - 1
         self.ws = None
         self.mods = [types.SimpleNamespace(layer_idx=l) for l in range(layers)]
@@ -99,29 +108,45 @@ class LlamaShaped:
             self.probes[l] = p
         return self.probes
 
+    def _qkv(self, l: int, qkv: torch.Tensor, pos: torch.Tensor):
+        """Layer l's query and key rows of a product, normalised where the model has head norms and turned
+        to their positions, and its value rows, each (N, heads, D)."""
+        N = qkv.shape[0]
+        q, k = ops.qk_norm_rope(qkv[:, :HQ * D].view(N, HQ, D), qkv[:, HQ * D:(HQ + HKV) * D].view(N, HKV, D), pos,
+                                *self.half, self.qn[l], self.kn[l], EPS)
+        return q, k, qkv[:, (HQ + HKV) * D:].view(N, HKV, D)
+
     @torch.no_grad()
     def prefill(self, tokens: torch.Tensor, qlen: int = 64) -> torch.Tensor:
         """Prompt prefill of every batch row (tokens (B, T) int64), one row at a time through all
         layers (graph_runner.py:615-622).  Each layer's attention is attn_hook's prefill branch:
         the row's K, V are written to C.K[l][b, :, :T], its causal attention is dense and the
         method builds the row's index (C.qlen[b] = qlen question rows).  Leaves C.phase at
-        "decode" and the greedy next token of every row in self.tok; returns it."""
+        "decode" and the greedy next token of every row in self.tok; returns it.  With a 4-bit cache the
+        row extends its request there (an empty one), its keys and values are written to the new slots and
+        its own attention is dense over the unrounded rows."""
         B, T = tokens.shape
         if B != self.B or T > self.Lmax:
             raise ValueError(f"tokens must be ({self.B}, <= {self.Lmax})")
+        if self.cache is not None:
+            return self._prefill_cache(tokens)
         CTX.phase = "prefill"
         CTX.qlen = [qlen] * B
         CTX.method = self.method if self.method is not None else Method(None, B, self.Lmax, self.dev)
         cos, sin = self.cos[:T].unsqueeze(1), self.sin[:T].unsqueeze(1)           # (T, 1, D)
+        where = torch.arange(T, device=self.dev)
         for b in range(B):
             CTX.brow = b
             x = self.embed.index_select(0, tokens[b])                              # (T, HID)
             for l in range(self.L):
                 h = rmsnorm(x, self.ln1[l])
                 qkv = h @ self.wqkv[l]
-                q = rope(qkv[:, :HQ * D].view(T, HQ, D), cos, sin).transpose(0, 1).unsqueeze(0)
-                k = rope(qkv[:, HQ * D:(HQ + HKV) * D].view(T, HKV, D), cos, sin).transpose(0, 1).unsqueeze(0)
-                v = qkv[:, (HQ + HKV) * D:].view(T, HKV, D).transpose(0, 1).unsqueeze(0)
+                if self.qk_norm:
+                    q, k, v = (t.transpose(0, 1).unsqueeze(0) for t in self._qkv(l, qkv, where))
+                else:
+                    q = rope(qkv[:, :HQ * D].view(T, HQ, D), cos, sin).transpose(0, 1).unsqueeze(0)
+                    k = rope(qkv[:, HQ * D:(HQ + HKV) * D].view(T, HKV, D), cos, sin).transpose(0, 1).unsqueeze(0)
+                    v = qkv[:, (HQ + HKV) * D:].view(T, HKV, D).transpose(0, 1).unsqueeze(0)
                 del qkv
                 o, _ = attn_hook(self.mods[l], q, k, v, None)                       # (1, T, HQ, D)
                 x = x + o.reshape(T, HQ * D) @ self.wo[l]
@@ -135,11 +160,57 @@ class LlamaShaped:
         CTX.phase = "decode"
         return self.tok
 
+    def _prefill_cache(self, tokens: torch.Tensor) -> torch.Tensor:
+        B, T = tokens.shape
+        cache = self.cache
+        if bool((cache.lens != 0).any()):
+            raise ValueError("prefill: the cache's requests must be empty (KV4Cache.truncate)")
+        for b in range(B):
+            add = torch.zeros(B, device=self.dev, dtype=torch.int32)
+            add[b] = T
+            slots, pos, _ = cache.extend(add, T)
+            cache.check()
+            x = self.embed.index_select(0, tokens[b])                              # (T, HID)
+            for l in range(self.L):
+                h = rmsnorm(x, self.ln1[l])
+                q, k, v = self._qkv(l, h @ self.wqkv[l], pos)
+                cache.write(l, k, v, slots)
+                o = prefill_attention(*(t.transpose(0, 1).unsqueeze(0) for t in (q, k, v)), D ** -0.5)
+                x = x + o[0].transpose(0, 1).reshape(T, HQ * D) @ self.wo[l]
+                del q, k, v, o
+                h = rmsnorm(x, self.ln2[l])
+                gu = h @ self.w13[l]
+                x = x + (torch.nn.functional.silu(gu[:, :FFN]) * gu[:, FFN:]) @ self.w2[l]
+                del gu
+            logits = rmsnorm(x[-1:], self.lnf) @ self.lm_head
+            self.tok[b] = logits.argmax(-1)[0]
+        return self.tok
+
+    def _step_cache(self) -> torch.Tensor:
+        B, cache = self.B, self.cache
+        slots, pos, _ = cache.extend()
+        x = self.embed.index_select(0, self.tok)                        # (B, HID)
+        for l in range(self.L):
+            h = rmsnorm(x, self.ln1[l])
+            q, k, v = self._qkv(l, h @ self.wqkv[l], pos)
+            cache.write(l, k, v, slots)
+            x = x + cache.attend(l, q).view(B, HQ * D) @ self.wo[l]
+            h = rmsnorm(x, self.ln2[l])
+            gu = h @ self.w13[l]
+            x = x + (torch.nn.functional.silu(gu[:, :FFN]) * gu[:, FFN:]) @ self.w2[l]
+        logits = rmsnorm(x, self.lnf) @ self.lm_head
+        self.tok.copy_(logits.argmax(-1))
+        return self.tok
+
     @torch.no_grad()
-    def step(self, n: int) -> torch.Tensor:
+    def step(self, n: int | None = None) -> torch.Tensor:
         """One decode step: the token in self.tok sits at position n - 1 (n = C.n_dev on the
         device; the host n only fixes the sparse stage's sink/local/top-k counts).  Writes the
-        greedy next token into self.tok and returns it."""
+        greedy next token into self.tok and returns it.  With a 4-bit cache n is not used: each token
+        sits at its request's length, which the step extends (a step that the cache refuses, out of
+        pages or past max_len, leaves lengths and rows as they were: KV4Cache.check)."""
+        if self.cache is not None:
+            return self._step_cache()
         B = self.B
         pos = (CTX.n_dev - 1).long()                                    # (1,) on the device
         cos = self.cos.index_select(0, pos).unsqueeze(0)                # (1, 1, D)
@@ -148,9 +219,12 @@ class LlamaShaped:
         for l in range(self.L):
             h = rmsnorm(x, self.ln1[l])
             qkv = h @ self.wqkv[l]
-            q = rope(qkv[:, :HQ * D].view(B, HQ, D), cos, sin)
-            k = rope(qkv[:, HQ * D:(HQ + HKV) * D].view(B, HKV, D), cos, sin)
-            v = qkv[:, (HQ + HKV) * D:].view(B, HKV, D)
+            if self.qk_norm:
+                q, k, v = self._qkv(l, qkv, pos.expand(B).contiguous())
+            else:
+                q = rope(qkv[:, :HQ * D].view(B, HQ, D), cos, sin)
+                k = rope(qkv[:, HQ * D:(HQ + HKV) * D].view(B, HKV, D), cos, sin)
+                v = qkv[:, (HQ + HKV) * D:].view(B, HKV, D)
             CTX.K[l].index_copy_(2, pos, k.unsqueeze(2))
             CTX.V[l].index_copy_(2, pos, v.unsqueeze(2))
             p = self.probes.get(l)
