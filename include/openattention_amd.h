@@ -572,7 +572,9 @@ int oa_qk_norm_rope(const void* q, long q_st, long q_sh, const void* k, long k_s
  *
  * Either takes effect for all requests or for none; then nothing changes (an extension's slots, pos are -1,
  * its cu 0) and *status |= 1 (a negative count, a length outside of the table's row), 2 (too few free pages,
- * or more than the stack holds), 4 (more than total tokens).  ws: 3 requests + 1 ints of scratch.
+ * or more than the stack holds), 4 (more than total tokens).  ws: 3 requests + 1 ints of scratch; NULL
+ * will do for an extension of at most 1024 requests by at most 2048 tokens and a truncation of at most 256
+ * requests.
  */
 int oa_kv_pages_extend(const int* add, int* lens, int* table, long table_stride, int* free, int* nfree, int* status,
                        int requests, int width, int pages, int page, int total, int* slots, int* pos, int* cu, int* ws,

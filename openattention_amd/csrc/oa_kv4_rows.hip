@@ -81,6 +81,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
   __shared__ unsigned s_ref[kWaves][8];                    // largest scales of the first V tile, by wave and part
   __shared__ unsigned s_wide;                              // a scale is out of fp16's span
 
+  if (TWO && !a.ws_flag[blockIdx.x]) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n32 = lane & 31, h = lane >> 5;
   const int units = a.B * a.HKV;
@@ -89,13 +90,13 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
   const int b = bh / a.HKV, head = bh - b * a.HKV;
   const Seq sq = seq_of(a, b);
   const int rows = min(sq.R, a.max_q) * a.G;
+  if (!TWO && tid == 0) a.ws_flag[blockIdx.x] = 0;
   if (row0 >= rows) return;
   const int first = sq.n - sq.R;         // position of the sequence's first query token
   const int hi = sq.bad ? 0 : first + (min(row0 + kRows, rows) - 1) / a.G + 1;         // keys any row sees
   const int all = first + row0 / a.G + 1;                                              // keys every row sees
   const int k0 = ch * a.chunk, k1 = min(k0 + a.chunk, hi);
   if (k0 >= k1 && a.nchunk > 1) return;
-  if (TWO && !a.ws_flag[blockIdx.x]) return;
   const int n = max(0, (k1 - k0 + kTile - 1) / kTile);     // tiles
   const int nfull = min(n, max(0, (all - k0) / kTile));    // those that every row sees whole
 
@@ -355,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
   }
   if (!TWO) {
     oa::lds_barrier();
-    if (tid == 0) a.ws_flag[blockIdx.x] = (int)s_wide;
+    if (tid == 0 && s_wide) a.ws_flag[blockIdx.x] = 1;
   }
 
   const auto lx = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);

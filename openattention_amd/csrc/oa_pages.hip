@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(THREADS) pages_extend_kernel(PagesArgs a, int 
     page0 += t1;
   }
   if (tid == 0) {
-    a.ws[2 * a.B] = nfree;
+    if (!alone) a.ws[2 * a.B] = nfree;
     if (!bad) *a.nfree = nfree - (int)pages;
   }
   if (!alone) return;
@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(THREADS) pages_truncate_kernel(PagesArgs a, in
     page0 = add_to(page0, t0);
   }
   if (tid == 0) {
-    a.ws[2 * a.B] = top;
+    if (!alone) a.ws[2 * a.B] = top;
     if (bad) *a.status |= 2;
     else *a.nfree = top;
   }
@@ -287,7 +287,7 @@ constexpr int kAloneRows = 256;
 
 int take(PagesArgs& a, const int* count, int* lens, int* table, long t_st, int* free, int* nfree, int* status, int B,
          int width, int NP, int page, int* ws) {
-  if (!count || !lens || !table || !free || !nfree || !status || !ws || B <= 0 || width <= 0 || t_st < width || NP <= 0 ||
+  if (!count || !lens || !table || !free || !nfree || !status || B <= 0 || width <= 0 || t_st < width || NP <= 0 ||
       page < 32 || page > 1024 || (page & (page - 1)) || (long)NP * page > 0x7fffffffL || (long)width * page > (1L << 30) ||
       B > (1 << 24))
     return OA_EINVAL;
@@ -304,7 +304,8 @@ extern "C" int oa_kv_pages_extend(const int* add, int* lens, int* table, long ta
                                   int* pos, int* cu, int* ws, void* stream) {
   PagesArgs a;
   if (const int e = take(a, add, lens, table, table_stride, free, nfree, status, requests, width, pages, page, ws)) return e;
-  if (total < 0 || total > 0x7fffff00 || (total && (!slots || !pos)) || !cu) return OA_EINVAL;
+  if (total < 0 || total > 0x7fffff00 || (total && (!slots || !pos)) || !cu || (!ws && (requests > kMost || total > kAlone)))
+    return OA_EINVAL;
   a.total = total; a.slots = slots; a.pos = pos; a.cu = cu;
   const hipStream_t st = (hipStream_t)stream;
   const int alone = total <= kAlone;
@@ -319,6 +320,7 @@ extern "C" int oa_kv_pages_truncate(const int* keep, int* lens, int* table, long
                                     int* status, int requests, int width, int pages, int page, int* ws, void* stream) {
   PagesArgs a;
   if (const int e = take(a, keep, lens, table, table_stride, free, nfree, status, requests, width, pages, page, ws)) return e;
+  if (!ws && requests > kAloneRows) return OA_EINVAL;
   const hipStream_t st = (hipStream_t)stream;
   const int alone = requests <= kAloneRows;
   if (requests <= 16) hipLaunchKernelGGL(pages_truncate_kernel<64>, dim3(1), dim3(64), 0, st, a, alone);

@@ -735,21 +735,22 @@ def qk_norm_rope(q, k, pos, cos, sin, wq=None, wk=None, eps: float = 1e-6, q_out
     or more NaN.  Returns (q_out, k_out), contiguous unless given; either may be its input."""
     i = _where(q, k, pos, cos, sin, wq, wk, q_out, k_out)
     dt = q.dtype
-    if q.dim() != 3 or k.dim() != 3 or k.shape[::2] != q.shape[::2] or dt not in _DT or k.dtype is not dt:
+    if q.dim() != 3 or k.dim() != 3 or dt not in _DT or k.dtype is not dt:
         raise ValueError("q, k: (T, HQ, D) and (T, HKV, D), both bf16, fp16 or fp32")
     T, HQ, Dh = q.shape
-    HKV = k.shape[1]
-    if Dh not in (64, 128, 256) or T * (HQ + HKV) > 1 << 27:
-        raise ValueError(f"head dimension 64, 128 or 256 (got {Dh}), at most 2^27 rows")
+    Tk, HKV, Dk = k.shape
+    if Tk != T or Dk != Dh or Dh not in (64, 128, 256) or T * (HQ + HKV) > 1 << 27:
+        raise ValueError(f"q, k: the same tokens, heads of 64, 128 or 256 (got {Dh}, {Dk}), at most 2^27 rows")
     pt = pos.dtype
-    if pt not in (torch.int32, torch.int64) or pos.shape != (T,) or T > 1 and pos.stride(0) != 1:
+    if pt is not torch.int32 and pt is not torch.int64 or pos.shape != (T,) or T > 1 and pos.stride(0) != 1:
         raise ValueError(f"pos: ({T},) int32 or int64, contiguous")
+    half = Dh // 2
     P = cos.shape[0]
-    cst, sst, cp, sp = cos.stride(), sin.stride(), cos.data_ptr(), sin.data_ptr()
-    if (cos.shape != (P, Dh // 2) or sin.shape != cos.shape or cos.dtype is not torch.float32
-            or sin.dtype is not torch.float32 or P < 1 or cst != sst or cst[1] != 1 or P > 1 and cst[0] % 4
+    cst, cp, sp = cos.stride(), cos.data_ptr(), sin.data_ptr()
+    if (cos.shape != (P, half) or sin.shape != cos.shape or cos.dtype is not torch.float32
+            or sin.dtype is not torch.float32 or P < 1 or cst != sin.stride() or cst[1] != 1 or P > 1 and cst[0] % 4
             or (cp | sp) % 16):
-        raise ValueError(f"cos, sin: (positions, {Dh // 2}) fp32 rows of one stride, starting at multiples of 16 bytes")
+        raise ValueError(f"cos, sin: (positions, {half}) fp32 rows of one stride, starting at multiples of 16 bytes")
     wqp = wkp = None
     if wq is not None:
         wqp = wq.data_ptr()
@@ -763,14 +764,21 @@ def qk_norm_rope(q, k, pos, cos, sin, wq=None, wk=None, eps: float = 1e-6, q_out
         raise ValueError("eps: not negative")
     _plain(q, k, cos, sin, wq, wk, q_out, k_out)
     if q_out is None:
-        q_out = q.new_empty((T, HQ, Dh))
+        q_out = q.new_empty(T, HQ, Dh)
+        qo = q_out.data_ptr(), HQ * Dh, Dh
+    else:
+        if q_out.shape != q.shape or q_out.dtype is not dt:
+            raise ValueError("q_out: as q")
+        qo = _rows(q_out, T, HQ, Dh, "q_out", True)
     if k_out is None:
-        k_out = k.new_empty((T, HKV, Dh))
-    if q_out.shape != q.shape or k_out.shape != k.shape or q_out.dtype is not dt or k_out.dtype is not dt:
-        raise ValueError("q_out, k_out: as q, k")
+        k_out = k.new_empty(T, HKV, Dh)
+        ko = k_out.data_ptr(), HKV * Dh, Dh
+    else:
+        if k_out.shape != k.shape or k_out.dtype is not dt:
+            raise ValueError("k_out: as k")
+        ko = _rows(k_out, T, HKV, Dh, "k_out", True)
     _run(i, "oa_qk_norm_rope", *_rows(q, T, HQ, Dh, "q"), *_rows(k, T, HKV, Dh, "k"), T, HQ, HKV, Dh, _DT[dt],
-         pos.data_ptr(), pt is torch.int64, cp, sp, cst[0] if P > 1 else 0, P, wqp, wkp, eps,
-         *_rows(q_out, T, HQ, Dh, "q_out", True), *_rows(k_out, T, HKV, Dh, "k_out", True))
+         pos.data_ptr(), pt is torch.int64, cp, sp, cst[0] if P > 1 else 0, P, wqp, wkp, eps, *qo, *ko)
     return q_out, k_out
 
 
@@ -814,9 +822,9 @@ def kv_pages_extend(add, lens, table, free, nfree, status, page: int, total: int
     if not 0 <= total <= 1 << 30:
         raise ValueError("total: 0 to 2^30")
     B = st[7]
-    slots, pos, cu, ws = add.new_empty(2 * total + 4 * B + 2).split((total, total, B + 1, 3 * B + 1))
-    p = cu.data_ptr()
-    _run(i, "oa_kv_pages_extend", *st, total, p - 8 * total, p - 4 * total, p, p + 4 * B + 4)
+    slots, pos, cu = add.new_empty(total), add.new_empty(total), add.new_empty(B + 1)
+    ws = add.new_empty(3 * B + 1) if B > 1024 or total > 2048 else None
+    _run(i, "oa_kv_pages_extend", *st, total, slots.data_ptr(), pos.data_ptr(), cu.data_ptr(), _ptr(ws))
     return slots, pos, cu
 
 
@@ -826,8 +834,8 @@ def kv_pages_truncate(keep, lens, table, free, nfree, status, page: int) -> None
     an extension undoes it.  Nothing changes where the stack would outgrow `free` (status |= 2)."""
     i = _where(keep, lens, table, free, nfree, status)
     st = _pages_state(keep, lens, table, free, nfree, status, page, "keep")
-    ws = keep.new_empty(3 * st[7] + 1)
-    _run(i, "oa_kv_pages_truncate", *st, ws.data_ptr())
+    ws = keep.new_empty(3 * st[7] + 1) if st[7] > 256 else None
+    _run(i, "oa_kv_pages_truncate", *st, _ptr(ws))
 
 
 def _kv4_cache(kc, ks, vc, vs) -> tuple:
@@ -878,8 +886,8 @@ def kv4_read(slots, kc, ks, vc, vs, dtype: torch.dtype = torch.bfloat16):
     sp = _ints(slots, T, "slots")
     if dtype not in (torch.bfloat16, torch.float32) or T * HKV > 1 << 26:
         raise ValueError("dtype: bf16 or fp32; at most 2^26 rows")
-    k = kc.new_empty((T, HKV, Dh), dtype=dtype)
-    v = kc.new_empty((T, HKV, Dh), dtype=dtype)
+    k = kc.new_empty(T, HKV, Dh, dtype=dtype)
+    v = kc.new_empty(T, HKV, Dh, dtype=dtype)
     _run(i, "oa_kv4_read", sp, *ps, *where, k.data_ptr(), HKV * Dh, Dh, v.data_ptr(), HKV * Dh, Dh, T, HKV, Dh, _DT[dtype])
     return k, v
 
@@ -922,10 +930,12 @@ def kv4_attn(q, kc, ks, vc, vs, table, lens, sm_scale: float | None = None, cu_q
     _plain(q, out)
     qa = _rows(q, T, HQ, Dh, "q")
     if out is None:
-        out = q.new_empty((T, HQ, Dh)) if cp is None else q.new_zeros((T, HQ, Dh))
+        out = q.new_empty(T, HQ, Dh) if cp is None else q.new_zeros(T, HQ, Dh)
+        oa = out.data_ptr(), HQ * Dh, Dh
     elif out.shape != q.shape or out.dtype is not torch.bfloat16:
         raise ValueError("out: as q")
-    oa = _rows(out, T, HQ, Dh, "out", True)
+    else:
+        oa = _rows(out, T, HQ, Dh, "out", True)
     if T == 0 or B == 0:
         return out
     rows = max_q * G

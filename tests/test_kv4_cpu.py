@@ -94,12 +94,16 @@ def test_pages_hand_on_their_buffers(calls):
         ops.kv_pages_extend(torch.zeros(3, dtype=torch.int32), **a, total=-1)
     slots, pos, cu = ops.kv_pages_extend(torch.zeros(3, dtype=torch.int32), **a, total=7)
     (name, c), = calls
-    assert len(c) + 1 == len(lib.SIGNATURES[name]) and c[12:15] == (slots.data_ptr(), pos.data_ptr(), cu.data_ptr())
-    assert slots.shape == pos.shape == (7,) and cu.shape == (4,) and c[15] == cu.data_ptr() + 16
-    # the scratch (3 B + 1) ends inside the buffer
-    assert c[15] + 4 * 10 <= slots.untyped_storage().data_ptr() + slots.untyped_storage().nbytes()
+    assert len(c) + 1 == len(lib.SIGNATURES[name]) and c[12:] == (slots.data_ptr(), pos.data_ptr(), cu.data_ptr(), None)
+    assert slots.shape == pos.shape == (7,) and cu.shape == (4,)
     ops.kv_pages_truncate(torch.zeros(3, dtype=torch.int32), **a)
-    assert len(calls[1][1]) + 1 == len(lib.SIGNATURES["oa_kv_pages_truncate"])
+    assert len(calls[1][1]) + 1 == len(lib.SIGNATURES["oa_kv_pages_truncate"]) and calls[1][1][-1] is None
+    # scratch where a second launch needs it
+    ops.kv_pages_extend(torch.zeros(3, dtype=torch.int32), **a, total=2049)
+    many = pool(B=1025)
+    ops.kv_pages_extend(torch.zeros(1025, dtype=torch.int32), **many, total=7)
+    ops.kv_pages_truncate(torch.zeros(1025, dtype=torch.int32), **many)
+    assert all(c[1][-1] is not None for c in calls[2:])
 
 
 def cache(NP=4, H=2, page=32, D=128, **kw):
@@ -202,10 +206,11 @@ def test_library_refuses_before_a_launch():
         assert L.oa_qk_norm_rope(*rope[:i], v, *rope[i + 1:]) == -22, (i, v)
     assert L.oa_qk_norm_rope(*rope[:6], 0, *rope[7:]) == 0
     ext = [16, 16, 16, 4, 16, 16, 16, 3, 4, 9, 64, 7, 16, 16, 16, 16, None]
-    for i, v in ((0, None), (2, None), (3, 3), (7, 0), (8, 0), (9, 0), (10, 48), (10, 16), (10, 2048), (11, -1), (12, None), (14, None), (15, None),
+    for i, v in ((0, None), (2, None), (3, 3), (7, 0), (8, 0), (9, 0), (10, 48), (10, 16), (10, 2048), (11, -1), (12, None), (14, None),
                  (9, 1 << 26), (8, 1 << 25)):
         assert L.oa_kv_pages_extend(*ext[:i], v, *ext[i + 1:]) == -22, (i, v)
-    assert L.oa_kv_pages_truncate(16, 16, 16, 4, 16, 16, 16, 3, 4, 9, 64, None, None) == -22
+    assert L.oa_kv_pages_extend(*ext[:7], 1025, *ext[8:15], None, None) == -22 and L.oa_kv_pages_extend(*ext[:11], 2049, *ext[12:15], None, None) == -22
+    assert L.oa_kv_pages_truncate(16, 16, 16, 4, 16, 16, 16, 257, 4, 9, 64, None, None) == -22
     wr = [16, 256, 128, 16, 256, 128, 3, 2, 128, 0, 16, 16, 16, 16, 16, 4096, 256, 4, 32, None]
     for i, v in ((0, 8), (1, 4), (6, -1), (7, 0), (8, 96), (9, 3), (10, None), (11, 8), (12, None), (15, 4080), (15, 4104), (16, 240), (17, 0), (18, 33),
                  (6, 1 << 26)):
