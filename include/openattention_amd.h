@@ -605,7 +605,7 @@ int oa_kv4_read(const int* slots, const void* kc, const void* ks, const void* vc
 /*
  * Causal attention over the 4-bit cache.  Sequence b holds lens[b] keys in the pages of its table row; its
  * query tokens are rows cu[b] .. cu[b + 1] - 1 of q (tokens, q_heads, head_dim) bf16 (cu NULL: row b alone),
- * the last of them its newest key's, so that token j of R sees keys 0 .. lens - R + j.  out as q.  fp32 scores,
+ * the last of them its newest key's, so that token j of R sees keys 0 .. lens - R + j.  out as q, not q.  fp32 scores,
  * softmax and sums; weights in 16 bits.  A row that sees no key gives 0; rows behind cu[sequences], and tokens
  * of a sequence from max_q on, are left as they were.  NaN: rows that need a page id outside of the cache, and
  * those of sequences longer than their table row or than nchunk * chunk keys.  Keys are split into nchunk pieces

@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(kThreads) kv4_join_kernel(AttnArgs a) {
   __shared__ __align__(16) float s_o[kGroups][D];
   __shared__ float s_l[kGroups];
   const int heads = a.HKV * a.G;
-  const int hd = blockIdx.x % heads, rest = blockIdx.x / heads, j = rest % a.max_q, b = rest / a.max_q;
+  const int hd = blockIdx.x % heads, j = blockIdx.x / heads, b = blockIdx.y;
   const Seq sq = seq_of(a, b);
   if (j >= sq.R) return;
   const int seen = sq.n - sq.R + j + 1, tid = threadIdx.x;
@@ -385,20 +385,22 @@ __global__ void __launch_bounds__(kThreads) kv4_join_kernel(AttnArgs a) {
 
 // query rows up to which every workgroup turns its own keys to bf16 (more: oa_kv4_rows.hip)
 constexpr int kFewRows = 64;
+constexpr long kGrid = 0xffffffffL / kThreads;
 
 template <int D>
 int launch(AttnArgs a, hipStream_t st) {
   const long rows = (long)a.max_q * a.G;
   const int cols = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= kFewRows ? 32 : 128;
   a.ntile = (int)((rows + cols - 1) / cols);
-  const long blocks = (long)a.ntile * a.nchunk * a.B * a.HKV, joins = (long)a.B * a.max_q * a.HKV * a.G;
-  if (blocks > 0x7fffffffL || joins > 0x7fffffffL) return OA_EINVAL;
+  const long blocks = (long)a.ntile * a.nchunk * a.B * a.HKV, joins = (long)a.max_q * a.HKV * a.G;
+  // (a grid's threads along one axis are counted in 32 bits)
+  if (blocks > kGrid || (a.nchunk > 1 && (joins > kGrid || a.B > 65535))) return OA_EINVAL;
   const dim3 grid((unsigned)blocks), blk(kThreads);
   if (cols == 8) hipLaunchKernelGGL((kv4_attn_kernel<D, 1, true>), grid, blk, 0, st, a);
   else if (cols == 16) hipLaunchKernelGGL((kv4_attn_kernel<D, 1, false>), grid, blk, 0, st, a);
   else if (cols == 32) hipLaunchKernelGGL((kv4_attn_kernel<D, 2, false>), grid, blk, 0, st, a);
   else launch_rows(a, D, grid, st);
-  if (a.nchunk > 1) hipLaunchKernelGGL((kv4_join_kernel<D>), dim3((unsigned)joins), blk, 0, st, a);
+  if (a.nchunk > 1) hipLaunchKernelGGL((kv4_join_kernel<D>), dim3((unsigned)joins, a.B), blk, 0, st, a);
   return OA_LAUNCH_STATUS();
 }
 
@@ -422,6 +424,7 @@ extern "C" int oa_kv4_attn(const void* q, long q_st, long q_sh, const void* kc, 
       scale_stride < (long)kv_heads * page * (head_dim / 32) || code_stride % 16 || scale_stride % 16 ||
       code_stride > 0xffffffffL || scale_stride > 0xffffffffL || !(sm_scale == sm_scale))
     return OA_EINVAL;
+  if (out == q) return OA_EINVAL;        // (rows may be read again after others were written)
   if ((nchunk > 1 && (odd(ws_o, 16) || odd(ws_ml, 8))) || ((long)max_q * (q_heads / kv_heads) > kFewRows && odd(ws_flag, 4)))
     return OA_EINVAL;
   AttnArgs a;

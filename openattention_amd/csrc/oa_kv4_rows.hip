@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
         } else if (s == 1) {
           const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
           mx = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * c;
-          moved = __any(mx > m + kLazy);
+          moved = __any(mx > m + (big ? 0.f : kLazy));
           if (moved) {
             const float mn = fmaxf(m, mx);
             alpha = __builtin_amdgcn_exp2f(m - mn);

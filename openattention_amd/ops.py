@@ -892,12 +892,15 @@ def kv4_read(slots, kc, ks, vc, vs, dtype: torch.dtype = torch.bfloat16):
     return k, v
 
 
-def kv4_chunk(cap: int, units: int) -> int:
-    """Keys per workgroup of kv4_attn, for `units` (sequence, KV head, query tile) triples of up to `cap` keys:
-    two workgroups to a compute unit, but pieces of at least 384 keys (their start and end cost as much
-    as some 300 keys) and at most an eighth of the longest sequence (or 1024), so that a batch does not
-    wait for one piece of it."""
-    n = max(min(max(cap * units // 512, 384), max(cap // 8, 1024)), 384)
+def kv4_chunk(cap: int, units: int, rows: int) -> int:
+    """Keys per workgroup of kv4_attn, for `units` (sequence, KV head, query tile) triples of up to `cap` keys and
+    `rows` query rows: two workgroups to a compute unit, but pieces of at least 384 keys (their start and end
+    cost as much as some 300).  Where the rows are few and reading keys is the work, at most an eighth of the
+    longest sequence (or 1024), so that a batch does not wait for one piece of it: 61 sequences of 1 to
+    16001 keys take 62 us in pieces of 4096 and 48 in pieces of 2048."""
+    n = max(cap * units // 512, 384)
+    if rows <= 64:
+        n = max(min(n, max(cap // 8, 1024)), 384)
     return min(-(-n // 128), -(-cap // 128)) * 128
 
 
@@ -910,7 +913,8 @@ def kv4_attn(q, kc, ks, vc, vs, table, lens, sm_scale: float | None = None, cu_q
     Token j of R sees keys 0 .. lens[b] - R + j; one that sees none gives 0.  max_len: a bound on lens
     that the caller knows (the table's width otherwise).  NaN: rows that need a page id outside of the
     cache, and those of sequences longer than their table row or than max_len (rounded up to whole pieces,
-    kv4_chunk).  Rows of `out` behind cu_q[B] are left as they were (0 where the call makes it)."""
+    kv4_chunk).  Rows of `out` behind cu_q[B], and tokens past max_q, are left as they
+    were (0 where the call makes it); `out` shares no memory with q."""
     i = _where(q, kc, ks, vc, vs, table, lens, cu_q, out)
     ps, where, HKV, Dh = _kv4_cache(kc, ks, vc, vs)
     tp, ts, B, width = _table(table, where[3])
@@ -932,8 +936,8 @@ def kv4_attn(q, kc, ks, vc, vs, table, lens, sm_scale: float | None = None, cu_q
     if out is None:
         out = q.new_empty(T, HQ, Dh) if cp is None else q.new_zeros(T, HQ, Dh)
         oa = out.data_ptr(), HQ * Dh, Dh
-    elif out.shape != q.shape or out.dtype is not torch.bfloat16:
-        raise ValueError("out: as q")
+    elif out.shape != q.shape or out.dtype is not torch.bfloat16 or out.data_ptr() == qa[0]:
+        raise ValueError("out: as q, and not q itself")
     else:
         oa = _rows(out, T, HQ, Dh, "out", True)
     if T == 0 or B == 0:
@@ -941,7 +945,7 @@ def kv4_attn(q, kc, ks, vc, vs, table, lens, sm_scale: float | None = None, cu_q
     rows = max_q * G
     cap = max(1, width * where[3] if max_len is None else min(max_len, width * where[3]))
     units = B * HKV * -(-rows // (8 if rows <= 8 else 16 if rows <= 16 else 32 if rows <= 64 else 128))
-    chunk = kv4_chunk(cap, units)
+    chunk = kv4_chunk(cap, units, rows)
     nchunk = -(-cap // chunk)
     wp = mp = fp = None
     parts = T * HQ * nchunk if nchunk > 1 else 0

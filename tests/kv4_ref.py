@@ -60,7 +60,8 @@ def attn(q, k, v, n, scale, weight=2.0 ** -16):
     and the fp32 kernel's error bound beside the output's own rounding: sums of D exact products (each
     sum off by D 2^-24 of its terms' sizes, as a score and once more in the maximum), weights rounded
     to `weight` of themselves (two bf16 terms 2^-16; fp16, for more than 64 rows of a KV head, 2^-11), exponentials and sums over n keys ((n + 64) 2^-24); and what fp32 does not hold:
-    a weight, or its second term, under 2^-126 counts as 0, so that each key may be off by 2^-125 |v|."""
+    a weight, or its second term, under 2^-126 counts as 0, so that each key may be off by 2^-125 |v|; fp16
+    weights are kept times 2^7, those under 2^-21 of the largest to half of 2^-24 / 2^7: 2^-32 |v|."""
     R, HQ, D = q.shape
     HKV = k.shape[1]
     G = HQ // HKV
@@ -77,7 +78,7 @@ def attn(q, k, v, n, scale, weight=2.0 ** -16):
         out[j] = torch.matmul(w, vv).reshape(HQ, D)
         a = torch.matmul(w, vv.abs()).reshape(HQ, D)
         err[j] = a * (2 * size.reshape(HQ, 1) * (D + 4) * 2.0 ** -24 + weight + (m + 64) * 2.0 ** -24)
-        err[j] += 2.0 ** -125 * vv.abs().sum(1).repeat_interleave(G, 0)
+        err[j] += (2.0 ** -32 if weight > 2.0 ** -16 else 2.0 ** -125) * vv.abs().sum(1).repeat_interleave(G, 0)
     return out, err
 
 

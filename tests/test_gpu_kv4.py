@@ -344,7 +344,7 @@ def test_attention(case, chunk, copies, monkeypatch):
     print(f"[case] attn {CASES[case]} chunk={chunk} copies={copies}", flush=True)
     lens, rows, HQ, HKV, D, page = CASES[case]
     if chunk:
-        monkeypatch.setattr(ops, "kv4_chunk", lambda cap, units: min(chunk, -(-cap // 128) * 128))
+        monkeypatch.setattr(ops, "kv4_chunk", lambda cap, units, rows: min(chunk, -(-cap // 128) * 128))
     lens, rows = lens * copies, rows and rows * copies
     g = gen(case)
     cache, table = paged(lens, HKV, D, page, g, extra_width=case % 3)
@@ -415,22 +415,48 @@ def test_attention_of_many_sequences():
     check_attn(out, *want_attn(q, cache, table, lens, list(range(701)), 0.125, 32))
 
 
-def test_attention_scales():
-    """A negative scale, one of zero, large scores (one key takes all), and equal keys."""
+@pytest.mark.parametrize("rows", [1, 3, 33])
+def test_attention_scales(rows):
+    """A negative scale, one of zero, large scores (one key takes all), scores past what fp32 tells apart, equal
+    keys, and queries that are not finite."""
     g = gen(5)
     lens = [150, 70]
     cache, table = paged(lens, 2, 128, 32, g)
-    q = randn(g, 2, 8, 128, dtype=torch.bfloat16)
+    cu = [0, rows, 2 * rows]
+    q = randn(g, 2 * rows, 8, 128, dtype=torch.bfloat16)
+
+    def run(q, scale):
+        return ops.kv4_attn(q, *cache, table, i32(lens), scale, cu_q=i32(cu), max_q=rows)
+
     for scale in (-0.09, 0.0, 30.0):
-        out = ops.kv4_attn(q, *cache, table, i32(lens), scale)
-        check_attn(out, *want_attn(q, cache, table, lens, [0, 1, 2], scale, 32))
+        check_attn(run(q, scale), *want_attn(q, cache, table, lens, cu, scale, 32))
+    for size in (2.0 ** 22, 2.0 ** 24, 2.0 ** 27, 2.0 ** 60):
+        out = run(q, size)
+        assert not out.isnan().any()
+        # the one key that takes all, wherever fp32 tells the best two apart
+        out, err = run(q, size), None
+        for b, slots in enumerate(ref.held(table, lens, 32)):
+            k, v = (ref.rows_at(cache[i], cache[i + 1], slots.to(DEV)) for i in (0, 2))
+            for j in range(rows):
+                n = lens[b] - rows + j + 1
+                x = q[cu[b] + j].double().view(2, 4, 1, 128)
+                s = (x * k[:n].transpose(0, 1)[:, None]).sum(-1)                     # (2, 4, n)
+                size_of = (x.abs() * k[:n].transpose(0, 1)[:, None].abs()).sum(-1).amax(-1)
+                top = s.topk(2, -1)
+                clear = (top.values[..., 0] - top.values[..., 1]) > 2 * size_of * 132 * 2.0 ** -24 + 40 / size
+                want = v.transpose(0, 1)[torch.arange(2, device=DEV)[:, None], top.indices[..., 0]]
+                got = out[cu[b] + j].double().view(2, 4, 128)
+                assert clear.any() and torch.equal(got[clear], want[clear])
     k = torch.ones(150, 2, 128, device=DEV)
     slots = ref.held(table, lens, 32)[0].int().to(DEV)
     v = randn(g, 150, 2, 128)
     ops.kv4_write(k * 2.0 ** 90, v, slots, *cache)
-    q = torch.full_like(q, 2.0 ** 30)
-    out = ops.kv4_attn(q, *cache, table, i32(lens), 1e-6)
-    check_attn(out[:1], *want_attn(q[:1], cache, table[:1], lens[:1], [0, 1], 1e-6, 32))
+    check_attn(run(torch.full_like(q, 2.0 ** 30), 1e-6)[:rows],
+               *want_attn(torch.full_like(q[:rows], 2.0 ** 30), cache, table[:1], lens[:1], cu[:2], 1e-6, 32))
+    q[0, 1, 5], q[rows, 3, 9] = math.nan, math.inf
+    out = run(q, 0.1)
+    assert out[0, 1].isnan().all() and out[rows, 3].isnan().all()
+    assert not out[0, 0].isnan().any() and not out[0, 2:].isnan().any() and not out[rows, :3].isnan().any()
 
 
 @pytest.mark.parametrize("rows", [1, 3, 40])

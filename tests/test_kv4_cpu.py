@@ -170,7 +170,7 @@ def test_attention_refused(calls):
                 dict(q=torch.zeros(3, 8, 136, dtype=torch.bfloat16)[..., 4:132]), dict(q=q.clone().requires_grad_()),
                 dict(table=t.long()), dict(table=t[0]), dict(table=torch.zeros(2, 3, dtype=torch.int32).t()), dict(table=t[:, :0]),
                 dict(lens=n.long()), dict(lens=n[:2]), dict(cu_q=cu.long()), dict(cu_q=cu[:3]), dict(max_q=2), dict(cu_q=cu, max_q=0),
-                dict(cu_q=cu, max_q=-1), dict(sm_scale=float("nan")), dict(max_len=-1), dict(out=q.float()), dict(out=q[:2]),
+                dict(cu_q=cu, max_q=-1), dict(sm_scale=float("nan")), dict(max_len=-1), dict(out=q.float()), dict(out=q[:2]), dict(out=q),
                 dict(out=torch.zeros(3, 1, 128, dtype=torch.bfloat16).expand(3, 8, 128)), dict(cu_q=cu, max_q=1 << 30)):
         with pytest.raises(ValueError):
             ops.kv4_attn(**dict(ok, **bad), **c)
@@ -218,10 +218,13 @@ def test_library_refuses_before_a_launch():
     assert L.oa_kv4_write(*wr[:6], 0, *wr[7:]) == 0
     rd = [16, 16, 16, 16, 16, 4096, 256, 4, 32, 16, 256, 128, 16, 256, 128, 3, 2, 128, 0, None]
     assert L.oa_kv4_read(*rd[:18], 1, None) == -22 and L.oa_kv4_read(None, *rd[1:]) == -22
-    at = [16, 1024, 128, 16, 16, 16, 16, 4096, 256, 4, 32, 16, 2, 2, 16, None, 3, 3, 1, 8, 2, 128, 0.1, 128, 2, 16, 16, 16, 16, 1024, 128, None]
+    at = [16, 1024, 128, 16, 16, 16, 16, 4096, 256, 4, 32, 16, 2, 2, 16, None, 3, 3, 1, 8, 2, 128, 0.1, 128, 2, 16, 16, 16, 32, 1024, 128, None]
     for i, v in ((0, 8), (1, 4), (3, 8), (7, 4000), (9, 0), (10, 31), (11, None), (12, 1), (13, 0), (13, 1 << 26), (14, None), (16, 2), (18, 0), (18, 2), (19, 7), (20, 0),
-                 (21, 96), (22, float("nan")), (23, 64), (23, 200), (24, 0), (25, None), (26, None), (28, None), (29, 2), (23, 1 << 30), (24, 1 << 24)):
+                 (21, 96), (22, float("nan")), (23, 64), (23, 200), (24, 0), (25, None), (26, None), (28, None), (29, 2), (23, 1 << 30), (24, 1 << 24), (28, 16)):
         assert L.oa_kv4_attn(*at[:i], v, *at[i + 1:]) == -22, (i, v)
     assert L.oa_kv4_attn(*at[:16], 0, 0, *at[18:]) == 0
     many = [*at[:15], 16, 3, 64, 17, *at[19:]]           # 68 rows of a KV head
+    # more workgroups, or rows to join, than a grid holds
+    assert L.oa_kv4_attn(*at[:15], 16, 1 << 20, 1 << 20, 1 << 10, *at[19:]) == -22
+    assert L.oa_kv4_attn(*at[:15], 16, 3, 1 << 22, 1 << 22, *at[19:]) == -22 and L.oa_kv4_attn(*at[:15], 16, 65536, 8, 1, *at[19:]) == -22
     assert L.oa_kv4_attn(*many[:27], None, *many[28:]) == -22 and L.oa_kv4_attn(*many[:27], 2, *many[28:]) == -22
