@@ -14,6 +14,9 @@ on a HIP device and the kernel library must be built.
 """
 from __future__ import annotations
 
+import functools
+from operator import index
+
 import torch
 from torch.overrides import _get_current_function_mode_stack
 from torch.utils._device import DeviceContext
@@ -663,12 +666,15 @@ def prefill_attn(q, k, v, sm_scale: float) -> torch.Tensor:
 
 
 # ================================================================== 4-bit paged cache
-# (eager decode steps call these once per layer: a call's checks are most of its time on the host, so
-# they run on sizes and strides fetched once, and format nothing unless they fail)
+# An eager decode step calls these once per layer, and their checks were two thirds of a call's time on the
+# host.  So what depends on sizes, strides and types alone (_*_sizes below) is looked up by those, and only
+# what can differ between tensors of the same sizes is looked at in every call: devices, alignment, gradients.
+# Numbers go in as Python's own, so that no tensor's value is taken for another's.
 _DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 KV4_BLOCK = 32             # values that share a scale
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _get_device = torch._C._cuda_getDevice
+_sizes = functools.lru_cache(maxsize=1024)
 
 
 def _where(*ts) -> int:
@@ -703,27 +709,57 @@ def _plain(*ts) -> None:
                 raise ValueError("a lazily negated view (call resolve_neg())")
 
 
-def _rows(t: torch.Tensor, T: int, H: int, Dh: int, name: str, out: bool = False) -> tuple:
-    """(pointer, token stride, head stride) of rows (T, H, Dh) that are loaded 16 bytes at a time; of an
-    output, rows that do not overlap.  The stride of a single token or head, which is free, counts as 0."""
-    s0, s1, s2 = t.stride()
+def _aligned(p: int) -> None:
+    """p: pointers or-ed together"""
+    if p % 16:
+        raise ValueError("rows, tables, weights and caches must start at multiples of 16 bytes")
+
+
+def _m(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype)
+
+
+def _row_strides(T: int, H: int, Dh: int, stride: tuple, dtype: torch.dtype, name: str, out: bool = False) -> tuple:
+    """(token stride, head stride) of rows (T, H, Dh) that are loaded 16 bytes at a time; of an output, rows that
+    do not overlap.  The stride of a single token or head, which is free, counts as 0."""
+    s0, s1, s2 = stride
     if T <= 1:
         s0 = 0
     if H <= 1:
         s1 = 0
-    p = t.data_ptr()
-    if p % 16 or (s0 | s1) % (4 if t.dtype is torch.float32 else 8) or s2 != 1:
-        _need(T * H == 0, f"{name}: contiguous rows that start at multiples of 16 bytes (strides {t.stride()})")
-    if out and not (H <= 1 or s1 >= Dh) & (T <= 1 or s0 >= s1 * (H - 1) + Dh):
-        _need(T * H == 0 or (T <= 1 or s0 >= Dh) and (H <= 1 or s1 >= s0 * (T - 1) + Dh), f"{name}: rows overlap")
-    return p, s0, s1
+    if T * H:
+        _need((s0 | s1) % (4 if dtype is torch.float32 else 8) == 0 and s2 == 1,
+              f"{name}: contiguous rows that start at multiples of 16 bytes (strides {stride})")
+        _need(not out or (H <= 1 or s1 >= Dh) and (T <= 1 or s0 >= s1 * (H - 1) + Dh)
+              or (T <= 1 or s0 >= Dh) and (H <= 1 or s1 >= s0 * (T - 1) + Dh), f"{name}: rows overlap")
+    return s0, s1
 
 
-def _ints(t: torch.Tensor, n: int, name: str) -> int:
-    """pointer of n contiguous int32"""
-    if t.dtype is not torch.int32 or t.shape != (n,) or n > 1 and t.stride(0) != 1:
-        raise ValueError(f"{name}: ({n},) int32, contiguous (got {tuple(t.shape)} {t.dtype})")
-    return t.data_ptr()
+def _int_vector(shape: tuple, stride: tuple, dtype: torch.dtype, n: int, name: str) -> None:
+    _need(dtype is torch.int32 and shape == (n,) and (n <= 1 or stride[0] == 1),
+          f"{name}: ({n},) int32, contiguous (got {tuple(shape)} {dtype})")
+
+
+@_sizes
+def _rope_sizes(qs, qst, dt, ks, kst, kt, ps, pst, pt, cs, cst, ct, ss, sst, st, wq, wk, eps, qo, ko) -> tuple:
+    _need(len(qs) == 3 and len(ks) == 3 and dt in _DT and kt is dt, "q, k: (T, HQ, D) and (T, HKV, D), both bf16, fp16 or fp32")
+    T, HQ, Dh = qs
+    HKV = ks[1]
+    _need(ks[0] == T and ks[2] == Dh and Dh in (64, 128, 256) and T * (HQ + HKV) <= 1 << 27,
+          "q, k: the same tokens, heads of 64, 128 or 256, at most 2^27 rows")
+    _need(pt in (torch.int32, torch.int64) and ps == (T,) and (T <= 1 or pst[0] == 1), f"pos: ({T},) int32 or int64, contiguous")
+    f32 = torch.float32
+    _need(len(cs) == 2 and cs[1] == Dh // 2 and cs[0] >= 1 and ss == cs and ct is f32 and st is f32 and cst == sst and cst[1] == 1
+          and (cs[0] == 1 or cst[0] % 4 == 0), f"cos, sin: (positions, {Dh // 2}) fp32 rows of one stride, of whole 16 bytes")
+    for w, name in ((wq, "wq"), (wk, "wk")):
+        _need(w is None or w[0] == (Dh,) and w[1] == (1,) and w[2] is dt, f"{name}: ({Dh},) of q's type, contiguous")
+    _need(eps >= 0, "eps: not negative")
+    for o, s, name in ((qo, qs, "q_out"), (ko, ks, "k_out")):
+        _need(o is None or o[0] == s and o[2] is dt, f"{name}: as {name[0]}")
+    return (T, HQ, HKV, Dh, _row_strides(T, HQ, Dh, qst, dt, "q"), _row_strides(T, HKV, Dh, kst, dt, "k"),
+            (HQ * Dh, Dh) if qo is None else _row_strides(T, HQ, Dh, qo[1], dt, "q_out", True),
+            (HKV * Dh, Dh) if ko is None else _row_strides(T, HKV, Dh, ko[1], dt, "k_out", True),
+            (T, HQ, HKV, Dh, _DT[dt]), pt is torch.int64, (cst[0] if cs[0] > 1 else 0, cs[0]))
 
 
 def qk_norm_rope(q, k, pos, cos, sin, wq=None, wk=None, eps: float = 1e-6, q_out=None, k_out=None):
@@ -734,79 +770,47 @@ def qk_norm_rope(q, k, pos, cos, sin, wq=None, wk=None, eps: float = 1e-6, q_out
     of q's type, None for a rotation alone.  A token of negative position (padding) gives zeros, one of P
     or more NaN.  Returns (q_out, k_out), contiguous unless given; either may be its input."""
     i = _where(q, k, pos, cos, sin, wq, wk, q_out, k_out)
-    dt = q.dtype
-    if q.dim() != 3 or k.dim() != 3 or dt not in _DT or k.dtype is not dt:
-        raise ValueError("q, k: (T, HQ, D) and (T, HKV, D), both bf16, fp16 or fp32")
-    T, HQ, Dh = q.shape
-    Tk, HKV, Dk = k.shape
-    if Tk != T or Dk != Dh or Dh not in (64, 128, 256) or T * (HQ + HKV) > 1 << 27:
-        raise ValueError(f"q, k: the same tokens, heads of 64, 128 or 256 (got {Dh}, {Dk}), at most 2^27 rows")
-    pt = pos.dtype
-    if pt is not torch.int32 and pt is not torch.int64 or pos.shape != (T,) or T > 1 and pos.stride(0) != 1:
-        raise ValueError(f"pos: ({T},) int32 or int64, contiguous")
-    half = Dh // 2
-    P = cos.shape[0]
-    cst, cp, sp = cos.stride(), cos.data_ptr(), sin.data_ptr()
-    if (cos.shape != (P, half) or sin.shape != cos.shape or cos.dtype is not torch.float32
-            or sin.dtype is not torch.float32 or P < 1 or cst != sin.stride() or cst[1] != 1 or P > 1 and cst[0] % 4
-            or (cp | sp) % 16):
-        raise ValueError(f"cos, sin: (positions, {half}) fp32 rows of one stride, starting at multiples of 16 bytes")
-    wqp = wkp = None
-    if wq is not None:
-        wqp = wq.data_ptr()
-        if wq.shape != (Dh,) or wq.dtype is not dt or wq.stride(0) != 1 or wqp % 16:
-            raise ValueError(f"wq: ({Dh},) of q's type, contiguous, 16-byte aligned")
-    if wk is not None:
-        wkp = wk.data_ptr()
-        if wk.shape != (Dh,) or wk.dtype is not dt or wk.stride(0) != 1 or wkp % 16:
-            raise ValueError(f"wk: ({Dh},) of q's type, contiguous, 16-byte aligned")
-    if not eps >= 0:
-        raise ValueError("eps: not negative")
+    T, HQ, HKV, Dh, qst, kst, qo, ko, sizes, wide, table = _rope_sizes(
+        q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, pos.shape, pos.stride(), pos.dtype, cos.shape, cos.stride(),
+        cos.dtype, sin.shape, sin.stride(), sin.dtype, _m(wq), _m(wk), float(eps), _m(q_out), _m(k_out))
     _plain(q, k, cos, sin, wq, wk, q_out, k_out)
     if q_out is None:
         q_out = q.new_empty(T, HQ, Dh)
-        qo = q_out.data_ptr(), HQ * Dh, Dh
-    else:
-        if q_out.shape != q.shape or q_out.dtype is not dt:
-            raise ValueError("q_out: as q")
-        qo = _rows(q_out, T, HQ, Dh, "q_out", True)
     if k_out is None:
         k_out = k.new_empty(T, HKV, Dh)
-        ko = k_out.data_ptr(), HKV * Dh, Dh
-    else:
-        if k_out.shape != k.shape or k_out.dtype is not dt:
-            raise ValueError("k_out: as k")
-        ko = _rows(k_out, T, HKV, Dh, "k_out", True)
-    _run(i, "oa_qk_norm_rope", *_rows(q, T, HQ, Dh, "q"), *_rows(k, T, HKV, Dh, "k"), T, HQ, HKV, Dh, _DT[dt],
-         pos.data_ptr(), pt is torch.int64, cp, sp, cst[0] if P > 1 else 0, P, wqp, wkp, eps, *qo, *ko)
+    qp, kp, cp, sp, qop, kop = q.data_ptr(), k.data_ptr(), cos.data_ptr(), sin.data_ptr(), q_out.data_ptr(), k_out.data_ptr()
+    wqp, wkp = _ptr(wq), _ptr(wk)
+    if T:
+        _aligned((qp | qop if HQ else 0) | (kp | kop if HKV else 0) | cp | sp | (wqp or 0) | (wkp or 0))
+    _run(i, "oa_qk_norm_rope", qp, *qst, kp, *kst, *sizes, pos.data_ptr(), wide, cp, sp, *table, wqp, wkp, eps, qop, *qo,
+         kop, *ko)
     return q_out, k_out
 
 
 def _page(page: int) -> None:
-    if not 32 <= page <= 1024 or page & (page - 1):
-        raise ValueError(f"page: a power of two, 32 to 1024 (got {page})")
+    _need(32 <= page <= 1024 and page & (page - 1) == 0, f"page: a power of two, 32 to 1024 (got {page})")
 
 
-def _table(table: torch.Tensor, page: int) -> tuple:
-    """(pointer, row stride, rows, width) of a table of page ids"""
-    if table.dim() != 2 or table.dtype is not torch.int32:
-        raise ValueError("table: (requests, width) int32")
-    B, width = table.shape
-    s0, s1 = table.stride()
-    if width < 1 or width * page > 1 << 30 or width > 1 and s1 != 1 or B > 1 and s0 < width or B > 1 << 24:
-        raise ValueError("table: contiguous rows of at most 2^30 tokens, at most 2^24 requests")
-    return table.data_ptr(), max(s0, width), B, width
+def _table_sizes(ts, tst, tt, page: int) -> tuple:
+    """(row stride, rows, width) of a table of page ids"""
+    _need(len(ts) == 2 and tt is torch.int32, "table: (requests, width) int32")
+    B, width = ts
+    _need(width >= 1 and width * page <= 1 << 30 and (width == 1 or tst[1] == 1) and (B <= 1 or tst[0] >= width) and B <= 1 << 24,
+          "table: contiguous rows of at most 2^30 tokens, at most 2^24 requests")
+    return max(tst[0], width), B, width
 
 
-def _pages_state(count, lens, table, free, nfree, status, page: int, what: str) -> tuple:
-    """The arguments that both calls of the page tables begin with."""
+@_sizes
+def _pages_sizes(page, ts, tst, tt, fs, fst, ft, count, lens, nfree, status, what) -> tuple:
     _page(page)
-    tp, ts, B, width = _table(table, page)
-    NP = free.shape[0] if free.dim() == 1 else 0
-    if B < 1 or NP < 1 or NP * page >= 1 << 31:
-        raise ValueError("at least one request; free: (pages,) int32, a pool of fewer than 2^31 tokens")
-    return (_ints(count, B, what), _ints(lens, B, "lens"), tp, ts, _ints(free, NP, "free"), _ints(nfree, 1, "nfree"),
-            _ints(status, 1, "status"), B, width, NP, page)
+    stride, B, width = _table_sizes(ts, tst, tt, page)
+    _need(len(fs) == 1, "free: (pages,) int32")
+    NP = fs[0]
+    _need(B >= 1 and NP >= 1 and NP * page < 1 << 31, "at least one request and page; a pool of fewer than 2^31 tokens")
+    _int_vector(fs, fst, ft, NP, "free")
+    for m, n, name in ((count, B, what), (lens, B, "lens"), (nfree, 1, "nfree"), (status, 1, "status")):
+        _int_vector(*m, n, name)
+    return stride, B, (B, width, NP, page)
 
 
 def kv_pages_extend(add, lens, table, free, nfree, status, page: int, total: int):
@@ -818,13 +822,14 @@ def kv_pages_extend(add, lens, table, free, nfree, status, page: int, total: int
     (status |= 1), free pages do not reach (2) or there are more than `total` new tokens (4), nothing
     changes, slots and pos are -1 and cu is 0; status (1,) is the caller's to look at and to clear."""
     i = _where(add, lens, table, free, nfree, status)
-    st = _pages_state(add, lens, table, free, nfree, status, page, "add")
+    stride, B, sizes = _pages_sizes(index(page), table.shape, table.stride(), table.dtype, free.shape, free.stride(), free.dtype,
+                                    _m(add), _m(lens), _m(nfree), _m(status), "add")
     if not 0 <= total <= 1 << 30:
         raise ValueError("total: 0 to 2^30")
-    B = st[7]
     slots, pos, cu = add.new_empty(total), add.new_empty(total), add.new_empty(B + 1)
     ws = add.new_empty(3 * B + 1) if B > 1024 or total > 2048 else None
-    _run(i, "oa_kv_pages_extend", *st, total, slots.data_ptr(), pos.data_ptr(), cu.data_ptr(), _ptr(ws))
+    _run(i, "oa_kv_pages_extend", add.data_ptr(), lens.data_ptr(), table.data_ptr(), stride, free.data_ptr(), nfree.data_ptr(),
+         status.data_ptr(), *sizes, total, slots.data_ptr(), pos.data_ptr(), cu.data_ptr(), _ptr(ws))
     return slots, pos, cu
 
 
@@ -833,33 +838,49 @@ def kv_pages_truncate(keep, lens, table, free, nfree, status, page: int) -> None
     it no longer needs go back to the stack and leave the table (-1).  A truncation to the lengths before
     an extension undoes it.  Nothing changes where the stack would outgrow `free` (status |= 2)."""
     i = _where(keep, lens, table, free, nfree, status)
-    st = _pages_state(keep, lens, table, free, nfree, status, page, "keep")
-    ws = keep.new_empty(3 * st[7] + 1) if st[7] > 256 else None
-    _run(i, "oa_kv_pages_truncate", *st, _ptr(ws))
+    stride, B, sizes = _pages_sizes(index(page), table.shape, table.stride(), table.dtype, free.shape, free.stride(), free.dtype,
+                                    _m(keep), _m(lens), _m(nfree), _m(status), "keep")
+    ws = keep.new_empty(3 * B + 1) if B > 256 else None
+    _run(i, "oa_kv_pages_truncate", keep.data_ptr(), lens.data_ptr(), table.data_ptr(), stride, free.data_ptr(),
+         nfree.data_ptr(), status.data_ptr(), *sizes, _ptr(ws))
+
+
+@_sizes
+def _kv4_sizes(kcs, kst, kct, kss, sst, ksdt, vcs, vst, vct, vss, vsst, vsdt) -> tuple:
+    """(page strides, pages, page) of a 4-bit cache's tensors, its heads and head dimension; pages may lie apart (a
+    layer of a larger tensor)."""
+    _need(len(kcs) == 4, "kc: (pages, heads, page, D / 2) uint8")
+    NP, HKV, page, half = kcs
+    blocks = half // (KV4_BLOCK // 2)
+    _page(page)
+    _need(half in (32, 64) and NP >= 1 and HKV >= 1 and NP * page < 1 << 31,
+          f"cache: head dimension 64 or 128 (got {2 * half}), at least one page and head, fewer than 2^31 slots")
+    u8 = torch.uint8
+    _need(vcs == kcs and kss == (NP, HKV, page, blocks) and vss == kss and kct is u8 and ksdt is u8 and vct is u8 and vsdt is u8,
+          f"cache: codes ({NP}, {HKV}, {page}, {half}), scales ({NP}, {HKV}, {page}, {blocks}), uint8")
+    c0, s0 = (kst[0], sst[0]) if NP > 1 else (HKV * page * half, HKV * page * blocks)
+    _need(vst == kst and vsst == sst and kst[1:] == (page * half, half, 1) and sst[1:] == (page * blocks, blocks, 1)
+          and c0 >= HKV * page * half and s0 >= HKV * page * blocks and c0 < 1 << 32 and (c0 | s0) % 16 == 0,
+          "cache: contiguous pages, those of k and v at one distance, of whole 16 bytes, under 2^32")
+    return (c0, s0, NP, page), HKV, 2 * half
 
 
 def _kv4_cache(kc, ks, vc, vs) -> tuple:
-    """(pointers, page strides, pages, page) of a 4-bit cache's tensors, its heads and head dimension; pages may
-    lie apart (a layer of a larger tensor)."""
-    if kc.dim() != 4:
-        raise ValueError("kc: (pages, heads, page, D / 2) uint8")
-    NP, HKV, page, half = kc.shape
-    blocks = half // (KV4_BLOCK // 2)
-    _page(page)
-    if half not in (32, 64) or NP < 1 or HKV < 1 or NP * page >= 1 << 31:
-        raise ValueError(f"cache: head dimension 64 or 128 (got {2 * half}), at least one page and head, fewer than 2^31 slots")
-    u8 = torch.uint8
-    if (vc.shape != kc.shape or ks.shape != (NP, HKV, page, blocks) or vs.shape != ks.shape
-            or kc.dtype is not u8 or ks.dtype is not u8 or vc.dtype is not u8 or vs.dtype is not u8):
-        raise ValueError(f"cache: codes ({NP}, {HKV}, {page}, {half}), scales ({NP}, {HKV}, {page}, {blocks}), uint8")
-    c, s = kc.stride(), ks.stride()
-    ps = kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr()
-    c0, s0 = (c[0], s[0]) if NP > 1 else (HKV * page * half, HKV * page * blocks)
-    if (vc.stride() != c or vs.stride() != s or c[1:] != (page * half, half, 1) or s[1:] != (page * blocks, blocks, 1)
-            or c0 < HKV * page * half or s0 < HKV * page * blocks or c0 >> 32 or (c0 | s0 | ps[0] | ps[1] | ps[2] | ps[3]) % 16):
-        raise ValueError("cache: contiguous pages that start at multiples of 16 bytes, those of k and v at one distance "
-                         "under 2^32 bytes")
-    return ps, (c0, s0, NP, page), HKV, 2 * half
+    """A 4-bit cache's pointers and sizes (_kv4_sizes)."""
+    sizes = _kv4_sizes(kc.shape, kc.stride(), kc.dtype, ks.shape, ks.stride(), ks.dtype, vc.shape, vc.stride(), vc.dtype,
+                       vs.shape, vs.stride(), vs.dtype)
+    p = kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr()
+    _aligned(p[0] | p[1] | p[2] | p[3])
+    return p, *sizes
+
+
+@_sizes
+def _write_sizes(HKV, Dh, ks, kst, kt, vs, vst, vt, ss, sst, st) -> tuple:
+    _need(len(ks) == 3 and ks[1:] == (HKV, Dh) and vs == ks and kt in _DT and vt is kt and ks[0] * HKV <= 1 << 26,
+          f"k, v: (T, {HKV}, {Dh}), both bf16, fp16 or fp32, at most 2^26 rows")
+    T = ks[0]
+    _int_vector(ss, sst, st, T, "slots")
+    return _row_strides(T, HKV, Dh, kst, kt, "k"), _row_strides(T, HKV, Dh, vst, kt, "v"), (T, HKV, Dh, _DT[kt])
 
 
 def kv4_write(k, v, slots, kc, ks, vc, vs) -> None:
@@ -869,12 +890,13 @@ def kv4_write(k, v, slots, kc, ks, vc, vs) -> None:
     over.  The slots of one call are distinct (a slot given twice ends with blocks of either row)."""
     i = _where(k, v, slots, kc, ks, vc, vs)
     ps, where, HKV, Dh = _kv4_cache(kc, ks, vc, vs)
-    T, dt = k.shape[0], k.dtype
-    if k.shape != (T, HKV, Dh) or v.shape != k.shape or dt not in _DT or v.dtype is not dt or T * HKV > 1 << 26:
-        raise ValueError(f"k, v: (T, {HKV}, {Dh}), both bf16, fp16 or fp32, at most 2^26 rows")
+    kst, vst, sizes = _write_sizes(HKV, Dh, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, slots.shape,
+                                   slots.stride(), slots.dtype)
     _plain(k, v)
-    _run(i, "oa_kv4_write", *_rows(k, T, HKV, Dh, "k"), *_rows(v, T, HKV, Dh, "v"), T, HKV, Dh, _DT[dt],
-         _ints(slots, T, "slots"), *ps, *where)
+    kp, vp = k.data_ptr(), v.data_ptr()
+    if sizes[0]:
+        _aligned(kp | vp)
+    _run(i, "oa_kv4_write", kp, *kst, vp, *vst, *sizes, slots.data_ptr(), *ps, *where)
 
 
 def kv4_read(slots, kc, ks, vc, vs, dtype: torch.dtype = torch.bfloat16):
@@ -883,12 +905,13 @@ def kv4_read(slots, kc, ks, vc, vs, dtype: torch.dtype = torch.bfloat16):
     i = _where(slots, kc, ks, vc, vs)
     ps, where, HKV, Dh = _kv4_cache(kc, ks, vc, vs)
     T = slots.shape[0] if slots.dim() == 1 else 0
-    sp = _ints(slots, T, "slots")
+    _int_vector(slots.shape, slots.stride(), slots.dtype, T, "slots")
     if dtype not in (torch.bfloat16, torch.float32) or T * HKV > 1 << 26:
         raise ValueError("dtype: bf16 or fp32; at most 2^26 rows")
     k = kc.new_empty(T, HKV, Dh, dtype=dtype)
     v = kc.new_empty(T, HKV, Dh, dtype=dtype)
-    _run(i, "oa_kv4_read", sp, *ps, *where, k.data_ptr(), HKV * Dh, Dh, v.data_ptr(), HKV * Dh, Dh, T, HKV, Dh, _DT[dtype])
+    _run(i, "oa_kv4_read", slots.data_ptr(), *ps, *where, k.data_ptr(), HKV * Dh, Dh, v.data_ptr(), HKV * Dh, Dh, T, HKV, Dh,
+         _DT[dtype])
     return k, v
 
 
@@ -904,6 +927,32 @@ def kv4_chunk(cap: int, units: int, rows: int) -> int:
     return min(-(-n // 128), -(-cap // 128)) * 128
 
 
+@_sizes
+def _attn_sizes(HKV, Dh, page, qs, qst, qt, ts, tst, tt, ls, lst, lt, cu, max_q, sm_scale, max_len, o) -> tuple:
+    tstride, B, width = _table_sizes(ts, tst, tt, page)
+    _need(len(qs) == 3 and qs[2] == Dh and qt is torch.bfloat16 and qs[1] >= 1 and qs[1] % HKV == 0,
+          f"q: (T, a multiple of {HKV}, {Dh}) bf16")
+    T, HQ, _ = qs
+    _int_vector(ls, lst, lt, B, "lens")
+    if cu is not None:
+        _int_vector(*cu, B + 1, "cu_q")
+    else:
+        _need(T == B and max_q == 1, "without cu_q every sequence has one row of q")
+    scale = Dh ** -0.5 if sm_scale is None else sm_scale
+    _need(1 <= max_q <= (1 << 30) // (HQ // HKV) and scale == scale and (max_len is None or max_len >= 0),
+          "max_q: at least 1; sm_scale: not NaN; max_len: not negative")
+    _need(o is None or o[0] == qs and o[2] is torch.bfloat16, "out: as q")
+    rows = max_q * (HQ // HKV)
+    cap = max(1, width * page if max_len is None else min(max_len, width * page))
+    units = B * HKV * -(-rows // (8 if rows <= 8 else 16 if rows <= 16 else 32 if rows <= 64 else 128))
+    chunk = kv4_chunk(cap, units, rows)
+    nchunk = -(-cap // chunk)
+    return (T, HQ, B, _row_strides(T, HQ, Dh, qst, qt, "q"),
+            (HQ * Dh, Dh) if o is None else _row_strides(T, HQ, Dh, o[1], qt, "out", True), (tstride, width),
+            (B, T, max_q, HQ, HKV, Dh, scale, chunk, nchunk), T * HQ * nchunk if nchunk > 1 else 0,
+            units * nchunk if rows > 64 else 0)
+
+
 def kv4_attn(q, kc, ks, vc, vs, table, lens, sm_scale: float | None = None, cu_q=None, max_q: int = 1, out=None,
              max_len: int | None = None) -> torch.Tensor:
     """Causal attention of the newest tokens of every sequence over a 4-bit paged cache.
@@ -917,46 +966,28 @@ def kv4_attn(q, kc, ks, vc, vs, table, lens, sm_scale: float | None = None, cu_q
     were (0 where the call makes it); `out` shares no memory with q."""
     i = _where(q, kc, ks, vc, vs, table, lens, cu_q, out)
     ps, where, HKV, Dh = _kv4_cache(kc, ks, vc, vs)
-    tp, ts, B, width = _table(table, where[3])
-    T, HQ = q.shape[:2] if q.dim() == 3 else (0, 0)
-    if q.shape != (T, HQ, Dh) or q.dtype is not torch.bfloat16 or HQ < 1 or HQ % HKV:
-        raise ValueError(f"q: (T, a multiple of {HKV}, {Dh}) bf16")
-    G = HQ // HKV
-    lp = _ints(lens, B, "lens")
-    cp = None
-    if cu_q is not None:
-        cp = _ints(cu_q, B + 1, "cu_q")
-    elif T != B or max_q != 1:
-        raise ValueError("without cu_q every sequence has one row of q")
-    scale = Dh ** -0.5 if sm_scale is None else sm_scale
-    if not 1 <= max_q <= (1 << 30) // G or scale != scale or max_len is not None and max_len < 0:
-        raise ValueError("max_q: at least 1; sm_scale: not NaN; max_len: not negative")
+    T, HQ, B, qst, ost, tsz, sizes, parts, flags = _attn_sizes(
+        HKV, Dh, where[3], q.shape, q.stride(), q.dtype, table.shape, table.stride(), table.dtype, lens.shape, lens.stride(),
+        lens.dtype, _m(cu_q), index(max_q), None if sm_scale is None else float(sm_scale),
+        None if max_len is None else index(max_len), _m(out))
     _plain(q, out)
-    qa = _rows(q, T, HQ, Dh, "q")
+    qp = q.data_ptr()
     if out is None:
-        out = q.new_empty(T, HQ, Dh) if cp is None else q.new_zeros(T, HQ, Dh)
-        oa = out.data_ptr(), HQ * Dh, Dh
-    elif out.shape != q.shape or out.dtype is not torch.bfloat16 or out.data_ptr() == qa[0]:
-        raise ValueError("out: as q, and not q itself")
-    else:
-        oa = _rows(out, T, HQ, Dh, "out", True)
+        out = q.new_empty(T, HQ, Dh) if cu_q is None else q.new_zeros(T, HQ, Dh)
+    op = out.data_ptr()
     if T == 0 or B == 0:
         return out
-    rows = max_q * G
-    cap = max(1, width * where[3] if max_len is None else min(max_len, width * where[3]))
-    units = B * HKV * -(-rows // (8 if rows <= 8 else 16 if rows <= 16 else 32 if rows <= 64 else 128))
-    chunk = kv4_chunk(cap, units, rows)
-    nchunk = -(-cap // chunk)
+    _aligned(qp | op)
+    if op == qp:
+        raise ValueError("out: not q itself")
     wp = mp = fp = None
-    parts = T * HQ * nchunk if nchunk > 1 else 0
-    flags = units * nchunk if rows > 64 else 0
     if parts or flags:
         ws = q.new_empty(parts * (Dh + 2) + flags, dtype=torch.float32)
         wp = ws.data_ptr()
         mp = wp + 4 * parts * Dh
         fp = mp + 8 * parts
-    _run(i, "oa_kv4_attn", *qa, *ps, *where, tp, ts, width, lp, cp, B, T, max_q, HQ, HKV, Dh, scale, chunk, nchunk, wp, mp,
-         fp, *oa)
+    _run(i, "oa_kv4_attn", qp, *qst, *ps, *where, table.data_ptr(), *tsz, lens.data_ptr(), _ptr(cu_q), *sizes, wp, mp, fp, op,
+         *ost)
     return out
 
 

@@ -228,3 +228,31 @@ def test_library_refuses_before_a_launch():
     assert L.oa_kv4_attn(*at[:15], 16, 1 << 20, 1 << 20, 1 << 10, *at[19:]) == -22
     assert L.oa_kv4_attn(*at[:15], 16, 3, 1 << 22, 1 << 22, *at[19:]) == -22 and L.oa_kv4_attn(*at[:15], 16, 65536, 8, 1, *at[19:]) == -22
     assert L.oa_kv4_attn(*many[:27], None, *many[28:]) == -22 and L.oa_kv4_attn(*many[:27], 2, *many[28:]) == -22
+
+
+def test_a_numbers_value_counts_in_every_call(calls):
+    """Sizes are looked up by value: a scalar tensor, or numpy's integer, that has changed since gives its new value,
+    and good sizes that were seen before do not let in a misaligned or a gradient-bearing tensor."""
+    c = cache()
+    q = torch.zeros(3, 8, 128, dtype=torch.bfloat16)
+    t, n, cu = torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
+    s, m = torch.tensor(0.5), torch.tensor(2)
+    for scale, rows in ((0.5, 2), (0.25, 3)):
+        s.fill_(scale)
+        m.fill_(rows)
+        ops.kv4_attn(q, table=t, lens=n, cu_q=cu, sm_scale=s, max_q=m, **c)
+        name, a = calls[-1]
+        types = [x.__name__ for x in lib.SIGNATURES[name]]
+        assert [x for x, k in zip(a, types) if k == "c_float"] == [scale] and rows in a
+    with pytest.raises(TypeError):
+        ops.kv4_attn(q, table=t, lens=n, cu_q=cu, max_q=2.0, **c)
+    wide = torch.zeros(3, 8, 136, dtype=torch.bfloat16)
+    ops.kv4_attn(wide[..., :128], table=t, lens=n, cu_q=cu, max_q=2, **c)
+    ops.kv4_attn(q, table=t, lens=n, cu_q=cu, max_q=2, out=wide[..., :128], **c)
+    count, off = len(calls), wide[..., 1:129]
+    for bad in (off, q.clone().requires_grad_()):
+        with pytest.raises(ValueError):
+            ops.kv4_attn(bad, table=t, lens=n, cu_q=cu, max_q=2, **c)
+        with pytest.raises(ValueError):
+            ops.kv4_attn(q, table=t, lens=n, cu_q=cu, max_q=2, out=bad, **c)
+    assert len(calls) == count
