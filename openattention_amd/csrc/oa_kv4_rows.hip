@@ -18,9 +18,9 @@
 // the transpose reads spread over the banks and every address is one register and a constant (exchanged
 // places instead, as in the prompt's kernel, take 16 more registers and spill).
 //
-// Bound by instruction issue between the products: 64 questions' tokens of 4 heads over 32768 keys, twice (69 GFLOP),
-// 94 us for this kernel, 730 TFLOP/s (a large bf16 product reaches 1256), 100 with the empty second launch and
-// the join.  Its matrix cores are busy 30% of the time, its vector units about 45%; two waves a SIMD at 254 registers.
+// Bound by instruction issue between the products: 64 tokens of 32 query heads over 32768 keys of 8 heads, for two
+// sequences (69 GFLOP), 94 us for this kernel, 730 TFLOP/s (a large bf16 product reaches 1256), 98 for the call: the
+// empty second launch (4.5) and the join (8.5) in part beside it.  Its matrix cores are busy 30% of the time, its vector units about 45%; two waves a SIMD at 254 registers.
 #include "oa_kv4_attn.h"
 
 namespace {

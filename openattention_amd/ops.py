@@ -674,6 +674,7 @@ _DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 KV4_BLOCK = 32             # values that share a scale
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _get_device = torch._C._cuda_getDevice
+_forward_ad = torch.autograd.forward_ad
 _sizes = functools.lru_cache(maxsize=1024)
 
 
@@ -699,12 +700,14 @@ def _run(i: int, name: str, *args) -> None:
 def _plain(*ts) -> None:
     """Tensors whose data a kernel may take as it stands, with no gradient to be formed: these
     operators have no backward pass, and would cut a graph in silence."""
-    grad = torch.is_grad_enabled()
+    grad, dual = torch.is_grad_enabled(), _forward_ad._current_level >= 0
     for t in ts:
         if t is not None:
             if grad and t.requires_grad:
                 raise ValueError("a tensor requires a gradient, and this operator has no backward pass (call it under "
                                  "torch.no_grad())")
+            if dual and _forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError("a tensor carries a forward-mode tangent, which this operator would drop")
             if t.is_neg():
                 raise ValueError("a lazily negated view (call resolve_neg())")
 
@@ -963,7 +966,8 @@ def kv4_attn(q, kc, ks, vc, vs, table, lens, sm_scale: float | None = None, cu_q
     that the caller knows (the table's width otherwise).  NaN: rows that need a page id outside of the
     cache, and those of sequences longer than their table row or than max_len (rounded up to whole pieces,
     kv4_chunk).  Rows of `out` behind cu_q[B], and tokens past max_q, are left as they
-    were (0 where the call makes it); `out` shares no memory with q."""
+    were (0 where the call makes it); `out` shares no memory with q.  Sums are held in fp32 and not divided
+    before their end: values up to 2^80 are safe at any length."""
     i = _where(q, kc, ks, vc, vs, table, lens, cu_q, out)
     ps, where, HKV, Dh = _kv4_cache(kc, ks, vc, vs)
     T, HQ, B, qst, ost, tsz, sizes, parts, flags = _attn_sizes(

@@ -256,3 +256,21 @@ def test_a_numbers_value_counts_in_every_call(calls):
         with pytest.raises(ValueError):
             ops.kv4_attn(q, table=t, lens=n, cu_q=cu, max_q=2, out=bad, **c)
     assert len(calls) == count
+
+
+def test_forward_tangents_refused(calls):
+    """An operator would drop the tangent of a dual tensor in silence."""
+    from torch.autograd import forward_ad as fw
+    c = cache()
+    q, k, s = torch.zeros(3, 8, 128, dtype=torch.bfloat16), torch.zeros(3, 2, 128, dtype=torch.bfloat16), torch.zeros(3, dtype=torch.int32)
+    t = torch.zeros(3, 2, dtype=torch.int32)
+    with fw.dual_level():
+        dq, dk = fw.make_dual(q, torch.ones_like(q)), fw.make_dual(k, torch.ones_like(k))
+        for call in (lambda: ops.kv4_attn(dq, table=t, lens=s, **c), lambda: ops.kv4_write(k, dk, s, **c),
+                     lambda: ops.qk_norm_rope(**rope_args(q=fw.make_dual(torch.zeros(5, 8, 128), torch.ones(5, 8, 128)), k=torch.zeros(5, 2, 128)))):
+            with pytest.raises(ValueError):
+                call()
+        assert not calls
+        ops.kv4_attn(q, table=t, lens=s, **c)
+        ops.kv4_write(k, k, s, **c)
+    assert len(calls) == 2
