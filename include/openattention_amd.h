@@ -604,11 +604,12 @@ int oa_kv4_read(const int* slots, const void* kc, const void* ks, const void* vc
 
 /*
  * Causal attention over the 4-bit cache.  Sequence b holds lens[b] keys in the pages of its table row; its
- * query tokens are rows cu[b] .. cu[b + 1] - 1 of q (tokens, q_heads, head_dim) bf16 (cu NULL: row b alone),
- * the last of them its newest key's, so that token j of R sees keys 0 .. lens - R + j.  out as q, not q.  fp32 scores,
+ * query tokens are rows cu[b] .. cu[b + 1] - 1 of q (tokens, q_heads, head_dim) bf16 (cu NULL: row b alone; a
+ * sequence whose starts decrease or leave the rows has none), the last of them its newest key's, so that token j
+ * of R sees keys 0 .. lens - R + j.  out as q, not q.  fp32 scores,
  * softmax and sums (values up to 2^80 are safe at any length); weights in 16 bits, 11 past 64 rows of a KV head.
- * A row that sees no key gives 0; rows behind cu[sequences], and tokens of a sequence from max_q on, are left as
- * they were.  NaN: rows that need a page id outside of the cache, and
+ * A row that sees no key gives 0; rows that no sequence takes, and tokens of a sequence from max_q on, are left as
+ * they were, or, with `clear` and more than one piece, set to 0 (then the starts do not decrease).  NaN: rows that need a page id outside of the cache, and
  * those of sequences longer than their table row or than nchunk * chunk keys.  Keys are split into nchunk pieces
  * of `chunk` (a multiple of 128); with more than one, ws_o (tokens * q_heads * nchunk * head_dim) and ws_ml (* 2)
  * floats hold the pieces' sums; with more than 64 rows of a KV head (max_q * q_heads / kv_heads), ws_flag holds
@@ -618,7 +619,7 @@ int oa_kv4_attn(const void* q, long q_st, long q_sh, const void* kc, const void*
                 long code_stride, long scale_stride, int pages, int page, const int* table, long table_stride, int width,
                 const int* lens, const int* cu, int sequences, int tokens, int max_q, int q_heads, int kv_heads,
                 int head_dim, float sm_scale, int chunk, int nchunk, float* ws_o, float* ws_ml, int* ws_flag, void* out,
-                long o_st, long o_sh, void* stream);
+                long o_st, long o_sh, int clear, void* stream);
 
 #ifdef __cplusplus
 }

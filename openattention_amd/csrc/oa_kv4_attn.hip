@@ -333,6 +333,32 @@ __global__ void __launch_bounds__(kThreads, NQ > 1 ? 2 : 3) kv4_attn_kernel(Attn
   }
 }
 
+// Zeros in the rows of out that no sequence takes: those before the first and behind the last by all workgroups
+// of the join together, and head hd of sequence b's rows past max_q (all of its rows, where they do not fit) by
+// the one of its first row.  In the join, as it costs a launch to fill out beforehand (5 drafts of 7 sequences
+// 19.5 us a call, 15.5 here) and the attention kernel 4 to 13 us (one sequence of 131072 keys 30.6 to 35.6, 32 of
+// 32768 184 to 197), even where there is nothing to clear.
+template <int D>
+__device__ __forceinline__ void clear_rows(const AttnArgs& a, int b, int hd, bool own) {
+  constexpr int kLanes = D / 4, kRows = kThreads / kLanes;     // lanes of a row, 8 bytes each
+  const int y = threadIdx.x % kLanes, x = threadIdx.x / kLanes, heads = a.HKV * a.G;
+  auto zero = [&](int tok, int head) {
+    *reinterpret_cast<uint2v*>(a.out + (long)tok * a.o_st + (long)head * a.o_sh + 4 * y) = uint2v(0u);
+  };
+  auto in_out = [&](int t) { return min(max(t, 0), a.tokens); };
+  const int lead = in_out(a.cu[0]), tail = in_out(a.cu[a.B]);
+  const long n = (long)(lead + a.tokens - tail) * heads, blocks = (long)gridDim.x * gridDim.y;
+  for (long i = ((long)blockIdx.y * gridDim.x + blockIdx.x) * kRows + x; i < n; i += blocks * kRows) {
+    const int t = (int)(i / heads);
+    zero(t < lead ? t : tail + t - lead, (int)(i % heads));
+  }
+  if (!own) return;
+  const int r0 = a.cu[b], r1 = a.cu[b + 1];
+  const bool fits = r0 >= 0 && r1 >= r0 && r1 <= a.tokens;
+  const int t0 = fits ? r0 + min(r1 - r0, a.max_q) : in_out(r0), t1 = fits ? r1 : in_out(r1);
+  for (int t = t0 + x; t < t1; t += kRows) zero(t, hd);
+}
+
 // joins a row's chunks: weights exp2(m_i - max m), by groups of D / 4 lanes
 template <int D>
 __global__ void __launch_bounds__(kThreads) kv4_join_kernel(AttnArgs a) {
@@ -343,6 +369,7 @@ __global__ void __launch_bounds__(kThreads) kv4_join_kernel(AttnArgs a) {
   const int heads = a.HKV * a.G;
   const int hd = blockIdx.x % heads, j = blockIdx.x / heads, b = blockIdx.y;
   const Seq sq = seq_of(a, b);
+  if (a.clear) clear_rows<D>(a, b, hd, j == 0);
   if (j >= sq.R) return;
   const int seen = sq.n - sq.R + j + 1, tid = threadIdx.x;
   const int nv = sq.bad || seen <= 0 ? 0 : (seen + a.chunk - 1) / a.chunk;
@@ -416,7 +443,8 @@ extern "C" int oa_kv4_attn(const void* q, long q_st, long q_sh, const void* kc, 
                            const void* vs, long code_stride, long scale_stride, int pages, int page, const int* table,
                            long table_stride, int width, const int* lens, const int* cu, int sequences, int tokens,
                            int max_q, int q_heads, int kv_heads, int head_dim, float sm_scale, int chunk, int nchunk,
-                           float* ws_o, float* ws_ml, int* ws_flag, void* out, long o_st, long o_sh, void* stream) {
+                           float* ws_o, float* ws_ml, int* ws_flag, void* out, long o_st, long o_sh, int clear,
+                           void* stream) {
   auto odd = [](const void* p, uintptr_t n) { return !p || (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0; };
   if ((head_dim != 64 && head_dim != 128) || sequences < 0 || tokens < 0 || max_q <= 0 || kv_heads <= 0 || q_heads <= 0 ||
       q_heads % kv_heads || (long)max_q * (q_heads / kv_heads) > (1L << 30) || pages <= 0 || page < 32 || page > 1024 ||
@@ -442,6 +470,7 @@ extern "C" int oa_kv4_attn(const void* q, long q_st, long q_sh, const void* kc, 
   a.ws_o = ws_o; a.ws_ml = ws_ml; a.ws_flag = ws_flag;
   a.B = sequences; a.HKV = kv_heads; a.G = q_heads / kv_heads; a.tokens = tokens; a.max_q = max_q;
   a.width = width; a.NP = pages; a.lp = __builtin_ctz(page); a.chunk = chunk; a.nchunk = nchunk;
+  a.clear = cu && clear;
   a.c = sm_scale * kLog2e;
   return head_dim == 64 ? launch<64>(a, (hipStream_t)stream) : launch<128>(a, (hipStream_t)stream);
 }

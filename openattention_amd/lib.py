@@ -85,7 +85,7 @@ SIGNATURES = {
     "oa_kv_pages_truncate": [P, P, P, L, P, P, P, I, I, I, I, P, P],
     "oa_kv4_write": [P, L, L, P, L, L, I, I, I, I, P, P, P, P, P, L, L, I, I, P],
     "oa_kv4_read": [P, P, P, P, P, L, L, I, I, P, L, L, P, L, L, I, I, I, I, P],
-    "oa_kv4_attn": [P, L, L, P, P, P, P, L, L, I, I, P, L, I, P, P, I, I, I, I, I, I, F, I, I, P, P, P, P, L, L, P],
+    "oa_kv4_attn": [P, L, L, P, P, P, P, L, L, I, I, P, L, I, P, P, I, I, I, I, I, I, F, I, I, P, P, P, P, L, L, I, P],
 }
 
 # must equal oa_abi_version() of the loaded library (OA_ABI_VERSION in the header): a library

@@ -961,12 +961,13 @@ def kv4_attn(q, kc, ks, vc, vs, table, lens, sm_scale: float | None = None, cu_q
     """Causal attention of the newest tokens of every sequence over a 4-bit paged cache.
     q (T, HQ, D) bf16, HQ any multiple of the cache's heads; table (B, width) int32 page ids; lens (B,)
     int32 keys that the sequences hold, these tokens among them.  Tokens cu_q[b] .. cu_q[b + 1] - 1
-    (cu_q (B + 1,) int32) are the last of sequence b, at most max_q of them; cu_q None: one token each.
+    (cu_q (B + 1,) int32, 0 to T, not decreasing) are the last of sequence b, at most max_q of them; cu_q
+    None: one token each.
     Token j of R sees keys 0 .. lens[b] - R + j; one that sees none gives 0.  max_len: a bound on lens
     that the caller knows (the table's width otherwise).  NaN: rows that need a page id outside of the
     cache, and those of sequences longer than their table row or than max_len (rounded up to whole pieces,
-    kv4_chunk).  Rows of `out` behind cu_q[B], and tokens past max_q, are left as they
-    were (0 where the call makes it); `out` shares no memory with q.  Sums are held in fp32 and not divided
+    kv4_chunk).  Rows of `out` that no sequence takes, and tokens past max_q, are left
+    as they were (0 where the call makes it); `out` shares no memory with q.  Sums are held in fp32 and not divided
     before their end: values up to 2^80 are safe at any length."""
     i = _where(q, kc, ks, vc, vs, table, lens, cu_q, out)
     ps, where, HKV, Dh = _kv4_cache(kc, ks, vc, vs)
@@ -976,8 +977,9 @@ def kv4_attn(q, kc, ks, vc, vs, table, lens, sm_scale: float | None = None, cu_q
         None if max_len is None else index(max_len), _m(out))
     _plain(q, out)
     qp = q.data_ptr()
+    clear = out is None and cu_q is not None and parts > 0 and B > 0     # (by the join)
     if out is None:
-        out = q.new_empty(T, HQ, Dh) if cu_q is None else q.new_zeros(T, HQ, Dh)
+        out = q.new_empty(T, HQ, Dh) if clear or cu_q is None else q.new_zeros(T, HQ, Dh)
     op = out.data_ptr()
     if T == 0 or B == 0:
         return out
@@ -991,7 +993,7 @@ def kv4_attn(q, kc, ks, vc, vs, table, lens, sm_scale: float | None = None, cu_q
         mp = wp + 4 * parts * Dh
         fp = mp + 8 * parts
     _run(i, "oa_kv4_attn", qp, *qst, *ps, *where, table.data_ptr(), *tsz, lens.data_ptr(), _ptr(cu_q), *sizes, wp, mp, fp, op,
-         *ost)
+         *ost, clear)
     return out
 
 

@@ -507,6 +507,29 @@ def test_attention_bad_pages_lengths_and_starts():
     assert ops.kv4_attn(q[:0], *cache, table[:0], i32([])).shape == (0, 8, 128)
 
 
+@pytest.mark.parametrize("D,HQ,HKV,rows,n", [(128, 8, 2, 3, 100), (128, 8, 2, 3, 5000), (64, 14, 2, 3, 900), (128, 32, 2, 3, 900),
+                                             (128, 64, 2, 3, 5000), (64, 80, 1, 3, 100)])
+def test_rows_of_no_sequence_are_zeros(D, HQ, HKV, rows, n):
+    """An output that the call makes: 0 before the first sequence, behind the last and past max_q, over memory that held
+    NaN, by every kernel and with one piece of keys or several; elsewhere what a given output gets."""
+    g = gen(31)
+    lens = [n, n // 2, n - 7]
+    cache, table = paged(lens, HKV, D, 32, g)
+    q = randn(g, 300, HQ, D, dtype=torch.bfloat16)
+    for cu in ([2, 4, 4, 9], [0, 1, 3, 8], [0, 0, 0, 0], [299, 300, 300, 300], [4, 9, 11, 301], [-1, 2, 3, 3]):
+        own = torch.full_like(q, float("nan"))
+        ops.kv4_attn(q, *cache, table, i32(lens), cu_q=i32(cu), max_q=rows, out=own)
+        used = torch.full_like(q, float("nan"))
+        del used
+        made = ops.kv4_attn(q, *cache, table, i32(lens), cu_q=i32(cu), max_q=rows)
+        taken = torch.zeros(300, dtype=torch.bool)
+        for r0, r1 in zip(cu, cu[1:]):
+            if 0 <= r0 <= r1 <= 300:
+                taken[r0:min(r1, r0 + rows)] = True
+        assert (own.isnan().all((1, 2)).cpu() != taken).all()
+        assert torch.equal(made, torch.where(taken.to(DEV)[:, None, None], own, 0.0))
+
+
 def test_pages_far_apart():
     """Offsets past 32 bits: pages of codes 2^31 + 4096 bytes apart."""
     step = (1 << 31) + 4096

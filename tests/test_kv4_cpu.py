@@ -218,7 +218,7 @@ def test_library_refuses_before_a_launch():
     assert L.oa_kv4_write(*wr[:6], 0, *wr[7:]) == 0
     rd = [16, 16, 16, 16, 16, 4096, 256, 4, 32, 16, 256, 128, 16, 256, 128, 3, 2, 128, 0, None]
     assert L.oa_kv4_read(*rd[:18], 1, None) == -22 and L.oa_kv4_read(None, *rd[1:]) == -22
-    at = [16, 1024, 128, 16, 16, 16, 16, 4096, 256, 4, 32, 16, 2, 2, 16, None, 3, 3, 1, 8, 2, 128, 0.1, 128, 2, 16, 16, 16, 32, 1024, 128, None]
+    at = [16, 1024, 128, 16, 16, 16, 16, 4096, 256, 4, 32, 16, 2, 2, 16, None, 3, 3, 1, 8, 2, 128, 0.1, 128, 2, 16, 16, 16, 32, 1024, 128, 0, None]
     for i, v in ((0, 8), (1, 4), (3, 8), (7, 4000), (9, 0), (10, 31), (11, None), (12, 1), (13, 0), (13, 1 << 26), (14, None), (16, 2), (18, 0), (18, 2), (19, 7), (20, 0),
                  (21, 96), (22, float("nan")), (23, 64), (23, 200), (24, 0), (25, None), (26, None), (28, None), (29, 2), (23, 1 << 30), (24, 1 << 24), (28, 16)):
         assert L.oa_kv4_attn(*at[:i], v, *at[i + 1:]) == -22, (i, v)
