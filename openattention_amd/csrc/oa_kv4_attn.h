@@ -32,6 +32,7 @@ struct AttnArgs {
   float* ws_o; float* ws_ml;             // partial sums, (maximum, sum) by (row, chunk)
   int* ws_flag;                          // by workgroup of oa_kv4_rows.hip
   int B, HKV, G, tokens, max_q, width, NP, lp, chunk, nchunk, ntile;
+  unsigned by_g, by_hkv;                 // 2^16 / G + 1; 2^32 / HKV, rounded up (0: HKV is 1)
   int clear;                             // the join sets rows of out that no sequence takes to 0
   float c;                               // scale * log2 e
 };
