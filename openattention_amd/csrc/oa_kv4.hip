@@ -10,12 +10,13 @@
 // Layout: codes (pages, heads, page, D / 2), scales (pages, heads, page, D / 32), bytes; slot = page id
 // * page + offset.
 //
-// A lane takes 8 values of a row (16 bytes of bf16, 4 of codes), four lanes a block, a workgroup one head
-// of K or V for 16 or 32 successive tokens: where their slots follow each other, as a prompt's do, codes
-// and scales are whole lines (by token, all its heads together, writing and reading 32767 tokens took 85 us).
-// Bound by the bytes moved: 32767 tokens of 8 heads of 128 in bf16, 170 MB each way, 34 us written (5.0 TB/s) and
-// 27 us read back (6.3 TB/s); 32 tokens 2.5 us each.  What passes once (rows in, values out) passes by the
-// caches (62 us together; 70 through them; codes past the caches too: 74).
+// A lane takes 8 values of a row of K and of V (16 bytes of bf16, 4 of codes), four lanes a block, a workgroup one
+// head for 16 or 32 successive tokens: where their slots follow each other, as a prompt's do, codes and scales
+// are whole lines (by token, all its heads together, writing and reading 32767 tokens took 85 us; K and V by
+// workgroups of their own 61; two or four tokens to a lane 58 and 60).
+// Bound by the bytes moved: 32767 tokens of 8 heads of 128 in bf16, 170 MB each way, 32 us written (5.3 TB/s) and
+// 25 us read back (6.7 TB/s), 58 together; 32 tokens 2.6 us each.  What passes once (rows in, values out) passes
+// by the caches (through them 8 us more; codes past the caches too: 12).
 #include "oa_common.h"
 
 namespace {
@@ -44,17 +45,16 @@ struct Kv4Args {
   unsigned nslots;
 };
 
-// a lane's row: its token, whether it is there, and where its values and codes lie
+// a lane's row: its token, whether it is there, and where its codes and scales lie in their tensors
 struct Row {
   int tok;
   unsigned slot;
   bool live;
-  uint8_t* codes;
-  uint8_t* scales;
+  long codes, scales;
 };
 
 template <int D>
-__device__ __forceinline__ Row row_of(const Kv4Args& a, int blk, bool isv, int head) {
+__device__ __forceinline__ Row row_of(const Kv4Args& a, int blk, int head) {
   constexpr int kLanes = D / 8;          // lanes of a row
   Row r;
   r.tok = blk * (kThreads / kLanes) + (int)threadIdx.x / kLanes;
@@ -62,8 +62,8 @@ __device__ __forceinline__ Row row_of(const Kv4Args& a, int blk, bool isv, int h
   r.slot = r.live ? (unsigned)a.slots[r.tok] : ~0u;
   const unsigned s = r.slot < a.nslots ? r.slot : 0, page = s >> a.lp, off = s & ((1u << a.lp) - 1);
   const long in = ((long)head << a.lp) + off;
-  r.codes = (isv ? a.vc : a.kc) + (long)page * a.c_sp + in * (D / 2);
-  r.scales = (isv ? a.vs : a.ks) + (long)page * a.s_sp + in * (D / 32);
+  r.codes = (long)page * a.c_sp + in * (D / 2);
+  r.scales = (long)page * a.s_sp + in * (D / 32);
   return r;
 }
 
@@ -83,16 +83,8 @@ __device__ __forceinline__ unsigned max4(unsigned v) {     // over the lanes of 
   return max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x4E, 0xf, 0xf, false));
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) kv4_write_kernel(Kv4Args a) {
-  typedef typename Vec8<T>::type vec;
-  const int head = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, l = threadIdx.x % (D / 8);
-  const bool isv = rest & 1;
-  const Row r = row_of<D>(a, rest >> 1, isv, head);
-  const int tok = min(r.tok, a.tokens - 1);          // (lanes past the end repeat the last row, unstored)
-  const T* x = isv ? (const T*)a.v + (long)tok * a.v_st + (long)head * a.v_sh
-                   : (const T*)a.k + (long)tok * a.k_st + (long)head * a.k_sh;
-  const f32x8 f = __builtin_convertvector(__builtin_nontemporal_load(reinterpret_cast<const vec*>(x + 8 * l)), f32x8);
+// 8 values of a block of four lanes to codes; the block's scale
+__device__ __forceinline__ unsigned to_codes(const f32x8& f, unsigned& scale) {
   unsigned top = 0;                      // of |x| as bits: NaN above infinity above all else
 #pragma unroll
   for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
@@ -106,23 +98,39 @@ __global__ void __launch_bounds__(kThreads) kv4_write_kernel(Kv4Args a) {
   c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[2] * inv, f[3] * inv, 1.f, 1);
   c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[4] * inv, f[5] * inv, 1.f, 2);
   c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[6] * inv, f[7] * inv, 1.f, 3);
-  const unsigned w = scales_of_row<D>(fine ? e + 127 : 255);
-  if (r.slot >= a.nslots) return;        // padding
-  *reinterpret_cast<unsigned*>(r.codes + 4 * l) = fine ? c : 0u;
-  if (l) return;
-  if (D == 128) *reinterpret_cast<unsigned*>(r.scales) = w;
-  else *reinterpret_cast<uint16_t*>(r.scales) = (uint16_t)w;
+  scale = fine ? e + 127 : 255;
+  return fine ? c : 0u;
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) kv4_read_kernel(Kv4Args a) {
+__global__ void __launch_bounds__(kThreads) kv4_write_kernel(Kv4Args a) {
   typedef typename Vec8<T>::type vec;
-  const int head = blockIdx.x % a.kv_heads, rest = blockIdx.x / a.kv_heads, l = threadIdx.x % (D / 8);
-  const bool isv = rest & 1;
-  const Row r = row_of<D>(a, rest >> 1, isv, head);
-  const bool held = r.slot < a.nslots;   // (padding reads slot 0 and gives zeros)
-  const unsigned c = *reinterpret_cast<const unsigned*>(r.codes + 4 * l);
-  const unsigned s = r.scales[l / 4];
+  const int head = blockIdx.x % a.kv_heads, l = threadIdx.x % (D / 8);
+  const Row r = row_of<D>(a, blockIdx.x / a.kv_heads, head);
+  const int tok = min(r.tok, a.tokens - 1);          // (lanes past the end repeat the last row, unstored)
+  const T* xk = (const T*)a.k + (long)tok * a.k_st + (long)head * a.k_sh + 8 * l;
+  const T* xv = (const T*)a.v + (long)tok * a.v_st + (long)head * a.v_sh + 8 * l;
+  const vec k = __builtin_nontemporal_load(reinterpret_cast<const vec*>(xk));
+  const vec v = __builtin_nontemporal_load(reinterpret_cast<const vec*>(xv));
+  unsigned sk, sv;
+  const unsigned ck = to_codes(__builtin_convertvector(k, f32x8), sk);
+  const unsigned cv = to_codes(__builtin_convertvector(v, f32x8), sv);
+  sk = scales_of_row<D>(sk);
+  sv = scales_of_row<D>(sv);
+  if (r.slot >= a.nslots) return;        // padding
+  *reinterpret_cast<unsigned*>(a.kc + r.codes + 4 * l) = ck;
+  *reinterpret_cast<unsigned*>(a.vc + r.codes + 4 * l) = cv;
+  if (l) return;
+  if (D == 128) {
+    *reinterpret_cast<unsigned*>(a.ks + r.scales) = sk;
+    *reinterpret_cast<unsigned*>(a.vs + r.scales) = sv;
+  } else {
+    *reinterpret_cast<uint16_t*>(a.ks + r.scales) = (uint16_t)sk;
+    *reinterpret_cast<uint16_t*>(a.vs + r.scales) = (uint16_t)sv;
+  }
+}
+
+__device__ __forceinline__ f32x8 to_values(unsigned c, unsigned s) {
   const float f = s == 255 ? __builtin_nanf("") : __uint_as_float(s << 23);
   const bf16x2 b[4] = {__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, 1.f, 0),
                        __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, 1.f, 1),
@@ -130,10 +138,24 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(Kv4Args a) {
                        __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, 1.f, 3)};
   f32x8 y;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = held ? (float)b[i / 2][i % 2] * f : 0.f;
+  for (int i = 0; i < 8; ++i) y[i] = (float)b[i / 2][i % 2] * f;
+  return y;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) kv4_read_kernel(Kv4Args a) {
+  typedef typename Vec8<T>::type vec;
+  const int head = blockIdx.x % a.kv_heads, l = threadIdx.x % (D / 8);
+  const Row r = row_of<D>(a, blockIdx.x / a.kv_heads, head);
+  const bool held = r.slot < a.nslots;   // (padding reads slot 0 and gives zeros)
+  const unsigned ck = *reinterpret_cast<const unsigned*>(a.kc + r.codes + 4 * l), sk = a.ks[r.scales + l / 4];
+  const unsigned cv = *reinterpret_cast<const unsigned*>(a.vc + r.codes + 4 * l), sv = a.vs[r.scales + l / 4];
+  const f32x8 k = held ? to_values(ck, sk) : f32x8(0.f), v = held ? to_values(cv, sv) : f32x8(0.f);
   if (!r.live) return;
-  T* o = isv ? (T*)a.v + (long)r.tok * a.v_st + (long)head * a.v_sh : (T*)a.k + (long)r.tok * a.k_st + (long)head * a.k_sh;
-  __builtin_nontemporal_store(__builtin_convertvector(y, vec), reinterpret_cast<vec*>(o + 8 * l));
+  T* ok = (T*)a.k + (long)r.tok * a.k_st + (long)head * a.k_sh + 8 * l;
+  T* ov = (T*)a.v + (long)r.tok * a.v_st + (long)head * a.v_sh + 8 * l;
+  __builtin_nontemporal_store(__builtin_convertvector(k, vec), reinterpret_cast<vec*>(ok));
+  __builtin_nontemporal_store(__builtin_convertvector(v, vec), reinterpret_cast<vec*>(ov));
 }
 
 // the checks that both directions share
@@ -166,7 +188,7 @@ int take(Kv4Args& a, const void* k, long k_st, long k_sh, const void* v, long v_
 
 dim3 grid_of(const Kv4Args& a, int D) {
   const int rows = kThreads / (D / 8);
-  return dim3((unsigned)((long)((a.tokens + rows - 1) / rows) * 2 * a.kv_heads));
+  return dim3((unsigned)((long)((a.tokens + rows - 1) / rows) * a.kv_heads));
 }
 
 template <typename T>
