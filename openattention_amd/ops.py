@@ -890,7 +890,7 @@ def kv4_write(k, v, slots, kc, ks, vc, vs) -> None:
     """Key and value rows (T, HKV, D) bf16, fp16 or fp32 rounded to 4 bits (blocks of 32 with a power-of-two
     scale) and put at slots (T,) int32 = page id * page + offset of the cache kc, vc (pages, HKV, page,
     D / 2), ks, vs (pages, HKV, page, D / 32) uint8.  Rows of a slot outside of the cache (-1) are passed
-    over.  The slots of one call are distinct (a slot given twice ends with blocks of either row)."""
+    over.  The slots of one call are distinct (one given twice ends with codes and scales of either row)."""
     i = _where(k, v, slots, kc, ks, vc, vs)
     ps, where, HKV, Dh = _kv4_cache(kc, ks, vc, vs)
     kst, vst, sizes = _write_sizes(HKV, Dh, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype, slots.shape,
