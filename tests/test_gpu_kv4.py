@@ -530,6 +530,37 @@ def test_rows_of_no_sequence_are_zeros(D, HQ, HKV, rows, n):
         assert torch.equal(made, torch.where(taken.to(DEV)[:, None, None], own, 0.0))
 
 
+@pytest.mark.parametrize("HQ,HKV,rows", [(8, 2, 4), (64, 2, 4)])
+def test_replays_follow_starts_and_lengths(HQ, HKV, rows):
+    """A captured call whose starts and lengths change between replays gives the eager call's rows, zeros among them."""
+    g = gen(33)
+    lens = [4000, 2500, 700]
+    cache, table = paged(lens, HKV, 128, 64, g)
+    q = randn(g, 16, HQ, 128, dtype=torch.bfloat16)
+    cu, n = i32([0, 4, 8, 12]), i32(lens)
+
+    def call():
+        return ops.kv4_attn(q, *cache, table, n, cu_q=cu, max_q=rows)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for starts, held in (([0, 4, 8, 12], lens), ([0, 1, 1, 2], [3999, 1, 0]), ([3, 3, 7, 10], [64, 2000, 3]), ([0, 0, 0, 0], lens),
+                         ([0, 4, 8, 12], lens)):
+        cu.copy_(i32(starts))
+        n.copy_(i32(held))
+        want = call().clone()
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and not want.isnan().any()
+        assert (out[:starts[0]] == 0).all() and (out[starts[-1]:] == 0).all()
+
+
 def test_pages_far_apart():
     """Offsets past 32 bits: pages of codes 2^31 + 4096 bytes apart."""
     step = (1 << 31) + 4096
