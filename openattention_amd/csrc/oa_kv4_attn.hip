@@ -375,25 +375,29 @@ __global__ void __launch_bounds__(kThreads) kv4_join_kernel(AttnArgs a) {
   const int nv = sq.bad || seen <= 0 ? 0 : (seen + a.chunk - 1) / a.chunk;
   const long row = ((long)(sq.r0 + j) * heads + hd) * a.nchunk;
   const float* ml = a.ws_ml + row * 2;
-  float M = -FLT_MAX;
-  for (int i = tid; i < nv; i += kThreads) M = fmaxf(M, ml[2 * i]);
-  M = oa::wave_max(M);
-  if ((tid & 63) == 0) s_r[tid >> 6] = M;
-  __syncthreads();
-  M = fmaxf(fmaxf(s_r[0], s_r[1]), fmaxf(s_r[2], s_r[3]));
   const int grp = tid / kLanes, y = tid % kLanes;
-  f32x4 o = f32x4(0.f);
-  float L = 0.f;
   constexpr int kAtOnce = 4;             // pieces whose loads are in flight together
-  for (int i = grp; i < nv; i += kAtOnce * kGroups) {
-    f32x4 x[kAtOnce];
-    f32x2 w[kAtOnce];
+  f32x4 x[kAtOnce];
+  f32x2 w[kAtOnce];
+  auto fetch = [&](int i) {
 #pragma unroll
     for (int k = 0; k < kAtOnce; ++k) {
       const int at = min(i + k * kGroups, nv - 1);
       x[k] = *reinterpret_cast<const f32x4*>(a.ws_o + (row + at) * D + 4 * y);
       w[k] = *reinterpret_cast<const f32x2*>(ml + 2 * at);
     }
+  };
+  if (grp < nv) fetch(grp);              // (beside the maxima: one sequence of 131072 keys 30.9 us, 32.2 after them)
+  float M = -FLT_MAX;
+  for (int i = tid; i < nv; i += kThreads) M = fmaxf(M, ml[2 * i]);
+  M = oa::wave_max(M);
+  if ((tid & 63) == 0) s_r[tid >> 6] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(s_r[0], s_r[1]), fmaxf(s_r[2], s_r[3]));
+  f32x4 o = f32x4(0.f);
+  float L = 0.f;
+  for (int i = grp; i < nv; i += kAtOnce * kGroups) {
+    if (i > grp) fetch(i);
 #pragma unroll
     for (int k = 0; k < kAtOnce; ++k) {
       if (i + k * kGroups >= nv) break;
