@@ -159,10 +159,11 @@ __global__ void __launch_bounds__(kThreads, 2) kv4_rows_kernel(AttnArgs a) {
     } else {
       unsigned any = y.v[0];
       if constexpr (kWords > 1) any |= y.v[1];
-      const bool zero = t.out || !(any & 0x77777777u);
+      // (NaN first: its codes are 0 where oa_kv4_write put them, and zeros have no scale to be out of span)
+      const bool nan = y.vs == 255 && !t.out, zero = t.out || !(any & 0x77777777u);
       const int x = (int)y.vs - (int)ref;
-      if (!zero && y.vs != 255 && (x < -kSpan || x > kSpan)) wide = 1;
-      t.f = __uint_as_float(zero ? 0x3f800000u : y.vs == 255 ? 0x7f800000u : (unsigned)(127 + x) << 23);
+      if (!zero && !nan && (x < -kSpan || x > kSpan)) wide = 1;
+      t.f = __uint_as_float(nan ? 0x7f800000u : zero ? 0x3f800000u : (unsigned)(127 + x) << 23);
     }
     return t;
   };

@@ -1,0 +1,50 @@
+"""The 4-bit paged cache on the GPU where its first tests do not reach: values that are not finite among keys that every
+row sees."""
+import math
+
+import pytest
+import torch
+
+from openattention_amd import ops
+from tests import kv4_ref as ref
+from tests.test_gpu_kv4 import DEV, check_attn, gen, i32, paged, randn, starts, want_attn
+
+pytestmark = pytest.mark.gpu
+
+
+# 380 keys are one piece of the many-row kernel's, 900 three; 40 tokens of 4 query heads are 160 rows (two workgroups),
+# 17 are 68 (one, most of whose waves have no row), 16 are 64: the other kernel
+@pytest.mark.parametrize("rows", [16, 17, 40])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n", [380, 900])
+def test_a_value_that_every_row_sees_and_is_not_finite(rows, D, n):
+    """It makes NaN of its block of 32 dims in every row, in the first tile and in a later one, of one block or of a whole
+    tile's, whatever codes lie under the scale of NaN; the other blocks, heads and sequences keep their numbers."""
+    print(f"[case] NaN values: {rows} tokens, D {D}, {n} keys", flush=True)
+    g = gen(n + rows)
+    lens, page, HKV = [n] * 4, 32, 2
+    cache, table = paged(lens, HKV, D, page, g)
+    held = ref.held(table, lens, page)
+
+    def put(b, keys, head, dim, value):
+        k, v = randn(g, len(keys), HKV, D), randn(g, len(keys), HKV, D)
+        v[:, head, dim] = value
+        ops.kv4_write(k, v, held[b][keys].int().to(DEV), *cache)
+    put(0, [3], 1, 40, math.nan)                              # the first tile
+    put(1, [n // 2], 0, D - 1, math.inf)                      # a tile in the middle
+    put(2, list(range(32)), 1, 1, -math.inf)                  # a whole tile, the first one
+    put(3, [n // 2 + 1], 0, 5, math.nan)                      # beside a value that fp16 does not hold by the others' scale
+    put(3, [9, 11], 0, D - 2, 2.0 ** 40)
+    at = int(held[2][n // 2])                                 # codes that are not 0 under NaN's scale
+    cache[3][at // page, 0, at % page, 1] = 255
+    assert (cache[2][at // page, 0, at % page, 16:32] & 0x77 != 0).any()
+    cu = starts([rows] * 4)
+    q = randn(g, cu[-1], 8, D, dtype=torch.bfloat16)
+    out = ops.kv4_attn(q, *cache, table, i32(lens), cu_q=i32(cu), max_q=rows)
+    want, err = want_attn(q, cache, table, lens, cu, D ** -0.5, page)
+    blocks = want.isnan().view(4, rows, HKV, 4, D // 32, 32)
+    there = torch.zeros(4, 1, HKV, 1, D // 32, 1, dtype=torch.bool, device=DEV)
+    there[0, :, 1, :, 1], there[1, :, 0, :, -1], there[2, :, 1, :, 0], there[2, :, 0, :, 1] = True, True, True, True
+    there[3, :, 0, :, 0] = True
+    assert torch.equal(blocks, there.expand_as(blocks))
+    check_attn(out, want, err)
