@@ -931,7 +931,8 @@ def kv4_chunk(cap: int, units: int, rows: int) -> int:
 
 
 @_sizes
-def _attn_sizes(HKV, Dh, page, qs, qst, qt, ts, tst, tt, ls, lst, lt, cu, max_q, sm_scale, max_len, o) -> tuple:
+def _attn_sizes(HKV, Dh, page, qs, qst, qt, ts, tst, tt, ls, lst, lt, cu, max_q, sm_scale, max_len, o, rule) -> tuple:
+    # rule: kv4_chunk, a part of what is looked up, so that no call gets the pieces of another rule
     tstride, B, width = _table_sizes(ts, tst, tt, page)
     _need(len(qs) == 3 and qs[2] == Dh and qt is torch.bfloat16 and qs[1] >= 1 and qs[1] % HKV == 0,
           f"q: (T, a multiple of {HKV}, {Dh}) bf16")
@@ -948,7 +949,7 @@ def _attn_sizes(HKV, Dh, page, qs, qst, qt, ts, tst, tt, ls, lst, lt, cu, max_q,
     rows = max_q * (HQ // HKV)
     cap = max(1, width * page if max_len is None else min(max_len, width * page))
     units = B * HKV * -(-rows // (8 if rows <= 8 else 16 if rows <= 16 else 32 if rows <= 64 else 128))
-    chunk = kv4_chunk(cap, units, rows)
+    chunk = rule(cap, units, rows)
     nchunk = -(-cap // chunk)
     return (T, HQ, B, _row_strides(T, HQ, Dh, qst, qt, "q"),
             (HQ * Dh, Dh) if o is None else _row_strides(T, HQ, Dh, o[1], qt, "out", True), (tstride, width),
@@ -974,7 +975,7 @@ def kv4_attn(q, kc, ks, vc, vs, table, lens, sm_scale: float | None = None, cu_q
     T, HQ, B, qst, ost, tsz, sizes, parts, flags = _attn_sizes(
         HKV, Dh, where[3], q.shape, q.stride(), q.dtype, table.shape, table.stride(), table.dtype, lens.shape, lens.stride(),
         lens.dtype, _m(cu_q), index(max_q), None if sm_scale is None else float(sm_scale),
-        None if max_len is None else index(max_len), _m(out))
+        None if max_len is None else index(max_len), _m(out), kv4_chunk)
     _plain(q, out)
     qp = q.data_ptr()
     clear = out is None and cu_q is not None and parts > 0 and B > 0     # (by the join)
