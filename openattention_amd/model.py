@@ -199,7 +199,8 @@ class LlamaShaped:
             gu = h @ self.w13[l]
             x = x + (torch.nn.functional.silu(gu[:, :FFN]) * gu[:, FFN:]) @ self.w2[l]
         logits = rmsnorm(x, self.lnf) @ self.lm_head
-        self.tok.copy_(logits.argmax(-1))
+        # (a refused step's positions are -1: its tokens wait for the next one)
+        self.tok.copy_(torch.where(pos >= 0, logits.argmax(-1), self.tok))
         return self.tok
 
     @torch.no_grad()
@@ -208,7 +209,7 @@ class LlamaShaped:
         device; the host n only fixes the sparse stage's sink/local/top-k counts).  Writes the
         greedy next token into self.tok and returns it.  With a 4-bit cache n is not used: each token
         sits at its request's length, which the step extends (a step that the cache refuses, out of
-        pages or past max_len, leaves lengths and rows as they were: KV4Cache.check)."""
+        pages or past max_len, leaves lengths, rows and self.tok as they were: KV4Cache.check)."""
         if self.cache is not None:
             return self._step_cache()
         B = self.B

@@ -1,0 +1,48 @@
+"""The Llama-shaped model over a 4-bit paged cache at the cache's limits: its last positions, steps and prompts that are
+refused."""
+import pytest
+import torch
+
+from openattention_amd.model import VOCAB
+from tests.test_gpu_kv4 import DEV, i32
+from tests.test_gpu_kv4_model import model_of
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_refused_steps_token_is_taken_up_again(captured):
+    """A step that lacks pages leaves the tokens where they were: the step after a request has ended gives the others
+    what they would have got with pages enough."""
+    B, T = 2, 31
+    tokens = torch.randint(0, VOCAB, (B, T), generator=torch.Generator().manual_seed(6)).to(DEV)
+    model, cache = model_of(B, T, 1, False)
+    model.prefill(tokens)
+    want = [model.step().clone() for _ in range(2)]
+    model, cache = model_of(B, T, 1, False, pages=3)
+    model.prefill(tokens)
+    step = model.step
+    if captured:
+        state = [t.clone() for t in (cache.lens, cache.table, cache.free, cache.nfree, *cache.rows[0], model.tok)]
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            model.step()
+        torch.cuda.current_stream().wait_stream(s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            model.step()
+        for t, u in zip((cache.lens, cache.table, cache.free, cache.nfree, *cache.rows[0], model.tok), state):
+            t.copy_(u)
+        step = graph.replay
+    step()
+    assert torch.equal(model.tok, want[0])
+    for _ in range(2):
+        step()
+        assert cache.lens.tolist() == [32, 32] and torch.equal(model.tok, want[0])
+        with pytest.raises(RuntimeError, match="free pages"):
+            cache.check()
+    cache.truncate(i32([-1, 0]))
+    step()
+    cache.check()
+    assert cache.lens.tolist() == [33, 1] and int(model.tok[0]) == int(want[1][0])
