@@ -55,7 +55,8 @@ class LlamaShaped:
                  qk_norm: bool = False):
         """method: an OursHIP over these layers (sparse attention) or None (dense attention).
         The KV cache is C.K / C.V (set by the caller), (B, 8, Lmax, 128) bf16 per layer, or `cache`, a
-        KV4Cache of B requests and these layers (method None)."""
+        KV4Cache of B requests and these layers (method None): steps go on to the end of its pages, also
+        past Lmax."""
         if cache is not None and (method is not None or cache.B != B or cache.layers != layers):
             raise ValueError("cache: for B requests and these layers, without a method")
         self.B, self.Lmax, self.dev, self.L = B, Lmax, dev, layers
@@ -76,10 +77,11 @@ class LlamaShaped:
         self.lnf = torch.ones(HID, **bf)
         self.lm_head = w(HID, VOCAB)
         inv = llama31_inv_freq().to(dev)
-        t = torch.arange(Lmax, device=dev, dtype=torch.float32)
+        P = Lmax if cache is None else max(Lmax, cache.width * cache.page)      # (a 4-bit cache's length is in whole pages)
+        t = torch.arange(P, device=dev, dtype=torch.float32)
         fr = torch.outer(t, inv)
         emb = torch.cat([fr, fr], -1)
-        self.cos, self.sin = emb.cos(), emb.sin()                       # (Lmax, D) fp32
+        self.cos, self.sin = emb.cos(), emb.sin()                       # (P, D) fp32
         self.half = self.cos[:, :D // 2], self.sin[:, :D // 2]           # (a head's halves turn by the same angles)
         self.qn, self.kn = ([1 + w(D) * 5 for _ in range(layers)] if qk_norm else [None] * layers for _ in range(2))
         self.tok = torch.zeros(B, device=dev, dtype=torch.long)         # token at position n - 1

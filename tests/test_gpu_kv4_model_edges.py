@@ -3,7 +3,9 @@ refused."""
 import pytest
 import torch
 
-from openattention_amd.model import VOCAB
+from openattention_amd import KV4Cache
+from openattention_amd.model import VOCAB, LlamaShaped
+from tests import kv4_ref as ref
 from tests.test_gpu_kv4 import DEV, i32
 from tests.test_gpu_kv4_model import model_of
 
@@ -46,3 +48,34 @@ def test_a_refused_steps_token_is_taken_up_again(captured):
     step()
     cache.check()
     assert cache.lens.tolist() == [33, 1] and int(model.tok[0]) == int(want[1][0])
+
+
+def test_steps_up_to_the_caches_last_token():
+    """A cache's length is rounded up to whole pages: steps behind the length that was asked for are as good as those of a
+    model made for all of them, and the first one past the pages is refused and changes nothing, the token included."""
+    B, T, Lmax = 2, 120, 125
+    tokens = torch.randint(0, VOCAB, (B, T), generator=torch.Generator().manual_seed(5)).to(DEV)
+    took, rows = [], []
+    for length in (Lmax, 128):
+        cache = KV4Cache(B, length, DEV, page=32)
+        model = LlamaShaped(B, length, DEV, layers=1, seed=3, cache=cache)
+        took.append([model.prefill(tokens).clone()] + [model.step().clone() for _ in range(8)])
+        cache.check()
+        assert cache.lens.tolist() == [128, 128]
+        rows.append(cache.read(0, ref.held(cache.table, [128, 128], 32)[1].int().to(DEV)))
+        now = [t.clone() for t in (cache.lens, cache.table, cache.free, cache.nfree, *cache.rows[0], model.tok)]
+        model.step()
+        assert all(torch.equal(a, b) for a, b in zip(now, (cache.lens, cache.table, cache.free, cache.nfree, *cache.rows[0], model.tok)))
+        with pytest.raises(RuntimeError, match="max_len"):
+            cache.check()
+    assert all(torch.equal(a, b) for a, b in zip(*took))
+    assert all(torch.equal(a, b) and not a.isnan().any() for a, b in zip(*rows))
+    # a cache for more tokens than the model was made for
+    cache = KV4Cache(B, 160, DEV, page=32)
+    model = LlamaShaped(B, Lmax, DEV, layers=1, seed=3, cache=cache)
+    assert torch.equal(model.prefill(tokens), took[0][0])
+    for want in took[0][1:]:
+        assert torch.equal(model.step(), want)
+    model.step()
+    cache.check()
+    assert cache.lens.tolist() == [129, 129] and not cache.read(0, ref.held(cache.table, [129, 129], 32)[0].int().to(DEV))[0].isnan().any()
