@@ -125,8 +125,9 @@ class LlamaShaped:
         the row's K, V are written to C.K[l][b, :, :T], its causal attention is dense and the
         method builds the row's index (C.qlen[b] = qlen question rows).  Leaves C.phase at
         "decode" and the greedy next token of every row in self.tok; returns it.  With a 4-bit cache the
-        row extends its request there (an empty one), its keys and values are written to the new slots and
-        its own attention is dense over the unrounded rows."""
+        rows extend its requests (empty ones; all of them, or none where the cache refuses: RuntimeError), a
+        row's keys and values are written to the new slots and its own attention is dense over the unrounded
+        rows."""
         B, T = tokens.shape
         if B != self.B or T > self.Lmax:
             raise ValueError(f"tokens must be ({self.B}, <= {self.Lmax})")
@@ -167,16 +168,17 @@ class LlamaShaped:
         cache = self.cache
         if bool((cache.lens != 0).any()):
             raise ValueError("prefill: the cache's requests must be empty (KV4Cache.truncate)")
+        cache.check()                                                              # (an earlier call's refusal)
+        slots, pos, _ = cache.extend(torch.full_like(cache.lens, T), B * T)        # all requests or none
+        cache.check()
+        where = pos[:T]
         for b in range(B):
-            add = torch.zeros(B, device=self.dev, dtype=torch.int32)
-            add[b] = T
-            slots, pos, _ = cache.extend(add, T)
-            cache.check()
+            at = slots[b * T:(b + 1) * T]
             x = self.embed.index_select(0, tokens[b])                              # (T, HID)
             for l in range(self.L):
                 h = rmsnorm(x, self.ln1[l])
-                q, k, v = self._qkv(l, h @ self.wqkv[l], pos)
-                cache.write(l, k, v, slots)
+                q, k, v = self._qkv(l, h @ self.wqkv[l], where)
+                cache.write(l, k, v, at)
                 o = prefill_attention(*(t.transpose(0, 1).unsqueeze(0) for t in (q, k, v)), D ** -0.5)
                 x = x + o[0].transpose(0, 1).reshape(T, HQ * D) @ self.wo[l]
                 del q, k, v, o

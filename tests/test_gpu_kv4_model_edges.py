@@ -79,3 +79,24 @@ def test_steps_up_to_the_caches_last_token():
     model.step()
     cache.check()
     assert cache.lens.tolist() == [129, 129] and not cache.read(0, ref.held(cache.table, [129, 129], 32)[0].int().to(DEV))[0].isnan().any()
+
+
+def test_prompts_that_do_not_fit_change_nothing():
+    """Prompts for which the pool has too few pages, or that meet a refusal nobody has looked at, are refused as a whole:
+    no request is extended, and the same prompts go through where they fit."""
+    B, T = 3, 40
+    tokens = torch.randint(0, VOCAB, (B, T), generator=torch.Generator().manual_seed(7)).to(DEV)
+    model, cache = model_of(B, T, 1, False, pages=5)
+    for _ in range(2):
+        model.tok.fill_(11)
+        with pytest.raises(RuntimeError, match="free pages"):
+            model.prefill(tokens)
+        assert cache.lens.tolist() == [0] * B and int(cache.nfree) == 5 and (cache.table == -1).all() and (model.tok == 11).all()
+    first = model.prefill(tokens[:, :32]).clone()
+    assert cache.lens.tolist() == [32] * B and int(cache.nfree) == 2
+    cache.truncate(i32([0] * B))
+    cache.extend(i32([999, 0, 0]), 999)                       # refused
+    with pytest.raises(RuntimeError, match="max_len"):
+        model.prefill(tokens[:, :32])
+    assert cache.lens.tolist() == [0] * B and int(cache.nfree) == 5
+    assert torch.equal(model.prefill(tokens[:, :32]), first)
