@@ -571,8 +571,8 @@ int oa_qk_norm_rope(const void* q, long q_st, long q_sh, const void* k, long k_s
  * lengths restores the stack that an extension changed.
  *
  * Either takes effect for all requests or for none; then nothing changes (an extension's slots, pos are -1,
- * its cu 0) and *status |= 1 (a negative count, a length outside of the table's row), 2 (too few free pages,
- * or more than the stack holds), 4 (more than total tokens).  ws: 3 requests + 1 ints of scratch; NULL
+ * its cu 0) and *status |= 1 (a negative count to add, a length outside of the table's row), 2 (too few free
+ * pages, or more than the stack holds), 4 (more than total tokens).  ws: 3 requests + 1 ints of scratch; NULL
  * will do for an extension of at most 1024 requests by at most 2048 tokens and a truncation of at most 256
  * requests.
  */

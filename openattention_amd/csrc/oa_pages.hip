@@ -7,7 +7,7 @@
 // their pages, a truncation pushes them so that the stack is what it was before the extension that it
 // undoes: page k of R popped pages was at nfree - 1 - k, page k of R returned ones goes to
 // nfree + R - 1 - k.  Both take effect for all requests or for none; what went wrong is or-ed into
-// *status (1: a negative count or a request longer than its row of the table; 2: too few free pages, or
+// *status (1: a negative count to add, a length outside of its row of the table; 2: too few free pages, or
 // more than a stack can hold; 4: more tokens than the caller has slots for).
 //
 // One workgroup adds up what every request needs (a scan over the requests, as many threads as there are up
@@ -217,16 +217,20 @@ __device__ __forceinline__ void give_back(const PagesArgs& a, int i, int left, i
 template <int THREADS>
 __global__ void __launch_bounds__(THREADS) pages_truncate_kernel(PagesArgs a, int alone) {
   __shared__ Scan<THREADS> s;
+  __shared__ int s_bad;
   __shared__ int s_left[THREADS], s_gone[THREADS], s_first[THREADS];
   const int tid = threadIdx.x;
   const bool once = a.B <= THREADS;
+  if (tid == 0) s_bad = 0;
   const int nfree = min(max(*a.nfree, 0), a.NP);
+  __syncthreads();
   unsigned pages = 0, e0 = 0, e1 = 0, t1;
   int gone = 0, keep = 0;
   auto returned = [&](int i) {
     gone = keep = 0;
     if (i < a.B) {
       const int len = held_len(a, i), k = a.count[i];
+      if (len != a.lens[i]) atomicOr(&s_bad, 1);
       keep = k < 0 ? len : min(k, len);
       gone = pages_of(len, a.lp) - pages_of(keep, a.lp);
     }
@@ -239,7 +243,8 @@ __global__ void __launch_bounds__(THREADS) pages_truncate_kernel(PagesArgs a, in
     block_scan<THREADS>(s, e0, e1, t0, t1);
     pages = add_to(pages, t0);
   }
-  const bool bad = pages > (unsigned)(a.NP - nfree);
+  __syncthreads();
+  const int bad = s_bad | (pages > (unsigned)(a.NP - nfree) ? 2 : 0);
   const int top = nfree + (bad ? 0 : (int)pages);
   unsigned page0 = 0;
   for (int i0 = 0; i0 < a.B; i0 += THREADS) {
@@ -268,7 +273,7 @@ __global__ void __launch_bounds__(THREADS) pages_truncate_kernel(PagesArgs a, in
   }
   if (tid == 0) {
     if (!alone) a.ws[2 * a.B] = top;
-    if (bad) *a.status |= 2;
+    if (bad) *a.status |= bad;
     else *a.nfree = top;
   }
   if (!alone) return;

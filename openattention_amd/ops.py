@@ -839,7 +839,8 @@ def kv_pages_extend(add, lens, table, free, nfree, status, page: int, total: int
 def kv_pages_truncate(keep, lens, table, free, nfree, status, page: int) -> None:
     """Request i keeps its first min(keep[i], lens[i]) tokens (keep[i] < 0: all; 0: the request ends); pages
     it no longer needs go back to the stack and leave the table (-1).  A truncation to the lengths before
-    an extension undoes it.  Nothing changes where the stack would outgrow `free` (status |= 2)."""
+    an extension undoes it.  For all requests or for none: nothing changes where the stack would outgrow `free`
+    (status |= 2) or a length lies outside of its row (1)."""
     i = _where(keep, lens, table, free, nfree, status)
     stride, B, sizes = _pages_sizes(index(page), table.shape, table.stride(), table.dtype, free.shape, free.stride(), free.dtype,
                                     _m(keep), _m(lens), _m(nfree), _m(status), "keep")

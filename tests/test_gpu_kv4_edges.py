@@ -1,5 +1,5 @@
 """The 4-bit paged cache on the GPU where its first tests do not reach: values that are not finite among keys that every
-row sees."""
+row sees, truncations that are refused."""
 import math
 
 import pytest
@@ -48,3 +48,24 @@ def test_a_value_that_every_row_sees_and_is_not_finite(rows, D, n):
     there[3, :, 0, :, 0] = True
     assert torch.equal(blocks, there.expand_as(blocks))
     check_attn(out, want, err)
+
+
+@pytest.mark.parametrize("B", [3, 40, 300, 1100])
+@pytest.mark.parametrize("wrong", [-5, 129, 1 << 30])
+def test_truncation_of_a_length_outside_of_the_row(B, wrong):
+    """It is refused as an extension is: the status says so, and nothing changes for any request, also not a length
+    that is to be kept as it is."""
+    g = gen(B)
+    table = torch.randperm(4 * B, generator=g, device=DEV).int().view(B, 4)
+    lens = torch.randint(0, 129, (B,), generator=g, device=DEV, dtype=torch.int32)
+    lens[B // 2] = wrong
+    for keep in (torch.full_like(lens, -1), torch.zeros_like(lens), lens // 2):
+        st = [lens.clone(), table.clone(), torch.full((8 * B,), 9, device=DEV, dtype=torch.int32), i32([B]), i32([8])]
+        before = [t.clone() for t in st]
+        ops.kv_pages_truncate(keep, *st, 32)
+        assert int(st[4]) == 8 | 1
+        assert all(torch.equal(a, b) for a, b in zip(st[:4], before[:4]))
+    # too many pages for the stack as well
+    st = [torch.where(lens == wrong, wrong, 128).int(), table.clone(), torch.full((B,), 9, device=DEV, dtype=torch.int32), i32([B]), i32([0])]
+    ops.kv_pages_truncate(torch.zeros_like(lens), *st, 32)
+    assert int(st[4]) == 3 and torch.equal(st[1], table) and int(st[3]) == B
