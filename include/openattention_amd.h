@@ -609,11 +609,13 @@ int oa_kv4_read(const int* slots, const void* kc, const void* ks, const void* vc
  * of R sees keys 0 .. lens - R + j.  out as q, not q.  fp32 scores,
  * softmax and sums (values up to 2^80 are safe at any length); weights in 16 bits, 11 past 64 rows of a KV head.
  * A row that sees no key gives 0; rows that no sequence takes, and tokens of a sequence from max_q on, are left as
- * they were, or, with `clear` and more than one piece, set to 0 (then the starts do not decrease).  NaN: rows that need a page id outside of the cache, and
- * those of sequences longer than their table row or than nchunk * chunk keys.  Keys are split into nchunk pieces
+ * they were, or, with `clear` and more than one piece, set to 0 (then the starts do not decrease).  NaN: rows that
+ * need a page id outside of the cache, and those of sequences longer than their table row or than nchunk * chunk keys.  Keys are split into nchunk pieces
  * of `chunk` (a multiple of 128); with more than one, ws_o (tokens * q_heads * nchunk * head_dim) and ws_ml (* 2)
  * floats hold the pieces' sums; with more than 64 rows of a KV head (max_q * q_heads / kv_heads), ws_flag holds
- * sequences * kv_heads * nchunk * ceil(rows / 128) ints.
+ * sequences * kv_heads * nchunk * ceil(rows / 128) ints.  Grids hold 2^24 - 1 workgroups (sequences * kv_heads *
+ * nchunk * tiles of 8, 16, 32 or, past 64 rows, 128 rows), 65535 pieces and, with more than one, 65535 sequences
+ * and 2^24 - 1 query rows of one (max_q * q_heads).
  */
 int oa_kv4_attn(const void* q, long q_st, long q_sh, const void* kc, const void* ks, const void* vc, const void* vs,
                 long code_stride, long scale_stride, int pages, int page, const int* table, long table_stride, int width,

@@ -672,6 +672,7 @@ def prefill_attn(q, k, v, sm_scale: float) -> torch.Tensor:
 # Numbers go in as Python's own, so that no tensor's value is taken for another's.
 _DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 KV4_BLOCK = 32             # values that share a scale
+_GRID = (1 << 24) - 1      # workgroups of 256 threads along a grid's axis, whose threads are counted in 32 bits
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _get_device = torch._C._cuda_getDevice
 _forward_ad = torch.autograd.forward_ad
@@ -950,8 +951,11 @@ def _attn_sizes(HKV, Dh, page, qs, qst, qt, ts, tst, tt, ls, lst, lt, cu, max_q,
     rows = max_q * (HQ // HKV)
     cap = max(1, width * page if max_len is None else min(max_len, width * page))
     units = B * HKV * -(-rows // (8 if rows <= 8 else 16 if rows <= 16 else 32 if rows <= 64 else 128))
-    chunk = rule(cap, units, rows)
+    # (the join's grid holds 65535 sequences; so many need no pieces to fill the card)
+    chunk = rule(cap, units, rows) if B <= 65535 else -(-cap // 128) * 128
     nchunk = -(-cap // chunk)
+    _need(units * nchunk <= _GRID and B * HKV * HKV < 1 << 32,
+          f"at most {_GRID} workgroups (sequences x heads x tiles of rows x pieces), sequences x heads^2 under 2^32")
     return (T, HQ, B, _row_strides(T, HQ, Dh, qst, qt, "q"),
             (HQ * Dh, Dh) if o is None else _row_strides(T, HQ, Dh, o[1], qt, "out", True), (tstride, width),
             (B, T, max_q, HQ, HKV, Dh, scale, chunk, nchunk), T * HQ * nchunk if nchunk > 1 else 0,
@@ -970,7 +974,9 @@ def kv4_attn(q, kc, ks, vc, vs, table, lens, sm_scale: float | None = None, cu_q
     cache, and those of sequences longer than their table row or than max_len (rounded up to whole pieces,
     kv4_chunk).  Rows of `out` that no sequence takes, and tokens past max_q, are left
     as they were (0 where the call makes it); `out` shares no memory with q.  Sums are held in fp32 and not divided
-    before their end: values up to 2^80 are safe at any length."""
+    before their end: values up to 2^80 are safe at any length.  Sequences are cut into pieces by kv4_chunk, more than
+    65535 of them not at all; at most 2^24 - 1 workgroups (a sequence's, by head, for 8, 16, 32 or, past 64
+    rows of a KV head, 128 rows each)."""
     i = _where(q, kc, ks, vc, vs, table, lens, cu_q, out)
     ps, where, HKV, Dh = _kv4_cache(kc, ks, vc, vs)
     T, HQ, B, qst, ost, tsz, sizes, parts, flags = _attn_sizes(

@@ -1,5 +1,5 @@
 """The 4-bit paged cache on the GPU where its first tests do not reach: values that are not finite among keys that every
-row sees, truncations that are refused."""
+row sees, truncations that are refused, very many sequences."""
 import math
 
 import pytest
@@ -7,7 +7,7 @@ import torch
 
 from openattention_amd import ops
 from tests import kv4_ref as ref
-from tests.test_gpu_kv4 import DEV, check_attn, gen, i32, paged, randn, starts, want_attn
+from tests.test_gpu_kv4 import DEV, check_attn, gen, i32, new_cache, paged, randn, starts, want_attn
 
 pytestmark = pytest.mark.gpu
 
@@ -69,3 +69,22 @@ def test_truncation_of_a_length_outside_of_the_row(B, wrong):
     st = [torch.where(lens == wrong, wrong, 128).int(), table.clone(), torch.full((B,), 9, device=DEV, dtype=torch.int32), i32([B]), i32([0])]
     ops.kv_pages_truncate(torch.zeros_like(lens), *st, 32)
     assert int(st[4]) == 3 and torch.equal(st[1], table) and int(st[3]) == B
+
+
+def test_attention_of_more_sequences_than_a_grids_axis_holds():
+    """65537 sequences in a table whose width alone would cut each into pieces."""
+    g = gen(65)
+    B, HQ, D, page, NP = 65537, 2, 64, 32, 300
+    cache = new_cache(NP, 1, page, D, g=g)
+    for slots in torch.arange(NP * page, device=DEV, dtype=torch.int32).split(4096):
+        ops.kv4_write(randn(g, slots.numel(), 1, D), randn(g, slots.numel(), 1, D), slots, *cache)
+    table = torch.randint(0, NP, (B, 40), generator=g, device=DEV, dtype=torch.int32)
+    lens = torch.randint(0, 90, (B,), generator=g, device=DEV, dtype=torch.int32)
+    some = [0, 1, 77, 32768, 65534, 65535, 65536]
+    lens[some] = i32([1280, 0, 1100, 33, 700, 1, 1280])
+    q = randn(g, B, HQ, D, dtype=torch.bfloat16)
+    out = ops.kv4_attn(q, *cache, table, lens)
+    at = torch.tensor(some, device=DEV)
+    check_attn(out[at], *want_attn(q[at], cache, table[at], lens[at].tolist(), list(range(len(some) + 1)), D ** -0.5, page))
+    # and the others as they are in a batch of their own
+    assert torch.equal(out[1000:9000], ops.kv4_attn(q[1000:9000], *cache, table[1000:9000], lens[1000:9000], max_len=96))

@@ -35,3 +35,29 @@ def test_the_rule_for_pieces_is_looked_up_in_every_call(calls, case, monkeypatch
             want = min(chunk, -(-cap // 128) * 128)
             assert call() == call() == (want, -(-cap // want))
     assert call() == own
+
+
+@pytest.mark.parametrize("B", [65535, 65536, 1 << 20])
+def test_more_sequences_than_a_grids_axis_holds_take_one_piece_each(calls, B):  # noqa: F811
+    """The join counts sequences along an axis of 65535; so many fill the card with a piece each."""
+    c = cache(NP=2, H=1, page=32, D=64)
+    q, lens = torch.zeros(B, 1, 64, dtype=torch.bfloat16), torch.zeros(B, dtype=torch.int32)
+    ops.kv4_attn(q, **c, table=torch.zeros(B, 40, dtype=torch.int32), lens=lens)
+    chunk, n = attn_sizes(calls[-1])
+    assert chunk * n >= 1280 and (n > 1) == (B == 65535) and (n > 1 or chunk == 1280)
+    ops.kv4_attn(q, **c, table=torch.zeros(B, 40, dtype=torch.int32), lens=lens, max_len=100)
+    assert attn_sizes(calls[-1]) == (128, 1)
+
+
+def test_what_a_grid_does_not_hold_is_refused_by_name(calls):  # noqa: F811
+    """More than 2^24 - 1 workgroups: the library's own answer would be its invalid argument."""
+    for H, HQ, B, width, rows in ((1, 1, 1 << 24, 2, None), (2, 8, 1 << 23, 2, None), (64, 64, 1 << 18, 1, None), (1, 65, 1 << 23, 2, 4),
+                                  (1, 1, 130, 400, 1 << 24), (1 << 16, 1 << 16, 1, 1, None)):
+        c = cache(NP=1, H=H, page=32, D=64)
+        T = B if rows is None else 9
+        q = torch.zeros(1, 1, 64, dtype=torch.bfloat16).expand(T, HQ, 64)
+        kw = {} if rows is None else dict(cu_q=torch.zeros(B + 1, dtype=torch.int32), max_q=rows)
+        table = torch.zeros(B, width, dtype=torch.int32)
+        with pytest.raises(ValueError, match="workgroups"):
+            ops.kv4_attn(q, **c, table=table, lens=torch.zeros(B, dtype=torch.int32), out=torch.empty(T, HQ, 64, dtype=torch.bfloat16), **kw)
+    assert not calls
