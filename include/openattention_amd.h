@@ -550,7 +550,7 @@ int oa_step(const oa_step_args* args, void* stream);
  * in fp32, rounded once.  dtype 0 / 1 / 2: bf16 / fp16 / fp32 rows; head_dim 64, 128 or 256; pos int32 or,
  * pos_is_64, int64; cos_t, sin_t: (positions, head_dim / 2) fp32 rows of table_stride.  A token of negative
  * position (padding) gives zeros, one past the tables NaN.  Bases 16-byte aligned, strides multiples of 16
- * bytes; outputs may be the inputs.
+ * bytes.  q_out may be q, k_out k, of the same strides; otherwise outputs share no memory with anything.
  */
 int oa_qk_norm_rope(const void* q, long q_st, long q_sh, const void* k, long k_st, long k_sh, int tokens,
                     int q_heads, int kv_heads, int head_dim, int dtype, const void* pos, int pos_is_64,
@@ -606,7 +606,7 @@ int oa_kv4_read(const int* slots, const void* kc, const void* ks, const void* vc
  * Causal attention over the 4-bit cache.  Sequence b holds lens[b] keys in the pages of its table row; its
  * query tokens are rows cu[b] .. cu[b + 1] - 1 of q (tokens, q_heads, head_dim) bf16 (cu NULL: row b alone; a
  * sequence whose starts decrease or leave the rows has none), the last of them its newest key's, so that token j
- * of R sees keys 0 .. lens - R + j.  out as q, not q.  fp32 scores,
+ * of R sees keys 0 .. lens - R + j.  out as q, apart from all that is read.  fp32 scores,
  * softmax and sums (values up to 2^80 are safe at any length); weights in 16 bits, 11 past 64 rows of a KV head.
  * A row that sees no key gives 0; rows that no sequence takes, and tokens of a sequence from max_q on, are left as
  * they were, or, with `clear` and more than one piece, set to 0 (then the starts do not decrease).  NaN: rows that

@@ -17,6 +17,7 @@ from __future__ import annotations
 import functools
 from operator import index
 
+import numpy as np
 import torch
 from torch.overrides import _get_current_function_mode_stack
 from torch.utils._device import DeviceContext
@@ -739,6 +740,43 @@ def _row_strides(T: int, H: int, Dh: int, stride: tuple, dtype: torch.dtype, nam
     return s0, s1
 
 
+def _rows(T: int, H: int, stride: tuple, n: int, Dh: int) -> tuple:
+    """Where rows of Dh values of n bytes lie from their first: (bytes to the last one's end, tokens, heads, bytes between
+    tokens and between heads, bytes of a row)"""
+    s0, s1 = stride
+    return (n * ((T - 1) * s0 + (H - 1) * s1 + Dh) if T * H else 0), T, H, n * s0, n * s1, n * Dh
+
+
+@_sizes
+def _meet(d: int, a: tuple, b: tuple) -> bool:
+    """Whether rows a (_rows), which do not overlap one another, share a byte with rows b that begin d bytes behind them.
+    Equal strides, as of views of one product: whether d is a sum of strides and less than a row, exactly, whatever the
+    sizes; others by the rows' sorted places."""
+    _, Ta, Ha, a0, a1, wa = a
+    _, Tb, Hb, b0, b1, wb = b
+    if not ((a0 == b0 or Ta == 1 or Tb == 1) and (a1 == b1 or Ha == 1 or Hb == 1)):
+        x, y = (np.add.outer(s0 * np.arange(T), s1 * np.arange(H)).ravel() for _, T, H, s0, s1, _ in (a, b))
+        x.sort()
+        y += d
+        at = np.searchsorted(x, y - wa, side="right")       # the first of a's rows that ends behind one of b's
+        return bool((x[np.minimum(at, x.size - 1)] < y + wb)[at < x.size].any())
+    # d = i S + j s + e: steps i, j from a row of b to one of a, -wb < e < wa
+    (S, lo, hi), (s, l, h) = sorted(((a0 if Ta > 1 else b0, 1 - Tb, Ta - 1), (a1 if Ha > 1 else b1, 1 - Hb, Ha - 1)), reverse=True)
+    for i in range(max(lo, -((h * s + wa - 1 - d) // S)), min(hi, (d - l * s + wb - 1) // S) + 1) if S else (0,):
+        x = d - i * S
+        if (max(l, -((wa - 1 - x) // s)) <= min(h, (x + wb - 1) // s)) if s else -wb < x < wa:
+            return True
+    return False
+
+
+def _apart(name: str, p: int, rows: tuple, *others) -> None:
+    """An output's rows at p, which share no byte with the others (address, _rows)."""
+    end = p + rows[0]
+    for x, r in others:
+        if x < end and p < x + r[0] and rows[0] and r[0] and _meet(x - p, rows, r):
+            raise ValueError(f"{name}: its rows share memory with what the call reads, or writes besides")
+
+
 def _int_vector(shape: tuple, stride: tuple, dtype: torch.dtype, n: int, name: str) -> None:
     _need(dtype is torch.int32 and shape == (n,) and (n <= 1 or stride[0] == 1),
           f"{name}: ({n},) int32, contiguous (got {tuple(shape)} {dtype})")
@@ -760,10 +798,13 @@ def _rope_sizes(qs, qst, dt, ks, kst, kt, ps, pst, pt, cs, cst, ct, ss, sst, st,
     _need(eps >= 0, "eps: not negative")
     for o, s, name in ((qo, qs, "q_out"), (ko, ks, "k_out")):
         _need(o is None or o[0] == s and o[2] is dt, f"{name}: as {name[0]}")
-    return (T, HQ, HKV, Dh, _row_strides(T, HQ, Dh, qst, dt, "q"), _row_strides(T, HKV, Dh, kst, dt, "k"),
-            (HQ * Dh, Dh) if qo is None else _row_strides(T, HQ, Dh, qo[1], dt, "q_out", True),
-            (HKV * Dh, Dh) if ko is None else _row_strides(T, HKV, Dh, ko[1], dt, "k_out", True),
-            (T, HQ, HKV, Dh, _DT[dt]), pt is torch.int64, (cst[0] if cs[0] > 1 else 0, cs[0]))
+    qst, kst = _row_strides(T, HQ, Dh, qst, dt, "q"), _row_strides(T, HKV, Dh, kst, dt, "k")
+    qo = (HQ * Dh, Dh) if qo is None else _row_strides(T, HQ, Dh, qo[1], dt, "q_out", True)
+    ko = (HKV * Dh, Dh) if ko is None else _row_strides(T, HKV, Dh, ko[1], dt, "k_out", True)
+    n, table = dt.itemsize, (cst[0] if cs[0] > 1 else 0, cs[0])
+    return (T, HQ, HKV, Dh, qst, kst, qo, ko, (T, HQ, HKV, Dh, _DT[dt]), pt is torch.int64, table,
+            (_rows(T, HQ, qst, n, Dh), _rows(T, HKV, kst, n, Dh), _rows(T, HQ, qo, n, Dh), _rows(T, HKV, ko, n, Dh),
+             _rows(1, 1, (0, 0), pt.itemsize, T), _rows(cs[0], 1, (table[0], 0), 4, Dh // 2), _rows(1, 1, (0, 0), n, Dh)))
 
 
 def qk_norm_rope(q, k, pos, cos, sin, wq=None, wk=None, eps: float = 1e-6, q_out=None, k_out=None):
@@ -772,12 +813,14 @@ def qk_norm_rope(q, k, pos, cos, sin, wq=None, wk=None, eps: float = 1e-6, q_out
     q (T, HQ, D), k (T, HKV, D) bf16, fp16 or fp32, D 64, 128 or 256, any token and head strides of whole
     16 bytes (views of one product, say); pos (T,) int32 or int64; cos, sin (P, D / 2) fp32; wq, wk (D,)
     of q's type, None for a rotation alone.  A token of negative position (padding) gives zeros, one of P
-    or more NaN.  Returns (q_out, k_out), contiguous unless given; either may be its input."""
+    or more NaN.  Returns (q_out, k_out), contiguous unless given; either may be its input, and shares no
+    memory with the other tensors."""
     i = _where(q, k, pos, cos, sin, wq, wk, q_out, k_out)
-    T, HQ, HKV, Dh, qst, kst, qo, ko, sizes, wide, table = _rope_sizes(
+    T, HQ, HKV, Dh, qst, kst, qo, ko, sizes, wide, table, lie = _rope_sizes(
         q.shape, q.stride(), q.dtype, k.shape, k.stride(), k.dtype, pos.shape, pos.stride(), pos.dtype, cos.shape, cos.stride(),
         cos.dtype, sin.shape, sin.stride(), sin.dtype, _m(wq), _m(wk), float(eps), _m(q_out), _m(k_out))
     _plain(q, k, cos, sin, wq, wk, q_out, k_out)
+    given = (q_out is not None) + 2 * (k_out is not None)
     if q_out is None:
         q_out = q.new_empty(T, HQ, Dh)
     if k_out is None:
@@ -786,6 +829,13 @@ def qk_norm_rope(q, k, pos, cos, sin, wq=None, wk=None, eps: float = 1e-6, q_out
     wqp, wkp = _ptr(wq), _ptr(wk)
     if T:
         _aligned((qp | qop if HQ else 0) | (kp | kop if HKV else 0) | cp | sp | (wqp or 0) | (wkp or 0))
+    if given:                              # each its own input, or apart from what is read and from each other
+        lq, lk, lqo, lko, lp, lt, lw = lie
+        rest = (pos.data_ptr(), lp), (cp, lt), (sp, lt), (wqp or 0, lw), (wkp or 0, lw)
+        if given & 1:
+            _apart("q_out", qop, lqo, (kp, lk), (kop, lko), *rest, *(() if qop == qp and qo == qst else ((qp, lq),)))
+        if given & 2:
+            _apart("k_out", kop, lko, (qp, lq), (qop, lqo), *rest, *(() if kop == kp and ko == kst else ((kp, lk),)))
     _run(i, "oa_qk_norm_rope", qp, *qst, kp, *kst, *sizes, pos.data_ptr(), wide, cp, sp, *table, wqp, wkp, eps, qop, *qo,
          kop, *ko)
     return q_out, k_out
@@ -933,8 +983,9 @@ def kv4_chunk(cap: int, units: int, rows: int) -> int:
 
 
 @_sizes
-def _attn_sizes(HKV, Dh, page, qs, qst, qt, ts, tst, tt, ls, lst, lt, cu, max_q, sm_scale, max_len, o, rule) -> tuple:
+def _attn_sizes(HKV, Dh, where, qs, qst, qt, ts, tst, tt, ls, lst, lt, cu, max_q, sm_scale, max_len, o, rule) -> tuple:
     # rule: kv4_chunk, a part of what is looked up, so that no call gets the pieces of another rule
+    c0, s0, NP, page = where
     tstride, B, width = _table_sizes(ts, tst, tt, page)
     _need(len(qs) == 3 and qs[2] == Dh and qt is torch.bfloat16 and qs[1] >= 1 and qs[1] % HKV == 0,
           f"q: (T, a multiple of {HKV}, {Dh}) bf16")
@@ -956,10 +1007,12 @@ def _attn_sizes(HKV, Dh, page, qs, qst, qt, ts, tst, tt, ls, lst, lt, cu, max_q,
     nchunk = -(-cap // chunk)
     _need(units * nchunk <= _GRID and B * HKV * HKV < 1 << 32,
           f"at most {_GRID} workgroups (sequences x heads x tiles of rows x pieces), sequences x heads^2 under 2^32")
-    return (T, HQ, B, _row_strides(T, HQ, Dh, qst, qt, "q"),
-            (HQ * Dh, Dh) if o is None else _row_strides(T, HQ, Dh, o[1], qt, "out", True), (tstride, width),
-            (B, T, max_q, HQ, HKV, Dh, scale, chunk, nchunk), T * HQ * nchunk if nchunk > 1 else 0,
-            units * nchunk if rows > 64 else 0)
+    qst, ost = _row_strides(T, HQ, Dh, qst, qt, "q"), (HQ * Dh, Dh) if o is None else _row_strides(T, HQ, Dh, o[1], qt, "out", True)
+    return (T, HQ, B, qst, ost, (tstride, width), (B, T, max_q, HQ, HKV, Dh, scale, chunk, nchunk),
+            T * HQ * nchunk if nchunk > 1 else 0, units * nchunk if rows > 64 else 0,
+            (_rows(T, HQ, qst, 2, Dh), _rows(T, HQ, ost, 2, Dh), _rows(B, 1, (tstride, 0), 4, width), _rows(1, 1, (0, 0), 4, B),
+             _rows(1, 1, (0, 0), 4, B + 1), _rows(NP, 1, (c0, 0), 1, HKV * page * Dh // 2),
+             _rows(NP, 1, (s0, 0), 1, HKV * page * Dh // KV4_BLOCK)))
 
 
 def kv4_attn(q, kc, ks, vc, vs, table, lens, sm_scale: float | None = None, cu_q=None, max_q: int = 1, out=None,
@@ -973,18 +1026,19 @@ def kv4_attn(q, kc, ks, vc, vs, table, lens, sm_scale: float | None = None, cu_q
     that the caller knows (the table's width otherwise).  NaN: rows that need a page id outside of the
     cache, and those of sequences longer than their table row or than max_len (rounded up to whole pieces,
     kv4_chunk).  Rows of `out` that no sequence takes, and tokens past max_q, are left
-    as they were (0 where the call makes it); `out` shares no memory with q.  Sums are held in fp32 and not divided
-    before their end: values up to 2^80 are safe at any length.  Sequences are cut into pieces by kv4_chunk, more than
-    65535 of them not at all; at most 2^24 - 1 workgroups (a sequence's, by head, for 8, 16, 32 or, past 64
-    rows of a KV head, 128 rows each)."""
+    as they were (0 where the call makes it); `out` shares no memory with the other tensors.  Sums are held in
+    fp32 and not divided before their end: values up to 2^80 are safe at any length.  Sequences are cut into
+    pieces by kv4_chunk, more than 65535 of them not at all; at most 2^24 - 1 workgroups (a sequence's, by head,
+    for 8, 16, 32 or, past 64 rows of a KV head, 128 rows each)."""
     i = _where(q, kc, ks, vc, vs, table, lens, cu_q, out)
     ps, where, HKV, Dh = _kv4_cache(kc, ks, vc, vs)
-    T, HQ, B, qst, ost, tsz, sizes, parts, flags = _attn_sizes(
-        HKV, Dh, where[3], q.shape, q.stride(), q.dtype, table.shape, table.stride(), table.dtype, lens.shape, lens.stride(),
+    T, HQ, B, qst, ost, tsz, sizes, parts, flags, lie = _attn_sizes(
+        HKV, Dh, where, q.shape, q.stride(), q.dtype, table.shape, table.stride(), table.dtype, lens.shape, lens.stride(),
         lens.dtype, _m(cu_q), index(max_q), None if sm_scale is None else float(sm_scale),
         None if max_len is None else index(max_len), _m(out), kv4_chunk)
     _plain(q, out)
     qp = q.data_ptr()
+    given = out is not None
     clear = out is None and cu_q is not None and parts > 0 and B > 0     # (by the join)
     if out is None:
         out = q.new_empty(T, HQ, Dh) if clear or cu_q is None else q.new_zeros(T, HQ, Dh)
@@ -992,8 +1046,10 @@ def kv4_attn(q, kc, ks, vc, vs, table, lens, sm_scale: float | None = None, cu_q
     if T == 0 or B == 0:
         return out
     _aligned(qp | op)
-    if op == qp:
-        raise ValueError("out: not q itself")
+    if given:
+        lq, lo, lt, ll, lc, lw, ls = lie
+        _apart("out", op, lo, (qp, lq), (table.data_ptr(), lt), (lens.data_ptr(), ll), (_ptr(cu_q) or 0, lc), (ps[0], lw), (ps[1], ls),
+               (ps[2], lw), (ps[3], ls))
     wp = mp = fp = None
     if parts or flags:
         ws = q.new_empty(parts * (Dh + 2) + flags, dtype=torch.float32)
