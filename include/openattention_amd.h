@@ -29,11 +29,16 @@ extern "C" {
 #endif
 
 #define OA_ABI_VERSION 9
+#define OA_ABI_REVISION 1
 #define OA_EINVAL (-22)
 #define OA_ENOSPC (-28)
 
-/* ABI version of the loaded library (OA_ABI_VERSION of the header it was built from). */
+/*
+ * ABI version of the loaded library (OA_ABI_VERSION of the header it was built from), and the revision of the
+ * entry points within it: either is raised with any change of arguments.
+ */
 int oa_abi_version(void);
+int oa_abi_revision(void);
 
 /* Text for a status returned by any entry point. */
 const char* oa_error_string(int status);

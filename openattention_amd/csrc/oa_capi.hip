@@ -2,6 +2,7 @@
 #include "oa_common.h"
 
 extern "C" int oa_abi_version(void) { return OA_ABI_VERSION; }
+extern "C" int oa_abi_revision(void) { return OA_ABI_REVISION; }
 
 extern "C" const char* oa_error_string(int status) {
   if (status == 0) return "success";

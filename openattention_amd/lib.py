@@ -36,6 +36,7 @@ class StepArgs(ct.Structure):
 # name -> argtypes, in the order of include/openattention_amd.h
 SIGNATURES = {
     "oa_abi_version": [],
+    "oa_abi_revision": [],
     "oa_error_string": [I],
     "oa_flash_decode": [P, L, P, P, L, L, P, L, I, P, L, I, P, P, L, L, I, I, P, L, I, P, L,
                         I, I, I, I, F, I, P, P, P, P],
@@ -88,16 +89,17 @@ SIGNATURES = {
     "oa_kv4_attn": [P, L, L, P, P, P, P, L, L, I, I, P, L, I, P, P, I, I, I, I, I, I, F, I, I, P, P, P, P, L, L, I, P],
 }
 
-# must equal oa_abi_version() of the loaded library (OA_ABI_VERSION in the header): a library
-# built from sources with other argument lists would be handed wrong pointers
+# must equal oa_abi_version() and oa_abi_revision() of the loaded library (OA_ABI_VERSION, OA_ABI_REVISION in the
+# header): a library built from sources with other argument lists would be handed wrong pointers
 ABI_VERSION = 9
+ABI_REVISION = 1
 
 _LIB = None
 
 
 def load() -> ct.CDLL:
     """Load the kernel library; raises if it has not been built (run __graft_entry__.build()) or
-    was built for another ABI version."""
+    was built for another ABI version or revision."""
     global _LIB
     if _LIB is not None:
         return _LIB
@@ -114,6 +116,11 @@ def load() -> ct.CDLL:
     if missing:
         raise RuntimeError(f"kernel library {path} lacks {', '.join(missing)}: it was built from older sources, "
                            "rebuild it (__graft_entry__.build())")
+    lib.oa_abi_revision.restype = ct.c_int
+    have = lib.oa_abi_revision()
+    if have != ABI_REVISION:
+        raise RuntimeError(f"kernel library {path} has ABI {ABI_VERSION} revision {have}, this binding expects revision "
+                           f"{ABI_REVISION}: rebuild it (__graft_entry__.build())")
     for name, argtypes in SIGNATURES.items():
         fn = getattr(lib, name)
         fn.argtypes = argtypes
