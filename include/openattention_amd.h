@@ -611,13 +611,13 @@ int oa_kv4_read(const int* slots, const void* kc, const void* ks, const void* vc
  * Causal attention over the 4-bit cache.  Sequence b holds lens[b] keys in the pages of its table row; its
  * query tokens are rows cu[b] .. cu[b + 1] - 1 of q (tokens, q_heads, head_dim) bf16 (cu NULL: row b alone; a
  * sequence whose starts decrease or leave the rows has none), the last of them its newest key's, so that token j
- * of R sees keys 0 .. lens - R + j.  out as q, apart from all that is read.  fp32 scores,
- * softmax and sums (values up to 2^80 are safe at any length); weights in 16 bits, 11 past 64 rows of a KV head.
+ * of R sees keys 0 .. lens - R + j.  out as q, apart from all that is read.  fp32 scores, softmax and sums (values
+ * up to 2^80 are safe at any length); weights in 16 bits, 11 past 64 rows of a KV head.
  * A row that sees no key gives 0; rows that no sequence takes, and tokens of a sequence from max_q on, are left as
  * they were, or, with `clear` and more than one piece, set to 0 (then the starts do not decrease).  NaN: rows that
- * need a page id outside of the cache, and those of sequences longer than their table row or than nchunk * chunk keys.  Keys are split into nchunk pieces
- * of `chunk` (a multiple of 128); with more than one, ws_o (tokens * q_heads * nchunk * head_dim) and ws_ml (* 2)
- * floats hold the pieces' sums; with more than 64 rows of a KV head (max_q * q_heads / kv_heads), ws_flag holds
+ * need a page id outside of the cache, and those of sequences longer than their table row or than nchunk * chunk
+ * keys.  Keys are split into nchunk pieces of `chunk` (a multiple of 128); with more than one, ws_o (tokens *
+ * q_heads * nchunk * head_dim) and ws_ml (* 2) floats hold the pieces' sums; with more than 64 rows of a KV head (max_q * q_heads / kv_heads), ws_flag holds
  * sequences * kv_heads * nchunk * ceil(rows / 128) ints.  Grids hold 2^24 - 1 workgroups (sequences * kv_heads *
  * nchunk * tiles of 8, 16, 32 or, past 64 rows, 128 rows), 65535 pieces and, with more than one, 65535 sequences
  * and 2^24 - 1 query rows of one (max_q * q_heads).

@@ -14,9 +14,9 @@
 // the second term sits in the tile's other 8 columns, otherwise it takes a second product.
 //
 // Bound by the codes read where rows are few: 32 sequences of 32768 keys, 8 KV heads, 1141 MB, 183 us with the
-// join, 6.2 TB/s; one of 131072 keys 30 us (142 MB: 26 us and 4 for the join), where 512 workgroups each begin with
-// three dependent accesses.  A workgroup's tile costs 64 conversions, 16 products and about 60 other vector
-// instructions a wave.  Up to 64 rows of a KV head every workgroup turns its own keys to bf16 for 32 of them (64
+// join, 6.2 TB/s (in a train of launches of more than 2 ms the card slows: 190 to 245); one of 131072 keys 30 us
+// (142 MB: 26 us and 4 for the join), where 512 workgroups each begin with three dependent accesses.  A workgroup's
+// tile costs 64 conversions, 16 products and about 60 other vector instructions a wave.  Up to 64 rows of a KV head every workgroup turns its own keys to bf16 for 32 of them (64
 // rows over 32768 keys, twice: 48 us against 59 in oa_kv4_rows.hip; from 96 rows on that one is faster).
 #include "oa_kv4_attn.h"
 

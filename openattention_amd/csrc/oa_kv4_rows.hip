@@ -18,10 +18,10 @@
 // the transpose reads spread over the banks and every address is one register and a constant (exchanged
 // places instead, as in the prompt's kernel, take 16 more registers and spill).
 //
-// Bound by instruction issue between the products: 64 tokens of 32 query heads over 32768 keys of 8 heads, for two
-// sequences (69 GFLOP), 94 us for this kernel, 730 TFLOP/s (a large bf16 product reaches 1256), 95 for the call
-// with the empty second launch and the join (4.5 and 8.5 under a profiler).  Its matrix cores are busy 30% of the
-// time, its vector units about 45%; two waves a SIMD at 254 registers.
+// 64 tokens of 32 query heads over 32768 keys of 8 heads, for two sequences (69 GFLOP): 94 us for the call with the
+// empty second launch and the join (4.8 and 8.5 under a profiler), 730 TFLOP/s (a large bf16 product reaches 1256).
+// The matrix cores are busy 30% of the time, the vector units about 45%, so that neither bounds it; two waves a SIMD
+// at 254 registers, which meet every 32 keys.
 #include "oa_kv4_attn.h"
 
 namespace {
