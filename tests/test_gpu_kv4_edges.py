@@ -1,5 +1,5 @@
 """The 4-bit paged cache on the GPU where its first tests do not reach: values that are not finite among keys that every
-row sees, truncations that are refused, very many sequences."""
+row sees, truncations that are refused, very many sequences, outputs among their inputs."""
 import math
 
 import pytest
@@ -88,3 +88,28 @@ def test_attention_of_more_sequences_than_a_grids_axis_holds():
     check_attn(out[at], *want_attn(q[at], cache, table[at], lens[at].tolist(), list(range(len(some) + 1)), D ** -0.5, page))
     # and the others as they are in a batch of their own
     assert torch.equal(out[1000:9000], ops.kv4_attn(q[1000:9000], *cache, table[1000:9000], lens[1000:9000], max_len=96))
+
+
+@pytest.mark.parametrize("T", [1, 33, 3001])
+def test_outputs_beside_their_inputs_in_one_product(T):
+    """Rows of a product turned in place, and attention written between the rows of its queries, give what outputs of
+    their own get; the product's other columns stay as they were."""
+    g = gen(T)
+    HQ, HKV, D, page = 8, 2, 128, 32
+    x = randn(g, T, (2 * HQ + 2 * HKV) * D, dtype=torch.bfloat16)
+    q, free, k, v = (t.unflatten(1, (-1, D)) for t in x.split([HQ * D, HQ * D, HKV * D, HKV * D], 1))
+    a = torch.arange(T, dtype=torch.float64)[:, None] * 0.7 ** torch.arange(D // 2, dtype=torch.float64)
+    cos, sin, pos = a.cos().float().to(DEV), a.sin().float().to(DEV), torch.arange(T, device=DEV)
+    w = randn(g, D, dtype=torch.bfloat16)
+    keep = x.clone()
+    want = ops.qk_norm_rope(q, k, pos, cos, sin, w, w)
+    ops.qk_norm_rope(q, k, pos, cos, sin, w, w, q_out=q, k_out=k)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+    q.copy_(want[0])
+    lens = [T + 70]
+    cache, table = paged(lens, HKV, D, page, g)
+    want = ops.kv4_attn(q, *cache, table, i32(lens), cu_q=i32([0, T]), max_q=T)
+    was = q.clone()
+    ops.kv4_attn(q, *cache, table, i32(lens), cu_q=i32([0, T]), max_q=T, out=free)
+    assert torch.equal(free, want) and not want.isnan().any() and torch.equal(q, was)
+    assert torch.equal(v, keep.view(T, -1, D)[:, 2 * HQ + HKV:])
