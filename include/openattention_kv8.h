@@ -1,0 +1,81 @@
+/*
+ * C ABI of the 8-bit paged KV cache: rows rounded into it and read back, blocks chosen by bounds, attention over all
+ * blocks or over chosen ones (gfx950).  The conventions are those of openattention_amd.h: device pointers, sizes and
+ * strides in elements unless said otherwise, a hipStream_t; 0 or a hipError_t comes back, -22 for arguments that are
+ * refused before any launch.  Nothing allocates, synchronises or reads back.  Page tables and lengths are those of
+ * oa_kv_pages_extend.
+ */
+#ifndef OPENATTENTION_KV8_H
+#define OPENATTENTION_KV8_H
+
+/* goes up where an entry point's arguments change */
+#define OA_KV8_REVISION 1
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+int oa_kv8_revision(void);
+
+/*
+ * The cache: codes kc, vc (pages, kv_heads, page, head_dim), pages code_stride (a multiple of 16) bytes apart; scales
+ * ks, vs (pages, kv_heads), scale_stride bytes apart; bounds kb (pages, kv_heads, 2, head_dim), bound_stride (a multiple
+ * of 16) bytes apart; page: 32, 64 or 128 tokens, head_dim: 64 or 128.  A page holds one block of each head: codes in
+ * e4m3 (largest 448) and a byte s that scales them by 2^e, e = s - 127, the smallest with max |x| <= 448 * 2^e,
+ * -117 <= e <= 120; rounding to nearest, ties to even.  e starts with the write of a block's first token and from then on
+ * only grows; where it does, the codes of the block's earlier tokens are rounded again.  A row (token and head) with a
+ * value that is not finite is held as NaN (0x7f) and counts neither for e nor for the bounds.
+ * Bounds of a channel of a block's keys, in steps of 4 * 2^e: hi, the least whole number with code <= 4 hi, and nlo, that
+ * with -code <= 4 nlo, over the codes written (-112 for none); where e grows by d they become ceil(. / 2^d).
+ *
+ * write: rows of tokens (strides per token and head; dtype 0 / 1 / 2: bf16 / fp16 / fp32).  Sequence b holds lens[b]
+ * tokens in the pages of its row of table (sequences, width), int32 rows of table_stride; rows cu[b] .. cu[b + 1] - 1
+ * (cu NULL: row b alone) are its last ones.  cu does not decrease.  kb NULL: no bounds.  Passed over: sequences whose
+ * starts leave the rows or whose length is negative or more than their table row holds, tokens of negative position,
+ * pages outside of the cache.  A page that two sequences of a call write into ends as some mixture.
+ * read: the values at slots (page id * page + offset; dtype 0 or 2: bf16, exact, or fp32); a slot outside of the cache
+ * gives zeros.
+ */
+int oa_kv8_write(const void* k, long k_st, long k_sh, const void* v, long v_st, long v_sh, int tokens, int kv_heads,
+                 int head_dim, int dtype, void* kc, void* ks, void* vc, void* vs, void* kb, long code_stride,
+                 long scale_stride, long bound_stride, int pages, int page, const int* table, long table_stride, int width,
+                 const int* lens, const int* cu, int sequences, void* stream);
+int oa_kv8_read(const int* slots, const void* kc, const void* ks, const void* vc, const void* vs, long code_stride,
+                long scale_stride, int pages, int page, void* k, long k_st, long k_sh, void* v, long v_st, long v_sh,
+                int tokens, int kv_heads, int head_dim, int dtype, void* stream);
+
+/*
+ * The n blocks (tokens, kv_heads, n), ascending, -1 behind the last, whose keys can score highest for each query token
+ * and KV head.  q (tokens, q_heads, head_dim), dtype 0 / 1: bf16 / fp16; rows cu[b] .. cu[b + 1] - 1 of q (cu NULL: row b
+ * alone) are sequence b's last tokens; block i of a sequence lies in the page that entry i of its table row names.  A
+ * token at position p sees the blocks 0 .. p / page: all of them where they are at most n, otherwise the `first` first,
+ * the `last` last (at least 1; first + last <= n) and those of the highest scores, ties to the lower.  A score is
+ * max over the query heads of sum_d max(q8, 0) hi + max(-q8, 0) nlo, times 2^min(e, 100), q8 = rint(q / 2^u), u >= -120
+ * the smallest with |q8| <= 127 for the heads together; values of q that are not finite count as 0, a block whose page
+ * id lies outside of the cache comes last.  cap: blocks (at most width) that sequences hold at most; -1 alone: rows that
+ * no sequence takes, sequences of more than cap blocks.  ws: tokens * kv_heads * cap ints of scratch (NULL will do where
+ * cap <= n).
+ */
+int oa_kv8_select(const void* q, long q_st, long q_sh, int dtype, const void* ks, const void* kb, long scale_stride,
+                  long bound_stride, int pages, int page, const int* table, long table_stride, int width, const int* lens,
+                  const int* cu, int sequences, int tokens, int q_heads, int kv_heads, int head_dim, int n, int first,
+                  int last, int cap, unsigned* ws, int* blocks, void* stream);
+
+/*
+ * Causal attention over the 8-bit cache, arguments as oa_kv4_attn's besides these.  q and out: dtype 0 / 1, bf16 / fp16.
+ * blocks (tokens, kv_heads, n): a token's rows of a KV head see the keys of these blocks alone, up to the token's own
+ * position; numbers outside of 0 .. width - 1 name nothing, one given twice counts twice (NULL: all keys).  Keys (with
+ * blocks: the n * page listed ones) are split into nchunk pieces of `chunk`, a multiple of 128, which with blocks cover
+ * them; with more than one, ws_o (tokens * q_heads * nchunk * head_dim) and ws_ml (* 2) floats hold the pieces' sums.
+ */
+int oa_kv8_attn(const void* q, long q_st, long q_sh, int dtype, const void* kc, const void* ks, const void* vc,
+                const void* vs, long code_stride, long scale_stride, int pages, int page, const int* table, long table_stride,
+                int width, const int* lens, const int* cu, int sequences, int tokens, int max_q, int q_heads, int kv_heads,
+                int head_dim, float sm_scale, const int* blocks, int n, int chunk, int nchunk, float* ws_o, float* ws_ml,
+                void* out, long o_st, long o_sh, int clear, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* OPENATTENTION_KV8_H */

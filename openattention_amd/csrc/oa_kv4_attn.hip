@@ -24,22 +24,6 @@ namespace {
 
 using namespace kv4;
 
-__device__ __forceinline__ float max_groups(float v) {     // over the four 16-lane groups
-  const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
-  const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
-}
-__device__ __forceinline__ float sum_groups(float v) {
-  const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = __uint_as_float(x[0]) + __uint_as_float(x[1]);
-  const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(y[0]) + __uint_as_float(y[1]);
-}
-
-// what the lanes of a wave exchange through its LDS tile stays in program order (the LDS keeps it)
-__device__ __forceinline__ void lane_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local"); }
-
 // one tile's codes and scales of this lane: keys lane % 16 and 16 + lane % 16, a quarter of the dims
 template <int D>
 struct Tile {
@@ -333,96 +317,13 @@ __global__ void __launch_bounds__(kThreads, NQ > 1 ? 2 : 3) kv4_attn_kernel(Attn
   }
 }
 
-// Zeros in the rows of out that no sequence takes: those before the first and behind the last by all workgroups
-// of the join together, and head hd of sequence b's rows past max_q (all of its rows, where they do not fit) by
-// the one of its first row.  In the join, as it costs a launch to fill out beforehand (5 drafts of 7 sequences
-// 19.5 us a call, 15.5 here) and the attention kernel 4 to 13 us (one sequence of 131072 keys 30.6 to 35.6, 32 of
-// 32768 184 to 197), even where there is nothing to clear.
-template <int D>
-__device__ __forceinline__ void clear_rows(const AttnArgs& a, int b, int hd, bool own) {
-  constexpr int kLanes = D / 4, kRows = kThreads / kLanes;     // lanes of a row, 8 bytes each
-  const int y = threadIdx.x % kLanes, x = threadIdx.x / kLanes, heads = a.HKV * a.G;
-  auto zero = [&](int tok, int head) {
-    *reinterpret_cast<uint2v*>(a.out + (long)tok * a.o_st + (long)head * a.o_sh + 4 * y) = uint2v(0u);
-  };
-  auto in_out = [&](int t) { return min(max(t, 0), a.tokens); };
-  const int lead = in_out(a.cu[0]), tail = in_out(a.cu[a.B]);
-  const long n = (long)(lead + a.tokens - tail) * heads, blocks = (long)gridDim.x * gridDim.y;
-  for (long i = ((long)blockIdx.y * gridDim.x + blockIdx.x) * kRows + x; i < n; i += blocks * kRows) {
-    const int t = (int)(i / heads);
-    zero(t < lead ? t : tail + t - lead, (int)(i % heads));
-  }
-  if (!own) return;
-  const int r0 = a.cu[b], r1 = a.cu[b + 1];
-  const bool fits = r0 >= 0 && r1 >= r0 && r1 <= a.tokens;
-  const int t0 = fits ? r0 + min(r1 - r0, a.max_q) : in_out(r0), t1 = fits ? r1 : in_out(r1);
-  for (int t = t0 + x; t < t1; t += kRows) zero(t, hd);
-}
-
-// joins a row's chunks: weights exp2(m_i - max m), by groups of D / 4 lanes
 template <int D>
 __global__ void __launch_bounds__(kThreads) kv4_join_kernel(AttnArgs a) {
-  constexpr int kLanes = D / 4, kGroups = kThreads / kLanes;
-  __shared__ float s_r[kWaves];
-  __shared__ __align__(16) float s_o[kGroups][D];
-  __shared__ float s_l[kGroups];
-  const int heads = a.HKV * a.G;
-  const int hd = blockIdx.x % heads, j = blockIdx.x / heads, b = blockIdx.y;
-  const Seq sq = seq_of(a, b);
-  if (a.clear) clear_rows<D>(a, b, hd, j == 0);
-  if (j >= sq.R) return;
-  const int seen = sq.n - sq.R + j + 1, tid = threadIdx.x;
-  const int nv = sq.bad || seen <= 0 ? 0 : (seen + a.chunk - 1) / a.chunk;
-  const long row = ((long)(sq.r0 + j) * heads + hd) * a.nchunk;
-  const float* ml = a.ws_ml + row * 2;
-  const int grp = tid / kLanes, y = tid % kLanes;
-  constexpr int kAtOnce = 4;             // pieces whose loads are in flight together
-  f32x4 x[kAtOnce];
-  f32x2 w[kAtOnce];
-  auto fetch = [&](int i) {
-#pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) {
-      const int at = min(i + k * kGroups, nv - 1);
-      x[k] = *reinterpret_cast<const f32x4*>(a.ws_o + (row + at) * D + 4 * y);
-      w[k] = *reinterpret_cast<const f32x2*>(ml + 2 * at);
-    }
-  };
-  if (grp < nv) fetch(grp);              // (beside the maxima: one sequence of 131072 keys 30.9 us, 32.2 after them)
-  float M = -FLT_MAX;
-  for (int i = tid; i < nv; i += kThreads) M = fmaxf(M, ml[2 * i]);
-  M = oa::wave_max(M);
-  if ((tid & 63) == 0) s_r[tid >> 6] = M;
-  __syncthreads();
-  M = fmaxf(fmaxf(s_r[0], s_r[1]), fmaxf(s_r[2], s_r[3]));
-  f32x4 o = f32x4(0.f);
-  float L = 0.f;
-  for (int i = grp; i < nv; i += kAtOnce * kGroups) {
-    if (i > grp) fetch(i);
-#pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) {
-      if (i + k * kGroups >= nv) break;
-      const float e = __builtin_amdgcn_exp2f(w[k][0] - M);
-      L += e * w[k][1];
-      o += x[k] * e;
-    }
-  }
-  *reinterpret_cast<f32x4*>(&s_o[grp][4 * y]) = o;
-  if (y == 0) s_l[grp] = L;
-  __syncthreads();
-  if (grp) return;
-#pragma unroll
-  for (int k = 1; k < kGroups; ++k) {
-    o += *reinterpret_cast<const f32x4*>(&s_o[k][4 * y]);
-    L += s_l[k];
-  }
-  o = sq.bad ? f32x4(__builtin_nanf("")) : nv ? o / L : f32x4(0.f);
-  *reinterpret_cast<uint2v*>(a.out + (long)(sq.r0 + j) * a.o_st + (long)hd * a.o_sh + 4 * y) =
-      uint2v{pack2(o[0], o[1]), pack2(o[2], o[3])};
+  join_pieces<D, __bf16, false>(a);
 }
 
 // query rows up to which every workgroup turns its own keys to bf16 (more: oa_kv4_rows.hip)
 constexpr int kFewRows = 64;
-constexpr long kGrid = 0xffffffffL / kThreads;
 
 template <int D>
 int launch(AttnArgs a, hipStream_t st) {

@@ -39,14 +39,9 @@ __device__ __forceinline__ float16v mfma(bf16x8 a, bf16x8 b, float16v c) {
 }
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ float16v mfma16(bf16x8 a, uint4v b, float16v c) {     // both hold fp16
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ uint32_t pack2h(float a, float b) {
-  const f32x2 x = {a, b};
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, f16x2));
 }
 // 8 codes to fp16, scaled by a power of two (all exponent bits set: NaN)
 __device__ __forceinline__ bf16x8 from4h(unsigned w, float f) {

@@ -1,0 +1,346 @@
+// The 8-bit paged KV cache: rows rounded into it (oa_kv8_write) and read back from it (oa_kv8_read).
+//
+// A page holds a block of tokens of every head: codes in e4m3 (sign, four bits of exponent, three of mantissa, the
+// largest 448) and one byte s for a block of a head, which scales them by 2^e, e = s - 127, the smallest with
+// max |x| <= 448 2^e, -117 <= e <= 120: no value is clipped, what a code stands for is a normal fp32 and bf16
+// number, and a scale that is a power of two makes both directions exact but for the one rounding (to nearest, ties
+// to even).  A block's scale starts with the write of its first token and from then on only grows: where later
+// tokens need a larger one, the codes of earlier tokens are rounded again.  A row (token and head) with a value that
+// is not finite is held as NaN and counts neither for the scale nor for the bounds.
+// Bounds of K: for every channel of a block hi = ceil(max / 4) and nlo = ceil(max of the negatives / 4) of its codes,
+// one byte each (-112 .. 112), so that 4 2^e hi and -4 2^e nlo enclose what the block holds.  Where the scale grows by
+// 2^d they shrink to ceil(. / 2^d), which encloses the codes as they are rounded again.
+// Layout: codes (pages, heads, page, D), scales (pages, heads), bounds (pages, heads, 2, D), bytes.
+//
+// One workgroup takes the new tokens of one block of a head: a lane 8 values of a row of K and of V, four rows (D = 128)
+// to a wave, the whole block in registers between its largest value and the rounding, so that rows are read once.
+// Workgroups find their block from the starts: sequence b owns the numbers from cu[b] / page + 2 b on, which are at
+// least as many as the blocks that its tokens can lie in.
+#include "oa_kv8.h"
+
+namespace {
+
+using namespace kv8;
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x8m __attribute__((ext_vector_type(8), aligned(16)));    // in memory
+typedef unsigned uint2v __attribute__((ext_vector_type(2)));
+
+template <typename T> struct Vec8;
+template <> struct Vec8<__bf16> { typedef bf16x8 type; };
+template <> struct Vec8<_Float16> { typedef f16x8 type; };
+template <> struct Vec8<float> { typedef f32x8m type; };
+
+constexpr int kThreads = 256, kWaves = 4;
+constexpr int kLow = -117, kHigh = 120;  // least and largest e
+constexpr unsigned kInf = 0x7f800000u;
+
+struct Kv8Args {
+  const void* k; long k_st, k_sh;        // rows in (write) or out (read)
+  const void* v; long v_st, v_sh;
+  uint8_t* kc; uint8_t* ks; uint8_t* vc; uint8_t* vs; int8_t* kb;
+  long c_sp, s_sp, b_sp;                 // bytes between pages of codes, scales, bounds
+  const int* table; long t_st; int width;
+  const int* lens; const int* cu;
+  const int* slots;
+  int tokens, kv_heads, B, NP, lp;
+};
+
+// the largest |x| of 8 values, as bits: NaN above infinity above all else
+__device__ __forceinline__ unsigned top8(const f32x8& f) {
+  unsigned t = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t = max(t, __float_as_uint(f[i]) & 0x7fffffffu);
+  return t;
+}
+template <int CTRL>
+__device__ __forceinline__ unsigned dpp_max(unsigned v) {
+  return max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false));
+}
+template <int D>
+__device__ __forceinline__ unsigned max_row(unsigned v) {  // over the D / 8 lanes of a row
+  v = dpp_max<0xB1>(v);
+  v = dpp_max<0x4E>(v);
+  v = dpp_max<0x141>(v);
+  return D == 128 ? dpp_max<0x140>(v) : v;
+}
+__device__ __forceinline__ unsigned max_wave(unsigned v) {  // of values that the lanes of a row share
+  v = dpp_max<0x140>(v);
+  const auto x = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max(x[0], x[1]);
+  const auto y = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return max(y[0], y[1]);
+}
+// over the rows of a wave, lane by lane
+template <int D>
+__device__ __forceinline__ float max_rows(float v) {
+  if (D == 64)
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), 0x128, 0xf, 0xf, false)));  // row_ror 8
+  const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+  const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+}
+
+// the exponent that a block of largest |x| (bits, finite) needs: floor(log2) - 8, one more past 1.75
+__device__ __forceinline__ int exponent(unsigned top) { return min(max((int)((top + 0x1fffffu) >> 23) - 135, kLow), kHigh); }
+
+__device__ __forceinline__ uint2v to_codes(const f32x8& f) {
+  int a = 0, b = 0;
+  a = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], a, false);
+  a = __builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], a, true);
+  b = __builtin_amdgcn_cvt_pk_fp8_f32(f[4], f[5], b, false);
+  b = __builtin_amdgcn_cvt_pk_fp8_f32(f[6], f[7], b, true);
+  return uint2v{(unsigned)a, (unsigned)b};
+}
+__device__ __forceinline__ f32x8 from_codes(uint2v c) {
+  const f32x2 p = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[0], false), q = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[0], true);
+  const f32x2 r = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[1], false), s = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[1], true);
+  return f32x8{p[0], p[1], q[0], q[1], r[0], r[1], s[0], s[1]};
+}
+
+// the bytes of w that hold NaN, all bits set
+__device__ __forceinline__ unsigned nan_bytes(unsigned w) {
+  const unsigned hit = (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+  return hit * 0xffu;
+}
+
+// codes of 8 values again, 2^-d times what they were; NaN stays
+__device__ __forceinline__ uint2v again(uint2v c, float f) {
+  f32x8 x = from_codes(c);
+  const unsigned n0 = nan_bytes(c[0]), n1 = nan_bytes(c[1]);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] *= f;
+  const uint2v y = to_codes(x);
+  return uint2v{(y[0] & ~n0) | (c[0] & n0), (y[1] & ~n1) | (c[1] & n1)};
+}
+
+// N: passes of the workgroup over a block, page * D / 2048
+template <typename T, int D, int N>
+__global__ void __launch_bounds__(kThreads) kv8_write_kernel(Kv8Args a) {
+  typedef typename Vec8<T>::type vec;
+  constexpr int kLanes = D / 8, kRows = kThreads / kLanes;
+  __shared__ unsigned s_top[2][kWaves];
+  __shared__ float s_b[kWaves][2 * D];
+  const int tid = threadIdx.x, wave = tid >> 6, l = tid % kLanes, r = tid / kLanes;
+  const int head = blockIdx.x % a.kv_heads, id = blockIdx.x / a.kv_heads;
+  const int b = a.cu ? sequence_of(a.B, id, [&](int i) { return (a.cu[i] >> a.lp) + 2 * i; }) : id;
+  const int r0 = a.cu ? a.cu[b] : b, r1 = a.cu ? a.cu[b + 1] : b + 1, n = a.lens[b];
+  if (r0 < 0 || r1 <= r0 || r1 > a.tokens || n < 0 || n > a.width << a.lp) return;
+  const int first = n - (r1 - r0), from = max(first, 0), k = a.cu ? id - ((r0 >> a.lp) + 2 * b) : 0;
+  const int page = 1 << a.lp, blk = (from >> a.lp) + k, base = blk << a.lp;
+  if (k < 0 || base >= n) return;
+  const unsigned pid = (unsigned)a.table[(long)b * a.t_st + blk];
+  if (pid >= (unsigned)a.NP) return;
+  const int begin = max(from - base, 0), end = min(n - base, page);      // the new tokens' places in the block
+  const long at = (long)pid * a.c_sp + ((long)head << a.lp) * D + 8 * l;
+  uint8_t* const ks = a.ks + (long)pid * a.s_sp + head;
+  uint8_t* const vs = a.vs + (long)pid * a.s_sp + head;
+  const int was_k = (int)*ks - 127, was_v = (int)*vs - 127;
+  int8_t* const kb = a.kb ? a.kb + (long)pid * a.b_sp + (long)head * (2 * D) : nullptr;
+  const int old = kb && tid < 2 * D ? kb[tid] : 0;
+
+  vec xk[N], xv[N];
+  unsigned top_k = 0, top_v = 0, bad_k = 0, bad_v = 0;     // bad: bit i of a row that is not finite
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int o = i * kRows + r;
+    if (o < begin || o >= end) {
+      xk[i] = xv[i] = vec(T(0.f));
+      continue;
+    }
+    const long tok = r0 + (base + o - first);
+    xk[i] = __builtin_nontemporal_load(reinterpret_cast<const vec*>((const T*)a.k + tok * a.k_st + (long)head * a.k_sh + 8 * l));
+    xv[i] = __builtin_nontemporal_load(reinterpret_cast<const vec*>((const T*)a.v + tok * a.v_st + (long)head * a.v_sh + 8 * l));
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const unsigned tk = max_row<D>(top8(__builtin_convertvector(xk[i], f32x8))), tv = max_row<D>(top8(__builtin_convertvector(xv[i], f32x8)));
+    if (tk < kInf) top_k = max(top_k, tk);
+    else bad_k |= 1u << i;
+    if (tv < kInf) top_v = max(top_v, tv);
+    else bad_v |= 1u << i;
+  }
+  top_k = max_wave(top_k);
+  top_v = max_wave(top_v);
+  if ((tid & 63) == 0) {
+    s_top[0][wave] = top_k;
+    s_top[1][wave] = top_v;
+  }
+  __syncthreads();
+  int ek = exponent(max(max(s_top[0][0], s_top[0][1]), max(s_top[0][2], s_top[0][3])));
+  int ev = exponent(max(max(s_top[1][0], s_top[1][1]), max(s_top[1][2], s_top[1][3])));
+  int drop_k = 0, drop_v = 0;
+  if (begin) {                           // (the block's first token was there before)
+    ek = max(ek, was_k);
+    ev = max(ev, was_v);
+    drop_k = ek - was_k;
+    drop_v = ev - was_v;
+  }
+  const float fk = power(max(-ek, -126)), fv = power(max(-ev, -126));
+  f32x8 hi = f32x8(-448.f), lo = f32x8(-448.f);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int o = i * kRows + r;
+    if (o < begin || o >= end) continue;
+    const f32x8 yk = __builtin_convertvector(xk[i], f32x8) * fk, yv = __builtin_convertvector(xv[i], f32x8) * fv;
+    const bool nk = bad_k >> i & 1, nv = bad_v >> i & 1;
+    const uint2v ck = nk ? uint2v(0x7f7f7f7fu) : to_codes(yk), cv = nv ? uint2v(0x7f7f7f7fu) : to_codes(yv);
+    *reinterpret_cast<uint2v*>(a.kc + at + (long)o * D) = ck;
+    *reinterpret_cast<uint2v*>(a.vc + at + (long)o * D) = cv;
+    if (kb && !nk) {
+      const f32x8 z = from_codes(ck);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        hi[j] = fmaxf(hi[j], z[j]);
+        lo[j] = fmaxf(lo[j], -z[j]);
+      }
+    }
+  }
+  if (drop_k > 0 || drop_v > 0) {        // (rare: a scale doubles a few times in a block's life)
+    const float gk = power(-min(drop_k, 126)), gv = power(-min(drop_v, 126));
+    for (int o = r; o < begin; o += kRows) {
+      uint2v* const pk = reinterpret_cast<uint2v*>(a.kc + at + (long)o * D);
+      uint2v* const pv = reinterpret_cast<uint2v*>(a.vc + at + (long)o * D);
+      if (drop_k > 0) *pk = again(*pk, gk);
+      if (drop_v > 0) *pv = again(*pv, gv);
+    }
+  }
+  if (tid == 0) {
+    *ks = (uint8_t)(ek + 127);
+    *vs = (uint8_t)(ev + 127);
+  }
+  if (!kb) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    hi[j] = max_rows<D>(hi[j]);
+    lo[j] = max_rows<D>(lo[j]);
+  }
+  if ((tid & 63) < kLanes) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      s_b[wave][8 * l + j] = hi[j];
+      s_b[wave][D + 8 * l + j] = lo[j];
+    }
+  }
+  __syncthreads();
+  if (tid < 2 * D) {
+    const int x = (int)ceilf(0.25f * fmaxf(fmaxf(s_b[0][tid], s_b[1][tid]), fmaxf(s_b[2][tid], s_b[3][tid])));
+    const int y = begin ? -(-old >> min(drop_k, 31)) : -112;
+    kb[tid] = (int8_t)max(x, y);
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) kv8_read_kernel(Kv8Args a) {
+  typedef typename Vec8<T>::type vec;
+  constexpr int kLanes = D / 8;
+  const int head = blockIdx.x % a.kv_heads, l = threadIdx.x % kLanes;
+  const int tok = blockIdx.x / a.kv_heads * (kThreads / kLanes) + (int)threadIdx.x / kLanes;
+  if (tok >= a.tokens) return;
+  const unsigned slot = (unsigned)a.slots[tok], nslots = (unsigned)a.NP << a.lp;
+  const bool held = slot < nslots;       // (padding reads slot 0 and gives zeros)
+  const unsigned s = held ? slot : 0, page = s >> a.lp, off = s & ((1u << a.lp) - 1);
+  const long at = (long)page * a.c_sp + (((long)head << a.lp) + off) * D + 8 * l;
+  const uint2v ck = *reinterpret_cast<const uint2v*>(a.kc + at), cv = *reinterpret_cast<const uint2v*>(a.vc + at);
+  const float fk = __uint_as_float((unsigned)a.ks[(long)page * a.s_sp + head] << 23);
+  const float fv = __uint_as_float((unsigned)a.vs[(long)page * a.s_sp + head] << 23);
+  const f32x8 k = held ? from_codes(ck) * fk : f32x8(0.f), v = held ? from_codes(cv) * fv : f32x8(0.f);
+  T* ok = (T*)a.k + (long)tok * a.k_st + (long)head * a.k_sh + 8 * l;
+  T* ov = (T*)a.v + (long)tok * a.v_st + (long)head * a.v_sh + 8 * l;
+  __builtin_nontemporal_store(__builtin_convertvector(k, vec), reinterpret_cast<vec*>(ok));
+  __builtin_nontemporal_store(__builtin_convertvector(v, vec), reinterpret_cast<vec*>(ov));
+}
+
+// the checks that both directions share
+int take(Kv8Args& a, const void* k, long k_st, long k_sh, const void* v, long v_st, long v_sh, int tokens, int kv_heads,
+         int D, int align, void* kc, void* ks, void* vc, void* vs, long code_stride, long scale_stride, int pages, int page) {
+  auto bad = [&](const void* p, long st, long sh) {
+    return !p || (reinterpret_cast<uintptr_t>(p) & 15) || st % align || sh % align;
+  };
+  auto odd = [](const void* p) { return !p || (reinterpret_cast<uintptr_t>(p) & 15) != 0; };
+  if ((D != 64 && D != 128) || tokens < 0 || kv_heads <= 0 || pages <= 0 || (page != 32 && page != 64 && page != 128) ||
+      (long)pages * page > 0x7fffffffL || (long)tokens * kv_heads > (1L << 26))
+    return OA_EINVAL;
+  a = Kv8Args{};
+  a.tokens = tokens;
+  if (!tokens) return 0;
+  if (bad(k, k_st, k_sh) || bad(v, v_st, v_sh) || odd(kc) || !ks || odd(vc) || !vs ||
+      code_stride < (long)kv_heads * page * D || scale_stride < kv_heads || code_stride % 16)
+    return OA_EINVAL;
+  a.k = k; a.k_st = k_st; a.k_sh = k_sh;
+  a.v = v; a.v_st = v_st; a.v_sh = v_sh;
+  a.kc = (uint8_t*)kc; a.ks = (uint8_t*)ks; a.vc = (uint8_t*)vc; a.vs = (uint8_t*)vs;
+  a.c_sp = code_stride; a.s_sp = scale_stride;
+  a.kv_heads = kv_heads; a.NP = pages;
+  a.lp = __builtin_ctz(page);
+  return 0;
+}
+
+template <typename T, int D>
+void write_rows(const Kv8Args& a, dim3 grid, hipStream_t st) {
+  const int passes = (D << a.lp) / (8 * kThreads);
+  if (D == 64 && passes == 1) hipLaunchKernelGGL((kv8_write_kernel<T, D, D == 64 ? 1 : 2>), grid, dim3(kThreads), 0, st, a);
+  else if (passes == 2) hipLaunchKernelGGL((kv8_write_kernel<T, D, 2>), grid, dim3(kThreads), 0, st, a);
+  else if (passes == 4) hipLaunchKernelGGL((kv8_write_kernel<T, D, 4>), grid, dim3(kThreads), 0, st, a);
+  else hipLaunchKernelGGL((kv8_write_kernel<T, D, D == 64 ? 4 : 8>), grid, dim3(kThreads), 0, st, a);
+}
+
+template <typename T>
+void read_rows(const Kv8Args& a, int D, hipStream_t st) {
+  const int rows = kThreads / (D / 8);
+  const dim3 grid((unsigned)((long)((a.tokens + rows - 1) / rows) * a.kv_heads));
+  if (D == 64) hipLaunchKernelGGL((kv8_read_kernel<T, 64>), grid, dim3(kThreads), 0, st, a);
+  else hipLaunchKernelGGL((kv8_read_kernel<T, 128>), grid, dim3(kThreads), 0, st, a);
+}
+
+}  // namespace
+
+extern "C" int oa_kv8_write(const void* k, long k_st, long k_sh, const void* v, long v_st, long v_sh, int tokens,
+                            int kv_heads, int head_dim, int dtype, void* kc, void* ks, void* vc, void* vs, void* kb,
+                            long code_stride, long scale_stride, long bound_stride, int pages, int page, const int* table,
+                            long table_stride, int width, const int* lens, const int* cu, int sequences, void* stream) {
+  if (dtype < 0 || dtype > 2 || sequences < 0 || (!cu && sequences != tokens)) return OA_EINVAL;
+  Kv8Args a;
+  if (const int e = take(a, k, k_st, k_sh, v, v_st, v_sh, tokens, kv_heads, head_dim, dtype == 2 ? 4 : 8, kc, ks, vc, vs,
+                         code_stride, scale_stride, pages, page))
+    return e;
+  if (!tokens || !sequences) return 0;
+  const long work = cu ? (long)(tokens >> a.lp) + 2L * sequences : sequences;
+  if (!table || !lens || width <= 0 || (long)width * page > (1L << 30) || table_stride < width || sequences > (1 << 24) ||
+      (kb && bound_stride < 2L * kv_heads * head_dim) || work * kv_heads > 0xffffffffL / kThreads)
+    return OA_EINVAL;
+  a.kb = (int8_t*)kb; a.b_sp = bound_stride;
+  a.table = table; a.t_st = table_stride; a.width = width; a.lens = lens; a.cu = cu; a.B = sequences;
+  const dim3 grid((unsigned)(work * kv_heads));
+  const hipStream_t st = (hipStream_t)stream;
+  const int x = dtype * 2 + (head_dim == 128);
+  if (x == 0) write_rows<__bf16, 64>(a, grid, st);
+  else if (x == 1) write_rows<__bf16, 128>(a, grid, st);
+  else if (x == 2) write_rows<_Float16, 64>(a, grid, st);
+  else if (x == 3) write_rows<_Float16, 128>(a, grid, st);
+  else if (x == 4) write_rows<float, 64>(a, grid, st);
+  else write_rows<float, 128>(a, grid, st);
+  return OA_LAUNCH_STATUS();
+}
+
+extern "C" int oa_kv8_read(const int* slots, const void* kc, const void* ks, const void* vc, const void* vs,
+                           long code_stride, long scale_stride, int pages, int page, void* k, long k_st, long k_sh,
+                           void* v, long v_st, long v_sh, int tokens, int kv_heads, int head_dim, int dtype,
+                           void* stream) {
+  if (dtype != 0 && dtype != 2) return OA_EINVAL;  // (fp16 does not hold what a scale may be)
+  Kv8Args a;
+  if (const int e = take(a, k, k_st, k_sh, v, v_st, v_sh, tokens, kv_heads, head_dim, dtype == 2 ? 4 : 8,
+                         const_cast<void*>(kc), const_cast<void*>(ks), const_cast<void*>(vc), const_cast<void*>(vs),
+                         code_stride, scale_stride, pages, page))
+    return e;
+  if (!tokens) return 0;
+  if (!slots) return OA_EINVAL;
+  a.slots = slots;
+  if (dtype == 0) read_rows<__bf16>(a, head_dim, (hipStream_t)stream);
+  else read_rows<float>(a, head_dim, (hipStream_t)stream);
+  return OA_LAUNCH_STATUS();
+}

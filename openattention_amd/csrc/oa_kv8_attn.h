@@ -1,0 +1,50 @@
+// What the attention kernels over the 8-bit paged cache share: arguments, codes to bf16 or fp16.
+#pragma once
+#include "oa_kv8.h"
+#include "oa_paged_attn.h"
+
+namespace kv8 {
+
+using namespace paged;
+
+struct AttnArgs {
+  const uint16_t* q; long q_st, q_sh;
+  const uint8_t* kc; const uint8_t* ks; const uint8_t* vc; const uint8_t* vs;
+  long c_sp, s_sp;                       // bytes between pages
+  const int* table; long t_st;
+  const int* lens; const int* cu;
+  const int* list;                       // the blocks that a (token, KV head) reads, n of them; null: all
+  uint16_t* out; long o_st, o_sh;
+  float* ws_o; float* ws_ml;             // partial sums, (maximum, sum) by (row, chunk)
+  int B, HKV, G, tokens, max_q, width, NP, lp, chunk, nchunk, ntile, n;
+  unsigned by_g, by_hkv;                 // 2^16 / G + 1; 2^32 / HKV, rounded up (0: HKV is 1)
+  int clear;                             // the join sets rows of out that no sequence takes to 0
+  float c;                               // scale * log2 e
+};
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// 8 codes to bf16, times a power of two
+__device__ __forceinline__ bf16x8 from8(unsigned w0, unsigned w1, float f) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, f, false);
+  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, f, true);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, f, false);
+  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, f, true);
+  const uint4v x = {__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, c),
+                    __builtin_bit_cast(uint32_t, d)};
+  return __builtin_bit_cast(bf16x8, x);
+}
+// 8 codes to fp16, which holds them as they are, times a power of two
+__device__ __forceinline__ bf16x8 from8h(unsigned w0, unsigned w1, float f) {
+  const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, f, false);
+  const f16x2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, f, true);
+  const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, f, false);
+  const f16x2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, f, true);
+  const uint4v x = {__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, c),
+                    __builtin_bit_cast(uint32_t, d)};
+  return __builtin_bit_cast(bf16x8, x);
+}
+// whether one of 4 codes is NaN
+__device__ __forceinline__ unsigned nan_codes(unsigned w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+}  // namespace kv8

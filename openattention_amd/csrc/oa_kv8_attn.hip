@@ -1,0 +1,452 @@
+// Causal attention of the newest tokens of every sequence over an 8-bit paged cache (layout and codes: oa_kv8.hip),
+// over all of their keys or over the blocks that a list names for each token and KV head:
+//   out = sum_t p_t v_t / sum_t p_t,  p_t = exp(scale q . k_t - max),
+// in one pass over the keys with a running maximum and sum.
+//
+// One workgroup of four waves takes 16 NQ query rows of a KV head (row = token * G + head, so that any number of
+// query heads fills the tiles; with a list the rows of one token, as each has its own) and a chunk of keys (ops.kv8_chunk
+// says how many and why); each wave walks its own tiles of 32 keys and the waves join at the end.  With several
+// chunks a second kernel joins them.
+//   scores   S^T = K Q^T by v_mfma_f32_16x16x32 of the queries' type, which holds the codes as they are: a lane of the K
+//            operand takes 16 dims of each 64 of a key.  A tile lies in one block, whose scale is a factor of the
+//            scores.  All products are exact.
+//   values   O^T = V^T P^T in bf16, the scale taken in by the conversion: the weights are the B operand as the scores
+//            left them; V goes through the wave's own LDS tile and comes back by the LDS transpose reads.
+// Weights go into the product as two bf16 terms, so that the sum keeps 16 bits of each: up to 8 rows
+// the second term sits in the tile's other 8 columns, otherwise it takes a second product.
+#include "oa_kv8_attn.h"
+
+namespace {
+
+using namespace kv8;
+
+// one tile's codes of this lane (keys lane % 16 and 16 + lane % 16, 16 dims of each 64) and its scales
+template <int D>
+struct Tile {
+  uint4v k[2][D / 64], v[2][D / 64];
+  unsigned ks, vs;
+  unsigned bad;                          // the exponent of NaN where the page is outside of the cache
+};
+
+template <bool ONCE>
+__device__ __forceinline__ uint4v load16(const uint8_t* p) {
+  const uint4v* q = reinterpret_cast<const uint4v*>(p);
+  return ONCE ? __builtin_nontemporal_load(q) : *q;
+}
+
+// NQ tiles of 16 query rows; DUP: at most 8 rows, columns 8.. repeat them for the weights' second terms; T: the rows'
+// type; LISTED: over listed blocks, the rows of one token
+template <int D, int NQ, bool DUP, typename T, bool LISTED>
+__global__ void __launch_bounds__(kThreads, NQ > 1 ? 2 : 3) kv8_attn_kernel(AttnArgs a) {
+  constexpr bool kHalf = !std::is_same<T, __bf16>::value;
+  constexpr int kPieces = D / 64;        // 16-byte loads of a lane for a key
+  constexpr int kSteps = D / 32;         // products of a 16 x 16 score tile
+  constexpr int kDims = D / 16;          // tiles of 16 dims
+  constexpr int kRowB = D * 2;           // bytes of a value row in LDS
+  constexpr int kStage = kTile * kRowB;
+  constexpr int kCols = DUP ? 8 : 16;
+  constexpr int kStride = kWaves * kTile;
+  // value tiles of the waves; at the end their sums, 16 rows of D floats each
+  __shared__ __align__(16) char s_v[kWaves * (kStage > 64 * D ? kStage : 64 * D)];
+  __shared__ float s_m[kWaves][NQ * 16], s_l[kWaves][NQ * 16];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, g = lane >> 4;
+  // (sequence or token, head) fastest: workgroups go to the XCDs in turn, so that a long sequence's pieces and a
+  // batch's short sequences spread over all of them, and the query tiles of a piece meet in one L2
+  const int unit = blockIdx.x, row0 = blockIdx.y * (NQ * kCols), ch = blockIdx.z;
+  const int u = a.by_hkv ? (int)__umulhi((unsigned)unit, a.by_hkv) : unit, h = unit - u * a.HKV;
+  const int b = LISTED && a.cu ? sequence_of(a.B, u, [&](int i) { return a.cu[i]; }) : u;
+  auto token_of = [&](int r) { return LISTED ? 0 : (int)((unsigned)r * a.by_g >> 16); };         // r / G
+  const int k0 = ch * a.chunk, tb = k0 + wave * kTile;
+  const int* const trow = a.table + (long)b * a.t_st;
+  auto page_at = [&](int t0) { return trow[min(t0 >> a.lp, a.width - 1)]; };
+  int page0 = 0, page = 0;
+  if (!LISTED) {                         // (requested beside the length: what lies past it is not used)
+    page0 = page_at(tb);
+    page = page_at(tb + kStride);
+  }
+  const Seq sq = LISTED ? seq_of(a, b, 1L << 32) : seq_of(a, b);
+  const int j0 = LISTED ? u - sq.r0 : 0;                   // the token whose rows these are, or the first
+  if (LISTED && (j0 < 0 || j0 >= min(sq.R, a.max_q))) return;
+  const int rows = LISTED ? a.G : min(sq.R, a.max_q) * a.G;
+  if (row0 >= rows) return;
+  const int first = sq.n - sq.R + j0;    // position of the first token
+  const int hi = sq.bad ? 0 : first + token_of(min(row0 + NQ * kCols, rows) - 1) + 1;    // keys any row sees
+  const int all = first + token_of(row0) + 1;                                              // keys every row sees
+  const int k1 = LISTED ? min(k0 + a.chunk, a.n << a.lp) : min(k0 + a.chunk, hi);
+  if (!LISTED && k0 >= k1 && a.nchunk > 1) return;
+
+  // a tile's addresses: a scalar base and fixed lane offsets
+  const int pmask = (1 << a.lp) - 1;
+  const long headc = ((long)h << a.lp) * D;
+  const unsigned oc = col * D + 16 * g;
+  auto load = [&](Tile<D>& t, int off, int page) {
+    const bool bad = (unsigned)page >= (unsigned)a.NP;
+    t.bad = bad ? 0x7f800000u : 0u;
+    const long pg = bad ? 0 : page;
+    const long bc = pg * a.c_sp + headc + (long)off * D, bs = pg * a.s_sp + h;
+    t.ks = a.ks[bs];
+    t.vs = a.vs[bs];
+    const uint8_t* kc = a.kc + bc + oc;
+    const uint8_t* vc = a.vc + bc + oc;
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int x = 0; x < kPieces; ++x) t.k[c][x] = load16<NQ == 1>(kc + 16 * c * D + 64 * x);
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int x = 0; x < kPieces; ++x) t.v[c][x] = load16<NQ == 1>(vc + 16 * c * D + 64 * x);
+  };
+  const int nt = max(0, (k1 - tb + kStride - 1) / kStride);                  // this wave's tiles
+  Tile<D> ta, tc;
+  // listed blocks: tile i's block, -1 past the last; whether a row sees something of it
+  const int* const list = LISTED ? a.list + ((long)u * a.HKV + h) * a.n : nullptr;
+  auto block_at = [&](int i) { return i < nt ? list[(tb + i * kStride) >> a.lp] : -1; };
+  auto place_of = [&](int blk, int i) { return (blk << a.lp) + ((tb + i * kStride) & pmask); };
+  auto page_of = [&](int blk) { return trow[min(max(blk, 0), a.width - 1)]; };
+  auto live = [&](int blk, int i) { return blk >= 0 && blk < a.width && place_of(blk, i) < hi; };
+  int b0 = -1, b1 = -1, b2 = -1;
+  if (LISTED) {
+    b0 = block_at(0);
+    b1 = block_at(1);
+    b2 = block_at(2);
+    page0 = page_of(b0);
+    page = page_of(b1);
+    if (live(b0, 0)) load(ta, tb & pmask, page0);
+  } else if (nt > 0) {
+    load(ta, tb & pmask, page0);
+  }
+
+  // this lane's columns: rows of q (negated under a negative scale: the maximum is taken before scaling)
+  // and how many keys they see (0: no such row)
+  const float c = fabsf(a.c);
+  const unsigned flip = a.c < 0.f ? 0x80008000u : 0u;
+  bf16x8 Q[NQ][kSteps];
+  int lim[NQ];
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    const int r = row0 + x * kCols + (DUP ? col & 7 : col);
+    const int rr = min(r, rows - 1), j = token_of(rr), hd = h * a.G + rr - j * a.G;
+    lim[x] = r < rows ? first + j + 1 : 0;
+    const uint16_t* p = a.q + (long)(sq.r0 + j0 + j) * a.q_st + (long)hd * a.q_sh + 16 * g;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const uint4v w = *reinterpret_cast<const uint4v*>(p + 64 * (s >> 1) + 8 * (s & 1));
+      Q[x][s] = __builtin_bit_cast(bf16x8, w ^ uint4v(flip));
+    }
+  }
+
+  // LDS tile of 32 value rows; 16-byte chunk x of row r lies at x ^ f(r): 16 rows written at one chunk
+  // and 16 rows read at two both spread over all banks
+  char* const sv = s_v + wave * kStage;
+  auto fsw = [](int r) { return D == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : ((r >> 1) & 3) << 1; };
+  const int wbase = col * kRowB, wf = fsw(col);
+  const int lr = 4 * g + ((lane & 15) >> 2), rf = fsw(lr), lc = lane & 3;
+  auto val_op = [&](int d) {
+    const int ad = lr * kRowB + (((2 * d + (lc >> 1)) ^ rf) << 4) + (lc & 1) * 8;
+    const short4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v*)(sv + ad));
+    const short4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v*)(sv + ad + 16 * kRowB));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+
+  f32x4 O[NQ][kDims];
+  float m[NQ], l[NQ];                    // running maximum, scaled, and sum of the lane's keys
+  bool big[NQ];                          // a maximum is past 2^24 (uniform)
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    m[x] = -FLT_MAX;
+    l[x] = 0.f;
+    big[x] = false;
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) O[x][d] = f32x4(0.f);
+  }
+
+  // a tile whose first key is at position t0
+  auto body = [&](auto mask_c, int t0, const Tile<D>& t) {
+    const bool MASK = mask_c;            // (known beforehand, or the same for the whole wave)
+    // (the block's scale, a factor of the scores; finite, so that it leaves a product of 0 what it is)
+    const float ck = fminf(c * __uint_as_float(t.ks << 23), FLT_MAX) + __uint_as_float(t.bad) * 0.f;
+    f32x4 S[NQ][2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+      for (int x = 0; x < NQ; ++x) S[x][c] = f32x4(0.f);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const unsigned w0 = t.k[c][s >> 1][2 * (s & 1)], w1 = t.k[c][s >> 1][2 * (s & 1) + 1];
+        const bf16x8 kop = kHalf ? from8h(w0, w1, 1.f) : from8(w0, w1, 1.f);
+#pragma unroll
+        for (int x = 0; x < NQ; ++x) {
+          if constexpr (kHalf)
+            S[x][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, kop), __builtin_bit_cast(f16x8, Q[x][s]),
+                                                             S[x][c], 0, 0, 0);
+          else
+            S[x][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop, Q[x][s], S[x][c], 0, 0, 0);
+        }
+      }
+    }
+    // values into the LDS tile.  In a masked tile keys past the last one any row sees count as zeros (their
+    // weights are 0, but what lies there may be anything), and so does NaN in keys that some rows see
+    const float fv = __uint_as_float(t.vs << 23);
+    bool nan[2] = {false, false};
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      uint4v w[kPieces];
+#pragma unroll
+      for (int x = 0; x < kPieces; ++x) w[x] = t.v[c][x];
+      if (MASK) {
+        const bool past = t0 + 16 * c + col >= hi;
+        unsigned any = 0;
+#pragma unroll
+        for (int x = 0; x < kPieces; ++x) any |= nan_codes(w[x][0]) | nan_codes(w[x][1]) | nan_codes(w[x][2]) | nan_codes(w[x][3]);
+        nan[c] = any && !past;
+#pragma unroll
+        for (int x = 0; x < kPieces; ++x) w[x] = any || past ? uint4v(0u) : w[x];
+      }
+#pragma unroll
+      for (int x = 0; x < kPieces; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+          *reinterpret_cast<bf16x8*>(sv + wbase + 16 * c * kRowB + (((8 * x + 2 * g + y) ^ wf) << 4)) =
+              from8(w[x][2 * y], w[x][2 * y + 1], fv);
+    }
+    lane_order();
+
+    uint4v P[NQ], Plo[NQ];
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
+      float v[8];
+      float mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] = S[x][i >> 2][i & 3];
+        mx = fmaxf(mx, v[i]);
+      }
+      mx *= ck;
+      if (MASK) {
+        mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          v[i] = t0 + 16 * (i >> 2) + 4 * g + (i & 3) < lim[x] ? v[i] * ck : -INFINITY;
+          mx = fmaxf(mx, v[i]);
+        }
+      }
+      if (__any(mx > m[x])) {
+        const float mn = fmaxf(m[x], max_groups(mx)), alpha = __builtin_amdgcn_exp2f(m[x] - mn);
+        m[x] = mn;
+        l[x] *= alpha;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) O[x][d] *= alpha;
+        // the maximum rounds S ck, so that the fma below leaves up to half its last place: past 2^24 more than
+        // the exponential should see, and an infinity in time.  There S ck is rounded first, as the maximum is
+        big[x] = __any(fabsf(mn) >= 16777216.f);
+      }
+      if (!MASK && big[x]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= ck;
+      }
+      const float cc = MASK || big[x] ? 1.f : ck;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] = __builtin_amdgcn_exp2f(fmaf(v[i], cc, -m[x]));
+        l[x] += v[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t u = pack2(v[2 * i], v[2 * i + 1]);
+        const uint32_t lo = pack2(v[2 * i] - __uint_as_float(u << 16), v[2 * i + 1] - __uint_as_float(u & 0xffff0000u));
+        P[x][i] = DUP && (lane & 8) ? lo : u;
+        Plo[x][i] = lo;
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) {
+      const bf16x8 vop = val_op(d);
+#pragma unroll
+      for (int x = 0; x < NQ; ++x) {
+        O[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vop, __builtin_bit_cast(bf16x8, P[x]), O[x][d], 0, 0, 0);
+        if (!DUP) O[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vop, __builtin_bit_cast(bf16x8, Plo[x]), O[x][d], 0, 0, 0);
+      }
+    }
+    lane_order();
+    if (MASK) {                          // NaN, into the rows that see it (rare): the lane's dims, 16 of each 64
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        unsigned long at_nan = __ballot(nan[c]);
+        while (at_nan) {
+          const int at = __builtin_ctzl(at_nan), key = t0 + 16 * c + (at & 15), part = at >> 4;
+          at_nan &= at_nan - 1;
+#pragma unroll
+          for (int x = 0; x < NQ; ++x)
+#pragma unroll
+            for (int d = 0; d < kDims; ++d)
+              if ((d & 3) == part && key < lim[x]) O[x][d] = f32x4(__builtin_nanf(""));
+        }
+      }
+    }
+  };
+  typedef std::integral_constant<bool, false> whole;
+  typedef std::integral_constant<bool, true> masked;
+  if (LISTED) {
+#pragma unroll 1
+    for (int i = 0; i < nt; ++i) {
+      if (live(b1, i + 1)) load(tc, (tb + (i + 1) * kStride) & pmask, page);
+      page = page_of(b2);
+      const int b3 = block_at(i + 3);
+      if (live(b0, i)) {
+        const int t0 = place_of(b0, i);
+        body(t0 + kTile > hi, t0, ta);
+      }
+      ta = tc;
+      b0 = b1;
+      b1 = b2;
+      b2 = b3;
+    }
+  } else {
+    const int nfull = min(nt, max(0, (all - tb - kTile + kStride) / kStride));    // tiles that every row sees whole
+    auto next = [&](int i) {             // tile i + 1, and the page of the one after
+      if (i + 1 < nt) {
+        const int t0 = tb + (i + 1) * kStride;
+        load(tc, t0 & pmask, page);
+        page = page_at(t0 + kStride);
+      }
+    };
+    int i = 0;
+#pragma unroll 1
+    for (; i < nfull; ++i) {
+      next(i);
+      body(whole(), tb + i * kStride, ta);
+      ta = tc;
+    }
+#pragma unroll 1
+    for (; i < nt; ++i) {
+      next(i);
+      body(masked(), tb + i * kStride, ta);
+      ta = tc;
+    }
+  }
+
+  // the four waves' sums, with a common maximum
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    const float lt = sum_groups(l[x]);
+    if (g == 0) {
+      s_m[wave][x * 16 + col] = m[x];
+      s_l[wave][x * 16 + col] = lt;
+    }
+  }
+  float* const so = reinterpret_cast<float*>(s_v);
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    __syncthreads();                     // (every wave is done with its tile, or with the previous sums)
+    const int sc = x * 16 + col;
+    const float M = fmaxf(fmaxf(s_m[0][sc], s_m[1][sc]), fmaxf(s_m[2][sc], s_m[3][sc]));
+    const float e = __builtin_amdgcn_exp2f(m[x] - M);
+#pragma unroll
+    for (int d = 0; d < kDims; ++d)      // 16-byte chunk y of column col at y ^ col
+      *reinterpret_cast<f32x4*>(so + (wave * 16 + col) * D + (((4 * d + g) ^ col) << 2)) = O[x][d] * e;
+    __syncthreads();
+    constexpr int kChunks = D / 4;
+    for (int i = threadIdx.x; i < kCols * kChunks; i += kThreads) {
+      const int cl = i / kChunks, y = i % kChunks, r = row0 + x * kCols + cl;
+      if (r >= rows) continue;
+      const int c16 = x * 16 + cl;
+      const float Mr = fmaxf(fmaxf(s_m[0][c16], s_m[1][c16]), fmaxf(s_m[2][c16], s_m[3][c16]));
+      float L = 0.f;
+      f32x4 o = f32x4(0.f);
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        L += s_l[w][c16] * __builtin_amdgcn_exp2f(s_m[w][c16] - Mr);
+        o += *reinterpret_cast<const f32x4*>(so + (w * 16 + cl) * D + ((y ^ cl) << 2));
+        if (DUP) o += *reinterpret_cast<const f32x4*>(so + (w * 16 + 8 + cl) * D + ((y ^ (8 + cl)) << 2));
+      }
+      const int j = token_of(r), hd = h * a.G + r - j * a.G;
+      if (a.nchunk == 1) {
+        const bool some = first + j >= 0 && !(LISTED && L == 0.f);
+        o = sq.bad ? f32x4(__builtin_nanf("")) : some ? o / L : f32x4(0.f);
+        *reinterpret_cast<uint2v*>(a.out + (long)(sq.r0 + j0 + j) * a.o_st + (long)hd * a.o_sh + 4 * y) =
+            uint2v{pack_out<T>(o[0], o[1]), pack_out<T>(o[2], o[3])};
+      } else {
+        const long at = ((long)(sq.r0 + j0 + j) * (a.HKV * a.G) + hd) * a.nchunk + ch;
+        *reinterpret_cast<f32x4*>(a.ws_o + at * D + 4 * y) = o;
+        if (y == 0) *reinterpret_cast<f32x2*>(a.ws_ml + at * 2) = f32x2{Mr, L};
+      }
+    }
+  }
+}
+
+template <int D, typename T, bool LISTED>
+__global__ void __launch_bounds__(kThreads) kv8_join_kernel(AttnArgs a) {
+  join_pieces<D, T, LISTED>(a);
+}
+
+template <int D, typename T, bool LISTED>
+int launch(AttnArgs a, hipStream_t st) {
+  const long rows = LISTED ? a.G : (long)a.max_q * a.G;
+  const int cols = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
+  a.ntile = (int)((rows + cols - 1) / cols);
+  const long units = (long)(LISTED ? a.tokens : a.B) * a.HKV, joins = (long)a.max_q * a.HKV * a.G;
+  // (workgroups along the other axes are counted in 16 bits)
+  if (units > kGrid || a.ntile > 65535 || a.nchunk > 65535 || units * a.ntile * a.nchunk > kGrid ||
+      (a.nchunk > 1 && (joins > kGrid || a.B > 65535)))
+    return OA_EINVAL;
+  // quotients as products with 2^16 / G + 1 and 2^32 / HKV, rounded up: exact while the number times the divisor is
+  // less than that power
+  if (units * a.HKV > 0xffffffffL || rows * a.G > 65535) return OA_EINVAL;
+  a.by_g = 65536u / a.G + 1;
+  a.by_hkv = a.HKV > 1 ? (unsigned)((0x100000000L + a.HKV - 1) / a.HKV) : 0;
+  const dim3 grid((unsigned)units, a.ntile, a.nchunk), blk(kThreads);
+  if (cols == 8) hipLaunchKernelGGL((kv8_attn_kernel<D, 1, true, T, LISTED>), grid, blk, 0, st, a);
+  else if (cols == 16) hipLaunchKernelGGL((kv8_attn_kernel<D, 1, false, T, LISTED>), grid, blk, 0, st, a);
+  else hipLaunchKernelGGL((kv8_attn_kernel<D, 2, false, T, LISTED>), grid, blk, 0, st, a);
+  if (a.nchunk > 1) hipLaunchKernelGGL((kv8_join_kernel<D, T, LISTED>), dim3((unsigned)joins, a.B), blk, 0, st, a);
+  return OA_LAUNCH_STATUS();
+}
+
+template <int D, typename T>
+int launch_over(const AttnArgs& a, hipStream_t st) {
+  return a.list ? launch<D, T, true>(a, st) : launch<D, T, false>(a, st);
+}
+
+}  // namespace
+
+extern "C" int oa_kv8_attn(const void* q, long q_st, long q_sh, int dtype, const void* kc, const void* ks, const void* vc,
+                           const void* vs, long code_stride, long scale_stride, int pages, int page, const int* table,
+                           long table_stride, int width, const int* lens, const int* cu, int sequences, int tokens,
+                           int max_q, int q_heads, int kv_heads, int head_dim, float sm_scale, const int* blocks, int n,
+                           int chunk, int nchunk, float* ws_o, float* ws_ml, void* out, long o_st, long o_sh, int clear,
+                           void* stream) {
+  auto odd = [](const void* p, uintptr_t n) { return !p || (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0; };
+  if ((head_dim != 64 && head_dim != 128) || dtype < 0 || dtype > 1 || sequences < 0 || tokens < 0 || max_q <= 0 ||
+      kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads || (long)max_q * (q_heads / kv_heads) > (1L << 30) || pages <= 0 ||
+      (page != 32 && page != 64 && page != 128) || (long)pages * page > 0x7fffffffL || width <= 0 ||
+      (long)width * page > (1L << 30) || table_stride < width || chunk < 128 || chunk % 128 || nchunk <= 0 ||
+      (long)nchunk * chunk > (1L << 30) + (1L << 29) ||
+      (blocks && (n <= 0 || (long)n * page > (1L << 30) || (long)nchunk * chunk < (long)n * page)))
+    return OA_EINVAL;
+  if (!cu && (max_q != 1 || sequences != tokens)) return OA_EINVAL;
+  if (!sequences || !tokens) return 0;
+  if (odd(q, 16) || q_st % 8 || q_sh % 8 || odd(out, 8) || o_st % 4 || o_sh % 4 || odd(kc, 16) || !ks || odd(vc, 16) || !vs ||
+      !table || !lens || (blocks && odd(blocks, 4)) || code_stride < (long)kv_heads * page * head_dim ||
+      scale_stride < kv_heads || code_stride % 16 || !(sm_scale == sm_scale))
+    return OA_EINVAL;
+  if (out == q) return OA_EINVAL;        // (rows may be read again after others were written)
+  if (nchunk > 1 && (odd(ws_o, 16) || odd(ws_ml, 8))) return OA_EINVAL;
+  AttnArgs a;
+  a.q = (const uint16_t*)q; a.q_st = q_st; a.q_sh = q_sh;
+  a.kc = (const uint8_t*)kc; a.ks = (const uint8_t*)ks; a.vc = (const uint8_t*)vc; a.vs = (const uint8_t*)vs;
+  a.c_sp = code_stride; a.s_sp = scale_stride;
+  a.table = table; a.t_st = table_stride; a.lens = lens; a.cu = cu;
+  a.list = blocks; a.n = n;
+  a.out = (uint16_t*)out; a.o_st = o_st; a.o_sh = o_sh;
+  a.ws_o = ws_o; a.ws_ml = ws_ml;
+  a.B = sequences; a.HKV = kv_heads; a.G = q_heads / kv_heads; a.tokens = tokens; a.max_q = max_q;
+  a.width = width; a.NP = pages; a.lp = __builtin_ctz(page); a.chunk = chunk; a.nchunk = nchunk;
+  a.clear = cu && clear;
+  a.c = sm_scale * kLog2e;
+  const hipStream_t st = (hipStream_t)stream;
+  if (head_dim == 64) return dtype ? launch_over<64, _Float16>(a, st) : launch_over<64, __bf16>(a, st);
+  return dtype ? launch_over<128, _Float16>(a, st) : launch_over<128, __bf16>(a, st);
+}

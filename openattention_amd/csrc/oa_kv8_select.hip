@@ -1,0 +1,336 @@
+// The blocks of an 8-bit paged cache whose keys can score highest for each query token and KV head (oa_kv8_select).
+//
+// A block's bounds hi, nlo of every channel (oa_kv8.hip) give the most that a key in it can score:
+//   sum_d max(q_d, 0) hi_d + max(-q_d, 0) nlo_d,  times 4 2^e,
+// here with q rounded to whole numbers q8 of at most 127 by one power of two for the query heads of a KV head
+// together, and the largest over these heads.  All of it is whole numbers below 2^24 times a power of two (past
+// 2^100 taken as 2^100), so that a score has one value whatever the order of its sums, and the choice (ties: the
+// lower block) is exact.
+//
+// The first kernel forms the scores by v_mfma_i32_16x16x64_i8: 16 query rows (a token's heads, padded to a power of
+// two by repeating the last; several tokens where heads are few) against 16 blocks, both sides as [max(x, 0),
+// max(-x, 0)].  A lane ends with the scores of one block for four rows, so that the largest over four heads takes no
+// exchange.  The second takes a row's scores as integers of the same order, finds the last one that is chosen by four
+// passes over its bytes, counted in LDS, and writes the chosen blocks in ascending order.
+#include "oa_kv8.h"
+
+namespace {
+
+using namespace kv8;
+
+typedef int int4v __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kThreads = 256, kWaves = 4;
+constexpr int kSpan = 128;               // blocks that a workgroup of the first kernel scores
+constexpr int kHeld = 8;                 // scores that a lane of the second keeps in registers
+
+struct SelectArgs {
+  const void* q; long q_st, q_sh;
+  const uint8_t* ks; const int8_t* kb;
+  long s_sp, b_sp;                       // bytes between pages of scales, bounds
+  const int* table; long t_st; int width;
+  const int* lens; const int* cu;
+  unsigned* ws;                          // scores by (token, head, block)
+  int* out;
+  int B, HKV, G, tokens, NP, lp, n, first, last, cap;
+  int head0;                             // the first query head of this launch; not 0: scores are raised, not set
+};
+
+// a sequence's rows and its keys (none that the call does not cover)
+struct Seq {
+  int n, r0, R;
+};
+__device__ __forceinline__ Seq seq_of(const SelectArgs& a, int b) {
+  Seq s;
+  s.n = a.lens[b];
+  s.r0 = a.cu ? a.cu[b] : b;
+  const int r1 = a.cu ? a.cu[b + 1] : b + 1;
+  s.R = s.r0 < 0 || r1 < s.r0 || r1 > a.tokens ? 0 : r1 - s.r0;
+  if (s.n < 0 || (long)s.n > (long)min(a.width, a.cap) << a.lp) s.n = 0;
+  return s;
+}
+
+template <int GP>
+__device__ __forceinline__ unsigned max_heads(unsigned v) {        // over GP lanes side by side, then the four groups
+  auto dpp = [](unsigned x, auto ctrl) {
+    return max(x, (unsigned)__builtin_amdgcn_update_dpp((int)x, (int)x, decltype(ctrl)::value, 0xf, 0xf, false));
+  };
+  if (GP >= 2) v = dpp(v, std::integral_constant<int, 0xB1>());
+  if (GP >= 4) v = dpp(v, std::integral_constant<int, 0x4E>());
+  if (GP >= 8) v = dpp(v, std::integral_constant<int, 0x141>());
+  if (GP >= 16) v = dpp(v, std::integral_constant<int, 0x140>());
+  const auto x = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max(x[0], x[1]);
+  const auto y = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return max(y[0], y[1]);
+}
+
+__device__ __forceinline__ float finite(float x) { return (__float_as_uint(x) & 0x7fffffffu) < 0x7f800000u ? x : 0.f; }
+
+// scores as integers of the same order
+__device__ __forceinline__ unsigned key_of(float f) {
+  const unsigned u = __float_as_uint(f);
+  return u ^ ((int)u < 0 ? 0xffffffffu : 0x80000000u);
+}
+
+// GP: rows of a token in a tile, the heads rounded up to a power of two
+template <typename T, int D, int GP>
+__global__ void __launch_bounds__(kThreads) kv8_score_kernel(SelectArgs a) {
+  constexpr int kTokens = 16 / GP, kPieces = D / 64, kSteps = 2 * kPieces;
+  typedef std::conditional_t<std::is_same<T, __bf16>::value, bf16x8, f16x8> vec;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+  const int h = blockIdx.x % a.HKV, id = blockIdx.x / a.HKV;
+  const int b = a.cu ? sequence_of(a.B, id, [&](int i) { return a.cu[i] / kTokens + 2 * i; }) : id;
+  const Seq sq = seq_of(a, b);
+  const int j0 = a.cu ? (id - (sq.r0 / kTokens + 2 * b)) * kTokens : 0;
+  if (j0 < 0 || j0 >= sq.R) return;
+  const int pos = sq.n - sq.R + min(j0 + kTokens, sq.R) - 1, seen = pos < 0 ? 0 : (pos >> a.lp) + 1;
+  const int from = blockIdx.y * kSpan;
+  if (seen <= a.n || from >= seen) return;               // (all blocks are chosen, or none are here)
+
+  // this wave's blocks: two tiles of 16
+  const int* trow = a.table + (long)b * a.t_st;
+  int at[2];
+  unsigned page[2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    at[x] = from + (wave + x * kWaves) * 16 + col;
+    page[x] = (unsigned)trow[min(at[x], a.width - 1)];
+  }
+  // this lane's row: dims 16 g and on of each 64
+  const int row = min(j0 + col / GP, sq.R - 1), hd = col % GP;
+  const T* const q = (const T*)a.q + (long)(sq.r0 + row) * a.q_st + (long)h * a.G * a.q_sh + 16 * g;
+  f32x8 x[kPieces][2];
+  unsigned top = 0;
+  auto fetch = [&](int head) {
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        x[p][y] = __builtin_convertvector(*reinterpret_cast<const vec*>(q + (long)head * a.q_sh + 64 * p + 8 * y), f32x8);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[p][y][i] = finite(x[p][y][i]);
+          top = max(top, __float_as_uint(x[p][y][i]) & 0x7fffffffu);
+        }
+      }
+  };
+  for (int i = hd; i < a.G; i += GP) fetch(i);           // (the scale is that of all heads)
+  fetch(min(a.head0 + hd, a.G - 1));
+  top = max_heads<GP>(top);
+  // the smallest u with top <= 127 2^u
+  const float f = power(-max((int)((top + 0x1ffffu) >> 23) - 133, -120));
+  int4v Q[kSteps];
+#pragma unroll
+  for (int p = 0; p < kPieces; ++p)
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      unsigned plus = 0, minus = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = (int)rintf(x[p][w >> 1][4 * (w & 1) + i] * f);
+        plus |= (unsigned)max(k, 0) << (8 * i);
+        minus |= (unsigned)max(-k, 0) << (8 * i);
+      }
+      Q[p][w] = (int)plus;
+      Q[kPieces + p][w] = (int)minus;
+    }
+
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const bool bad = page[x] >= (unsigned)a.NP;
+    const long pg = bad ? 0 : page[x];
+    const int4v* kb = reinterpret_cast<const int4v*>(a.kb + pg * a.b_sp + (long)h * (2 * D) + 16 * g);
+    const int e = min((int)a.ks[pg * a.s_sp + h] - 127, 100);
+    int4v S = int4v(0);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) S = __builtin_amdgcn_mfma_i32_16x16x64_i8(Q[s], kb[4 * s], S, 0, 0, 0);
+    // S[i]: row 4 g + i, this lane's block
+    int best[4] = {S[0], S[1], S[2], S[3]};
+    constexpr int kOut = GP == 1 ? 4 : GP == 2 ? 2 : 1;
+    if (GP == 2) {
+      best[0] = max(S[0], S[1]);
+      best[1] = max(S[2], S[3]);
+    } else if (GP >= 4) {
+      best[0] = max(max(S[0], S[1]), max(S[2], S[3]));
+      if (GP >= 8) {
+        const auto y = __builtin_amdgcn_permlane16_swap((unsigned)best[0], (unsigned)best[0], false, false);
+        best[0] = max((int)y[0], (int)y[1]);
+      }
+      if (GP >= 16) {
+        const auto y = __builtin_amdgcn_permlane32_swap((unsigned)best[0], (unsigned)best[0], false, false);
+        best[0] = max((int)y[0], (int)y[1]);
+      }
+    }
+    const int tok = GP <= 4 ? g * kOut : GP == 8 ? g >> 1 : 0;       // the first token of the tile that this lane holds
+    if ((GP == 8 && (g & 1)) || (GP == 16 && g)) continue;
+#pragma unroll
+    for (int i = 0; i < kOut; ++i) {
+      if (at[x] >= seen || j0 + tok + i >= sq.R) continue;
+      unsigned* const to = a.ws + ((long)(sq.r0 + j0 + tok + i) * a.HKV + h) * a.cap + at[x];
+      const unsigned key = key_of(bad ? -3.4028234e38f : (float)best[i] * power(e));
+      *to = a.head0 ? max(*to, key) : key;
+    }
+  }
+}
+
+// inclusive sum over the lanes of a wave
+__device__ __forceinline__ unsigned wave_scan(unsigned v) {
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);     // row_shr 1, 2, 4, 8
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);     // rows 0 to 1, 2 to 3
+  return v + (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);   // rows 1 to 2, 3
+}
+
+__global__ void __launch_bounds__(kThreads) kv8_choose_kernel(SelectArgs a) {
+  __shared__ int s_hist[256];
+  __shared__ unsigned s_part[kWaves];
+  __shared__ int s_bin, s_left;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int h = blockIdx.x % a.HKV, t = blockIdx.x / a.HKV;
+  const int b = a.cu ? sequence_of(a.B, t, [&](int i) { return a.cu[i]; }) : t;
+  const Seq sq = seq_of(a, b);
+  const int j = t - sq.r0, pos = sq.n - sq.R + j;
+  const int seen = j < 0 || j >= sq.R || pos < 0 ? 0 : (pos >> a.lp) + 1;
+  int* const out = a.out + ((long)t * a.HKV + h) * a.n;
+  if (seen <= a.n) {
+    for (int i = tid; i < a.n; i += kThreads) out[i] = i < seen ? i : -1;
+    return;
+  }
+  const unsigned* const ws = a.ws + ((long)t * a.HKV + h) * a.cap;
+  const int lo = a.first, hi = seen - a.last;             // blocks to choose from (more than are wanted)
+  const int per = (seen + kThreads - 1) / kThreads, mine = tid * per;
+  const bool held = per <= kHeld;
+  unsigned key[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) key[i] = held && i < per && mine + i < seen ? ws[mine + i] : 0;
+  // the score of the last that is chosen, byte by byte: of those that agree with it so far, `left` are to be chosen
+  int left = a.n - a.first - a.last;
+  unsigned have = 0;
+  for (int shift = 24; shift >= 0 && left; shift -= 8) {
+    s_hist[tid] = 0;
+    __syncthreads();
+    auto count = [&](int i, unsigned k) {
+      if (i >= lo && i < hi && (shift == 24 || (k ^ have) >> (shift + 8) == 0)) atomicAdd(&s_hist[k >> shift & 255], 1);
+    };
+    if (held) {
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i)
+        if (i < per) count(mine + i, key[i]);
+    } else {
+      for (int i = lo + tid; i < hi; i += kThreads) count(i, ws[i]);
+    }
+    __syncthreads();
+    // numbers from the highest bin down
+    const unsigned c = (unsigned)s_hist[255 - tid];
+    unsigned sum = wave_scan(c);
+    if (lane == 63) s_part[wave] = sum;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) sum += s_part[w];
+    if ((int)sum >= left && (int)(sum - c) < left) {      // (one lane: the bin that holds the last one)
+      s_bin = 255 - tid;
+      s_left = left - (int)(sum - c);
+    }
+    __syncthreads();
+    have |= (unsigned)s_bin << shift;
+    left = s_left;
+  }
+  // chosen: the first and last blocks, scores above `have`, and the lowest `left` of those that equal it
+  unsigned above = 0, equal = 0;
+  auto kind = [&](int i, unsigned k) { return i < lo || i >= hi ? 2 : left && k >= have ? (k > have ? 2 : 1) : 0; };
+  const int end = min(mine + per, seen);
+  if (held) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (mine + i < end) {
+        const int x = kind(mine + i, key[i]);
+        above += x == 2;
+        equal += x == 1;
+      }
+  } else {
+    for (int i = mine; i < end; ++i) {
+      const int x = kind(i, ws[i]);
+      above += x == 2;
+      equal += x == 1;
+    }
+  }
+  unsigned sa = wave_scan(above), se = wave_scan(equal);
+  __shared__ unsigned s_above[kWaves], s_equal[kWaves];
+  if (lane == 63) {
+    s_above[wave] = sa;
+    s_equal[wave] = se;
+  }
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) {
+    sa += s_above[w];
+    se += s_equal[w];
+  }
+  int na = (int)(sa - above), ne = (int)(se - equal);     // before this lane's
+  auto put = [&](int i, unsigned k) {
+    const int x = kind(i, k);
+    if (x == 2 || (x == 1 && ne < left)) out[na + min(ne, left)] = i;
+    na += x == 2;
+    ne += x == 1;
+  };
+  if (held) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (mine + i < end) put(mine + i, key[i]);
+  } else {
+    for (int i = mine; i < end; ++i) put(i, ws[i]);
+  }
+}
+
+template <typename T, int D>
+void score(SelectArgs a, dim3 grid, int gp, hipStream_t st) {
+  if (gp == 1) hipLaunchKernelGGL((kv8_score_kernel<T, D, 1>), grid, dim3(kThreads), 0, st, a);
+  else if (gp == 2) hipLaunchKernelGGL((kv8_score_kernel<T, D, 2>), grid, dim3(kThreads), 0, st, a);
+  else if (gp == 4) hipLaunchKernelGGL((kv8_score_kernel<T, D, 4>), grid, dim3(kThreads), 0, st, a);
+  else if (gp == 8) hipLaunchKernelGGL((kv8_score_kernel<T, D, 8>), grid, dim3(kThreads), 0, st, a);
+  else
+    for (; a.head0 < a.G; a.head0 += 16) hipLaunchKernelGGL((kv8_score_kernel<T, D, 16>), grid, dim3(kThreads), 0, st, a);
+}
+
+}  // namespace
+
+extern "C" int oa_kv8_select(const void* q, long q_st, long q_sh, int dtype, const void* ks, const void* kb,
+                             long scale_stride, long bound_stride, int pages, int page, const int* table, long table_stride,
+                             int width, const int* lens, const int* cu, int sequences, int tokens, int q_heads, int kv_heads,
+                             int head_dim, int n, int first, int last, int cap, unsigned* ws, int* blocks, void* stream) {
+  if ((head_dim != 64 && head_dim != 128) || dtype < 0 || dtype > 1 || sequences < 0 || tokens < 0 || kv_heads <= 0 ||
+      q_heads <= 0 || q_heads % kv_heads || pages <= 0 || (page != 32 && page != 64 && page != 128) ||
+      (long)pages * page > 0x7fffffffL || width <= 0 || (long)width * page > (1L << 30) || table_stride < width ||
+      sequences > (1 << 24) || n <= 0 || first < 0 || last < 1 || (long)first + last > n || cap <= 0 || cap > width ||
+      (!cu && sequences != tokens))
+    return OA_EINVAL;
+  if (!sequences || !tokens) return 0;
+  auto odd = [](const void* p, uintptr_t x) { return !p || (reinterpret_cast<uintptr_t>(p) & (x - 1)) != 0; };
+  if (odd(q, 16) || q_st % 8 || q_sh % 8 || !ks || odd(kb, 16) || scale_stride < kv_heads || bound_stride % 16 ||
+      bound_stride < 2L * kv_heads * head_dim || !table || !lens || (cap > n && odd(ws, 4)) || odd(blocks, 4))
+    return OA_EINVAL;
+  SelectArgs a;
+  a.q = q; a.q_st = q_st; a.q_sh = q_sh;
+  a.ks = (const uint8_t*)ks; a.kb = (const int8_t*)kb; a.s_sp = scale_stride; a.b_sp = bound_stride;
+  a.table = table; a.t_st = table_stride; a.width = width; a.lens = lens; a.cu = cu; a.ws = ws; a.out = blocks;
+  a.B = sequences; a.HKV = kv_heads; a.G = q_heads / kv_heads; a.tokens = tokens; a.NP = pages; a.lp = __builtin_ctz(page);
+  a.n = n; a.first = first; a.last = last; a.cap = cap; a.head0 = 0;
+  int gp = 1;
+  while (gp < a.G && gp < 16) gp *= 2;
+  const long tiles = (cu ? (long)tokens / (16 / gp) + 2L * sequences : sequences) * kv_heads, spans = (cap + kSpan - 1) / kSpan;
+  if (tiles > 0xffffffffL / kThreads || spans > 65535 || (long)tokens * kv_heads > 0xffffffffL / kThreads) return OA_EINVAL;
+  const dim3 grid((unsigned)tiles, (unsigned)spans);
+  const hipStream_t st = (hipStream_t)stream;
+  if (cap > n) {                         // (otherwise every row takes all of its blocks)
+    if (dtype == 0 && head_dim == 64) score<__bf16, 64>(a, grid, gp, st);
+    else if (dtype == 0) score<__bf16, 128>(a, grid, gp, st);
+    else if (head_dim == 64) score<_Float16, 64>(a, grid, gp, st);
+    else score<_Float16, 128>(a, grid, gp, st);
+  }
+  hipLaunchKernelGGL(kv8_choose_kernel, dim3((unsigned)(tokens * kv_heads)), dim3(kThreads), 0, st, a);
+  return OA_LAUNCH_STATUS();
+}

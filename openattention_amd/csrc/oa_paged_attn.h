@@ -1,0 +1,171 @@
+// What the attention kernels over a paged cache share, whatever its codes: a sequence's rows and lengths, exchanges
+// between the lanes of a wave, and the join of a row's pieces.  Args: the kernels' arguments, whose fields these name.
+#pragma once
+#include <cfloat>
+#include <type_traits>
+
+#include "oa_common.h"
+
+namespace paged {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef unsigned int uint4v __attribute__((ext_vector_type(4)));
+typedef unsigned int uint2v __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) short4v lds_short4v;
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * 64;
+constexpr int kTile = 32;                // keys per tile
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr long kGrid = 0xffffffffL / kThreads;             // a grid's threads along an axis are counted in 32 bits
+
+// what a sequence asks: its rows and how many keys they see
+struct Seq {
+  int n, r0, R;
+  bool bad;                              // more keys than the table or the call covers
+};
+
+template <typename Args>
+__device__ __forceinline__ Seq seq_of(const Args& a, int b, long covered) {
+  Seq s;
+  s.n = max(a.lens[b], 0);
+  s.r0 = a.cu ? a.cu[b] : b;
+  const int r1 = a.cu ? a.cu[b + 1] : b + 1;
+  s.R = s.r0 < 0 || r1 < s.r0 || r1 > a.tokens ? 0 : r1 - s.r0;         // (starts that do not fit the rows: none)
+  s.bad = (long)s.n > min((long)a.width << a.lp, covered);
+  return s;
+}
+template <typename Args>
+__device__ __forceinline__ Seq seq_of(const Args& a, int b) { return seq_of(a, b, (long)a.nchunk * a.chunk); }
+
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  const f32x2 x = {a, b};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2));
+}
+__device__ __forceinline__ uint32_t pack2h(float a, float b) {
+  const f32x2 x = {a, b};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, f16x2));
+}
+// two values in the type of the rows
+template <typename T>
+__device__ __forceinline__ uint32_t pack_out(float a, float b) {
+  return std::is_same<T, __bf16>::value ? pack2(a, b) : pack2h(a, b);
+}
+// An entry of a table's row, the same for all lanes, by a vector load: scalar loads come back in no order, and
+// beside one in flight every wait for LDS waits for all of it.
+__device__ __forceinline__ int table_entry(const int* row, int i) {
+  int zero;
+  asm("v_mov_b32 %0, 0" : "=v"(zero));
+  return row[i + zero];
+}
+
+__device__ __forceinline__ float max_groups(float v) {     // over the four 16-lane groups
+  const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+  const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+}
+__device__ __forceinline__ float sum_groups(float v) {
+  const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+  const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(y[0]) + __uint_as_float(y[1]);
+}
+
+// what the lanes of a wave exchange through its LDS tile stays in program order (the LDS keeps it)
+__device__ __forceinline__ void lane_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local"); }
+
+// Zeros in the rows of out that no sequence takes: those before the first and behind the last by all workgroups
+// of the join together, and head hd of sequence b's rows past max_q (all of its rows, where they do not fit) by
+// the one of its first row.  In the join, as it costs a launch to fill out beforehand (5 drafts of 7 sequences
+// 19.5 us a call, 15.5 here) and the attention kernel 4 to 13 us (one sequence of 131072 keys 30.6 to 35.6, 32 of
+// 32768 184 to 197), even where there is nothing to clear.
+template <int D, typename Args>
+__device__ __forceinline__ void clear_rows(const Args& a, int b, int hd, bool own) {
+  constexpr int kLanes = D / 4, kRows = kThreads / kLanes;     // lanes of a row, 8 bytes each
+  const int y = threadIdx.x % kLanes, x = threadIdx.x / kLanes, heads = a.HKV * a.G;
+  auto zero = [&](int tok, int head) {
+    *reinterpret_cast<uint2v*>(a.out + (long)tok * a.o_st + (long)head * a.o_sh + 4 * y) = uint2v(0u);
+  };
+  auto in_out = [&](int t) { return min(max(t, 0), a.tokens); };
+  const int lead = in_out(a.cu[0]), tail = in_out(a.cu[a.B]);
+  const long n = (long)(lead + a.tokens - tail) * heads, blocks = (long)gridDim.x * gridDim.y;
+  for (long i = ((long)blockIdx.y * gridDim.x + blockIdx.x) * kRows + x; i < n; i += blocks * kRows) {
+    const int t = (int)(i / heads);
+    zero(t < lead ? t : tail + t - lead, (int)(i % heads));
+  }
+  if (!own) return;
+  const int r0 = a.cu[b], r1 = a.cu[b + 1];
+  const bool fits = r0 >= 0 && r1 >= r0 && r1 <= a.tokens;
+  const int t0 = fits ? r0 + min(r1 - r0, a.max_q) : in_out(r0), t1 = fits ? r1 : in_out(r1);
+  for (int t = t0 + x; t < t1; t += kRows) zero(t, hd);
+}
+
+// joins a row's chunks: weights exp2(m_i - max m), by groups of D / 4 lanes.  T: the rows' type; LISTED: all chunks count
+// (those of a list of blocks, which may hold nothing that the row sees)
+template <int D, typename T, bool LISTED, typename Args>
+__device__ __forceinline__ void join_pieces(const Args& a) {
+  constexpr int kLanes = D / 4, kGroups = kThreads / kLanes;
+  __shared__ float s_r[kWaves];
+  __shared__ __align__(16) float s_o[kGroups][D];
+  __shared__ float s_l[kGroups];
+  const int heads = a.HKV * a.G;
+  const int hd = blockIdx.x % heads, j = blockIdx.x / heads, b = blockIdx.y;
+  const Seq sq = LISTED ? seq_of(a, b, 1L << 32) : seq_of(a, b);
+  if (a.clear) clear_rows<D>(a, b, hd, j == 0);
+  if (j >= sq.R) return;
+  const int seen = sq.n - sq.R + j + 1, tid = threadIdx.x;
+  const int nv = sq.bad || seen <= 0 ? 0 : LISTED ? a.nchunk : (seen + a.chunk - 1) / a.chunk;
+  const long row = ((long)(sq.r0 + j) * heads + hd) * a.nchunk;
+  const float* ml = a.ws_ml + row * 2;
+  const int grp = tid / kLanes, y = tid % kLanes;
+  constexpr int kAtOnce = 4;             // pieces whose loads are in flight together
+  f32x4 x[kAtOnce];
+  f32x2 w[kAtOnce];
+  auto fetch = [&](int i) {
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int at = min(i + k * kGroups, nv - 1);
+      x[k] = *reinterpret_cast<const f32x4*>(a.ws_o + (row + at) * D + 4 * y);
+      w[k] = *reinterpret_cast<const f32x2*>(ml + 2 * at);
+    }
+  };
+  if (grp < nv) fetch(grp);              // (beside the maxima: one sequence of 131072 keys 30.9 us, 32.2 after them)
+  float M = -FLT_MAX;
+  for (int i = tid; i < nv; i += kThreads) M = fmaxf(M, ml[2 * i]);
+  M = oa::wave_max(M);
+  if ((tid & 63) == 0) s_r[tid >> 6] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(s_r[0], s_r[1]), fmaxf(s_r[2], s_r[3]));
+  f32x4 o = f32x4(0.f);
+  float L = 0.f;
+  for (int i = grp; i < nv; i += kAtOnce * kGroups) {
+    if (i > grp) fetch(i);
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      if (i + k * kGroups >= nv) break;
+      const float e = __builtin_amdgcn_exp2f(w[k][0] - M);
+      L += e * w[k][1];
+      o += x[k] * e;
+    }
+  }
+  *reinterpret_cast<f32x4*>(&s_o[grp][4 * y]) = o;
+  if (y == 0) s_l[grp] = L;
+  __syncthreads();
+  if (grp) return;
+#pragma unroll
+  for (int k = 1; k < kGroups; ++k) {
+    o += *reinterpret_cast<const f32x4*>(&s_o[k][4 * y]);
+    L += s_l[k];
+  }
+  o = sq.bad ? f32x4(__builtin_nanf("")) : nv && !(LISTED && L == 0.f) ? o / L : f32x4(0.f);
+  *reinterpret_cast<uint2v*>(a.out + (long)(sq.r0 + j) * a.o_st + (long)hd * a.o_sh + 4 * y) =
+      uint2v{pack_out<T>(o[0], o[1]), pack_out<T>(o[2], o[3])};
+}
+
+}  // namespace paged

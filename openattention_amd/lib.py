@@ -1,4 +1,5 @@
-"""ctypes binding of the gfx950 kernel library (C ABI declared in include/openattention_amd.h).
+"""ctypes binding of the gfx950 kernel library (C ABI declared in include/openattention_amd.h and, for the 8-bit
+paged cache, in include/openattention_kv8.h).
 
 torch is imported first on purpose: the library links the HIP runtime that ships inside torch,
 and loading torch first makes both share that one runtime (device pointers and streams are
@@ -89,10 +90,20 @@ SIGNATURES = {
     "oa_kv4_attn": [P, L, L, P, P, P, P, L, L, I, I, P, L, I, P, P, I, I, I, I, I, I, F, I, I, P, P, P, P, L, L, I, P],
 }
 
+# the 8-bit paged cache's, in the order of include/openattention_kv8.h
+SIGNATURES_KV8 = {
+    "oa_kv8_revision": [],
+    "oa_kv8_write": [P, L, L, P, L, L, I, I, I, I, P, P, P, P, P, L, L, L, I, I, P, L, I, P, P, I, P],
+    "oa_kv8_read": [P, P, P, P, P, L, L, I, I, P, L, L, P, L, L, I, I, I, I, P],
+    "oa_kv8_select": [P, L, L, I, P, P, L, L, I, I, P, L, I, P, P, I, I, I, I, I, I, I, I, I, P, P, P],
+    "oa_kv8_attn": [P, L, L, I, P, P, P, P, L, L, I, I, P, L, I, P, P, I, I, I, I, I, I, F, P, I, I, I, P, P, P, L, L, I, P],
+}
+
 # must equal oa_abi_version() and oa_abi_revision() of the loaded library (OA_ABI_VERSION, OA_ABI_REVISION in the
 # header): a library built from sources with other argument lists would be handed wrong pointers
 ABI_VERSION = 9
 ABI_REVISION = 1
+KV8_REVISION = 1           # oa_kv8_revision(), OA_KV8_REVISION
 
 _LIB = None
 
@@ -121,7 +132,16 @@ def load() -> ct.CDLL:
     if have != ABI_REVISION:
         raise RuntimeError(f"kernel library {path} has ABI {ABI_VERSION} revision {have}, this binding expects revision "
                            f"{ABI_REVISION}: rebuild it (__graft_entry__.build())")
-    for name, argtypes in SIGNATURES.items():
+    missing = [name for name in SIGNATURES_KV8 if not hasattr(lib, name)]
+    if missing:
+        raise RuntimeError(f"kernel library {path} lacks {', '.join(missing)}: it was built from older sources, "
+                           "rebuild it (__graft_entry__.build())")
+    lib.oa_kv8_revision.restype = ct.c_int
+    have = lib.oa_kv8_revision()
+    if have != KV8_REVISION:
+        raise RuntimeError(f"kernel library {path} has revision {have} of the 8-bit cache's entry points, this binding expects "
+                           f"{KV8_REVISION}: rebuild it (__graft_entry__.build())")
+    for name, argtypes in {**SIGNATURES, **SIGNATURES_KV8}.items():
         fn = getattr(lib, name)
         fn.argtypes = argtypes
         fn.restype = {"oa_error_string": ct.c_char_p, "oa_kmeans_step_ws": ct.c_long}.get(name, ct.c_int)

@@ -7,8 +7,9 @@ Operator surface kept from the reference:
                                                                         triton_expand_decode.py:139-165
 plus one function per decode stage (index_update, qgs_prep, qgs_scan, topk_select, errorgate,
 waterfill, topq, residual, residual_flash, dense_decode) and the operators of the 4-bit paged cache
-(qk_norm_rope, kv_pages_extend, kv_pages_truncate, kv4_write, kv4_read, kv4_attn), each a thin checked
-call of the C ABI (include/openattention_amd.h) on torch's current HIP stream.  Shape, dtype, device, alignment
+(qk_norm_rope, kv_pages_extend, kv_pages_truncate, kv4_write, kv4_read, kv4_attn) and of the 8-bit one
+(kv8_write, kv8_read, kv8_select, kv8_attn), each a thin checked call of the C ABI
+(include/openattention_amd.h, include/openattention_kv8.h) on torch's current HIP stream.  Shape, dtype, device, alignment
 and stride checks happen here; the kernels trust them.  There is no CPU path: tensors must live
 on a HIP device and the kernel library must be built.
 """
@@ -1060,6 +1061,267 @@ def kv4_attn(q, kc, ks, vc, vs, table, lens, sm_scale: float | None = None, cu_q
          *ost, clear)
     return out
 
+
+# ================================================================== 8-bit paged cache
+_PAGES8 = (32, 64, 128)    # tokens of a block, which share a scale and bounds
+
+
+@_sizes
+def _kv8_sizes(kcs, kst, kct, vcs, vst, vct, kss, sst, ksdt, vss, vsst, vsdt) -> tuple:
+    """((page strides of codes and scales, pages, page), heads, head dimension) of an 8-bit cache's tensors; pages may lie
+    apart (a layer of a larger tensor)."""
+    _need(len(kcs) == 4, "kc: (pages, heads, page, D) uint8")
+    NP, HKV, page, Dh = kcs
+    _need(page in _PAGES8, f"page: 32, 64 or 128 (got {page})")
+    _need(Dh in (64, 128) and NP >= 1 and HKV >= 1 and NP * page < 1 << 31,
+          f"cache: head dimension 64 or 128 (got {Dh}), at least one page and head, fewer than 2^31 slots")
+    u8 = torch.uint8
+    _need(vcs == kcs and kss == (NP, HKV) and vss == kss and kct is u8 and ksdt is u8 and vct is u8 and vsdt is u8,
+          f"cache: codes ({NP}, {HKV}, {page}, {Dh}), scales ({NP}, {HKV}), uint8")
+    c0, s0 = (kst[0], sst[0]) if NP > 1 else (HKV * page * Dh, HKV)
+    _need((NP == 1 or vst[0] == c0 and vsst[0] == s0) and kst[1:] == vst[1:] == (page * Dh, Dh, 1) and (HKV == 1 or sst[1] == vsst[1] == 1)
+          and c0 >= HKV * page * Dh and s0 >= HKV and c0 % 16 == 0,
+          "cache: contiguous pages, those of k and v at one distance, codes' of whole 16 bytes")
+    return (c0, s0, NP, page), HKV, Dh
+
+
+@_sizes
+def _bound_sizes(shape, stride, dtype, NP, HKV, Dh) -> int:
+    """The page stride of a cache's bounds."""
+    _need(shape == (NP, HKV, 2, Dh) and dtype is torch.int8, f"kb: ({NP}, {HKV}, 2, {Dh}) int8")
+    b0 = stride[0] if NP > 1 else HKV * 2 * Dh
+    _need((HKV == 1 or stride[1] == 2 * Dh) and stride[2:] == (Dh, 1) and b0 >= HKV * 2 * Dh and b0 % 16 == 0,
+          "kb: contiguous pages, at a distance of whole 16 bytes")
+    return b0
+
+
+def _kv8_cache(kc, ks, vc, vs) -> tuple:
+    """An 8-bit cache's pointers and sizes (_kv8_sizes)."""
+    sizes = _kv8_sizes(kc.shape, kc.stride(), kc.dtype, vc.shape, vc.stride(), vc.dtype, ks.shape, ks.stride(), ks.dtype,
+                       vs.shape, vs.stride(), vs.dtype)
+    p = kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr()
+    _aligned(p[0] | p[2])
+    return p, *sizes
+
+
+@_sizes
+def _write8_sizes(HKV, Dh, page, ks, kst, kt, vs, vst, vt, ts, tst, tt, lens, cu) -> tuple:
+    _need(len(ks) == 3 and ks[1:] == (HKV, Dh) and vs == ks and kt in _DT and vt is kt and ks[0] * HKV <= 1 << 26,
+          f"k, v: (T, {HKV}, {Dh}), both bf16, fp16 or fp32, at most 2^26 rows")
+    T = ks[0]
+    tstride, B, width = _table_sizes(ts, tst, tt, page)
+    _int_vector(*lens, B, "lens")
+    if cu is not None:
+        _int_vector(*cu, B + 1, "cu")
+    else:
+        _need(T == B, "without cu every sequence adds one row")
+    _need(((T // page + 2 * B) if cu is not None else B) * HKV <= _GRID,
+          f"at most {_GRID} workgroups ((tokens / page + 2 x sequences) x heads)")
+    return (_row_strides(T, HKV, Dh, kst, kt, "k"), _row_strides(T, HKV, Dh, vst, kt, "v"), (T, HKV, Dh, _DT[kt]),
+            (tstride, width), B)
+
+
+def kv8_write(k, v, kc, ks, vc, vs, kb, table, lens, cu=None) -> None:
+    """Key and value rows (T, HKV, D) bf16, fp16 or fp32 of the newest tokens of every sequence, rounded to 8 bits in the
+    sequences' pages: tokens cu[b] .. cu[b + 1] - 1 (cu (B + 1,) int32, 0 to T, not decreasing; None: one token
+    each) are the last of the lens[b] that sequence b holds (lens (B,) int32), in the pages of its row of table
+    (B, width) int32.  Cache: kc, vc (pages, HKV, page, D) uint8 codes in e4m3, ks, vs (pages, HKV) uint8 scales s,
+    which stand for 2^(s - 127), one for a page's block of 32, 64 or 128 tokens of a head; kb (pages, HKV, 2, D) int8
+    bounds of the keys' channels, which kv8_select reads, or None.
+    A block's scale is the smallest power of two that clips nothing of it.  It starts with the write of the block's
+    first token; a later token that needs a larger one raises it, and the block's earlier codes are rounded again.  A
+    row with a value that is not finite is held as NaN.  Sequences longer than their table row, tokens of negative
+    position and pages outside of the cache are passed over.  A page that two sequences of one call write into ends as
+    some mixture."""
+    i = _where(k, v, kc, ks, vc, vs, kb, table, lens, cu)
+    ps, where, HKV, Dh = _kv8_cache(kc, ks, vc, vs)
+    b0 = 0 if kb is None else _bound_sizes(kb.shape, kb.stride(), kb.dtype, where[2], HKV, Dh)
+    kst, vst, sizes, tsz, B = _write8_sizes(HKV, Dh, where[3], k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype,
+                                            table.shape, table.stride(), table.dtype, _m(lens), _m(cu))
+    _plain(k, v)
+    kp, vp, bp = k.data_ptr(), v.data_ptr(), _ptr(kb)
+    if sizes[0]:
+        _aligned(kp | vp | (bp or 0))
+    _run(i, "oa_kv8_write", kp, *kst, vp, *vst, *sizes, *ps, bp, where[0], where[1], b0, where[2], where[3],
+         table.data_ptr(), *tsz, lens.data_ptr(), _ptr(cu), B)
+
+
+def kv8_read(slots, kc, ks, vc, vs, dtype: torch.dtype = torch.bfloat16):
+    """The values (k, v), each (T, HKV, D) bf16 (which holds them exactly) or fp32, at slots (T,) int32 = page id * page +
+    offset of an 8-bit cache; zeros for a slot outside of it."""
+    i = _where(slots, kc, ks, vc, vs)
+    ps, where, HKV, Dh = _kv8_cache(kc, ks, vc, vs)
+    T = slots.shape[0] if slots.dim() == 1 else 0
+    _int_vector(slots.shape, slots.stride(), slots.dtype, T, "slots")
+    if dtype not in (torch.bfloat16, torch.float32) or T * HKV > 1 << 26:
+        raise ValueError("dtype: bf16 or fp32; at most 2^26 rows")
+    k = kc.new_empty(T, HKV, Dh, dtype=dtype)
+    v = kc.new_empty(T, HKV, Dh, dtype=dtype)
+    _run(i, "oa_kv8_read", slots.data_ptr(), *ps, *where, k.data_ptr(), HKV * Dh, Dh, v.data_ptr(), HKV * Dh, Dh, T, HKV, Dh,
+         _DT[dtype])
+    return k, v
+
+
+@_sizes
+def _select_sizes(qs, qst, qt, ks, kst, kt, bs, bst, bt, ts, tst, tt, lens, page, n, cu, first, last, max_len) -> tuple:
+    _need(page in _PAGES8, f"page: 32, 64 or 128 (got {page})")
+    _need(len(bs) == 4 and bs[2] == 2 and bs[3] in (64, 128) and bs[0] >= 1 and bs[1] >= 1 and bs[0] * page < 1 << 31,
+          "kb: (pages, heads, 2, D) int8, head dimension 64 or 128, fewer than 2^31 slots")
+    NP, HKV, _, Dh = bs
+    b0 = _bound_sizes(bs, bst, bt, NP, HKV, Dh)
+    _need(ks == (NP, HKV) and kt is torch.uint8 and (HKV == 1 or kst[1] == 1) and (NP == 1 or kst[0] >= HKV),
+          f"ks: ({NP}, {HKV}) uint8, contiguous pages")
+    _need(len(qs) == 3 and qs[2] == Dh and qt in (torch.bfloat16, torch.float16) and qs[1] >= 1 and qs[1] % HKV == 0,
+          f"q: (T, a multiple of {HKV}, {Dh}) bf16 or fp16")
+    T, HQ, _ = qs
+    tstride, B, width = _table_sizes(ts, tst, tt, page)
+    _int_vector(*lens, B, "lens")
+    if cu is not None:
+        _int_vector(*cu, B + 1, "cu_q")
+    else:
+        _need(T == B, "without cu_q every sequence has one row of q")
+    _need(first >= 0 and last >= 1 and first + last <= n < 1 << 25, "n: at least first + last, first: not negative, last: at least 1")
+    _need(max_len is None or max_len >= 0, "max_len: not negative")
+    cap = width if max_len is None else max(1, min(width, -(-max_len // page)))
+    rows = next(x for x in (16, 8, 4, 2, 1) if x == 1 or x * (HQ // HKV) <= 16)            # tokens of a tile
+    _need(((T // rows + 2 * B) if cu is not None else B) * HKV <= _GRID and T * HKV <= _GRID and cap <= 65535 * 128,
+          f"at most {_GRID} workgroups (tokens x heads)")
+    qst = _row_strides(T, HQ, Dh, qst, qt, "q")
+    return (T, HKV, qst, _DT[qt], (kst[0] if NP > 1 else HKV, b0, NP, page), (tstride, width), (B, T, HQ, HKV, Dh, n, first, last, cap),
+            T * HKV * cap if cap > n else 0)
+
+
+def kv8_select(q, ks, kb, table, lens, page: int, n: int, cu_q=None, first: int = 1, last: int = 2, max_len: int | None = None):
+    """The blocks whose keys can score highest for every query token and KV head: (T, HKV, n) int32 block numbers (a
+    sequence's page number from 0 on), ascending, -1 behind the last.  q (T, HQ, D) bf16 or fp16; ks, kb, table, lens as
+    kv8_write leaves them; cu_q as kv8_attn takes it.  A token sees the blocks that hold a key at or before its own
+    position: all of them where they are at most n, otherwise the `first` first and the `last` last (its own among
+    them) and those of the highest scores, ties to the lower.  A block's score is
+    max over the query heads of sum_d max(q8_d, 0) hi_d + max(-q8_d, 0) nlo_d, times 2^(s - 127) (at most 2^100), with
+    q8 = rint(q / 2^u), u the smallest for which the heads' |q8| are at most 127: up to q's rounding the most that a
+    key of the block can score.  Scores are whole numbers times powers of two, and the choice is exact.  Values of q
+    that are not finite count as 0.  A block whose page id lies outside of the cache comes last.  max_len: a bound on
+    lens that the caller knows.  -1 alone: tokens that no sequence takes, and those of sequences longer than their
+    table row or than max_len (rounded up to whole pages).  A workspace of T HKV blocks integers is taken from torch's
+    allocator."""
+    i = _where(q, ks, kb, table, lens, cu_q)
+    T, HKV, qst, dt, where, tsz, sizes, scores = _select_sizes(
+        q.shape, q.stride(), q.dtype, ks.shape, ks.stride(), ks.dtype, kb.shape, kb.stride(), kb.dtype, table.shape,
+        table.stride(), table.dtype, _m(lens), index(page), index(n), _m(cu_q), index(first), index(last),
+        None if max_len is None else index(max_len))
+    _plain(q)
+    qp, bp = q.data_ptr(), kb.data_ptr()
+    if T:
+        _aligned(qp | bp)
+    out = table.new_empty(T, HKV, sizes[5])
+    ws = table.new_empty(scores) if scores else None
+    _run(i, "oa_kv8_select", qp, *qst, dt, ks.data_ptr(), bp, *where, table.data_ptr(), *tsz, lens.data_ptr(), _ptr(cu_q),
+         *sizes, _ptr(ws), out.data_ptr())
+    return out
+
+
+def kv8_chunk(cap: int, units: int, rows: int) -> int:
+    """Keys per workgroup of kv8_attn, for `units` (sequence or token, KV head, query tile) triples of up to `cap` keys and
+    `rows` query rows: as kv4_chunk."""
+    n = max(cap * units // 512, 256)
+    if rows <= 64:
+        n = max(min(n, max(cap // 8, 1024)), 256)
+    return min(-(-n // 128), -(-cap // 128)) * 128
+
+
+@_sizes
+def _attn8_sizes(HKV, Dh, where, qs, qst, qt, ts, tst, tt, lens, cu, max_q, sm_scale, blocks, max_len, o, rule) -> tuple:
+    # rule: kv8_chunk, a part of what is looked up, so that no call gets the pieces of another rule
+    c0, s0, NP, page = where
+    tstride, B, width = _table_sizes(ts, tst, tt, page)
+    _need(len(qs) == 3 and qs[2] == Dh and qt in (torch.bfloat16, torch.float16) and qs[1] >= 1 and qs[1] % HKV == 0,
+          f"q: (T, a multiple of {HKV}, {Dh}) bf16 or fp16")
+    T, HQ, _ = qs
+    G = HQ // HKV
+    _int_vector(*lens, B, "lens")
+    if cu is not None:
+        _int_vector(*cu, B + 1, "cu_q")
+    else:
+        _need(T == B and max_q == 1, "without cu_q every sequence has one row of q")
+    scale = Dh ** -0.5 if sm_scale is None else sm_scale
+    _need(1 <= max_q <= (1 << 30) // G and scale == scale and (max_len is None or max_len >= 0),
+          "max_q: at least 1; sm_scale: not NaN; max_len: not negative")
+    _need(o is None or o[0] == qs and o[2] is qt, "out: as q")
+    n = 0
+    if blocks is not None:
+        bs, bst, bt = blocks
+        _need(len(bs) == 3 and bs[:2] == (T, HKV) and bs[2] >= 1 and bs[2] * page <= 1 << 30 and bt is torch.int32
+              and _packed(bs, bst), f"blocks: ({T}, {HKV}, n) int32, contiguous")
+        n = bs[2]
+    rows = G if n else max_q * G
+    cap = n * page if n else max(1, width * page if max_len is None else min(max_len, width * page))
+    units = (T if n else B) * HKV
+    tiles = -(-rows // (8 if rows <= 8 else 16 if rows <= 16 else 32))
+    # (the join's grid holds 65535 sequences; so many need no pieces to fill the card)
+    chunk = rule(cap, units * tiles, rows) if B <= 65535 else -(-cap // 128) * 128
+    nchunk = -(-cap // chunk)
+    _need(units * tiles * nchunk <= _GRID and units * HKV < 1 << 32,
+          f"at most {_GRID} workgroups (sequences, or tokens with blocks, x heads x tiles of rows x pieces), heads^2 times those under 2^32")
+    qst, ost = _row_strides(T, HQ, Dh, qst, qt, "q"), (HQ * Dh, Dh) if o is None else _row_strides(T, HQ, Dh, o[1], qt, "out", True)
+    return (T, HQ, B, qst, ost, _DT[qt], (tstride, width), (B, T, max_q, HQ, HKV, Dh, scale), (n, chunk, nchunk),
+            T * HQ * nchunk if nchunk > 1 else 0,
+            (_rows(T, HQ, qst, 2, Dh), _rows(T, HQ, ost, 2, Dh), _rows(B, 1, (tstride, 0), 4, width), _rows(1, 1, (0, 0), 4, B),
+             _rows(1, 1, (0, 0), 4, B + 1), _rows(NP, 1, (c0, 0), 1, HKV * page * Dh), _rows(NP, 1, (s0, 0), 1, HKV),
+             _rows(1, 1, (0, 0), 4, T * HKV * n)))
+
+
+def _packed(shape, stride) -> bool:
+    """Whether a tensor of these sizes is contiguous"""
+    want = 1
+    for n, s in zip(reversed(shape), reversed(stride)):
+        if n > 1 and s != want:
+            return False
+        want *= n
+    return True
+
+
+def kv8_attn(q, kc, ks, vc, vs, table, lens, sm_scale: float | None = None, cu_q=None, max_q: int = 1, blocks=None, out=None,
+             max_len: int | None = None) -> torch.Tensor:
+    """Causal attention of the newest tokens of every sequence over an 8-bit paged cache (kv8_write).
+    q (T, HQ, D) bf16 or fp16, HQ any multiple of the cache's heads; table (B, width) int32 page ids; lens (B,) int32 keys
+    that the sequences hold, these tokens among them.  Tokens cu_q[b] .. cu_q[b + 1] - 1 (cu_q (B + 1,) int32, 0 to T, not
+    decreasing) are the last of sequence b, at most max_q of them; cu_q None: one token each.
+    Token j of R sees keys 0 .. lens[b] - R + j; one that sees none gives 0.  blocks (T, HKV, n) int32: a token's rows
+    of a KV head see of these the keys in the blocks listed for them alone (kv8_select; in any order, each once; numbers
+    under 0 and those of blocks that the token does not see name nothing).  max_len: a bound on lens that the caller knows
+    (the table's width otherwise; with blocks it is not used).  NaN: rows that need a page id outside of the cache, and
+    those of sequences longer than their table row or than max_len (rounded up to whole pieces, kv8_chunk).  Rows of `out`
+    that no sequence takes, and tokens past max_q, are left as they were (0 where the call makes it); `out` shares no
+    memory with the other tensors.  Sums are held in fp32 and not divided before their end: values up to 2^80 are safe at
+    any length."""
+    i = _where(q, kc, ks, vc, vs, table, lens, cu_q, blocks, out)
+    ps, where, HKV, Dh = _kv8_cache(kc, ks, vc, vs)
+    T, HQ, B, qst, ost, dt, tsz, sizes, pieces, parts, lie = _attn8_sizes(
+        HKV, Dh, where, q.shape, q.stride(), q.dtype, table.shape, table.stride(), table.dtype, _m(lens), _m(cu_q),
+        index(max_q), None if sm_scale is None else float(sm_scale), _m(blocks),
+        None if max_len is None else index(max_len), _m(out), kv8_chunk)
+    _plain(q, out)
+    qp = q.data_ptr()
+    given = out is not None
+    clear = out is None and cu_q is not None and parts > 0 and B > 0     # (by the join)
+    if out is None:
+        out = q.new_empty(T, HQ, Dh) if clear or cu_q is None else q.new_zeros(T, HQ, Dh)
+    op = out.data_ptr()
+    if T == 0 or B == 0:
+        return out
+    _aligned(qp | op)
+    if given:
+        lq, lo, lt, ll, lc, lw, ls, lb = lie
+        _apart("out", op, lo, (qp, lq), (table.data_ptr(), lt), (lens.data_ptr(), ll), (_ptr(cu_q) or 0, lc), (ps[0], lw), (ps[1], ls),
+               (ps[2], lw), (ps[3], ls), (_ptr(blocks) or 0, lb))
+    wp = mp = None
+    if parts:
+        ws = q.new_empty(parts * (Dh + 2), dtype=torch.float32)
+        wp = ws.data_ptr()
+        mp = wp + 4 * parts * Dh
+    _run(i, "oa_kv8_attn", qp, *qst, dt, *ps, *where, table.data_ptr(), *tsz, lens.data_ptr(), _ptr(cu_q), *sizes, _ptr(blocks),
+         *pieces, wp, mp, op, *ost, clear)
+    return out
 
 # ================================================================== prefill index build
 def qgs_codes(K, T: int, U, codes, scale, amax_ws, zc_ws=None) -> None:

@@ -1,0 +1,215 @@
+"""What the operators of the 8-bit paged cache refuse on the host, before anything is launched, and what they hand to
+the library (CPU tensors stand in for device ones; the launch is recorded instead)."""
+import re
+import subprocess
+
+import pytest
+import torch
+
+from openattention_amd import _build, lib, ops
+
+BF = torch.bfloat16
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    got = []
+    monkeypatch.setattr(ops, "_where", lambda *ts: 0)
+    monkeypatch.setattr(ops, "_run", lambda i, name, *a: got.append((name, a)))
+    return got
+
+
+def z(*s, dtype=torch.uint8):
+    return torch.zeros(*s, dtype=dtype)
+
+
+def i32(*s):
+    return z(*s, dtype=torch.int32)
+
+
+def cache(NP=4, H=2, page=32, D=128, **kw):
+    a = dict(kc=z(NP, H, page, D), ks=z(NP, H), vc=z(NP, H, page, D), vs=z(NP, H))
+    a.update(kw)
+    return a
+
+
+def bounds(NP=4, H=2, D=128):
+    return z(NP, H, 2, D, dtype=torch.int8)
+
+
+BAD = [cache(D=96), cache(D=256), cache(page=16), cache(page=48), cache(page=256), cache(NP=0), cache(H=0),
+       cache(kc=z(4, 2, 32, 128, dtype=torch.int8)), cache(kc=z(4, 2, 32, 128).float()), cache(vc=z(4, 2, 64, 128)),
+       cache(ks=z(4, 2, 1)), cache(ks=z(4, 3)), cache(vs=z(4, 2, dtype=torch.int8)), cache(ks=z(2, 4).t(), vs=z(2, 4).t()),
+       cache(kc=z(4, 32, 2, 128).transpose(1, 2)), cache(vc=z(4, 3, 2, 32, 128)[:, 1]), cache(vs=z(4, 3, 2)[:, 1]),
+       cache(kc=z(1, 2, 32, 128).expand(4, 2, 32, 128), vc=z(1, 2, 32, 128).expand(4, 2, 32, 128)),
+       cache(kc=z(4 * 8192 + 16)[1:32769].view(4, 2, 32, 128)), cache(kc=z(4, 8200)[:, :8192].view(4, 2, 32, 128), vc=z(4, 8200)[:, :8192].view(4, 2, 32, 128))]
+
+
+@pytest.mark.parametrize("bad", range(len(BAD)))
+def test_cache_tensors_refused(calls, bad):
+    c = BAD[bad]
+    k, n = z(3, 2, 128, dtype=BF), i32(3)
+    with pytest.raises(ValueError):
+        ops.kv8_write(k, k, **c, kb=bounds(), table=i32(3, 2), lens=n)
+    with pytest.raises(ValueError):
+        ops.kv8_read(n, **c)
+    with pytest.raises(ValueError):
+        ops.kv8_attn(z(3, 8, 128, dtype=BF), **c, table=i32(3, 2), lens=n)
+    assert not calls
+
+
+def test_writes_refused(calls):
+    c = cache()
+    k, t, n = z(3, 2, 128, dtype=BF), i32(3, 2), i32(3)
+    ok = dict(k=k, v=k, kb=bounds(), table=t, lens=n)
+    for bad in (dict(k=k[:, :1]), dict(v=k.float()), dict(v=k[:2]), dict(k=k[0], v=k[0]), dict(k=k.to(torch.int16), v=k.to(torch.int16)),
+                dict(v=k.clone().requires_grad_()), dict(k=z(3, 2, 129, dtype=BF)[..., 1:]), dict(v=z(3, 2, 132, dtype=BF)[..., :128]),
+                dict(table=t.long()), dict(table=t[0]), dict(table=i32(2, 3).t()), dict(table=t[:, :0]), dict(lens=n.long()), dict(lens=n[:2]),
+                dict(cu=i32(3)), dict(cu=i32(4).long()), dict(cu=i32(8)[::2]), dict(table=i32(2, 2), lens=i32(2)), dict(kb=bounds(H=3)), dict(kb=bounds().to(torch.uint8)),
+                dict(kb=bounds(D=64)), dict(kb=z(4, 2, 128, 2, dtype=torch.int8).transpose(2, 3)), dict(kb=z(4, 600, dtype=torch.int8)[:, 1:513].view(4, 2, 2, 128)),
+                dict(kb=z(2049, dtype=torch.int8)[1:].view(4, 2, 2, 128)), dict(kb=z(1, 2, 2, 128, dtype=torch.int8).expand(4, 2, 2, 128))):
+        with pytest.raises(ValueError):
+            ops.kv8_write(**dict(ok, **bad), **c)
+    for s, dt in ((n.long(), BF), (n[None], BF), (n, torch.float16), (i32(6)[::2], torch.float32)):
+        with pytest.raises(ValueError):
+            ops.kv8_read(s, **c, dtype=dt)
+    assert not calls
+    ops.kv8_write(**ok, **c)
+    ops.kv8_write(**dict(ok, kb=None, cu=i32(4)), **c)
+    ops.kv8_read(n, **c)
+    # layers of one tensor: pages 3 layers apart
+    big = [z(4, 3, *s)[:, 1] for s in ((2, 32, 128), (2,), (2, 32, 128), (2,))]
+    ops.kv8_write(k, k, *big, z(4, 3, 2, 2, 128, dtype=torch.int8)[:, 2], t, n)
+    for name, a in calls:
+        assert len(a) + 1 == len(lib.SIGNATURES_KV8[name])
+    assert calls[1][1][14] is None and calls[3][1][15:20] == (3 * 8192, 6, 3 * 512, 4, 32)
+
+
+def test_selections_refused(calls):
+    q, t, n = z(3, 8, 128, dtype=BF), i32(3, 9), i32(3)
+    ok = dict(q=q, ks=z(4, 2), kb=bounds(), table=t, lens=n, page=32, n=4)
+    for bad in (dict(q=q.float()), dict(q=q[:, :7]), dict(q=q[..., :64]), dict(q=q[0]), dict(q=q[:2]), dict(q=q[:, :0]), dict(q=q.clone().requires_grad_()),
+                dict(q=z(3, 8, 136, dtype=BF)[..., 4:132]), dict(ks=z(4, 3)), dict(ks=z(4, 2, dtype=torch.int8)), dict(ks=z(1, 2).expand(4, 2)), dict(kb=bounds(D=96)),
+                dict(kb=bounds().to(torch.uint8)), dict(kb=bounds()[:, :, 0]), dict(kb=z(4, 3, 2, 2, 128, dtype=torch.int8)[:, :, 1]), dict(table=t.long()), dict(table=t[:2]),
+                dict(lens=n[:2]), dict(page=48), dict(page=256), dict(n=0), dict(n=2), dict(first=-1), dict(last=0), dict(first=3), dict(n=1 << 25), dict(max_len=-1),
+                dict(cu_q=i32(3)), dict(cu_q=i32(4).long())):
+        with pytest.raises(ValueError):
+            ops.kv8_select(**dict(ok, **bad))
+    with pytest.raises(TypeError):
+        ops.kv8_select(**dict(ok, n=4.0))
+    assert not calls
+    assert ops.kv8_select(**ok).shape == (3, 2, 4)
+    ops.kv8_select(**dict(ok, cu_q=i32(4), max_len=70, n=3, q=z(5, 8, 128, dtype=torch.float16)))
+    ops.kv8_select(**dict(ok, n=9))
+    for name, a in calls:
+        assert len(a) + 1 == len(lib.SIGNATURES_KV8[name])
+    # blocks, from the table's width or max_len; no scratch where all are chosen
+    assert calls[0][1][-3] == 9 and calls[0][1][-2] is not None and calls[1][1][-3] == 3 and calls[1][1][-2] is None and calls[2][1][-2] is None
+
+
+def test_attention_refused(calls):
+    c = cache()
+    q, t, n, cu = z(3, 8, 128, dtype=BF), i32(3, 2), i32(3), i32(4)
+    ok = dict(q=q, table=t, lens=n)
+    for bad in (dict(q=q.float()), dict(q=q[:, :7]), dict(q=q[..., :64]), dict(q=q[0]), dict(q=q[:2]), dict(q=q[:, :0]),
+                dict(q=z(3, 8, 136, dtype=BF)[..., 4:132]), dict(q=q.clone().requires_grad_()), dict(table=t.long()), dict(table=t[0]),
+                dict(table=i32(2, 3).t()), dict(table=t[:, :0]), dict(lens=n.long()), dict(lens=n[:2]), dict(cu_q=cu.long()), dict(cu_q=cu[:3]),
+                dict(max_q=2), dict(cu_q=cu, max_q=0), dict(cu_q=cu, max_q=-1), dict(sm_scale=float("nan")), dict(max_len=-1), dict(out=q.half()),
+                dict(out=q[:2]), dict(out=q), dict(out=z(3, 1, 128, dtype=BF).expand(3, 8, 128)), dict(cu_q=cu, max_q=1 << 30),
+                dict(blocks=i32(3, 2)), dict(blocks=i32(3, 2, 0)), dict(blocks=i32(3, 1, 4)), dict(blocks=i32(2, 2, 4)), dict(blocks=i32(3, 2, 4).long()),
+                dict(blocks=i32(3, 2, 8)[..., ::2]), dict(blocks=i32(2, 3, 4).transpose(0, 1)), dict(blocks=i32(3, 2, 1).expand(3, 2, 4))):
+        with pytest.raises(ValueError):
+            ops.kv8_attn(**dict(ok, **bad), **c)
+    with pytest.raises(TypeError):
+        ops.kv8_attn(**ok, **c, cu_q=cu, max_q=2.0)
+    assert not calls
+    ops.kv8_attn(**ok, **c)
+    ops.kv8_attn(**dict(ok, q=q.half()), **c, cu_q=cu, max_q=5, max_len=4000)
+    ops.kv8_attn(**ok, **c, blocks=i32(3, 2, 5))
+    for name, a in calls:
+        assert len(a) + 1 == len(lib.SIGNATURES_KV8[name])
+    assert calls[0][1][3] == 0 and calls[1][1][3] == 1
+    # an output over what the call reads
+    held = z(4 * 8192 * 4)
+    kc = held[:32768].view(4, 2, 32, 128)
+    for out in (held[32752:32752 + 6144].view(BF).view(3, 8, 128), held[:6144].view(BF).view(3, 8, 128)):
+        with pytest.raises(ValueError, match="shares? memory"):
+            ops.kv8_attn(**ok, **dict(c, kc=kc), out=out)
+    blocks = i32(3 * 2 * 2000).view(3, 2, 2000)
+    with pytest.raises(ValueError, match="shares? memory"):
+        ops.kv8_attn(**ok, **c, blocks=blocks, out=blocks.view(-1)[-1536:].view(BF).view(3, 8, 128))
+
+
+def test_forward_tangents_refused(calls):
+    from torch.autograd import forward_ad as fw
+    c = cache()
+    q, k, s, t = z(3, 8, 128, dtype=BF), z(3, 2, 128, dtype=BF), i32(3), i32(3, 2)
+    with fw.dual_level():
+        dq, dk = fw.make_dual(q, torch.ones_like(q)), fw.make_dual(k, torch.ones_like(k))
+        for call in (lambda: ops.kv8_attn(dq, table=t, lens=s, **c), lambda: ops.kv8_write(k, dk, **c, kb=None, table=t, lens=s),
+                     lambda: ops.kv8_select(dq, c["ks"], bounds(), t, s, 32, 4)):
+            with pytest.raises(ValueError):
+                call()
+    assert not calls
+
+
+def test_tensors_on_the_host():
+    c = cache()
+    with pytest.raises(RuntimeError, match="HIP device"):
+        ops.kv8_read(i32(3), **c)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        ops.kv8_select(z(3, 8, 128, dtype=BF), c["ks"], bounds(), i32(3, 2), i32(3), 32, 4)
+
+
+def test_library_refuses_before_a_launch():
+    """The C entry points' own checks (no device is touched)."""
+    L = lib.load()
+    assert L.oa_kv8_revision() == lib.KV8_REVISION
+    wr = [16, 256, 128, 16, 256, 128, 3, 2, 128, 0, 16, 16, 16, 16, 16, 8192, 2, 512, 4, 32, 16, 2, 2, 16, None, 3, None]
+    for i, v in ((0, 8), (1, 4), (6, -1), (7, 0), (8, 96), (9, 3), (10, None), (10, 8), (11, None), (15, 8176), (15, 8200), (16, 1), (17, 500), (18, 0), (19, 16),
+                 (19, 256), (20, None), (21, 1), (22, 0), (22, 1 << 26), (23, None), (25, 2), (25, -1), (6, 1 << 26)):
+        assert L.oa_kv8_write(*wr[:i], v, *wr[i + 1:]) == -22, (i, v)
+    assert L.oa_kv8_write(*wr[:6], 0, *wr[7:25], 0, None) == 0
+    rd = [16, 16, 16, 16, 16, 8192, 2, 4, 32, 16, 256, 128, 16, 256, 128, 3, 2, 128, 0, None]
+    assert L.oa_kv8_read(*rd[:18], 1, None) == -22 and L.oa_kv8_read(None, *rd[1:]) == -22
+    se = [16, 1024, 128, 0, 16, 16, 2, 512, 4, 32, 16, 9, 9, 16, None, 3, 3, 8, 2, 128, 4, 1, 2, 9, 16, 16, None]
+    for i, v in ((0, 8), (1, 4), (3, 2), (4, None), (5, 8), (6, 1), (7, 500), (7, 520), (8, 0), (9, 16), (10, None), (11, 8), (12, 0), (13, None), (15, 2), (17, 7),
+                 (18, 0), (19, 96), (20, 2), (21, -1), (22, 0), (23, 0), (23, 10), (24, None), (25, None), (25, 2)):
+        assert L.oa_kv8_select(*se[:i], v, *se[i + 1:]) == -22, (i, v)
+    assert L.oa_kv8_select(*se[:15], 0, 0, *se[17:]) == 0
+    at = [16, 1024, 128, 0, 16, 16, 16, 16, 8192, 2, 4, 32, 16, 2, 2, 16, None, 3, 3, 1, 8, 2, 128, 0.1, None, 0, 128, 2, 16, 16, 32, 1024, 128, 0, None]
+    for i, v in ((0, 8), (1, 4), (3, 2), (4, 8), (5, None), (8, 8000), (9, 1), (10, 0), (11, 31), (11, 256), (12, None), (13, 1), (14, 0), (15, None), (17, 2), (19, 0),
+                 (19, 2), (20, 7), (21, 0), (22, 96), (23, float("nan")), (26, 64), (26, 200), (27, 0), (28, None), (29, None), (30, None), (31, 2), (30, 16),
+                 (26, 1 << 30), (27, 1 << 24)):
+        assert L.oa_kv8_attn(*at[:i], v, *at[i + 1:]) == -22, (i, v)
+    for blocks, n in ((16, 0), (16, -1), (16, 9), (2, 4), (16, 1 << 26)):                  # (two pieces of 128 hold 8 blocks of 32)
+        assert L.oa_kv8_attn(*at[:24], blocks, n, *at[26:]) == -22
+    assert L.oa_kv8_attn(*at[:17], 0, 0, *at[19:]) == 0
+
+
+def test_binding_matches_header():
+    import os
+    path = os.path.join(os.path.dirname(_build.HERE), "include", "openattention_kv8.h")
+    text = re.sub(r"/\*.*?\*/", "", open(path).read(), flags=re.S)
+    assert f"OA_KV8_REVISION {lib.KV8_REVISION}\n" in text
+    found = {}
+    for name, args in re.findall(r"int (oa_kv8_\w+)\(([^;]*)\);", text, re.S):
+        args = [a.strip() for a in args.split(",") if a.strip() != "void"]
+        found[name] = [lib.P if "*" in a else lib.L if a.startswith("long") else lib.F if a.startswith("float") else lib.I for a in args]
+    assert found == lib.SIGNATURES_KV8
+    out = subprocess.run(["nm", "-D", "--defined-only", _build.lib_path()], capture_output=True, text=True, check=True).stdout
+    assert set(found) <= set(re.findall(r"\bT (oa_[a-z0-9_]+)", out))
+
+
+@pytest.mark.parametrize("lacks,want", [("oa_kv8_attn", "lacks oa_kv8_attn"), (None, "revision 99 of the 8-bit")])
+def test_a_library_of_other_entry_points_is_refused(lacks, want, tmp_path, monkeypatch):
+    answers = {"oa_abi_version": lib.ABI_VERSION, "oa_abi_revision": lib.ABI_REVISION, "oa_kv8_revision": 99}
+    names = [n for n in (*lib.SIGNATURES, *lib.SIGNATURES_KV8) if n != lacks]
+    src, so = tmp_path / "old.c", tmp_path / "old.so"
+    src.write_text("".join(f"int {n}(void) {{ return {answers.get(n, 0)}; }}\n" for n in names))
+    subprocess.run(["gcc", "-shared", "-fPIC", "-o", str(so), str(src)], check=True)
+    monkeypatch.setattr(_build, "lib_path", lambda: str(so))
+    monkeypatch.setattr(lib, "_LIB", None)
+    with pytest.raises(RuntimeError, match=want) as e:
+        lib.load()
+    assert "rebuild it" in str(e.value)
