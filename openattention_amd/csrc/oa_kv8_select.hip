@@ -7,11 +7,16 @@
 // 2^100 taken as 2^100), so that a score has one value whatever the order of its sums, and the choice (ties: the
 // lower block) is exact.
 //
-// The first kernel forms the scores by v_mfma_i32_16x16x64_i8: 16 query rows (a token's heads, padded to a power of
-// two by repeating the last; several tokens where heads are few) against 16 blocks, both sides as [max(x, 0),
-// max(-x, 0)].  A lane ends with the scores of one block for four rows, so that the largest over four heads takes no
-// exchange.  The second takes a row's scores as integers of the same order, finds the last one that is chosen by four
-// passes over its bytes, counted in LDS, and writes the chosen blocks in ascending order.
+// Scores come from v_mfma_i32_16x16x64_i8: 16 query rows (a token's heads, padded to a power of two by repeating the
+// last; several tokens where heads are few) against 16 blocks, both sides as [max(x, 0), max(-x, 0)].  A lane ends with
+// the scores of one block for four rows, so that the largest over four heads takes no exchange.  They are kept as
+// integers of the same order.
+//   up to 1024 blocks  one launch: a workgroup scores all blocks of a tile's tokens into LDS, then a wave chooses for a
+//                      token (choose);
+//   more               scores into a workspace by as many workgroups as there are spans of 128 blocks, then a
+//                      workgroup for each token and head finds the last score that is chosen by four passes over its
+//                      bytes, counted in LDS.
+// Either writes the chosen blocks in ascending order.
 #include "oa_kv8.h"
 
 namespace {
@@ -68,39 +73,19 @@ __device__ __forceinline__ unsigned max_heads(unsigned v) {        // over GP la
   return max(y[0], y[1]);
 }
 
-__device__ __forceinline__ float finite(float x) { return (__float_as_uint(x) & 0x7fffffffu) < 0x7f800000u ? x : 0.f; }
-
 // scores as integers of the same order
 __device__ __forceinline__ unsigned key_of(float f) {
   const unsigned u = __float_as_uint(f);
   return u ^ ((int)u < 0 ? 0xffffffffu : 0x80000000u);
 }
 
-// GP: rows of a token in a tile, the heads rounded up to a power of two
+// The tile's query rows as operands: lane (row, g) holds dims 16 g and on of each 64, their positive parts first.  GP:
+// rows of a token in a tile, the heads rounded up to a power of two.
 template <typename T, int D, int GP>
-__global__ void __launch_bounds__(kThreads) kv8_score_kernel(SelectArgs a) {
-  constexpr int kTokens = 16 / GP, kPieces = D / 64, kSteps = 2 * kPieces;
+__device__ __forceinline__ void query_rows(const SelectArgs& a, const Seq& sq, int j0, int h, int4v (&Q)[D / 32]) {
+  constexpr int kPieces = D / 64;
   typedef std::conditional_t<std::is_same<T, __bf16>::value, bf16x8, f16x8> vec;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
-  const int h = blockIdx.x % a.HKV, id = blockIdx.x / a.HKV;
-  const int b = a.cu ? sequence_of(a.B, id, [&](int i) { return a.cu[i] / kTokens + 2 * i; }) : id;
-  const Seq sq = seq_of(a, b);
-  const int j0 = a.cu ? (id - (sq.r0 / kTokens + 2 * b)) * kTokens : 0;
-  if (j0 < 0 || j0 >= sq.R) return;
-  const int pos = sq.n - sq.R + min(j0 + kTokens, sq.R) - 1, seen = pos < 0 ? 0 : (pos >> a.lp) + 1;
-  const int from = blockIdx.y * kSpan;
-  if (seen <= a.n || from >= seen) return;               // (all blocks are chosen, or none are here)
-
-  // this wave's blocks: two tiles of 16
-  const int* trow = a.table + (long)b * a.t_st;
-  int at[2];
-  unsigned page[2];
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    at[x] = from + (wave + x * kWaves) * 16 + col;
-    page[x] = (unsigned)trow[min(at[x], a.width - 1)];
-  }
-  // this lane's row: dims 16 g and on of each 64
+  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int row = min(j0 + col / GP, sq.R - 1), hd = col % GP;
   const T* const q = (const T*)a.q + (long)(sq.r0 + row) * a.q_st + (long)h * a.G * a.q_sh + 16 * g;
   f32x8 x[kPieces][2];
@@ -112,68 +97,268 @@ __global__ void __launch_bounds__(kThreads) kv8_score_kernel(SelectArgs a) {
       for (int y = 0; y < 2; ++y) {
         x[p][y] = __builtin_convertvector(*reinterpret_cast<const vec*>(q + (long)head * a.q_sh + 64 * p + 8 * y), f32x8);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[p][y][i] = finite(x[p][y][i]);
-          top = max(top, __float_as_uint(x[p][y][i]) & 0x7fffffffu);
-        }
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[p][y][i]) & 0x7fffffffu);
       }
   };
-  for (int i = hd; i < a.G; i += GP) fetch(i);           // (the scale is that of all heads)
+  auto finite = [&] {                    // values that are not count as 0
+    top = 0;
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const unsigned u = __float_as_uint(x[p][i >> 3][i & 7]) & 0x7fffffffu;
+        if (u >= 0x7f800000u) x[p][i >> 3][i & 7] = 0.f;
+        else top = max(top, u);
+      }
+  };
+  unsigned others = 0;
+  if (GP == 16)                          // (more heads than rows: the scale is that of all of them)
+    for (int i = hd + (a.head0 ? 0 : 16); i < a.G; i += 16) {
+      fetch(i);
+      if (__any(top >= 0x7f800000u)) finite();
+      others = max(others, top);
+      top = 0;
+    }
   fetch(min(a.head0 + hd, a.G - 1));
-  top = max_heads<GP>(top);
-  // the smallest u with top <= 127 2^u
+  if (__any(top >= 0x7f800000u)) finite();
+  top = max_heads<GP>(max(top, others));
+  // the smallest u with top <= 127 2^u; q / 2^u rounded in the sum with 1.5 * 2^23, whose low byte is then the number
   const float f = power(-max((int)((top + 0x1ffffu) >> 23) - 133, -120));
-  int4v Q[kSteps];
 #pragma unroll
   for (int p = 0; p < kPieces; ++p)
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      unsigned plus = 0, minus = 0;
+      unsigned k[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int k = (int)rintf(x[p][w >> 1][4 * (w & 1) + i] * f);
-        plus |= (unsigned)max(k, 0) << (8 * i);
-        minus |= (unsigned)max(-k, 0) << (8 * i);
-      }
-      Q[p][w] = (int)plus;
-      Q[kPieces + p][w] = (int)minus;
+      for (int i = 0; i < 4; ++i) k[i] = __float_as_uint(fmaf(x[p][w >> 1][4 * (w & 1) + i], f, 12582912.f));
+      const unsigned b = __builtin_amdgcn_perm(__builtin_amdgcn_perm(k[3], k[2], 0x0c0c0400u), __builtin_amdgcn_perm(k[1], k[0], 0x0c0c0400u), 0x05040100u);
+      const unsigned sign = b >> 7 & 0x01010101u, mask = (sign << 8) - sign;             // (bytes of negative numbers)
+      Q[p][w] = (int)(b & ~mask);
+      Q[kPieces + p][w] = (int)((~b & mask) + sign);
     }
+}
 
+// a lane's part of 16 blocks' bounds: block lane % 16, bytes 16 g and on of each 64; and its scale
+template <int D>
+struct Bounds {
+  int4v b[D / 32];
+  unsigned s;
+  bool bad;
+};
+template <int D>
+__device__ __forceinline__ void fetch_bounds(const SelectArgs& a, Bounds<D>& t, unsigned page, int h) {
+  t.bad = page >= (unsigned)a.NP;
+  const long pg = t.bad ? 0 : page;
+  const int4v* kb = reinterpret_cast<const int4v*>(a.kb + pg * a.b_sp + (long)h * (2 * D) + 16 * ((threadIdx.x & 63) >> 4));
+  t.s = a.ks[pg * a.s_sp + h];
+#pragma unroll
+  for (int s = 0; s < D / 32; ++s) t.b[s] = kb[4 * s];
+}
+
+// The scores of the tile's tokens for this lane's block, as integers of the same order, given to put(token of the tile,
+// key).
+template <int D, int GP, typename Put>
+__device__ __forceinline__ void score_tile(const int4v (&Q)[D / 32], const Bounds<D>& t, Put put) {
+  const int g = (threadIdx.x & 63) >> 4;
+  int4v S = int4v(0);
+#pragma unroll
+  for (int s = 0; s < D / 32; ++s) S = __builtin_amdgcn_mfma_i32_16x16x64_i8(Q[s], t.b[s], S, 0, 0, 0);
+  // S[i]: row 4 g + i, this lane's block
+  int best[4] = {S[0], S[1], S[2], S[3]};
+  constexpr int kOut = GP == 1 ? 4 : GP == 2 ? 2 : 1;
+  if (GP == 2) {
+    best[0] = max(S[0], S[1]);
+    best[1] = max(S[2], S[3]);
+  } else if (GP >= 4) {
+    best[0] = max(max(S[0], S[1]), max(S[2], S[3]));
+    if (GP >= 8) {
+      const auto y = __builtin_amdgcn_permlane16_swap((unsigned)best[0], (unsigned)best[0], false, false);
+      best[0] = max((int)y[0], (int)y[1]);
+    }
+    if (GP >= 16) {
+      const auto y = __builtin_amdgcn_permlane32_swap((unsigned)best[0], (unsigned)best[0], false, false);
+      best[0] = max((int)y[0], (int)y[1]);
+    }
+  }
+  const int tok = GP <= 4 ? g * kOut : GP == 8 ? g >> 1 : 0;       // the first token of the tile that this lane holds
+  if ((GP == 8 && (g & 1)) || (GP == 16 && g)) return;
+  const float f = power(min((int)t.s - 127, 100));
+#pragma unroll
+  for (int i = 0; i < kOut; ++i) put(tok + i, key_of(t.bad ? -3.4028234e38f : (float)best[i] * f));
+}
+
+// scores of kSpan blocks for a tile's tokens into ws
+template <typename T, int D, int GP>
+__global__ void __launch_bounds__(kThreads) kv8_score_kernel(SelectArgs a) {
+  constexpr int kTokens = 16 / GP;
+  const int wave = threadIdx.x >> 6, col = threadIdx.x & 15;
+  const int h = blockIdx.x % a.HKV, id = blockIdx.x / a.HKV;
+  const int b = a.cu ? sequence_of(a.B, id, [&](int i) { return a.cu[i] / kTokens + 2 * i; }) : id;
+  const int from = blockIdx.y * kSpan;
+  // this wave's blocks: two tiles of 16
+  const int* trow = a.table + (long)b * a.t_st;
+  int at[2];
+  unsigned page[2];
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
-    const bool bad = page[x] >= (unsigned)a.NP;
-    const long pg = bad ? 0 : page[x];
-    const int4v* kb = reinterpret_cast<const int4v*>(a.kb + pg * a.b_sp + (long)h * (2 * D) + 16 * g);
-    const int e = min((int)a.ks[pg * a.s_sp + h] - 127, 100);
-    int4v S = int4v(0);
+    at[x] = from + (wave + x * kWaves) * 16 + col;
+    page[x] = (unsigned)trow[min(at[x], a.width - 1)];
+  }
+  const Seq sq = seq_of(a, b);
+  const int j0 = a.cu ? (id - (sq.r0 / kTokens + 2 * b)) * kTokens : 0;
+  if (j0 < 0 || j0 >= sq.R) return;
+  const int pos = sq.n - sq.R + min(j0 + kTokens, sq.R) - 1, seen = pos < 0 ? 0 : (pos >> a.lp) + 1;
+  if (seen <= a.n || from >= seen) return;               // (all blocks are chosen, or none are here)
+  Bounds<D> t[2];
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) S = __builtin_amdgcn_mfma_i32_16x16x64_i8(Q[s], kb[4 * s], S, 0, 0, 0);
-    // S[i]: row 4 g + i, this lane's block
-    int best[4] = {S[0], S[1], S[2], S[3]};
-    constexpr int kOut = GP == 1 ? 4 : GP == 2 ? 2 : 1;
-    if (GP == 2) {
-      best[0] = max(S[0], S[1]);
-      best[1] = max(S[2], S[3]);
-    } else if (GP >= 4) {
-      best[0] = max(max(S[0], S[1]), max(S[2], S[3]));
-      if (GP >= 8) {
-        const auto y = __builtin_amdgcn_permlane16_swap((unsigned)best[0], (unsigned)best[0], false, false);
-        best[0] = max((int)y[0], (int)y[1]);
-      }
-      if (GP >= 16) {
-        const auto y = __builtin_amdgcn_permlane32_swap((unsigned)best[0], (unsigned)best[0], false, false);
-        best[0] = max((int)y[0], (int)y[1]);
-      }
-    }
-    const int tok = GP <= 4 ? g * kOut : GP == 8 ? g >> 1 : 0;       // the first token of the tile that this lane holds
-    if ((GP == 8 && (g & 1)) || (GP == 16 && g)) continue;
+  for (int x = 0; x < 2; ++x) fetch_bounds(a, t[x], page[x], h);
+  int4v Q[D / 32];
+  query_rows<T, D, GP>(a, sq, j0, h, Q);
 #pragma unroll
-    for (int i = 0; i < kOut; ++i) {
-      if (at[x] >= seen || j0 + tok + i >= sq.R) continue;
-      unsigned* const to = a.ws + ((long)(sq.r0 + j0 + tok + i) * a.HKV + h) * a.cap + at[x];
-      const unsigned key = key_of(bad ? -3.4028234e38f : (float)best[i] * power(e));
+  for (int x = 0; x < 2; ++x)
+    score_tile<D, GP>(Q, t[x], [&](int tok, unsigned key) {
+      if (at[x] >= seen || j0 + tok >= sq.R) return;
+      unsigned* const to = a.ws + ((long)(sq.r0 + j0 + tok) * a.HKV + h) * a.cap + at[x];
       *to = a.head0 ? max(*to, key) : key;
+    });
+}
+
+// A row's choice by one wave, from scores in registers: lane l holds blocks l + 64 k, all ones for those that are chosen
+// whatever they score and 0 for none; `want` of them in all.  The score of the last one chosen by bisection over the
+// bits in which the scores differ, until as many as wanted are at or above it: some 12 steps for 512 blocks, each a
+// comparison and a count of lanes for 64 blocks.
+template <int N>
+__device__ __forceinline__ void choose(const unsigned (&key)[N], int want, int* out) {
+  unsigned most = 0, least = ~0u;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    most = max(most, key[k] == ~0u ? 0u : key[k]);
+    least = min(least, key[k] ? key[k] : ~0u);
+  }
+  most = (unsigned)__builtin_amdgcn_readfirstlane((int)max_heads<16>(most));
+  least = ~(unsigned)__builtin_amdgcn_readfirstlane((int)max_heads<16>(~least));
+  const auto count = [&](unsigned x) {
+    int c = 0;
+#pragma unroll
+    for (int k = 0; k < N; ++k) c += __popcll(__ballot(key[k] >= x));
+    return c;
+  };
+  // have: at least `want` are at or above it, and no more once `exact`.  (Where the ones chosen whatever they score are
+  // all that is wanted, no bit is taken below the first that lies above every other score.)
+  const unsigned differ = most ^ least;
+  const int bits = differ ? 32 - __builtin_clz(differ) : 0;
+  unsigned have = bits >= 32 ? 0 : most >> bits << bits;
+  bool exact = false;
+  if (count(most + 1) == want) {
+    have = most + 1;
+    exact = true;
+  }
+  for (int bit = bits - 1; bit >= 0 && !exact; --bit) {
+    const unsigned x = have | 1u << bit;
+    const int c = count(x);
+    if (c >= want) {
+      have = x;
+      exact = c == want;
     }
+  }
+  const int lane = threadIdx.x & 63;
+  const auto before = [](unsigned long m, int at) {        // at + the lanes of m before this one
+    return (int)__builtin_amdgcn_mbcnt_hi((unsigned)(m >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)m, (unsigned)at));
+  };
+  int at = 0;
+  if (exact) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const unsigned long m = __ballot(key[k] >= have);
+      const int to = before(m, at);
+      if (key[k] >= have) out[to] = lane + 64 * k;
+      at += __popcll(m);
+    }
+    return;
+  }
+  int left = want - count(have + 1);     // of those that equal it, the lowest
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const unsigned long tie = __ballot(key[k] == have);
+    const bool take = key[k] > have || (key[k] == have && before(tie, 0) < left);
+    left = max(left - (int)__popcll(tie), 0);
+    const unsigned long m = __ballot(take);
+    const int to = before(m, at);
+    if (take) out[to] = lane + 64 * k;
+    at += __popcll(m);
+  }
+}
+
+constexpr int kPickThreads = 512, kPickWaves = 8;
+constexpr int kPickMost = 1024;          // blocks that a row may have
+constexpr int kAtOnce = 4;               // tiles of bounds that a wave has on their way
+
+// both in one launch, for short rows: scores of a tile's tokens in LDS, a wave to a token's choice
+template <typename T, int D, int GP, int N>
+__global__ void __launch_bounds__(kPickThreads) kv8_pick_kernel(SelectArgs a) {
+  constexpr int kTokens = 16 / GP;
+  extern __shared__ unsigned s_key[];    // (kTokens, cap)
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15;
+  const int h = blockIdx.x % a.HKV, id = blockIdx.x / a.HKV;
+  const int b = a.cu ? sequence_of(a.B, id, [&](int i) { return a.cu[i] / kTokens + 2 * i; }) : id;
+  const int* trow = a.table + (long)b * a.t_st;
+  unsigned page[kAtOnce];
+  auto look = [&](int i) {
+#pragma unroll
+    for (int x = 0; x < kAtOnce; ++x) page[x] = (unsigned)trow[min(i + (wave + x * kPickWaves) * 16 + col, a.width - 1)];
+  };
+  look(0);
+  const Seq sq = seq_of(a, b);
+  const int j0 = a.cu ? (id - (sq.r0 / kTokens + 2 * b)) * kTokens : 0, end = j0 < 0 ? j0 : min(j0 + kTokens, sq.R);
+  const int last = j0 < end ? sq.n - sq.R + end - 1 : -1, most = last < 0 ? 0 : (last >> a.lp) + 1;
+  if (most > a.n) {
+    constexpr int kStep = kAtOnce * kPickWaves * 16;
+    int4v Q[D / 32];
+    Bounds<D> t[kAtOnce];
+    // (tiles past the last block too: what lies there is not used)
+#pragma unroll
+    for (int x = 0; x < kAtOnce; ++x) fetch_bounds(a, t[x], page[x], h);
+    query_rows<T, D, GP>(a, sq, j0, h, Q);
+#pragma unroll 1
+    for (int i = 0;;) {
+#pragma unroll
+      for (int x = 0; x < kAtOnce; ++x) {
+        const int at = i + (wave + x * kPickWaves) * 16 + col;
+        score_tile<D, GP>(Q, t[x], [&](int tok, unsigned key) {
+          if (at < most) s_key[tok * a.cap + at] = key;
+        });
+      }
+      if ((i += kStep) >= most) break;
+      look(i);
+#pragma unroll
+      for (int x = 0; x < kAtOnce; ++x) fetch_bounds(a, t[x], page[x], h);
+    }
+  }
+  __syncthreads();
+  for (int tok = wave; j0 + tok < end; tok += kPickWaves) {
+    const int pos = sq.n - sq.R + j0 + tok, seen = pos < 0 ? 0 : (pos >> a.lp) + 1;
+    int* const out = a.out + ((long)(sq.r0 + j0 + tok) * a.HKV + h) * a.n;
+    if (seen <= a.n) {
+      for (int i = lane; i < a.n; i += 64) out[i] = i < seen ? i : -1;
+      continue;
+    }
+    unsigned key[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int i = lane + 64 * k;
+      const unsigned x = s_key[tok * a.cap + min(i, seen - 1)];
+      key[k] = i >= seen ? 0 : i < a.first || i >= seen - a.last ? ~0u : x;
+    }
+    choose<N>(key, a.n, out);
+  }
+  if (!a.cu) return;
+  // -1 for the tokens that no sequence takes: each workgroup looks at as many as a tile has, from its number on
+  for (int x = kPickWaves - 1 - wave; x < kTokens; x += kPickWaves) {
+    const long t = (long)id * kTokens + x;
+    if (t >= a.tokens) continue;
+    const Seq own = seq_of(a, sequence_of(a.B, (int)t, [&](int i) { return a.cu[i]; }));
+    if (t >= own.r0 && t < own.r0 + own.R) continue;
+    for (int i = lane; i < a.n; i += 64) a.out[(t * a.HKV + h) * a.n + i] = -1;
   }
 }
 
@@ -286,6 +471,21 @@ __global__ void __launch_bounds__(kThreads) kv8_choose_kernel(SelectArgs a) {
   }
 }
 
+template <typename T, int D, int GP>
+void pick(const SelectArgs& a, unsigned tiles, hipStream_t st) {
+  const size_t lds = (size_t)(16 / GP) * a.cap * sizeof(unsigned);
+  if (a.cap <= 512) hipLaunchKernelGGL((kv8_pick_kernel<T, D, GP, 8>), dim3(tiles), dim3(kPickThreads), lds, st, a);
+  else hipLaunchKernelGGL((kv8_pick_kernel<T, D, GP, kPickMost / 64>), dim3(tiles), dim3(kPickThreads), lds, st, a);
+}
+template <typename T, int D>
+void pick(const SelectArgs& a, unsigned tiles, int gp, hipStream_t st) {
+  if (gp == 1) pick<T, D, 1>(a, tiles, st);
+  else if (gp == 2) pick<T, D, 2>(a, tiles, st);
+  else if (gp == 4) pick<T, D, 4>(a, tiles, st);
+  else if (gp == 8) pick<T, D, 8>(a, tiles, st);
+  else pick<T, D, 16>(a, tiles, st);
+}
+
 template <typename T, int D>
 void score(SelectArgs a, dim3 grid, int gp, hipStream_t st) {
   if (gp == 1) hipLaunchKernelGGL((kv8_score_kernel<T, D, 1>), grid, dim3(kThreads), 0, st, a);
@@ -311,7 +511,7 @@ extern "C" int oa_kv8_select(const void* q, long q_st, long q_sh, int dtype, con
   if (!sequences || !tokens) return 0;
   auto odd = [](const void* p, uintptr_t x) { return !p || (reinterpret_cast<uintptr_t>(p) & (x - 1)) != 0; };
   if (odd(q, 16) || q_st % 8 || q_sh % 8 || !ks || odd(kb, 16) || scale_stride < kv_heads || bound_stride % 16 ||
-      bound_stride < 2L * kv_heads * head_dim || !table || !lens || (cap > n && odd(ws, 4)) || odd(blocks, 4))
+      bound_stride < 2L * kv_heads * head_dim || !table || !lens || (cap > n && !(cap <= kPickMost && q_heads / kv_heads <= 16) && odd(ws, 4)) || odd(blocks, 4))
     return OA_EINVAL;
   SelectArgs a;
   a.q = q; a.q_st = q_st; a.q_sh = q_sh;
@@ -325,6 +525,14 @@ extern "C" int oa_kv8_select(const void* q, long q_st, long q_sh, int dtype, con
   if (tiles > 0xffffffffL / kThreads || spans > 65535 || (long)tokens * kv_heads > 0xffffffffL / kThreads) return OA_EINVAL;
   const dim3 grid((unsigned)tiles, (unsigned)spans);
   const hipStream_t st = (hipStream_t)stream;
+  if (cap <= kPickMost && a.G <= 16) {
+    if (tiles > 0xffffffffL / kPickThreads) return OA_EINVAL;
+    if (dtype == 0 && head_dim == 64) pick<__bf16, 64>(a, (unsigned)tiles, gp, st);
+    else if (dtype == 0) pick<__bf16, 128>(a, (unsigned)tiles, gp, st);
+    else if (head_dim == 64) pick<_Float16, 64>(a, (unsigned)tiles, gp, st);
+    else pick<_Float16, 128>(a, (unsigned)tiles, gp, st);
+    return OA_LAUNCH_STATUS();
+  }
   if (cap > n) {                         // (otherwise every row takes all of its blocks)
     if (dtype == 0 && head_dim == 64) score<__bf16, 64>(a, grid, gp, st);
     else if (dtype == 0) score<__bf16, 128>(a, grid, gp, st);

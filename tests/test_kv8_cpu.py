@@ -101,10 +101,12 @@ def test_selections_refused(calls):
     assert ops.kv8_select(**ok).shape == (3, 2, 4)
     ops.kv8_select(**dict(ok, cu_q=i32(4), max_len=70, n=3, q=z(5, 8, 128, dtype=torch.float16)))
     ops.kv8_select(**dict(ok, n=9))
+    ops.kv8_select(**dict(ok, table=i32(3, 1025)))
+    ops.kv8_select(**dict(ok, q=z(3, 34, 128, dtype=BF)))
     for name, a in calls:
         assert len(a) + 1 == len(lib.SIGNATURES_KV8[name])
-    # blocks, from the table's width or max_len; no scratch where all are chosen
-    assert calls[0][1][-3] == 9 and calls[0][1][-2] is not None and calls[1][1][-3] == 3 and calls[1][1][-2] is None and calls[2][1][-2] is None
+    # blocks, from the table's width or max_len; scratch where one launch does not do
+    assert [a[-3] for _, a in calls] == [9, 3, 9, 1025, 9] and [a[-2] is None for _, a in calls] == [True, True, True, False, False]
 
 
 def test_attention_refused(calls):
@@ -174,9 +176,11 @@ def test_library_refuses_before_a_launch():
     assert L.oa_kv8_read(*rd[:18], 1, None) == -22 and L.oa_kv8_read(None, *rd[1:]) == -22
     se = [16, 1024, 128, 0, 16, 16, 2, 512, 4, 32, 16, 9, 9, 16, None, 3, 3, 8, 2, 128, 4, 1, 2, 9, 16, 16, None]
     for i, v in ((0, 8), (1, 4), (3, 2), (4, None), (5, 8), (6, 1), (7, 500), (7, 520), (8, 0), (9, 16), (10, None), (11, 8), (12, 0), (13, None), (15, 2), (17, 7),
-                 (18, 0), (19, 96), (20, 2), (21, -1), (22, 0), (23, 0), (23, 10), (24, None), (25, None), (25, 2)):
+                 (18, 0), (19, 96), (20, 2), (21, -1), (22, 0), (23, 0), (23, 10), (25, None), (25, 2)):
         assert L.oa_kv8_select(*se[:i], v, *se[i + 1:]) == -22, (i, v)
     assert L.oa_kv8_select(*se[:15], 0, 0, *se[17:]) == 0
+    wide = [*se[:11], 1025, 1025, *se[13:23], 1025, None, 16, None]                          # no scratch
+    assert L.oa_kv8_select(*wide) == -22 and L.oa_kv8_select(*se[:17], 34, *se[18:24], None, *se[25:]) == -22
     at = [16, 1024, 128, 0, 16, 16, 16, 16, 8192, 2, 4, 32, 16, 2, 2, 16, None, 3, 3, 1, 8, 2, 128, 0.1, None, 0, 128, 2, 16, 16, 32, 1024, 128, 0, None]
     for i, v in ((0, 8), (1, 4), (3, 2), (4, 8), (5, None), (8, 8000), (9, 1), (10, 0), (11, 31), (11, 256), (12, None), (13, 1), (14, 0), (15, None), (17, 2), (19, 0),
                  (19, 2), (20, 7), (21, 0), (22, 96), (23, float("nan")), (26, 64), (26, 200), (27, 0), (28, None), (29, None), (30, None), (31, 2), (30, 16),
