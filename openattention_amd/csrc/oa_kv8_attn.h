@@ -17,6 +17,7 @@ struct AttnArgs {
   uint16_t* out; long o_st, o_sh;
   float* ws_o; float* ws_ml;             // partial sums, (maximum, sum) by (row, chunk)
   int B, HKV, G, tokens, max_q, width, NP, lp, chunk, nchunk, ntile, n;
+  int rows;                              // rows of a workgroup of oa_kv8_rows.hip
   unsigned by_g, by_hkv;                 // 2^16 / G + 1; 2^32 / HKV, rounded up (0: HKV is 1)
   int clear;                             // the join sets rows of out that no sequence takes to 0
   float c;                               // scale * log2 e
@@ -46,5 +47,8 @@ __device__ __forceinline__ bf16x8 from8h(unsigned w0, unsigned w1, float f) {
 }
 // whether one of 4 codes is NaN
 __device__ __forceinline__ unsigned nan_codes(unsigned w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+// many rows over shared keys (oa_kv8_rows.hip)
+void launch_rows(const AttnArgs& a, int head_dim, bool half, dim3 grid, hipStream_t st);
 
 }  // namespace kv8

@@ -7,11 +7,15 @@
 // query heads fills the tiles; with a list the rows of one token, as each has its own) and a chunk of keys (ops.kv8_chunk
 // says how many and why); each wave walks its own tiles of 32 keys and the waves join at the end.  With several
 // chunks a second kernel joins them.
+// A tile's codes are 4096 (D = 64: 2048) successive bytes of K and of V, loaded as such, 16 bytes to a lane, while the
+// tile before is worked on; the wave puts them into its own part of LDS and takes its operands from there.  (Loaded in
+// the operands' order, where a lane's neighbours take other keys, every access touches half lines: the same loop without
+// any work took 365 us for 32 sequences of 32768 keys, so 327, and 117 us for the blocks of two questions, so 49.)
 //   scores   S^T = K Q^T by v_mfma_f32_16x16x32 of the queries' type, which holds the codes as they are: a lane of the K
 //            operand takes 16 dims of each 64 of a key.  A tile lies in one block, whose scale is a factor of the
 //            scores.  All products are exact.
 //   values   O^T = V^T P^T in bf16, the scale taken in by the conversion: the weights are the B operand as the scores
-//            left them; V goes through the wave's own LDS tile and comes back by the LDS transpose reads.
+//            left them; V^T comes out of LDS by the transpose reads, as codes.
 // Weights go into the product as two bf16 terms, so that the sum keeps 16 bits of each: up to 8 rows
 // the second term sits in the tile's other 8 columns, otherwise it takes a second product.
 #include "oa_kv8_attn.h"
@@ -20,10 +24,13 @@ namespace {
 
 using namespace kv8;
 
-// one tile's codes of this lane (keys lane % 16 and 16 + lane % 16, 16 dims of each 64) and its scales
+typedef int int2v __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) int2v lds_int2v;
+
+// one tile's codes as they lie in memory, lane by lane 16 bytes, and its scales
 template <int D>
 struct Tile {
-  uint4v k[2][D / 64], v[2][D / 64];
+  uint4v k[D / 32], v[D / 32];
   unsigned ks, vs;
   unsigned bad;                          // the exponent of NaN where the page is outside of the cache
 };
@@ -35,18 +42,19 @@ __device__ __forceinline__ uint4v load16(const uint8_t* p) {
 }
 
 // NQ tiles of 16 query rows; DUP: at most 8 rows, columns 8.. repeat them for the weights' second terms; T: the rows'
-// type; LISTED: over listed blocks, the rows of one token
-template <int D, int NQ, bool DUP, typename T, bool LISTED>
+// type; LISTED: over listed blocks, the rows of one token; ONCE: no other workgroup reads these codes, which then pass by
+// the caches (32 sequences of 32768 keys: 365 us through them, 327)
+template <int D, int NQ, bool DUP, typename T, bool LISTED, bool ONCE>
 __global__ void __launch_bounds__(kThreads, NQ > 1 ? 2 : 3) kv8_attn_kernel(AttnArgs a) {
   constexpr bool kHalf = !std::is_same<T, __bf16>::value;
-  constexpr int kPieces = D / 64;        // 16-byte loads of a lane for a key
+  constexpr int kLoads = D / 32;         // 16-byte loads of a lane for a tile of K or V
   constexpr int kSteps = D / 32;         // products of a 16 x 16 score tile
-  constexpr int kDims = D / 16;          // tiles of 16 dims
-  constexpr int kRowB = D * 2;           // bytes of a value row in LDS
-  constexpr int kStage = kTile * kRowB;
+  constexpr int kDims = D / 16;          // tiles of 16 dims, 16-byte chunks of a row
+  constexpr int kTileB = kTile * D;      // bytes of a tile
+  constexpr int kStage = 2 * kTileB;
   constexpr int kCols = DUP ? 8 : 16;
   constexpr int kStride = kWaves * kTile;
-  // value tiles of the waves; at the end their sums, 16 rows of D floats each
+  // tiles of the waves, K then V; at the end their sums, 16 rows of D floats each
   __shared__ __align__(16) char s_v[kWaves * (kStage > 64 * D ? kStage : 64 * D)];
   __shared__ float s_m[kWaves][NQ * 16], s_l[kWaves][NQ * 16];
 
@@ -77,10 +85,9 @@ __global__ void __launch_bounds__(kThreads, NQ > 1 ? 2 : 3) kv8_attn_kernel(Attn
   const int k1 = LISTED ? min(k0 + a.chunk, a.n << a.lp) : min(k0 + a.chunk, hi);
   if (!LISTED && k0 >= k1 && a.nchunk > 1) return;
 
-  // a tile's addresses: a scalar base and fixed lane offsets
+  // a tile's addresses: a scalar base and the lane's place
   const int pmask = (1 << a.lp) - 1;
   const long headc = ((long)h << a.lp) * D;
-  const unsigned oc = col * D + 16 * g;
   auto load = [&](Tile<D>& t, int off, int page) {
     const bool bad = (unsigned)page >= (unsigned)a.NP;
     t.bad = bad ? 0x7f800000u : 0u;
@@ -88,19 +95,13 @@ __global__ void __launch_bounds__(kThreads, NQ > 1 ? 2 : 3) kv8_attn_kernel(Attn
     const long bc = pg * a.c_sp + headc + (long)off * D, bs = pg * a.s_sp + h;
     t.ks = a.ks[bs];
     t.vs = a.vs[bs];
-    const uint8_t* kc = a.kc + bc + oc;
-    const uint8_t* vc = a.vc + bc + oc;
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
+    for (int n = 0; n < kLoads; ++n) t.k[n] = load16<ONCE>(a.kc + bc + 16 * lane + 1024 * n);
 #pragma unroll
-      for (int x = 0; x < kPieces; ++x) t.k[c][x] = load16<NQ == 1>(kc + 16 * c * D + 64 * x);
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-      for (int x = 0; x < kPieces; ++x) t.v[c][x] = load16<NQ == 1>(vc + 16 * c * D + 64 * x);
+    for (int n = 0; n < kLoads; ++n) t.v[n] = load16<ONCE>(a.vc + bc + 16 * lane + 1024 * n);
   };
   const int nt = max(0, (k1 - tb + kStride - 1) / kStride);                  // this wave's tiles
-  Tile<D> ta, tc;
+  Tile<D> t;
   // listed blocks: tile i's block, -1 past the last; whether a row sees something of it
   const int* const list = LISTED ? a.list + ((long)u * a.HKV + h) * a.n : nullptr;
   auto block_at = [&](int i) { return i < nt ? list[(tb + i * kStride) >> a.lp] : -1; };
@@ -114,9 +115,9 @@ __global__ void __launch_bounds__(kThreads, NQ > 1 ? 2 : 3) kv8_attn_kernel(Attn
     b2 = block_at(2);
     page0 = page_of(b0);
     page = page_of(b1);
-    if (live(b0, 0)) load(ta, tb & pmask, page0);
+    if (live(b0, 0)) load(t, tb & pmask, page0);
   } else if (nt > 0) {
-    load(ta, tb & pmask, page0);
+    load(t, tb & pmask, page0);
   }
 
   // this lane's columns: rows of q (negated under a negative scale: the maximum is taken before scaling)
@@ -138,18 +139,26 @@ __global__ void __launch_bounds__(kThreads, NQ > 1 ? 2 : 3) kv8_attn_kernel(Attn
     }
   }
 
-  // LDS tile of 32 value rows; 16-byte chunk x of row r lies at x ^ f(r): 16 rows written at one chunk
-  // and 16 rows read at two both spread over all banks
-  char* const sv = s_v + wave * kStage;
-  auto fsw = [](int r) { return D == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : ((r >> 1) & 3) << 1; };
-  const int wbase = col * kRowB, wf = fsw(col);
-  const int lr = 4 * g + ((lane & 15) >> 2), rf = fsw(lr), lc = lane & 3;
-  auto val_op = [&](int d) {
-    const int ad = lr * kRowB + (((2 * d + (lc >> 1)) ^ rf) << 4) + (lc & 1) * 8;
-    const short4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v*)(sv + ad));
-    const short4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v*)(sv + ad + 16 * kRowB));
-    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  // LDS tiles of 32 rows of D bytes; 16-byte chunk x of row r lies at x ^ f(r), so that rows written as they come (8 or
+  // 16 of them whole), 16 rows read at one chunk and the transpose reads' 16 (keys 8 g' .. and 16 more) spread over all banks
+  char* const sk = s_v + wave * kStage;
+  char* const sv = sk + kTileB;
+  auto f = [](int r) {
+    return D == 128 ? ((r >> 1) & 3) | (((r >> 3) ^ (r >> 4)) & 1) << 2 : ((r >> 2) & 1) | (((r >> 3) ^ (r >> 4)) & 1) << 1;
   };
+  // the lane's row and chunk of load n, and where it goes
+  const int wrow = lane / kDims, wchunk = lane % kDims;
+  auto put_at = [&](int n) {
+    const int r = wrow + n * (1024 / D);
+    return r * D + ((wchunk ^ f(r)) << 4);
+  };
+  auto key_op = [&](int c, int x) {      // dims 64 x + 16 g .. of key 16 c + col
+    const int r = col + 16 * c;
+    return *reinterpret_cast<const uint4v*>(sk + r * D + (((4 * x + g) ^ f(r)) << 4));
+  };
+  // dims 16 d .. of keys 4 g .. and 16 + 4 g .., the order in which the scores leave the weights
+  const int vrow = 4 * g + ((lane >> 1) & 3) + ((lane & 8) << 1), vat = vrow * D + 8 * (lane & 1);
+  auto val_op = [&](int d) { return __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_int2v*)(sv + vat + ((d ^ f(vrow)) << 4))); };
 
   f32x4 O[NQ][kDims];
   float m[NQ], l[NQ];                    // running maximum, scaled, and sum of the lane's keys
@@ -163,56 +172,51 @@ __global__ void __launch_bounds__(kThreads, NQ > 1 ? 2 : 3) kv8_attn_kernel(Attn
     for (int d = 0; d < kDims; ++d) O[x][d] = f32x4(0.f);
   }
 
-  // a tile whose first key is at position t0
-  auto body = [&](auto mask_c, int t0, const Tile<D>& t) {
+  // the tile in t, whose first key is at position t0; next() requests what comes after it
+  auto body = [&](auto mask_c, int t0, auto next) {
     const bool MASK = mask_c;            // (known beforehand, or the same for the whole wave)
     // (the block's scale, a factor of the scores; finite, so that it leaves a product of 0 what it is)
     const float ck = fminf(c * __uint_as_float(t.ks << 23), FLT_MAX) + __uint_as_float(t.bad) * 0.f;
+    const float fv = __uint_as_float(t.vs << 23);
+    // In a masked tile the values of keys past the last one any row sees count as zeros (their weights are 0, but what
+    // lies there may be anything), and so do chunks with NaN of keys that some rows see
+    unsigned nan = 0;                    // bit n: such a chunk
+#pragma unroll
+    for (int n = 0; n < kLoads; ++n) {
+      uint4v w = t.v[n];
+      if (MASK) {
+        const bool past = t0 + wrow + n * (1024 / D) >= hi;
+        const bool any = (nan_codes(w[0]) | nan_codes(w[1]) | nan_codes(w[2]) | nan_codes(w[3])) != 0;
+        nan |= any && !past ? 1u << n : 0u;
+        w = any || past ? uint4v(0u) : w;
+      }
+      *reinterpret_cast<uint4v*>(sk + put_at(n)) = t.k[n];
+      *reinterpret_cast<uint4v*>(sv + put_at(n)) = w;
+    }
+    lane_order();
+    next();
     f32x4 S[NQ][2];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
 #pragma unroll
       for (int x = 0; x < NQ; ++x) S[x][c] = f32x4(0.f);
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const unsigned w0 = t.k[c][s >> 1][2 * (s & 1)], w1 = t.k[c][s >> 1][2 * (s & 1) + 1];
-        const bf16x8 kop = kHalf ? from8h(w0, w1, 1.f) : from8(w0, w1, 1.f);
+      for (int y = 0; y < D / 64; ++y) {
+        const uint4v w = key_op(c, y);
 #pragma unroll
-        for (int x = 0; x < NQ; ++x) {
-          if constexpr (kHalf)
-            S[x][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, kop), __builtin_bit_cast(f16x8, Q[x][s]),
-                                                             S[x][c], 0, 0, 0);
-          else
-            S[x][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop, Q[x][s], S[x][c], 0, 0, 0);
+        for (int z = 0; z < 2; ++z) {
+          const bf16x8 kop = kHalf ? from8h(w[2 * z], w[2 * z + 1], 1.f) : from8(w[2 * z], w[2 * z + 1], 1.f);
+#pragma unroll
+          for (int x = 0; x < NQ; ++x) {
+            if constexpr (kHalf)
+              S[x][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, kop),
+                                                               __builtin_bit_cast(f16x8, Q[x][2 * y + z]), S[x][c], 0, 0, 0);
+            else
+              S[x][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop, Q[x][2 * y + z], S[x][c], 0, 0, 0);
+          }
         }
       }
     }
-    // values into the LDS tile.  In a masked tile keys past the last one any row sees count as zeros (their
-    // weights are 0, but what lies there may be anything), and so does NaN in keys that some rows see
-    const float fv = __uint_as_float(t.vs << 23);
-    bool nan[2] = {false, false};
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      uint4v w[kPieces];
-#pragma unroll
-      for (int x = 0; x < kPieces; ++x) w[x] = t.v[c][x];
-      if (MASK) {
-        const bool past = t0 + 16 * c + col >= hi;
-        unsigned any = 0;
-#pragma unroll
-        for (int x = 0; x < kPieces; ++x) any |= nan_codes(w[x][0]) | nan_codes(w[x][1]) | nan_codes(w[x][2]) | nan_codes(w[x][3]);
-        nan[c] = any && !past;
-#pragma unroll
-        for (int x = 0; x < kPieces; ++x) w[x] = any || past ? uint4v(0u) : w[x];
-      }
-#pragma unroll
-      for (int x = 0; x < kPieces; ++x)
-#pragma unroll
-        for (int y = 0; y < 2; ++y)
-          *reinterpret_cast<bf16x8*>(sv + wbase + 16 * c * kRowB + (((8 * x + 2 * g + y) ^ wf) << 4)) =
-              from8(w[x][2 * y], w[x][2 * y + 1], fv);
-    }
-    lane_order();
 
     uint4v P[NQ], Plo[NQ];
 #pragma unroll
@@ -263,7 +267,8 @@ __global__ void __launch_bounds__(kThreads, NQ > 1 ? 2 : 3) kv8_attn_kernel(Attn
     }
 #pragma unroll
     for (int d = 0; d < kDims; ++d) {
-      const bf16x8 vop = val_op(d);
+      const int2v w = val_op(d);
+      const bf16x8 vop = from8((unsigned)w[0], (unsigned)w[1], fv);
 #pragma unroll
       for (int x = 0; x < NQ; ++x) {
         O[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vop, __builtin_bit_cast(bf16x8, P[x]), O[x][d], 0, 0, 0);
@@ -271,18 +276,18 @@ __global__ void __launch_bounds__(kThreads, NQ > 1 ? 2 : 3) kv8_attn_kernel(Attn
       }
     }
     lane_order();
-    if (MASK) {                          // NaN, into the rows that see it (rare): the lane's dims, 16 of each 64
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        unsigned long at_nan = __ballot(nan[c]);
+    if (MASK && __any(nan != 0)) {       // NaN, into the rows that see it (rare)
+#pragma unroll 1
+      for (int n = 0; n < kLoads; ++n) {
+        unsigned long at_nan = __ballot(nan >> n & 1);
         while (at_nan) {
-          const int at = __builtin_ctzl(at_nan), key = t0 + 16 * c + (at & 15), part = at >> 4;
+          const int at = __builtin_ctzl(at_nan), key = t0 + at / kDims + n * (1024 / D), part = at % kDims;
           at_nan &= at_nan - 1;
 #pragma unroll
           for (int x = 0; x < NQ; ++x)
 #pragma unroll
             for (int d = 0; d < kDims; ++d)
-              if ((d & 3) == part && key < lim[x]) O[x][d] = f32x4(__builtin_nanf(""));
+              if (d == part && key < lim[x]) O[x][d] = f32x4(__builtin_nanf(""));
         }
       }
     }
@@ -292,40 +297,35 @@ __global__ void __launch_bounds__(kThreads, NQ > 1 ? 2 : 3) kv8_attn_kernel(Attn
   if (LISTED) {
 #pragma unroll 1
     for (int i = 0; i < nt; ++i) {
-      if (live(b1, i + 1)) load(tc, (tb + (i + 1) * kStride) & pmask, page);
-      page = page_of(b2);
-      const int b3 = block_at(i + 3);
+      auto next = [&] {
+        if (live(b1, i + 1)) load(t, (tb + (i + 1) * kStride) & pmask, page);
+      };
       if (live(b0, i)) {
         const int t0 = place_of(b0, i);
-        body(t0 + kTile > hi, t0, ta);
+        body(t0 + kTile > hi, t0, next);
+      } else {
+        next();
       }
-      ta = tc;
+      page = page_of(b2);
+      const int b3 = block_at(i + 3);
       b0 = b1;
       b1 = b2;
       b2 = b3;
     }
   } else {
     const int nfull = min(nt, max(0, (all - tb - kTile + kStride) / kStride));    // tiles that every row sees whole
-    auto next = [&](int i) {             // tile i + 1, and the page of the one after
+    int i = 0;
+    auto next = [&] {                    // tile i + 1, and the page of the one after
       if (i + 1 < nt) {
         const int t0 = tb + (i + 1) * kStride;
-        load(tc, t0 & pmask, page);
+        load(t, t0 & pmask, page);
         page = page_at(t0 + kStride);
       }
     };
-    int i = 0;
 #pragma unroll 1
-    for (; i < nfull; ++i) {
-      next(i);
-      body(whole(), tb + i * kStride, ta);
-      ta = tc;
-    }
+    for (; i < nfull; ++i) body(whole(), tb + i * kStride, next);
 #pragma unroll 1
-    for (; i < nt; ++i) {
-      next(i);
-      body(masked(), tb + i * kStride, ta);
-      ta = tc;
-    }
+    for (; i < nt; ++i) body(masked(), tb + i * kStride, next);
   }
 
   // the four waves' sums, with a common maximum
@@ -382,25 +382,38 @@ __global__ void __launch_bounds__(kThreads) kv8_join_kernel(AttnArgs a) {
   join_pieces<D, T, LISTED>(a);
 }
 
+// query rows up to which every workgroup turns its own keys to 16 bits (more: oa_kv8_rows.hip)
+constexpr int kFewRows = 64;
+
 template <int D, typename T, bool LISTED>
 int launch(AttnArgs a, hipStream_t st) {
   const long rows = LISTED ? a.G : (long)a.max_q * a.G;
-  const int cols = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
+  const int cols = rows <= 8 ? 8 : rows <= 16 ? 16 : LISTED || rows <= kFewRows ? 32 : 128;
   a.ntile = (int)((rows + cols - 1) / cols);
   const long units = (long)(LISTED ? a.tokens : a.B) * a.HKV, joins = (long)a.max_q * a.HKV * a.G;
   // (workgroups along the other axes are counted in 16 bits)
-  if (units > kGrid || a.ntile > 65535 || a.nchunk > 65535 || units * a.ntile * a.nchunk > kGrid ||
+  if (units > kGrid || a.nchunk > 65535 || units * a.ntile * a.nchunk > kGrid || (cols < 128 && a.ntile > 65535) ||
       (a.nchunk > 1 && (joins > kGrid || a.B > 65535)))
     return OA_EINVAL;
   // quotients as products with 2^16 / G + 1 and 2^32 / HKV, rounded up: exact while the number times the divisor is
-  // less than that power
-  if (units * a.HKV > 0xffffffffL || rows * a.G > 65535) return OA_EINVAL;
+  // less than that power (without a list rows and G are at most 64 here; with one rows are not divided)
+  if (cols < 128 && units * a.HKV > 0xffffffffL) return OA_EINVAL;
   a.by_g = 65536u / a.G + 1;
   a.by_hkv = a.HKV > 1 ? (unsigned)((0x100000000L + a.HKV - 1) / a.HKV) : 0;
   const dim3 grid((unsigned)units, a.ntile, a.nchunk), blk(kThreads);
-  if (cols == 8) hipLaunchKernelGGL((kv8_attn_kernel<D, 1, true, T, LISTED>), grid, blk, 0, st, a);
-  else if (cols == 16) hipLaunchKernelGGL((kv8_attn_kernel<D, 1, false, T, LISTED>), grid, blk, 0, st, a);
-  else hipLaunchKernelGGL((kv8_attn_kernel<D, 2, false, T, LISTED>), grid, blk, 0, st, a);
+  // (the tokens of a sequence, where it has several, have blocks in common: through the caches)
+  if (cols == 8) {
+    if (LISTED && a.cu) hipLaunchKernelGGL((kv8_attn_kernel<D, 1, true, T, LISTED, !LISTED>), grid, blk, 0, st, a);
+    else hipLaunchKernelGGL((kv8_attn_kernel<D, 1, true, T, LISTED, true>), grid, blk, 0, st, a);
+  } else if (cols == 16) {
+    if (LISTED && a.cu) hipLaunchKernelGGL((kv8_attn_kernel<D, 1, false, T, LISTED, !LISTED>), grid, blk, 0, st, a);
+    else hipLaunchKernelGGL((kv8_attn_kernel<D, 1, false, T, LISTED, true>), grid, blk, 0, st, a);
+  } else if (cols == 32) {
+    hipLaunchKernelGGL((kv8_attn_kernel<D, 2, false, T, LISTED, false>), grid, blk, 0, st, a);
+  } else {
+    a.rows = cols;
+    launch_rows(a, D, !std::is_same<T, __bf16>::value, dim3((unsigned)(units * a.ntile * a.nchunk)), st);
+  }
   if (a.nchunk > 1) hipLaunchKernelGGL((kv8_join_kernel<D, T, LISTED>), dim3((unsigned)joins, a.B), blk, 0, st, a);
   return OA_LAUNCH_STATUS();
 }

@@ -1220,12 +1220,12 @@ def kv8_select(q, ks, kb, table, lens, page: int, n: int, cu_q=None, first: int 
     return out
 
 
-def kv8_chunk(cap: int, units: int, rows: int) -> int:
+def kv8_chunk(cap: int, units: int, rows: int, listed: bool = False) -> int:
     """Keys per workgroup of kv8_attn, for `units` (sequence or token, KV head, query tile) triples of up to `cap` keys and
-    `rows` query rows: as kv4_chunk."""
-    n = max(cap * units // 512, 256)
-    if rows <= 64:
-        n = max(min(n, max(cap // 8, 1024)), 256)
+    `rows` query rows."""
+    n = max(cap * units // (256 if rows <= 16 else 512), 128)
+    if rows <= 64 and not listed:
+        n = min(n, max(cap // 8, 1024))
     return min(-(-n // 128), -(-cap // 128)) * 128
 
 
@@ -1256,9 +1256,9 @@ def _attn8_sizes(HKV, Dh, where, qs, qst, qt, ts, tst, tt, lens, cu, max_q, sm_s
     rows = G if n else max_q * G
     cap = n * page if n else max(1, width * page if max_len is None else min(max_len, width * page))
     units = (T if n else B) * HKV
-    tiles = -(-rows // (8 if rows <= 8 else 16 if rows <= 16 else 32))
+    tiles = -(-rows // (8 if rows <= 8 else 16 if rows <= 16 else 32 if n or rows <= 64 else 128))
     # (the join's grid holds 65535 sequences; so many need no pieces to fill the card)
-    chunk = rule(cap, units * tiles, rows) if B <= 65535 else -(-cap // 128) * 128
+    chunk = rule(cap, units * tiles, rows, n > 0) if B <= 65535 else -(-cap // 128) * 128
     nchunk = -(-cap // chunk)
     _need(units * tiles * nchunk <= _GRID and units * HKV < 1 << 32,
           f"at most {_GRID} workgroups (sequences, or tokens with blocks, x heads x tiles of rows x pieces), heads^2 times those under 2^32")

@@ -363,7 +363,7 @@ def test_attention(case, chunk, copies, monkeypatch):
     print(f"[case] kv8 attn {CASES[case]} chunk={chunk} copies={copies}", flush=True)
     lens, rows, HQ, HKV, D, page, dtype = CASES[case]
     if chunk:
-        monkeypatch.setattr(ops, "kv8_chunk", lambda cap, units, rows: min(chunk, -(-cap // 128) * 128))
+        monkeypatch.setattr(ops, "kv8_chunk", lambda cap, units, rows, listed: min(chunk, -(-cap // 128) * 128))
     lens, rows = lens * copies, rows and rows * copies
     g = gen(case)
     cache, table = filled(lens, HKV, D, page, g, extra_width=case % 3)
@@ -388,7 +388,7 @@ def test_attention_over_blocks(case, n, chunk, monkeypatch):
     print(f"[case] kv8 blocks {CASES[case]} n={n} chunk={chunk}", flush=True)
     lens, rows, HQ, HKV, D, page, dtype = CASES[case]
     if chunk:
-        monkeypatch.setattr(ops, "kv8_chunk", lambda cap, units, rows: min(chunk, -(-cap // 128) * 128))
+        monkeypatch.setattr(ops, "kv8_chunk", lambda cap, units, rows, listed: min(chunk, -(-cap // 128) * 128))
     g = gen(case + 30)
     cache, table = filled(lens, HKV, D, page, g, extra_width=case % 3)
     cu = starts(rows or [1] * len(lens))
