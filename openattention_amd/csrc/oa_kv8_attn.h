@@ -17,7 +17,6 @@ struct AttnArgs {
   uint16_t* out; long o_st, o_sh;
   float* ws_o; float* ws_ml;             // partial sums, (maximum, sum) by (row, chunk)
   int B, HKV, G, tokens, max_q, width, NP, lp, chunk, nchunk, ntile, n;
-  int rows;                              // rows of a workgroup of oa_kv8_rows.hip
   unsigned by_g, by_hkv;                 // 2^16 / G + 1; 2^32 / HKV, rounded up (0: HKV is 1)
   int clear;                             // the join sets rows of out that no sequence takes to 0
   float c;                               // scale * log2 e

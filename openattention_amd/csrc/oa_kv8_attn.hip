@@ -411,7 +411,6 @@ int launch(AttnArgs a, hipStream_t st) {
   } else if (cols == 32) {
     hipLaunchKernelGGL((kv8_attn_kernel<D, 2, false, T, LISTED, false>), grid, blk, 0, st, a);
   } else {
-    a.rows = cols;
     launch_rows(a, D, !std::is_same<T, __bf16>::value, dim3((unsigned)(units * a.ntile * a.nchunk)), st);
   }
   if (a.nchunk > 1) hipLaunchKernelGGL((kv8_join_kernel<D, T, LISTED>), dim3((unsigned)joins, a.B), blk, 0, st, a);
