@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_rows_kernel(AttnArgs a) {
       asm volatile("" : "+v"(ck2));      // (formed here, before the next loads take the scale's register)
       const Put to = put_begin(st[kOdd], i + 2);
       rescale(refp);
-      float mx = -INFINITY, alpha = 1.f, p0 = 0.f;
+      float mx = -INFINITY, alpha = 1.f, p0 = 0.f, f = ck0;    // f: what the scores are still to be multiplied by
       bool moved = false;
       Sn = float16v(0.f);
       bf16x8 kop[kSteps], vop[kSteps];
@@ -261,16 +261,17 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_rows_kernel(AttnArgs a) {
         Sn = mfma<kHalf>(kop[s], Q[s], Sn);
         O[s >> 1] = mfma<true>(vop[s], __builtin_bit_cast(bf16x8, Pp.p[s & 1]), O[s >> 1]);
         if (s == 0) {                    // the tile's maximum
-          if (i >= nfull) {
+          if (i >= nfull) {              // (scaled first: the scale of a page outside of the cache is NaN)
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-              if (k0 + i * kTile + 8 * (r >> 2) + 4 * h + (r & 3) >= lim) S[r] = -INFINITY;
+              S[r] = k0 + i * kTile + 8 * (r >> 2) + 4 * h + (r & 3) < lim ? S[r] * ck0 : -INFINITY;
+            f = 1.f;
           }
 #pragma unroll
           for (int r = 0; r < 16; ++r) mx = fmaxf(mx, S[r]);
         } else if (s == 1) {
           const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-          mx = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1])) * ck0;
+          mx = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1])) * f;
           moved = __any(mx > m + (big ? 0.f : kLazy));
           if (moved) {
             const float mn = fmaxf(m, mx);
@@ -282,12 +283,13 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_rows_kernel(AttnArgs a) {
           }
           if (big) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) S[r] *= ck0;
+            for (int r = 0; r < 16; ++r) S[r] *= f;
+            f = 1.f;
           }
         } else {
 #pragma unroll
           for (int r = (s - 2) * 16 / (kSteps - 2); r < (s - 1) * 16 / (kSteps - 2); ++r) {
-            const float p1 = __builtin_amdgcn_exp2f(fmaf(S[r], big ? 1.f : ck0, kLift - m));
+            const float p1 = __builtin_amdgcn_exp2f(fmaf(S[r], f, kLift - m));
             l += p1;
             if (r & 1) {
               uint32_t u = pack2h(p0, p1);

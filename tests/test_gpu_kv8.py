@@ -571,3 +571,22 @@ def test_all_blocks_are_all_keys():
     a = ops.kv8_attn(q, *cache[:4], table, i32(lens), cu_q=i32(cu), max_q=4, blocks=blocks)
     b = ops.kv8_attn(q, *cache[:4], table, i32(lens), cu_q=i32(cu), max_q=4)
     assert ((a.float() - b.float()).abs() <= 2.0 ** -7 * b.float().abs().clamp(min=2.0 ** -8)).all()
+
+
+@pytest.mark.parametrize("rows", [2, 20, 70])
+def test_bad_pages_reach_the_rows_that_see_them(rows):
+    """A page outside of the cache makes NaN of the tokens behind its beginning and of no others, however many rows share
+    their keys."""
+    g = gen(14)
+    page, n = 32, 97
+    cache, table = filled([n], 2, 128, page, g)
+    bad = table.clone()
+    bad[0, 3] = -1
+    for HQ in (4, 8):
+        q = randn(g, rows, HQ, 128, dtype=BF)
+        good = ops.kv8_attn(q, *cache[:4], table, i32([n]), cu_q=i32([0, rows]), max_q=rows)
+        out = ops.kv8_attn(q, *cache[:4], bad, i32([n]), cu_q=i32([0, rows]), max_q=rows)
+        assert out[-1].isnan().all() and torch.equal(out[:-1], good[:-1])
+        last = ops.kv8_attn(q, *cache[:4], table, i32([n - 1]), cu_q=i32([0, rows]), max_q=rows)
+        none = ops.kv8_attn(q, *cache[:4], bad, i32([n - 1]), cu_q=i32([0, rows]), max_q=rows)
+        assert torch.equal(last, none) and not none.isnan().any()
