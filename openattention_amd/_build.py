@@ -4,6 +4,7 @@ Every ``csrc/*.hip`` file is compiled to an object with ``hipcc --offload-arch=g
 objects are linked with g++ into one shared library.  The library is linked against the HIP
 runtime that ships inside torch (same file name the torch extension libraries resolve), so a
 process that imports torch first runs both torch and this library on one HIP runtime.
+``csrc/oa_fast.cpp`` becomes a Python module beside it (``_oa_fast.so``, g++).
 
 Flags: -O3, -ffp-contract=off (a fused multiply-add only where the source asks for one:
 the decision path is replayed bit for bit by the CPU restatement), packed-fp32 code
@@ -22,6 +23,7 @@ INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "_lib")
 LIBNAME = "liboa_hip.so"
+FASTNAME = "_oa_fast.so"
 ARCH = os.environ.get("OA_OFFLOAD_ARCH", "gfx950")
 
 HIPCC_FLAGS = [
@@ -35,12 +37,29 @@ def lib_path() -> str:
     return os.path.join(LIBDIR, LIBNAME)
 
 
-def _torch_libdir() -> str:
+def fast_path() -> str:
+    return os.path.join(LIBDIR, FASTNAME)
+
+
+def _torch_dir() -> str:
     import importlib.util
     spec = importlib.util.find_spec("torch")
     if spec is None or not spec.origin:
         raise RuntimeError("torch is required to locate the HIP runtime to link against")
-    return os.path.join(os.path.dirname(spec.origin), "lib")
+    return os.path.dirname(spec.origin)
+
+
+def _torch_libdir() -> str:
+    return os.path.join(_torch_dir(), "lib")
+
+
+def _fast_cmd(out: str) -> list[str]:
+    """The host module that calls the library's entry points on torch tensors (csrc/oa_fast.cpp): for this Python and torch."""
+    import sysconfig
+    t, tl = os.path.join(_torch_dir(), "include"), _torch_libdir()
+    return ["g++", "-std=c++17", "-O2", "-Wall", "-fPIC", "-shared", os.path.join(CSRC, "oa_fast.cpp"), "-o", out, "-I", INCLUDE,
+            "-isystem", t, "-isystem", os.path.join(t, "torch", "csrc", "api", "include"), "-isystem", sysconfig.get_paths()["include"],
+            f"-L{tl}", "-ltorch_python", "-ltorch_cpu", "-lc10", f"-Wl,-rpath,{tl}"]
 
 
 def _hipcc() -> str:
@@ -70,6 +89,8 @@ def build(verbose: bool = False, jobs: int | None = None) -> str:
         procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
         if jobs and len([p for _, p in procs if p.poll() is None]) >= jobs:
             procs[0][1].wait()
+    fast = fast_path() + ".tmp"
+    procs.append(("oa_fast.cpp", subprocess.Popen(_fast_cmd(fast), stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
     failed = []
     for src, p in procs:
         out, _ = p.communicate()
@@ -90,6 +111,7 @@ def build(verbose: bool = False, jobs: int | None = None) -> str:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
     os.replace(tmp, lib_path())
+    os.replace(fast, fast_path())
     return lib_path()
 
 

@@ -1,0 +1,286 @@
+// Calls of the 8-bit cache's operators without Python's part.
+//
+// The checks of ops.py depend on sizes, strides, types and numbers alone, but for a few that can differ between tensors
+// of the same sizes.  What a call's first pass through Python has worked out (its plan: the numbers that the C entry
+// takes) is kept here under those sizes; a later call with the same ones looks at the few others (device, alignment,
+// gradients, lazily negated views) and launches at once.  Whatever is unusual is left to Python (NotImplemented), which
+// refuses it or handles it as before.  A step's call took 9 to 15 us on the host, most of it here now: see ops.py.
+// Nothing is kept by a tensor's address: pointers are taken anew in every call.
+#include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/version.h>
+
+#include <ATen/core/grad_mode.h>
+#include <ATen/ops/empty.h>
+#include <ATen/ops/zeros.h>
+
+#include <cstring>
+#include <unordered_map>
+#include <vector>
+
+#include "openattention_kv8.h"
+
+namespace {
+
+constexpr int kWords = 256, kTensors = 12, kPlans = 1024;
+
+enum Op { kWrite, kRead, kSelect, kAttn, kOps };
+
+// a call's arguments: what a plan is kept under, and the tensors
+struct Call {
+  int64_t key[kWords];
+  int words = 0, count = 0, device = -1;
+  const at::Tensor* t[kTensors] = {};    // null: None
+  void* p(int i) const { return t[i] ? t[i]->data_ptr() : nullptr; }
+  void push(int64_t x) { key[words++] = x; }
+};
+
+struct Plan {
+  std::vector<int64_t> key, c;           // c: the numbers, as ops.py lists them for the operator
+  std::vector<PyObject*> held;           // objects that the key names, so that nothing else takes their place
+  double scale = 0;
+};
+
+std::unordered_multimap<uint64_t, Plan> plans;
+void* entry[kOps] = {};
+PyObject* raw_stream = nullptr;
+PyObject* get_device = nullptr;
+
+uint64_t hash_of(const int64_t* k, int n) {
+  uint64_t h = 0x9e3779b97f4a7c15ull;
+  for (int i = 0; i < n; ++i) {
+    h = (h ^ (uint64_t)k[i]) * 0xff51afd7ed558ccdull;
+    h ^= h >> 32;
+  }
+  return h;
+}
+
+// false: something that Python has to look at
+bool take_tensor(Call& call, PyObject* o) {
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.defined() || t.layout() != at::kStrided || !t.is_cuda() || t.is_neg() || t.is_conj()) return false;
+  const c10::TensorImpl* impl = t.unsafeGetTensorImpl();
+  if (!impl->has_storage() || call.count >= kTensors || t.dim() > 8 || call.words + 4 + 2 * t.dim() > kWords - 8) return false;
+  if (impl->autograd_meta() && ((at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined())) return false;
+  const int d = t.get_device();
+  if (call.device >= 0 && d != call.device) return false;
+  call.device = d;
+  call.push(1);
+  call.push((int64_t)t.scalar_type());
+  call.push(d);
+  call.push(t.dim());
+  for (const int64_t x : t.sizes()) call.push(x);
+  for (const int64_t x : t.strides()) call.push(x);
+  call.t[call.count++] = &t;
+  return true;
+}
+
+bool take(Call& call, int op, PyObject* const* args, Py_ssize_t n, std::vector<PyObject*>* held) {
+  call.push(op);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* o = args[i];
+    if (call.words > kWords - 16) return false;
+    if (THPVariable_CheckExact(o)) {
+      if (!take_tensor(call, o)) return false;
+    } else if (o == Py_None) {
+      call.push(0);
+      if (call.count >= kTensors) return false;
+      call.t[call.count++] = nullptr;    // (numbers that may be None come behind the tensors)
+    } else if (PyLong_CheckExact(o)) {
+      int overflow = 0;
+      const long long x = PyLong_AsLongLongAndOverflow(o, &overflow);
+      if (overflow) return false;
+      call.push(2);
+      call.push(x);
+    } else if (PyFloat_CheckExact(o)) {
+      const double x = PyFloat_AS_DOUBLE(o);
+      int64_t b;
+      std::memcpy(&b, &x, sizeof b);
+      call.push(3);
+      call.push(b);
+    } else if (PyFunction_Check(o) || THPDtype_Check(o)) {
+      call.push(4);
+      call.push((int64_t)(intptr_t)o);
+      if (held) held->push_back(o);
+    } else {
+      return false;
+    }
+  }
+  return call.device >= 0;
+}
+
+Plan* find(const Call& call, uint64_t h) {
+  const auto range = plans.equal_range(h);
+  for (auto it = range.first; it != range.second; ++it)
+    if ((int)it->second.key.size() == call.words && !std::memcmp(it->second.key.data(), call.key, call.words * sizeof(int64_t)))
+      return &it->second;
+  return nullptr;
+}
+
+long number(PyObject* o) { return o ? PyLong_AsLong(o) : -1; }
+
+bool aligned(const void* a, const void* b = nullptr, const void* c = nullptr, const void* d = nullptr, const void* e = nullptr) {
+  return !(((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)d | (uintptr_t)e) & 15);
+}
+
+// the operators: NotImplemented by a null status pointer's -1 (misaligned), otherwise the entry's status
+constexpr int kElse = -1000;
+
+int run_write(const Call& a, const Plan& p, void* stream, PyObject**) {
+  const auto& c = p.c;
+  void *k = a.p(0), *v = a.p(1), *kc = a.p(2), *ks = a.p(3), *vc = a.p(4), *vs = a.p(5), *kb = a.p(6);
+  if (!aligned(k, v, kc, vc, kb)) return kElse;
+  return ((decltype(&oa_kv8_write))entry[kWrite])(k, c[0], c[1], v, c[2], c[3], c[4], c[5], c[6], c[7], kc, ks, vc, vs, kb, c[8], c[9],
+                                                  c[10], c[11], c[12], (const int*)a.p(7), c[13], c[14], (const int*)a.p(8),
+                                                  (const int*)a.p(9), c[15], stream);
+}
+
+int run_read(const Call& a, const Plan& p, void* stream, PyObject** out) {
+  const auto& c = p.c;                   // page strides, pages, page, tokens, heads, dims, type
+  void *kc = a.p(1), *ks = a.p(2), *vc = a.p(3), *vs = a.p(4);
+  if (!aligned(kc, vc)) return kElse;
+  const auto opt = a.t[1]->options().dtype(c[7] == 2 ? at::kFloat : at::kBFloat16);
+  const at::Tensor k = at::empty({c[4], c[5], c[6]}, opt), v = at::empty({c[4], c[5], c[6]}, opt);
+  const int st = ((decltype(&oa_kv8_read))entry[kRead])((const int*)a.p(0), kc, ks, vc, vs, c[0], c[1], c[2], c[3], k.data_ptr(),
+                                                        c[5] * c[6], c[6], v.data_ptr(), c[5] * c[6], c[6], c[4], c[5], c[6], c[7],
+                                                        stream);
+  if (!st) *out = Py_BuildValue("(NN)", THPVariable_Wrap(k), THPVariable_Wrap(v));
+  return st;
+}
+
+int run_select(const Call& a, const Plan& p, void* stream, PyObject** out) {
+  const auto& c = p.c;
+  void *q = a.p(0), *kb = a.p(2);
+  if (!aligned(q, kb)) return kElse;
+  const auto opt = a.t[3]->options();
+  const at::Tensor o = at::empty({c[8], c[16], c[12]}, opt);
+  at::Tensor ws;
+  if (c[17]) ws = at::empty({c[17]}, opt);
+  const int st = ((decltype(&oa_kv8_select))entry[kSelect])(
+      q, c[0], c[1], c[2], a.p(1), kb, c[3], c[4], c[5], c[6], (const int*)a.p(3), c[18], c[19], (const int*)a.p(4), (const int*)a.p(5),
+      c[7], c[8], c[9], c[10], c[11], c[12], c[13], c[14], c[15], c[17] ? (unsigned*)ws.data_ptr() : nullptr, (int*)o.data_ptr(),
+      stream);
+  if (!st) *out = THPVariable_Wrap(o);
+  return st;
+}
+
+int run_attn(const Call& a, const Plan& p, void* stream, PyObject** out) {
+  const auto& c = p.c;
+  void *q = a.p(0), *kc = a.p(1), *vc = a.p(3);
+  if (!aligned(q, kc, vc)) return kElse;
+  const auto opt = a.t[0]->options();
+  const at::Tensor o = c[20] ? at::zeros({c[0], c[1], c[2]}, opt) : at::empty({c[0], c[1], c[2]}, opt);
+  at::Tensor ws;
+  float* wo = nullptr;
+  if (c[18]) {
+    ws = at::empty({c[18] * (c[2] + 2)}, opt.dtype(at::kFloat));
+    wo = (float*)ws.data_ptr();
+  }
+  const int st = ((decltype(&oa_kv8_attn))entry[kAttn])(
+      q, c[3], c[4], c[5], kc, a.p(2), vc, a.p(4), c[6], c[7], c[8], c[9], (const int*)a.p(5), c[10], c[11], (const int*)a.p(6),
+      (const int*)a.p(7), c[12], c[0], c[13], c[1], c[14], c[2], (float)p.scale, (const int*)a.p(8), c[15], c[16], c[17], wo,
+      wo ? wo + c[18] * c[2] : nullptr, o.data_ptr(), c[1] * c[2], c[2], c[19], stream);
+  if (!st) *out = THPVariable_Wrap(o);
+  return st;
+}
+
+const char* const kNames[kOps] = {"oa_kv8_write", "oa_kv8_read", "oa_kv8_select", "oa_kv8_attn"};
+constexpr size_t kNumbers[kOps] = {16, 8, 20, 21};
+constexpr int kArgs[kOps] = {10, 5, 6, 9};               // tensors, None among them, that come first
+
+// call(op, arguments): the operator's answer, or NotImplemented where Python has to look at the call
+PyObject* call_op(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const long op = n > 0 ? number(args[0]) : -1;
+  if (op < 0 || op >= kOps || !entry[op]) Py_RETURN_NOTIMPLEMENTED;
+  Call a;
+  if (!take(a, op, args + 1, n - 1, nullptr) || a.count < kArgs[op]) Py_RETURN_NOTIMPLEMENTED;
+  const Plan* plan = find(a, hash_of(a.key, a.words));
+  if (!plan) Py_RETURN_NOTIMPLEMENTED;
+  PyObject* d = PyObject_CallNoArgs(get_device);
+  if (!d) return nullptr;
+  const long current = PyLong_AsLong(d);
+  Py_DECREF(d);
+  if (current != a.device) Py_RETURN_NOTIMPLEMENTED;
+  PyObject* which = PyLong_FromLong(a.device);
+  PyObject* s = which ? PyObject_CallOneArg(raw_stream, which) : nullptr;
+  Py_XDECREF(which);
+  if (!s) return nullptr;
+  void* stream = PyLong_AsVoidPtr(s);
+  Py_DECREF(s);
+  if (PyErr_Occurred()) return nullptr;
+  PyObject* out = nullptr;
+  constexpr int (*run[kOps])(const Call&, const Plan&, void*, PyObject**) = {run_write, run_read, run_select, run_attn};
+  const int st = run[op](a, *plan, stream, &out);
+  if (st == kElse) Py_RETURN_NOTIMPLEMENTED;
+  if (st) return PyErr_Format(PyExc_RuntimeError, "%s failed with status %d", kNames[op], st);
+  if (op == kWrite) Py_RETURN_NONE;
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
+// keep(op, numbers, scale, arguments): the plan of later calls with such arguments
+PyObject* keep(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const long op = n > 2 ? number(args[0]) : -1;
+  if (op < 0 || op >= kOps || !PyTuple_CheckExact(args[1]) || !PyFloat_CheckExact(args[2]) ||
+      (size_t)PyTuple_GET_SIZE(args[1]) != kNumbers[op])
+    return PyErr_Format(PyExc_ValueError, "keep: an operator, its numbers and a scale");
+  Call a;
+  Plan p;
+  if (!take(a, op, args + 3, n - 3, &p.held) || a.count < kArgs[op]) Py_RETURN_NONE;
+  for (size_t i = 0; i < kNumbers[op]; ++i) {
+    p.c.push_back(PyLong_AsLongLong(PyTuple_GET_ITEM(args[1], i)));
+    if (PyErr_Occurred()) return nullptr;
+  }
+  const uint64_t h = hash_of(a.key, a.words);
+  if (find(a, h)) Py_RETURN_NONE;
+  if (plans.size() >= kPlans) {
+    std::unordered_multimap<uint64_t, Plan> old;
+    old.swap(plans);
+    for (auto& x : old)
+      for (PyObject* o : x.second.held) Py_DECREF(o);
+  }
+  p.key.assign(a.key, a.key + a.words);
+  p.scale = PyFloat_AS_DOUBLE(args[2]);
+  for (PyObject* o : p.held) Py_INCREF(o);
+  plans.emplace(h, std::move(p));
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+// bind(addresses of the entry points, torch's raw stream of a device, the current device)
+PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 3 || !PyTuple_CheckExact(args[0]) || PyTuple_GET_SIZE(args[0]) != kOps)
+    return PyErr_Format(PyExc_ValueError, "bind: %d addresses and two functions", (int)kOps);
+  void* at[kOps];
+  for (int i = 0; i < kOps; ++i) {
+    at[i] = PyLong_AsVoidPtr(PyTuple_GET_ITEM(args[0], i));
+    if (PyErr_Occurred()) return nullptr;
+  }
+  std::memcpy(entry, at, sizeof entry);
+  Py_INCREF(args[1]);
+  Py_INCREF(args[2]);
+  Py_XDECREF(raw_stream);
+  Py_XDECREF(get_device);
+  raw_stream = args[1];
+  get_device = args[2];
+  Py_RETURN_NONE;
+}
+
+// what this was built for: torch's version, the revision of the entry points
+PyObject* built_for(PyObject*, PyObject*) { return Py_BuildValue("(si)", TORCH_VERSION, OA_KV8_REVISION); }
+
+PyObject* kept(PyObject*, PyObject*) { return PyLong_FromSize_t(plans.size()); }
+
+PyMethodDef methods[] = {{"call", (PyCFunction)(void (*)(void))call_op, METH_FASTCALL, nullptr},
+                         {"keep", (PyCFunction)(void (*)(void))keep, METH_FASTCALL, nullptr},
+                         {"bind", (PyCFunction)(void (*)(void))bind, METH_FASTCALL, nullptr},
+                         {"built_for", built_for, METH_NOARGS, nullptr},
+                         {"kept", kept, METH_NOARGS, nullptr},
+                         {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_oa_fast", nullptr, -1, methods};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__oa_fast(void) { return PyModule_Create(&module); }

@@ -157,3 +157,33 @@ def call(name: str, *args) -> None:
         msg = lib.oa_error_string(st).decode()
         sizes = [a for a in args if isinstance(a, (int, float)) and not isinstance(a, bool)]
         raise RuntimeError(f"{name} failed with status {st}: {msg} (numeric arguments {sizes})")
+
+
+_FAST = None
+
+
+def fast():
+    """The module that repeats calls of the 8-bit cache's operators without Python's part (csrc/oa_fast.cpp), bound to the
+    library; raises if it has not been built, or for another torch or other entry points."""
+    global _FAST
+    if _FAST is not None:
+        return _FAST
+    lib, path = load(), _build.fast_path()
+    if not os.path.exists(path):
+        raise RuntimeError(f"host module not built: {path} (run __graft_entry__.build())")
+    import importlib.machinery
+    import importlib.util
+    loader = importlib.machinery.ExtensionFileLoader("_oa_fast", path)
+    try:
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_oa_fast", loader))
+        loader.exec_module(module)
+    except ImportError as e:
+        raise RuntimeError(f"host module {path} does not load ({e}): rebuild it (__graft_entry__.build())") from e
+    have, want = module.built_for(), (torch.__version__.split("+")[0], KV8_REVISION)
+    if have != want:
+        raise RuntimeError(f"host module {path} was built for torch and revision {have}, not {want}: rebuild it "
+                           "(__graft_entry__.build())")
+    module.bind(tuple(ct.cast(getattr(lib, n), ct.c_void_p).value for n in ("oa_kv8_write", "oa_kv8_read", "oa_kv8_select", "oa_kv8_attn")),
+                torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice)
+    _FAST = module
+    return module

@@ -1063,7 +1063,20 @@ def kv4_attn(q, kc, ks, vc, vs, table, lens, sm_scale: float | None = None, cu_q
 
 
 # ================================================================== 8-bit paged cache
+# What was said of the 4-bit cache's checks goes further here: a call's plan, once Python has made it, is kept in a host
+# module (csrc/oa_fast.cpp) under the sizes, strides, types and numbers that it depends on, and later calls with such
+# arguments go there first.  It answers NotImplemented wherever something has to be looked at.
 _PAGES8 = (32, 64, 128)    # tokens of a block, which share a scale and bounds
+_WRITE8, _READ8, _SELECT8, _ATTN8 = range(4)
+_fast = None               # the module, from the first call that was checked
+
+
+def _keep(op: int, numbers: tuple, scale: float, *args) -> None:
+    """The plan of a call that has been made: `numbers` as the module's function for it takes them."""
+    global _fast
+    if _fast is None:
+        _fast = lib.fast()
+    _fast.keep(op, tuple(map(int, numbers)), scale, *args)
 
 
 @_sizes
@@ -1133,6 +1146,8 @@ def kv8_write(k, v, kc, ks, vc, vs, kb, table, lens, cu=None) -> None:
     row with a value that is not finite is held as NaN.  Sequences longer than their table row, tokens of negative
     position and pages outside of the cache are passed over.  A page that two sequences of one call write into ends as
     some mixture."""
+    if _fast is not None and _fast.call(_WRITE8, k, v, kc, ks, vc, vs, kb, table, lens, cu) is not NotImplemented:
+        return
     i = _where(k, v, kc, ks, vc, vs, kb, table, lens, cu)
     ps, where, HKV, Dh = _kv8_cache(kc, ks, vc, vs)
     b0 = 0 if kb is None else _bound_sizes(kb.shape, kb.stride(), kb.dtype, where[2], HKV, Dh)
@@ -1144,11 +1159,17 @@ def kv8_write(k, v, kc, ks, vc, vs, kb, table, lens, cu=None) -> None:
         _aligned(kp | vp | (bp or 0))
     _run(i, "oa_kv8_write", kp, *kst, vp, *vst, *sizes, *ps, bp, where[0], where[1], b0, where[2], where[3],
          table.data_ptr(), *tsz, lens.data_ptr(), _ptr(cu), B)
+    _keep(_WRITE8, (*kst, *vst, *sizes, where[0], where[1], b0, where[2], where[3], *tsz, B), 0.0, k, v, kc, ks, vc, vs, kb, table,
+          lens, cu)
 
 
 def kv8_read(slots, kc, ks, vc, vs, dtype: torch.dtype = torch.bfloat16):
     """The values (k, v), each (T, HKV, D) bf16 (which holds them exactly) or fp32, at slots (T,) int32 = page id * page +
     offset of an 8-bit cache; zeros for a slot outside of it."""
+    if _fast is not None:
+        got = _fast.call(_READ8, slots, kc, ks, vc, vs, dtype)
+        if got is not NotImplemented:
+            return got
     i = _where(slots, kc, ks, vc, vs)
     ps, where, HKV, Dh = _kv8_cache(kc, ks, vc, vs)
     T = slots.shape[0] if slots.dim() == 1 else 0
@@ -1159,6 +1180,7 @@ def kv8_read(slots, kc, ks, vc, vs, dtype: torch.dtype = torch.bfloat16):
     v = kc.new_empty(T, HKV, Dh, dtype=dtype)
     _run(i, "oa_kv8_read", slots.data_ptr(), *ps, *where, k.data_ptr(), HKV * Dh, Dh, v.data_ptr(), HKV * Dh, Dh, T, HKV, Dh,
          _DT[dtype])
+    _keep(_READ8, (*where, T, HKV, Dh, _DT[dtype]), 0.0, slots, kc, ks, vc, vs, dtype)
     return k, v
 
 
@@ -1204,6 +1226,10 @@ def kv8_select(q, ks, kb, table, lens, page: int, n: int, cu_q=None, first: int 
     lens that the caller knows.  -1 alone: tokens that no sequence takes, and those of sequences longer than their
     table row or than max_len (rounded up to whole pages).  Over more than 1024 blocks (or 16 query heads to a KV head) a
     workspace of T HKV blocks integers is taken from torch's allocator."""
+    if _fast is not None:
+        got = _fast.call(_SELECT8, q, ks, kb, table, lens, cu_q, page, n, first, last, max_len)
+        if got is not NotImplemented:
+            return got
     i = _where(q, ks, kb, table, lens, cu_q)
     T, HKV, qst, dt, where, tsz, sizes, scores = _select_sizes(
         q.shape, q.stride(), q.dtype, ks.shape, ks.stride(), ks.dtype, kb.shape, kb.stride(), kb.dtype, table.shape,
@@ -1217,6 +1243,8 @@ def kv8_select(q, ks, kb, table, lens, page: int, n: int, cu_q=None, first: int 
     ws = table.new_empty(scores) if scores else None
     _run(i, "oa_kv8_select", qp, *qst, dt, ks.data_ptr(), bp, *where, table.data_ptr(), *tsz, lens.data_ptr(), _ptr(cu_q),
          *sizes, _ptr(ws), out.data_ptr())
+    if T:
+        _keep(_SELECT8, (*qst, dt, *where, *sizes, HKV, scores, *tsz), 0.0, q, ks, kb, table, lens, cu_q, page, n, first, last, max_len)
     return out
 
 
@@ -1294,6 +1322,10 @@ def kv8_attn(q, kc, ks, vc, vs, table, lens, sm_scale: float | None = None, cu_q
     that no sequence takes, and tokens past max_q, are left as they were (0 where the call makes it); `out` shares no
     memory with the other tensors.  Sums are held in fp32 and not divided before their end: values up to 2^80 are safe at
     any length."""
+    if _fast is not None and out is None:
+        got = _fast.call(_ATTN8, q, kc, ks, vc, vs, table, lens, cu_q, blocks, sm_scale, max_q, max_len, kv8_chunk)
+        if got is not NotImplemented:
+            return got
     i = _where(q, kc, ks, vc, vs, table, lens, cu_q, blocks, out)
     ps, where, HKV, Dh = _kv8_cache(kc, ks, vc, vs)
     T, HQ, B, qst, ost, dt, tsz, sizes, pieces, parts, lie = _attn8_sizes(
@@ -1321,6 +1353,9 @@ def kv8_attn(q, kc, ks, vc, vs, table, lens, sm_scale: float | None = None, cu_q
         mp = wp + 4 * parts * Dh
     _run(i, "oa_kv8_attn", qp, *qst, dt, *ps, *where, table.data_ptr(), *tsz, lens.data_ptr(), _ptr(cu_q), *sizes, _ptr(blocks),
          *pieces, wp, mp, op, *ost, clear)
+    if not given:
+        _keep(_ATTN8, (T, HQ, Dh, *qst, dt, *where, *tsz, B, sizes[2], HKV, *pieces, parts, clear, not (clear or cu_q is None)),
+              float(sizes[6]), q, kc, ks, vc, vs, table, lens, cu_q, blocks, sm_scale, max_q, max_len, kv8_chunk)
     return out
 
 # ================================================================== prefill index build
