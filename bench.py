@@ -67,6 +67,10 @@ def parse():
                    help="batch sizes of --config5, comma-separated (default 1,32)")
     p.add_argument("--kv4", action="store_true",
                    help="with --config5: the same decode step over a 4-bit paged cache (KV4Cache) instead")
+    p.add_argument("--kv8", action="store_true",
+                   help="with --config5: the same decode step over an 8-bit paged cache (KV8Cache) instead")
+    p.add_argument("--blocks", type=int, default=None,
+                   help="with --config5 --kv8: read only so many blocks of 64 tokens for every sequence and KV head")
     p.add_argument("--config4", action="store_true",
                    help="long-context sweep instead: B=8, N in {65536, 131072}, 1%% and 3%%, 512-centre "
                         "mixture with 8 needles per KV head; one JSON line per point (us/layer-step, "
@@ -381,14 +385,15 @@ def config5_run(a):
         torch.cuda.empty_cache()
 
 
-def config5_kv4_run(a):
-    """The whole decode step of config5_run over a 4-bit paged cache: the prompt prefilled through the model
+def config5_paged_run(a):
+    """The whole decode step of config5_run over a 4-bit or 8-bit paged cache: the prompt prefilled through the model
     (dense causal attention, K/V written to the cache's pages), then the step -- pages extended on the
-    device, 32 x (RMSNorm, QKV, RoPE, K/V rounded into their slots, attention over the pages, O, RMSNorm,
-    SwiGLU), final norm, LM head, greedy token -- captured in one hipGraph and replayed over page borders."""
+    device, 32 x (RMSNorm, QKV, RoPE, K/V rounded into their slots, attention over the pages or over the blocks
+    chosen of them, O, RMSNorm, SwiGLU), final norm, LM head, greedy token -- captured in one hipGraph and
+    replayed over page borders."""
     import torch
 
-    from openattention_amd import KV4Cache, _build, lib
+    from openattention_amd import KV4Cache, KV8Cache, _build, lib
     if not os.path.exists(_build.lib_path()):
         _build.build()
     lib.load()
@@ -399,8 +404,8 @@ def config5_kv4_run(a):
     N = a.ctx
     for B in (int(x) for x in a.c5_batches.split(",")):
         cap = N + a.warmup + a.steps + 4
-        cache = KV4Cache(B, cap, dev, layers=NLAYER)
-        model = LlamaShaped(B, cap, dev, cache=cache)
+        cache = (KV8Cache if a.kv8 else KV4Cache)(B, cap, dev, layers=NLAYER)
+        model = LlamaShaped(B, cap, dev, cache=cache, blocks=a.blocks)
         tokens = torch.randint(0, VOCAB, (B, N), generator=torch.Generator(device="cpu").manual_seed(1000 + B)).to(dev)
         if B == 1:
             model.prefill(tokens[:, :4096])                 # (first-call set-up is not part of a request's prefill)
@@ -410,7 +415,8 @@ def config5_kv4_run(a):
         model.prefill(tokens)
         torch.cuda.synchronize()
         prefill_s = time.time() - p0
-        log(f"[config5 kv4] B={B}: prompt of {N} tokens prefilled through {NLAYER} layers in {prefill_s:.1f}s")
+        name = "kv8" if a.kv8 else "kv4"
+        log(f"[config5 {name}] B={B}: prompt of {N} tokens prefilled through {NLAYER} layers in {prefill_s:.1f}s")
         s = torch.cuda.Stream()
         s.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(s):
@@ -430,10 +436,12 @@ def config5_kv4_run(a):
         torch.cuda.synchronize()
         cache.check()
         ms = e0.elapsed_time(e1) / a.steps
-        rec = {"config": "config5", "cache": "kv4 (4.25 bits a value, pages of 64)",
+        size = D + (2 + 2 * D) / (2 * cache.page) if a.kv8 else D // 2 + D // 32          # bytes of a token and head of K or V
+        rec = {"config": "config5", "cache": "kv8 (8.1 bits a value, pages of 64)" if a.kv8 else "kv4 (4.25 bits a value, pages of 64)",
+               "blocks": a.blocks,
                "model": "Llama-3.1-8B-shaped, random-init bf16 weights", "params": model.params(), "layers": NLAYER, "B": B,
                "N": N, "ms_per_step": round(ms, 3), "tokens_per_s": round(B / (ms * 1e-3), 1),
-               "cache_bytes_per_token": NLAYER * 2 * HKV * (D // 2 + D // 32), "prefill_s": round(prefill_s, 2),
+               "cache_bytes_per_token": round(NLAYER * 2 * HKV * size), "prefill_s": round(prefill_s, 2),
                "data": "synthetic: a 32K random-token prompt per sequence prefilled through the model; decode steps run "
                        "through the full model"}
         print(json.dumps(rec), flush=True)
@@ -547,7 +555,7 @@ def main():
         config4_sweep(a)
         return
     if a.config5:
-        config5_kv4_run(a) if a.kv4 else config5_run(a)
+        config5_paged_run(a) if a.kv4 or a.kv8 else config5_run(a)
         return
     if a.pmc_calibration:
         pmc_calibration()

@@ -11,9 +11,10 @@ token -- is captured once in a hipGraph and replayed with n advancing on the dev
 
 With `method` an OursHIP the attention is its decode (the gfx950 sparse stage); with
 method = None it is the dense split-K decode kernel over [0, n) on the same cache.  With `cache` a
-KV4Cache keys and values are held in 4 bits in its pages instead: the step extends every sequence by
-its token, and positions and lengths are the cache's, one for each sequence.  `qk_norm` gives every
-layer norms of the query and key heads.
+KV4Cache or a KV8Cache keys and values are held in 4 or 8 bits in its pages instead: the step extends every
+sequence by its token, and positions and lengths are the cache's, one for each sequence.  With `blocks` a step
+reads of a KV8Cache only so many blocks for every sequence and KV head, those whose keys can score highest.
+`qk_norm` gives every layer norms of the query and key heads.
 
 `prefill` runs a prompt through the model one batch row at a time, as the reference's runner
 does (graph_runner.py:615-622): every layer's attention goes through the hook's prefill branch
@@ -29,6 +30,7 @@ import torch
 import types
 
 from openattention_amd import ops
+from openattention_amd.kv8 import KV8Cache
 from openattention_amd.method import C as CTX, Method, attn_hook, prefill_attention
 from openattention_amd.synth import llama31_inv_freq
 
@@ -52,15 +54,18 @@ def rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
 
 class LlamaShaped:
     def __init__(self, B: int, Lmax: int, dev, layers: int = NLAYER, seed: int = 0, method=None, cache=None,
-                 qk_norm: bool = False):
+                 qk_norm: bool = False, blocks: int | None = None):
         """method: an OursHIP over these layers (sparse attention) or None (dense attention).
         The KV cache is C.K / C.V (set by the caller), (B, 8, Lmax, 128) bf16 per layer, or `cache`, a
-        KV4Cache of B requests and these layers (method None): steps go on to the end of its pages, also
-        past Lmax."""
+        KV4Cache or KV8Cache of B requests and these layers (method None): steps go on to the end of its pages, also
+        past Lmax.  blocks: a step's attention reads that many blocks (at least 3) of a KV8Cache (KV8Cache.select);
+        prompts are attended to densely."""
+        if blocks is not None and (not isinstance(cache, KV8Cache) or blocks < 3):
+            raise ValueError("blocks: at least 3, of a KV8Cache")
         if cache is not None and (method is not None or cache.B != B or cache.layers != layers):
             raise ValueError("cache: for B requests and these layers, without a method")
         self.B, self.Lmax, self.dev, self.L = B, Lmax, dev, layers
-        self.method, self.cache, self.qk_norm = method, cache, qk_norm
+        self.method, self.cache, self.qk_norm, self.blocks = method, cache, qk_norm, blocks
         g = torch.Generator(device=dev).manual_seed(seed)
 
         def w(*shape):
@@ -77,7 +82,7 @@ class LlamaShaped:
         self.lnf = torch.ones(HID, **bf)
         self.lm_head = w(HID, VOCAB)
         inv = llama31_inv_freq().to(dev)
-        P = Lmax if cache is None else max(Lmax, cache.width * cache.page)      # (a 4-bit cache's length is in whole pages)
+        P = Lmax if cache is None else max(Lmax, cache.width * cache.page)      # (a paged cache's length is in whole pages)
         t = torch.arange(P, device=dev, dtype=torch.float32)
         fr = torch.outer(t, inv)
         emb = torch.cat([fr, fr], -1)
@@ -124,7 +129,7 @@ class LlamaShaped:
         layers (graph_runner.py:615-622).  Each layer's attention is attn_hook's prefill branch:
         the row's K, V are written to C.K[l][b, :, :T], its causal attention is dense and the
         method builds the row's index (C.qlen[b] = qlen question rows).  Leaves C.phase at
-        "decode" and the greedy next token of every row in self.tok; returns it.  With a 4-bit cache the
+        "decode" and the greedy next token of every row in self.tok; returns it.  With a paged cache the
         rows extend its requests (empty ones; all of them, or none where the cache refuses: RuntimeError), a
         row's keys and values are written to the new slots and its own attention is dense over the unrounded
         rows."""
@@ -167,18 +172,22 @@ class LlamaShaped:
         B, T = tokens.shape
         cache = self.cache
         if bool((cache.lens != 0).any()):
-            raise ValueError("prefill: the cache's requests must be empty (KV4Cache.truncate)")
+            raise ValueError("prefill: the cache's requests must be empty (truncate)")
         cache.check()                                                              # (an earlier call's refusal)
-        slots, pos, _ = cache.extend(torch.full_like(cache.lens, T), B * T)        # all requests or none
+        slots, pos, cu = cache.extend(torch.full_like(cache.lens, T), B * T)       # all requests or none
         cache.check()
         where = pos[:T]
+        eight = isinstance(cache, KV8Cache)
         for b in range(B):
             at = slots[b * T:(b + 1) * T]
             x = self.embed.index_select(0, tokens[b])                              # (T, HID)
             for l in range(self.L):
                 h = rmsnorm(x, self.ln1[l])
                 q, k, v = self._qkv(l, h @ self.wqkv[l], where)
-                cache.write(l, k, v, at)
+                if eight:
+                    cache.write(l, k, v, cu[:2], b)                                # (0 and T)
+                else:
+                    cache.write(l, k, v, at)
                 o = prefill_attention(*(t.transpose(0, 1).unsqueeze(0) for t in (q, k, v)), D ** -0.5)
                 x = x + o[0].transpose(0, 1).reshape(T, HQ * D) @ self.wo[l]
                 del q, k, v, o
@@ -192,13 +201,18 @@ class LlamaShaped:
 
     def _step_cache(self) -> torch.Tensor:
         B, cache = self.B, self.cache
-        slots, pos, _ = cache.extend()
+        slots, pos, cu = cache.extend()
+        eight = isinstance(cache, KV8Cache)
         x = self.embed.index_select(0, self.tok)                        # (B, HID)
         for l in range(self.L):
             h = rmsnorm(x, self.ln1[l])
             q, k, v = self._qkv(l, h @ self.wqkv[l], pos)
-            cache.write(l, k, v, slots)
-            x = x + cache.attend(l, q).view(B, HQ * D) @ self.wo[l]
+            cache.write(l, k, v, cu if eight else slots)
+            if self.blocks is None:
+                o = cache.attend(l, q)
+            else:
+                o = cache.attend(l, q, blocks=cache.select(l, q, self.blocks))
+            x = x + o.view(B, HQ * D) @ self.wo[l]
             h = rmsnorm(x, self.ln2[l])
             gu = h @ self.w13[l]
             x = x + (torch.nn.functional.silu(gu[:, :FFN]) * gu[:, FFN:]) @ self.w2[l]
@@ -211,9 +225,9 @@ class LlamaShaped:
     def step(self, n: int | None = None) -> torch.Tensor:
         """One decode step: the token in self.tok sits at position n - 1 (n = C.n_dev on the
         device; the host n only fixes the sparse stage's sink/local/top-k counts).  Writes the
-        greedy next token into self.tok and returns it.  With a 4-bit cache n is not used: each token
+        greedy next token into self.tok and returns it.  With a paged cache n is not used: each token
         sits at its request's length, which the step extends (a step that the cache refuses, out of
-        pages or past max_len, leaves lengths, rows and self.tok as they were: KV4Cache.check)."""
+        pages or past max_len, leaves lengths, rows and self.tok as they were: its check())."""
         if self.cache is not None:
             return self._step_cache()
         B = self.B
