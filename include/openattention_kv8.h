@@ -54,7 +54,7 @@ int oa_kv8_read(const int* slots, const void* kc, const void* ks, const void* vc
  * the smallest with |q8| <= 127 for the heads together; values of q that are not finite count as 0, a block whose page
  * id lies outside of the cache comes last.  cap: blocks (at most width) that sequences hold at most; -1 alone: rows that
  * no sequence takes, sequences of more than cap blocks.  ws: tokens * kv_heads * cap ints of scratch (NULL will do where
- * cap <= n, and for cap <= 1024 with at most 16 query heads to a KV head).
+ * cap <= n, and for cap <= 1024 with 2 to 16 query heads to a KV head, cap <= 512 with one).
  */
 int oa_kv8_select(const void* q, long q_st, long q_sh, int dtype, const void* ks, const void* kb, long scale_stride,
                   long bound_stride, int pages, int page, const int* table, long table_stride, int width, const int* lens,

@@ -11,8 +11,8 @@
 // last; several tokens where heads are few) against 16 blocks, both sides as [max(x, 0), max(-x, 0)].  A lane ends with
 // the scores of one block for four rows, so that the largest over four heads takes no exchange.  They are kept as
 // integers of the same order.
-//   up to 1024 blocks  one launch: a workgroup scores all blocks of a tile's tokens into LDS, then a wave chooses for a
-//                      token (choose);
+//   up to 1024 blocks  (512 where a KV head has one query head) one launch: a workgroup scores all blocks of a tile's
+//                      tokens into LDS, then a wave chooses for a token (choose);
 //   more               scores into a workspace by as many workgroups as there are spans of 128 blocks, then a
 //                      workgroup for each token and head finds the last score that is chosen by four passes over its
 //                      bytes, counted in LDS.
@@ -24,6 +24,7 @@ namespace {
 using namespace kv8;
 
 typedef int int4v __attribute__((ext_vector_type(4)));
+typedef unsigned uint4v __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
@@ -73,55 +74,74 @@ __device__ __forceinline__ unsigned max_heads(unsigned v) {        // over GP la
   return max(y[0], y[1]);
 }
 
+// what the lanes of a wave exchange through LDS stays in program order (the LDS keeps it)
+__device__ __forceinline__ void lane_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local"); }
+
 // scores as integers of the same order
 __device__ __forceinline__ unsigned key_of(float f) {
   const unsigned u = __float_as_uint(f);
   return u ^ ((int)u < 0 ? 0xffffffffu : 0x80000000u);
 }
 
-// The tile's query rows as operands: lane (row, g) holds dims 16 g and on of each 64, their positive parts first.  GP:
-// rows of a token in a tile, the heads rounded up to a power of two.
-template <typename T, int D, int GP>
-__device__ __forceinline__ void query_rows(const SelectArgs& a, const Seq& sq, int j0, int h, int4v (&Q)[D / 32]) {
-  constexpr int kPieces = D / 64;
+// The tile's query rows: lane (row, g) holds dims 16 g and on of each 64.  GP: rows of a token in a tile, the heads
+// rounded up to a power of two.
+template <typename T, int D>
+struct Rows {
   typedef std::conditional_t<std::is_same<T, __bf16>::value, bf16x8, f16x8> vec;
-  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
-  const int row = min(j0 + col / GP, sq.R - 1), hd = col % GP;
-  const T* const q = (const T*)a.q + (long)(sq.r0 + row) * a.q_st + (long)h * a.G * a.q_sh + 16 * g;
+  vec x[D / 64][2];
+};
+template <typename T, int D, int GP>
+__device__ __forceinline__ const T* row_of(const SelectArgs& a, const Seq& sq, int j0, int h) {
+  const int lane = threadIdx.x & 63, row = min(j0 + (lane & 15) / GP, sq.R - 1);
+  return (const T*)a.q + (long)(sq.r0 + row) * a.q_st + (long)h * a.G * a.q_sh + 16 * (lane >> 4);
+}
+template <typename T, int D>
+__device__ __forceinline__ void fetch_row(Rows<T, D>& t, const T* p) {
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+    for (int y = 0; y < 2; ++y) t.x[i][y] = *reinterpret_cast<const typename Rows<T, D>::vec*>(p + 64 * i + 8 * y);
+}
+// the lane's own head of this launch
+template <int GP>
+__device__ __forceinline__ int head_of(const SelectArgs& a) { return min(a.head0 + (int)(threadIdx.x & 15) % GP, a.G - 1); }
+
+// rows as operands: their positive parts first, then the negative ones'
+template <typename T, int D, int GP>
+__device__ __forceinline__ void quantise(const SelectArgs& a, const Rows<T, D>& own, const T* row, int4v (&Q)[D / 32]) {
+  constexpr int kPieces = D / 64;
   f32x8 x[kPieces][2];
-  unsigned top = 0;
-  auto fetch = [&](int head) {
+  auto load = [&](const Rows<T, D>& r) {                   // the largest |x|; values that are not finite count as 0
+    unsigned top = 0;
 #pragma unroll
     for (int p = 0; p < kPieces; ++p)
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        x[p][y] = __builtin_convertvector(*reinterpret_cast<const vec*>(q + (long)head * a.q_sh + 64 * p + 8 * y), f32x8);
+        x[p][y] = __builtin_convertvector(r.x[p][y], f32x8);
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[p][y][i]) & 0x7fffffffu);
       }
-  };
-  auto finite = [&] {                    // values that are not count as 0
-    top = 0;
-#pragma unroll
-    for (int p = 0; p < kPieces; ++p)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const unsigned u = __float_as_uint(x[p][i >> 3][i & 7]) & 0x7fffffffu;
-        if (u >= 0x7f800000u) x[p][i >> 3][i & 7] = 0.f;
-        else top = max(top, u);
-      }
-  };
-  unsigned others = 0;
-  if (GP == 16)                          // (more heads than rows: the scale is that of all of them)
-    for (int i = hd + (a.head0 ? 0 : 16); i < a.G; i += 16) {
-      fetch(i);
-      if (__any(top >= 0x7f800000u)) finite();
-      others = max(others, top);
+    if (__any(top >= 0x7f800000u)) {
       top = 0;
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const unsigned u = __float_as_uint(x[p][i >> 3][i & 7]) & 0x7fffffffu;
+          if (u >= 0x7f800000u) x[p][i >> 3][i & 7] = 0.f;
+          else top = max(top, u);
+        }
     }
-  fetch(min(a.head0 + hd, a.G - 1));
-  if (__any(top >= 0x7f800000u)) finite();
-  top = max_heads<GP>(max(top, others));
+    return top;
+  };
+  unsigned top = 0;
+  if (GP == 16)                          // (more heads than rows: the scale is that of all of them)
+    for (int i = (int)(threadIdx.x & 15) + (a.head0 ? 0 : 16); i < a.G; i += 16) {
+      Rows<T, D> other;
+      fetch_row(other, row + (long)i * a.q_sh);
+      top = max(top, load(other));
+    }
+  top = max_heads<GP>(max(top, load(own)));
   // the smallest u with top <= 127 2^u; q / 2^u rounded in the sum with 1.5 * 2^23, whose low byte is then the number
   const float f = power(-max((int)((top + 0x1ffffu) >> 23) - 133, -120));
 #pragma unroll
@@ -138,7 +158,8 @@ __device__ __forceinline__ void query_rows(const SelectArgs& a, const Seq& sq, i
     }
 }
 
-// a lane's part of 16 blocks' bounds: block lane % 16, bytes 16 g and on of each 64; and its scale
+// 16 blocks' bounds as they lie in memory, 256 (D = 64: 128) successive bytes of a block, 16 of them to a lane; and the
+// scale of block lane % 16.  `page`: its page.
 template <int D>
 struct Bounds {
   int4v b[D / 32];
@@ -147,22 +168,44 @@ struct Bounds {
 };
 template <int D>
 __device__ __forceinline__ void fetch_bounds(const SelectArgs& a, Bounds<D>& t, unsigned page, int h) {
+  constexpr int kLanes = D / 8;          // lanes of a block
+  const int lane = threadIdx.x & 63;
   t.bad = page >= (unsigned)a.NP;
-  const long pg = t.bad ? 0 : page;
-  const int4v* kb = reinterpret_cast<const int4v*>(a.kb + pg * a.b_sp + (long)h * (2 * D) + 16 * ((threadIdx.x & 63) >> 4));
-  t.s = a.ks[pg * a.s_sp + h];
+  const unsigned pg = t.bad ? 0 : page;
 #pragma unroll
-  for (int s = 0; s < D / 32; ++s) t.b[s] = kb[4 * s];
+  for (int n = 0; n < D / 32; ++n) {
+    const unsigned from = (unsigned)__builtin_amdgcn_ds_bpermute(4 * (lane / kLanes + n * (64 / kLanes)), (int)pg);
+    t.b[n] = *reinterpret_cast<const int4v*>(a.kb + (long)from * a.b_sp + (long)h * (2 * D) + 16 * (lane % kLanes));
+  }
+  t.s = a.ks[(long)pg * a.s_sp + h];
+}
+// The blocks through the wave's part of LDS (32 D bytes) into operands: lane (block, g) takes bytes 16 g and on of
+// each 64.  (Loaded in that order every access touches half lines: two questions' blocks 15.3 us for ...)  16-byte
+// chunk c of row r lies at c ^ f(r), so that 16 rows read at one chunk spread over all banks.
+template <int D>
+__device__ __forceinline__ void turn(const Bounds<D>& t, char* lds, int4v (&b)[D / 32]) {
+  constexpr int kLanes = D / 8;
+  auto place = [](int r, int c) { return r * (2 * D) + ((c ^ (D == 128 ? r & 15 : (r >> 1) & 7)) << 4); };
+  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int n = 0; n < D / 32; ++n)
+    *reinterpret_cast<int4v*>(lds + place(lane / kLanes + n * (64 / kLanes), lane % kLanes)) = t.b[n];
+  lane_order();
+#pragma unroll
+  for (int s = 0; s < D / 32; ++s) b[s] = *reinterpret_cast<const int4v*>(lds + place(col, 4 * s + g));
+  lane_order();
 }
 
 // The scores of the tile's tokens for this lane's block, as integers of the same order, given to put(token of the tile,
 // key).
 template <int D, int GP, typename Put>
-__device__ __forceinline__ void score_tile(const int4v (&Q)[D / 32], const Bounds<D>& t, Put put) {
+__device__ __forceinline__ void score_tile(const int4v (&Q)[D / 32], const Bounds<D>& t, char* lds, Put put) {
   const int g = (threadIdx.x & 63) >> 4;
+  int4v b[D / 32];
+  turn(t, lds, b);
   int4v S = int4v(0);
 #pragma unroll
-  for (int s = 0; s < D / 32; ++s) S = __builtin_amdgcn_mfma_i32_16x16x64_i8(Q[s], t.b[s], S, 0, 0, 0);
+  for (int s = 0; s < D / 32; ++s) S = __builtin_amdgcn_mfma_i32_16x16x64_i8(Q[s], b[s], S, 0, 0, 0);
   // S[i]: row 4 g + i, this lane's block
   int best[4] = {S[0], S[1], S[2], S[3]};
   constexpr int kOut = GP == 1 ? 4 : GP == 2 ? 2 : 1;
@@ -191,6 +234,7 @@ __device__ __forceinline__ void score_tile(const int4v (&Q)[D / 32], const Bound
 template <typename T, int D, int GP>
 __global__ void __launch_bounds__(kThreads) kv8_score_kernel(SelectArgs a) {
   constexpr int kTokens = 16 / GP;
+  __shared__ __align__(16) char s_turn[kWaves][32 * D];
   const int wave = threadIdx.x >> 6, col = threadIdx.x & 15;
   const int h = blockIdx.x % a.HKV, id = blockIdx.x / a.HKV;
   const int b = a.cu ? sequence_of(a.B, id, [&](int i) { return a.cu[i] / kTokens + 2 * i; }) : id;
@@ -209,32 +253,47 @@ __global__ void __launch_bounds__(kThreads) kv8_score_kernel(SelectArgs a) {
   if (j0 < 0 || j0 >= sq.R) return;
   const int pos = sq.n - sq.R + min(j0 + kTokens, sq.R) - 1, seen = pos < 0 ? 0 : (pos >> a.lp) + 1;
   if (seen <= a.n || from >= seen) return;               // (all blocks are chosen, or none are here)
+  // (the rows are requested first: answers come back in order)
+  const T* const row = row_of<T, D, GP>(a, sq, j0, h);
+  Rows<T, D> own;
+  fetch_row(own, row + (long)head_of<GP>(a) * a.q_sh);
   Bounds<D> t[2];
 #pragma unroll
   for (int x = 0; x < 2; ++x) fetch_bounds(a, t[x], page[x], h);
   int4v Q[D / 32];
-  query_rows<T, D, GP>(a, sq, j0, h, Q);
+  quantise<T, D, GP>(a, own, row, Q);
 #pragma unroll
   for (int x = 0; x < 2; ++x)
-    score_tile<D, GP>(Q, t[x], [&](int tok, unsigned key) {
+    score_tile<D, GP>(Q, t[x], s_turn[wave], [&](int tok, unsigned key) {
       if (at[x] >= seen || j0 + tok >= sq.R) return;
       unsigned* const to = a.ws + ((long)(sq.r0 + j0 + tok) * a.HKV + h) * a.cap + at[x];
       *to = a.head0 ? max(*to, key) : key;
     });
 }
 
+// inclusive sum over the lanes of a wave
+__device__ __forceinline__ unsigned wave_scan(unsigned v) {
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);     // row_shr 1, 2, 4, 8
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
+  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);     // rows 0 to 1, 2 to 3
+  return v + (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);   // rows 1 to 2, 3
+}
+
 // A row's choice by one wave, from scores in registers: lane l holds blocks l + 64 k, all ones for those that are chosen
-// whatever they score and 0 for none; `want` of them in all.  The score of the last one chosen by bisection over the
-// bits in which the scores differ, until as many as wanted are at or above it: some 12 steps for 512 blocks, each a
-// comparison and a count of lanes for 64 blocks.
+// whatever they score and 0 for none; `want` of them in all.  hist: 256 counters of the wave in LDS.  The scores'
+// range is cut into 256 steps and the one that holds the last score chosen found by counting; what it is among the few
+// that lie in it by bisection, until as many as wanted are at or above it.
 template <int N>
-__device__ __forceinline__ void choose(const unsigned (&key)[N], int want, int* out) {
+__device__ __forceinline__ void choose(const unsigned (&key)[N], int want, unsigned* hist, int* out) {
   unsigned most = 0, least = ~0u;
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     most = max(most, key[k] == ~0u ? 0u : key[k]);
     least = min(least, key[k] ? key[k] : ~0u);
   }
+  *reinterpret_cast<uint4v*>(hist + 4 * (threadIdx.x & 63)) = uint4v(0u);
   most = (unsigned)__builtin_amdgcn_readfirstlane((int)max_heads<16>(most));
   least = ~(unsigned)__builtin_amdgcn_readfirstlane((int)max_heads<16>(~least));
   const auto count = [&](unsigned x) {
@@ -243,22 +302,40 @@ __device__ __forceinline__ void choose(const unsigned (&key)[N], int want, int* 
     for (int k = 0; k < N; ++k) c += __popcll(__ballot(key[k] >= x));
     return c;
   };
-  // have: at least `want` are at or above it, and no more once `exact`.  (Where the ones chosen whatever they score are
-  // all that is wanted, no bit is taken below the first that lies above every other score.)
-  const unsigned differ = most ^ least;
-  const int bits = differ ? 32 - __builtin_clz(differ) : 0;
-  unsigned have = bits >= 32 ? 0 : most >> bits << bits;
-  bool exact = false;
-  if (count(most + 1) == want) {
-    have = most + 1;
-    exact = true;
+  const int range = 32 - __builtin_clz((most - least) | 1), shift = max(range - 8, 0);
+  int rest = want;                       // what is not chosen whatever it scores
+  lane_order();
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    rest -= __popcll(__ballot(key[k] == ~0u));
+    if (key[k] != ~0u && key[k]) atomicAdd(&hist[255 - ((key[k] - least) >> shift)], 1u);      // the highest step first
   }
-  for (int bit = bits - 1; bit >= 0 && !exact; --bit) {
-    const unsigned x = have | 1u << bit;
-    const int c = count(x);
-    if (c >= want) {
-      have = x;
-      exact = c == want;
+  lane_order();
+  const uint4v c4 = *reinterpret_cast<const uint4v*>(hist + 4 * (threadIdx.x & 63));
+  const unsigned sum = c4[0] + c4[1] + c4[2] + c4[3], upto = wave_scan(sum);
+  // have: at least `want` are at or above it, and no more once `exact`
+  unsigned have = most + 1;
+  bool exact = rest <= 0;
+  if (!exact) {
+    const int at = __builtin_ctzll(__ballot((int)upto >= rest));         // (the counters hold more than are wanted)
+    int over = (int)(__builtin_amdgcn_readlane((int)upto, at) - __builtin_amdgcn_readlane((int)sum, at)), step = 4 * at;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = __builtin_amdgcn_readlane((int)c4[i], at);
+      if (over < rest) {
+        over += c;
+        step = 4 * at + i;
+      }
+    }
+    have = least + ((unsigned)(255 - step) << shift);
+    exact = over == rest;
+    for (int bit = shift - 1; bit >= 0 && !exact; --bit) {
+      const unsigned x = have + (1u << bit);
+      const int c = count(x);
+      if (c >= want) {
+        have = x;
+        exact = c == want;
+      }
     }
   }
   const int lane = threadIdx.x & 63;
@@ -298,6 +375,8 @@ template <typename T, int D, int GP, int N>
 __global__ void __launch_bounds__(kPickThreads) kv8_pick_kernel(SelectArgs a) {
   constexpr int kTokens = 16 / GP;
   extern __shared__ unsigned s_key[];    // (kTokens, cap)
+  __shared__ __align__(16) char s_turn[kPickWaves][32 * D];
+  __shared__ __align__(16) unsigned s_count[kPickWaves][256];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15;
   const int h = blockIdx.x % a.HKV, id = blockIdx.x / a.HKV;
   const int b = a.cu ? sequence_of(a.B, id, [&](int i) { return a.cu[i] / kTokens + 2 * i; }) : id;
@@ -313,18 +392,21 @@ __global__ void __launch_bounds__(kPickThreads) kv8_pick_kernel(SelectArgs a) {
   const int last = j0 < end ? sq.n - sq.R + end - 1 : -1, most = last < 0 ? 0 : (last >> a.lp) + 1;
   if (most > a.n) {
     constexpr int kStep = kAtOnce * kPickWaves * 16;
-    int4v Q[D / 32];
+    const T* const row = row_of<T, D, GP>(a, sq, j0, h);
+    Rows<T, D> own;
+    fetch_row(own, row + (long)head_of<GP>(a) * a.q_sh);
     Bounds<D> t[kAtOnce];
     // (tiles past the last block too: what lies there is not used)
 #pragma unroll
     for (int x = 0; x < kAtOnce; ++x) fetch_bounds(a, t[x], page[x], h);
-    query_rows<T, D, GP>(a, sq, j0, h, Q);
+    int4v Q[D / 32];
+    quantise<T, D, GP>(a, own, row, Q);
 #pragma unroll 1
     for (int i = 0;;) {
 #pragma unroll
       for (int x = 0; x < kAtOnce; ++x) {
         const int at = i + (wave + x * kPickWaves) * 16 + col;
-        score_tile<D, GP>(Q, t[x], [&](int tok, unsigned key) {
+        score_tile<D, GP>(Q, t[x], s_turn[wave], [&](int tok, unsigned key) {
           if (at < most) s_key[tok * a.cap + at] = key;
         });
       }
@@ -349,7 +431,7 @@ __global__ void __launch_bounds__(kPickThreads) kv8_pick_kernel(SelectArgs a) {
       const unsigned x = s_key[tok * a.cap + min(i, seen - 1)];
       key[k] = i >= seen ? 0 : i < a.first || i >= seen - a.last ? ~0u : x;
     }
-    choose<N>(key, a.n, out);
+    choose<N>(key, a.n, s_count[wave], out);
   }
   if (!a.cu) return;
   // -1 for the tokens that no sequence takes: each workgroup looks at as many as a tile has, from its number on
@@ -360,16 +442,6 @@ __global__ void __launch_bounds__(kPickThreads) kv8_pick_kernel(SelectArgs a) {
     if (t >= own.r0 && t < own.r0 + own.R) continue;
     for (int i = lane; i < a.n; i += 64) a.out[(t * a.HKV + h) * a.n + i] = -1;
   }
-}
-
-// inclusive sum over the lanes of a wave
-__device__ __forceinline__ unsigned wave_scan(unsigned v) {
-  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);     // row_shr 1, 2, 4, 8
-  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
-  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
-  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
-  v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);     // rows 0 to 1, 2 to 3
-  return v + (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);   // rows 1 to 2, 3
 }
 
 __global__ void __launch_bounds__(kThreads) kv8_choose_kernel(SelectArgs a) {
@@ -496,6 +568,15 @@ void score(SelectArgs a, dim3 grid, int gp, hipStream_t st) {
     for (; a.head0 < a.G; a.head0 += 16) hipLaunchKernelGGL((kv8_score_kernel<T, D, 16>), grid, dim3(kThreads), 0, st, a);
 }
 
+// rows of a token in a tile
+int rows_of_token(int heads) {
+  int gp = 1;
+  while (gp < heads && gp < 16) gp *= 2;
+  return gp;
+}
+// whether a tile's scores fit the workgroup's LDS (32 KB of it) and a wave's registers
+bool one_launch(int cap, int heads) { return cap <= kPickMost && heads <= 16 && 16 / rows_of_token(heads) * cap <= 8192; }
+
 }  // namespace
 
 extern "C" int oa_kv8_select(const void* q, long q_st, long q_sh, int dtype, const void* ks, const void* kb,
@@ -511,7 +592,7 @@ extern "C" int oa_kv8_select(const void* q, long q_st, long q_sh, int dtype, con
   if (!sequences || !tokens) return 0;
   auto odd = [](const void* p, uintptr_t x) { return !p || (reinterpret_cast<uintptr_t>(p) & (x - 1)) != 0; };
   if (odd(q, 16) || q_st % 8 || q_sh % 8 || !ks || odd(kb, 16) || scale_stride < kv_heads || bound_stride % 16 ||
-      bound_stride < 2L * kv_heads * head_dim || !table || !lens || (cap > n && !(cap <= kPickMost && q_heads / kv_heads <= 16) && odd(ws, 4)) || odd(blocks, 4))
+      bound_stride < 2L * kv_heads * head_dim || !table || !lens || (cap > n && !one_launch(cap, q_heads / kv_heads) && odd(ws, 4)) || odd(blocks, 4))
     return OA_EINVAL;
   SelectArgs a;
   a.q = q; a.q_st = q_st; a.q_sh = q_sh;
@@ -519,13 +600,12 @@ extern "C" int oa_kv8_select(const void* q, long q_st, long q_sh, int dtype, con
   a.table = table; a.t_st = table_stride; a.width = width; a.lens = lens; a.cu = cu; a.ws = ws; a.out = blocks;
   a.B = sequences; a.HKV = kv_heads; a.G = q_heads / kv_heads; a.tokens = tokens; a.NP = pages; a.lp = __builtin_ctz(page);
   a.n = n; a.first = first; a.last = last; a.cap = cap; a.head0 = 0;
-  int gp = 1;
-  while (gp < a.G && gp < 16) gp *= 2;
+  const int gp = rows_of_token(a.G);
   const long tiles = (cu ? (long)tokens / (16 / gp) + 2L * sequences : sequences) * kv_heads, spans = (cap + kSpan - 1) / kSpan;
   if (tiles > 0xffffffffL / kThreads || spans > 65535 || (long)tokens * kv_heads > 0xffffffffL / kThreads) return OA_EINVAL;
   const dim3 grid((unsigned)tiles, (unsigned)spans);
   const hipStream_t st = (hipStream_t)stream;
-  if (cap <= kPickMost && a.G <= 16) {
+  if (one_launch(cap, a.G)) {
     if (tiles > 0xffffffffL / kPickThreads) return OA_EINVAL;
     if (dtype == 0 && head_dim == 64) pick<__bf16, 64>(a, (unsigned)tiles, gp, st);
     else if (dtype == 0) pick<__bf16, 128>(a, (unsigned)tiles, gp, st);

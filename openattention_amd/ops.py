@@ -1210,7 +1210,7 @@ def _select_sizes(qs, qst, qt, ks, kst, kt, bs, bst, bt, ts, tst, tt, lens, page
           f"at most {_GRID} workgroups (tokens x heads)")
     qst = _row_strides(T, HQ, Dh, qst, qt, "q")
     return (T, HKV, qst, _DT[qt], (kst[0] if NP > 1 else HKV, b0, NP, page), (tstride, width), (B, T, HQ, HKV, Dh, n, first, last, cap),
-            T * HKV * cap if cap > n and (cap > 1024 or HQ // HKV > 16) else 0)
+            T * HKV * cap if cap > n and (cap > 1024 or rows * cap > 8192 or HQ // HKV > 16) else 0)
 
 
 def kv8_select(q, ks, kb, table, lens, page: int, n: int, cu_q=None, first: int = 1, last: int = 2, max_len: int | None = None):
@@ -1224,7 +1224,8 @@ def kv8_select(q, ks, kb, table, lens, page: int, n: int, cu_q=None, first: int 
     key of the block can score.  Scores are whole numbers times powers of two, and the choice is exact.  Values of q
     that are not finite count as 0.  A block whose page id lies outside of the cache comes last.  max_len: a bound on
     lens that the caller knows.  -1 alone: tokens that no sequence takes, and those of sequences longer than their
-    table row or than max_len (rounded up to whole pages).  Over more than 1024 blocks (or 16 query heads to a KV head) a
+    table row or than max_len (rounded up to whole pages).  Over more than 1024 blocks (512 where a KV head has one
+    query head), or with more than 16 query heads to a KV head, a
     workspace of T HKV blocks integers is taken from torch's allocator."""
     if _fast is not None:
         got = _fast.call(_SELECT8, q, ks, kb, table, lens, cu_q, page, n, first, last, max_len)

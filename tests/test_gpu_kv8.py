@@ -233,7 +233,8 @@ SELECTS = [  # lens, rows, HQ, HKV, D, page, n, first, last, type
     ([1], None, 4, 1, 128, 32, 3, 1, 2, BF), ([400, 0, 1, 31, 700, 64], None, 32, 8, 128, 32, 5, 1, 2, BF),
     ([900, 300], [40, 5], 14, 2, 64, 32, 6, 0, 1, FH), ([3000], [9], 8, 8, 128, 64, 4, 2, 2, BF), ([1500, 2, 800], [3, 2, 1], 40, 2, 128, 32, 9, 1, 1, FH),
     ([700], [1], 48, 1, 64, 32, 7, 1, 2, BF), ([640, 100, 500], [30, 0, 2], 6, 2, 64, 32, 8, 1, 2, BF), ([2000], [7], 3, 1, 128, 128, 3, 1, 2, BF),
-    ([5, 1000], [9, 4], 16, 1, 128, 32, 10, 3, 4, BF)]
+    ([5, 1000], [9, 4], 16, 1, 128, 32, 10, 3, 4, BF), ([16000, 300], [17, 3], 2, 2, 64, 32, 20, 1, 2, BF), ([32700, 40, 9000], None, 4, 2, 64, 32, 300, 1, 2, FH),
+    ([17000], [3], 1, 1, 64, 32, 5, 1, 2, BF)]
 
 
 def want_select(q, cache, table, lens, cu, page, n, first, last):

@@ -103,10 +103,12 @@ def test_selections_refused(calls):
     ops.kv8_select(**dict(ok, n=9))
     ops.kv8_select(**dict(ok, table=i32(3, 1025)))
     ops.kv8_select(**dict(ok, q=z(3, 34, 128, dtype=BF)))
+    ops.kv8_select(**dict(ok, q=z(3, 2, 128, dtype=BF), table=i32(3, 512)))
+    ops.kv8_select(**dict(ok, q=z(3, 2, 128, dtype=BF), table=i32(3, 513)))
     for name, a in calls:
         assert len(a) + 1 == len(lib.SIGNATURES_KV8[name])
     # blocks, from the table's width or max_len; scratch where one launch does not do
-    assert [a[-3] for _, a in calls] == [9, 3, 9, 1025, 9] and [a[-2] is None for _, a in calls] == [True, True, True, False, False]
+    assert [a[-3] for _, a in calls] == [9, 3, 9, 1025, 9, 512, 513] and [a[-2] is None for _, a in calls] == [True, True, True, False, False, True, False]
 
 
 def test_attention_refused(calls):
