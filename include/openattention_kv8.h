@@ -53,7 +53,7 @@ int oa_kv8_read(const int* slots, const void* kc, const void* ks, const void* vc
  * max over the query heads of sum_d max(q8, 0) hi + max(-q8, 0) nlo, times 2^min(e, 100), q8 = rint(q / 2^u), u >= -120
  * the smallest with |q8| <= 127 for the heads together; values of q that are not finite count as 0, a block whose page
  * id lies outside of the cache comes last.  cap: blocks (at most width) that sequences hold at most; -1 alone: rows that
- * no sequence takes, sequences of more than cap blocks.  ws: tokens * kv_heads * cap ints of scratch (NULL will do where
+ * no sequence takes (of no sequences: nothing is written), sequences of more than cap blocks.  ws: tokens * kv_heads * cap ints of scratch (NULL will do where
  * cap <= n, and for cap <= 1024 with 2 to 16 query heads to a KV head, cap <= 512 with one).
  */
 int oa_kv8_select(const void* q, long q_st, long q_sh, int dtype, const void* ks, const void* kb, long scale_stride,

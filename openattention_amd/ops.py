@@ -1240,6 +1240,8 @@ def kv8_select(q, ks, kb, table, lens, page: int, n: int, cu_q=None, first: int 
     qp, bp = q.data_ptr(), kb.data_ptr()
     if T:
         _aligned(qp | bp)
+    if not sizes[0]:
+        return table.new_full((T, HKV, sizes[5]), -1)
     out = table.new_empty(T, HKV, sizes[5])
     ws = table.new_empty(scores) if scores else None
     _run(i, "oa_kv8_select", qp, *qst, dt, ks.data_ptr(), bp, *where, table.data_ptr(), *tsz, lens.data_ptr(), _ptr(cu_q),

@@ -318,6 +318,33 @@ def test_selection_that_has_no_place():
     assert ops.kv8_select(q[:0], cache[1], cache[4], table, i32([300, 200]), 32, 4, cu_q=i32([0, 0, 0])).shape == (0, 2, 4)
 
 
+def test_selection_of_no_sequences():
+    """Rows that no sequence takes, as there is none: -1 alone, at once and again."""
+    cache, table = filled([100], 2, 64, 32, gen(61))
+    q = randn(gen(62), 3, 4, 64, dtype=BF)
+    for _ in range(3):
+        junk = torch.full((3 * 2 * 4,), 7, device=DEV, dtype=torch.int32)
+        del junk                                             # (what the next tensor of this size is likely to hold)
+        got = ops.kv8_select(q, cache[1], cache[4], table[:0], i32([]), 32, 4, cu_q=i32([0]))
+        assert got.shape == (3, 2, 4) and (got == -1).all()
+
+
+@pytest.mark.parametrize("HQ,blocks,rows", [(1, 512, 16), (1, 512, 1), (2, 1024, 9), (16, 1024, 2), (16, 8, 1)])
+def test_selection_of_the_largest_tiles(HQ, blocks, rows):
+    """As many scores as one launch holds, with rows of the larger head dimension."""
+    g = gen(63)
+    page, D = 32, 128
+    table = torch.randperm(blocks, generator=g, device=DEV).int()[None].contiguous()
+    kb = torch.randint(-5, 113, (blocks, 1, 2, D), generator=g, device=DEV, dtype=torch.int8)
+    ks = torch.randint(118, 124, (blocks, 1), generator=g, device=DEV, dtype=torch.uint8)
+    q = randn(g, rows, HQ, D, dtype=BF)
+    for n in (4, blocks // 2, blocks - 1):
+        if n < 3:
+            continue
+        got = ops.kv8_select(q, ks, kb, table, i32([blocks * page]), page, n, cu_q=i32([0, rows]))
+        assert torch.equal(got.cpu(), want_select(q, [None, ks, None, None, kb], table, [blocks * page], [0, rows], page, n, 1, 2))
+
+
 # ================================================================== attention
 def values_of(cache, table, lens, page):
     """fp64 keys and values of every sequence"""
