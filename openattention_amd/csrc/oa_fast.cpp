@@ -195,8 +195,8 @@ PyObject* call_op(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (op < 0 || op >= kOps || !entry[op]) Py_RETURN_NOTIMPLEMENTED;
   Call a;
   if (!take(a, op, args + 1, n - 1, nullptr) || a.count < kArgs[op]) Py_RETURN_NOTIMPLEMENTED;
-  const Plan* plan = find(a, hash_of(a.key, a.words));
-  if (!plan) Py_RETURN_NOTIMPLEMENTED;
+  const uint64_t hash = hash_of(a.key, a.words);
+  if (!plans.count(hash)) Py_RETURN_NOTIMPLEMENTED;
   PyObject* d = PyObject_CallNoArgs(get_device);
   if (!d) return nullptr;
   const long current = PyLong_AsLong(d);
@@ -209,6 +209,9 @@ PyObject* call_op(PyObject*, PyObject* const* args, Py_ssize_t n) {
   void* stream = PyLong_AsVoidPtr(s);
   Py_DECREF(s);
   if (PyErr_Occurred()) return nullptr;
+  // (after the calls into Python, which another thread's may come between: keep() may drop plans)
+  const Plan* plan = find(a, hash);
+  if (!plan) Py_RETURN_NOTIMPLEMENTED;
   PyObject* out = nullptr;
   constexpr int (*run[kOps])(const Call&, const Plan&, void*, PyObject**) = {run_write, run_read, run_select, run_attn};
   const int st = run[op](a, *plan, stream, &out);
@@ -271,13 +274,10 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
 // what this was built for: torch's version, the revision of the entry points
 PyObject* built_for(PyObject*, PyObject*) { return Py_BuildValue("(si)", TORCH_VERSION, OA_KV8_REVISION); }
 
-PyObject* kept(PyObject*, PyObject*) { return PyLong_FromSize_t(plans.size()); }
-
 PyMethodDef methods[] = {{"call", (PyCFunction)(void (*)(void))call_op, METH_FASTCALL, nullptr},
                          {"keep", (PyCFunction)(void (*)(void))keep, METH_FASTCALL, nullptr},
                          {"bind", (PyCFunction)(void (*)(void))bind, METH_FASTCALL, nullptr},
                          {"built_for", built_for, METH_NOARGS, nullptr},
-                         {"kept", kept, METH_NOARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_oa_fast", nullptr, -1, methods};
 

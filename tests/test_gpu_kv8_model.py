@@ -268,3 +268,42 @@ def test_kept_plans_look_at_every_call(monkeypatch):
     with pytest.raises(ValueError):
         ops.kv8_write(bad, x, *cache, table, n)
     assert values_of(cache, table, lens, page)[0][0].shape == (700, 2, 128)
+
+
+def test_calls_of_two_threads():
+    """Calls of two host threads at once, each on a stream and a cache of its own, by plans that both keep."""
+    import threading
+    g = gen(9)
+    page, lens = 32, [300, 64]
+    work, errors = [], []
+    for _ in range(2):
+        cache, table = filled(lens, 2, 128, page, g)
+        work.append((cache, table, i32(lens), randn(g, 2, 8, 128, dtype=BF), torch.cuda.Stream()))
+
+    def run(cache, table, n, q, stream, times):
+        outs = []
+        with torch.cuda.stream(stream):
+            for i in range(times):
+                blocks = ops.kv8_select(q, cache[1], cache[4], table, n, page, 4 + i % 3)
+                outs.append(ops.kv8_attn(q, *cache[:4], table, n, blocks=blocks, sm_scale=0.05 + 0.01 * (i % 5)))
+        stream.synchronize()
+        return outs
+
+    torch.cuda.synchronize()
+    want = [run(*w, 15) for w in work]
+    got = [None, None]
+
+    def thread(i):
+        try:
+            got[i] = run(*work[i], 60)
+        except Exception as e:                              # (said by the test's own thread)
+            errors.append(e)
+
+    threads = [threading.Thread(target=thread, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for w, o in zip(want, got):
+        assert len(o) == 60 and all(torch.equal(x, w[i % 15]) for i, x in enumerate(o))
