@@ -618,3 +618,31 @@ def test_bad_pages_reach_the_rows_that_see_them(rows):
         last = ops.kv8_attn(q, *cache[:4], table, i32([n - 1]), cu_q=i32([0, rows]), max_q=rows)
         none = ops.kv8_attn(q, *cache[:4], bad, i32([n - 1]), cu_q=i32([0, rows]), max_q=rows)
         assert torch.equal(last, none) and not none.isnan().any()
+
+
+def test_pages_past_32_bits():
+    """Codes more than 2^32 bytes from the first page's: every operator gives what it gives over near pages, bit by bit."""
+    g = gen(31)
+    HKV, page, D, lens, rows = 8, 64, 128, [700, 150], [70, 40]
+    table, NP = new_table(lens, page, g)
+    far = (1 << 32) // (HKV * page * D) + NP + 3
+    near, cu = new_cache(NP, HKV, page, D, g), i32(starts(lens))
+    wide = [torch.empty(far, *t.shape[1:], device=DEV, dtype=t.dtype) for t in near]
+    away = torch.where(table >= 0, far - 1 - table, table)
+    assert (away[table >= 0].long() * HKV * page * D >= 1 << 32).all()
+    k, v = randn(g, sum(lens), HKV, D, dtype=BF), randn(g, sum(lens), HKV, D, dtype=BF)
+    n = i32(lens)
+    ops.kv8_write(k, v, *near, table, n, cu)
+    ops.kv8_write(k, v, *wide, away, n, cu)
+    slots, back = [i32([int(t[b, i // page]) * page + i % page for b, m in enumerate(lens) for i in range(m)]) for t in (table, away)]
+    for a, b in zip(ops.kv8_read(slots, *near[:4]), ops.kv8_read(back, *wide[:4])):
+        assert torch.equal(a, b)
+    for r, HQ in ((None, 32), ([1, 1], 64), ([5, 3], 32), (rows, 16)):
+        c = None if r is None else i32(starts(r))
+        q = randn(g, 2 if r is None else sum(r), HQ, D, dtype=BF)
+        m = 1 if r is None else max(r)
+        assert torch.equal(ops.kv8_attn(q, *near[:4], table, n, cu_q=c, max_q=m), ops.kv8_attn(q, *wide[:4], away, n, cu_q=c, max_q=m))
+        x, y = ops.kv8_select(q, near[1], near[4], table, n, page, 5, c), ops.kv8_select(q, wide[1], wide[4], away, n, page, 5, c)
+        assert torch.equal(x, y)
+        assert torch.equal(ops.kv8_attn(q, *near[:4], table, n, cu_q=c, max_q=m, blocks=x),
+                           ops.kv8_attn(q, *wide[:4], away, n, cu_q=c, max_q=m, blocks=x))
