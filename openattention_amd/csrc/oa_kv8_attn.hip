@@ -198,16 +198,18 @@ __global__ void __launch_bounds__(kThreads, NQ > 1 ? 2 : 3) kv8_attn_kernel(Attn
     }
     lane_order();
     next();
+    // (16 keys and the other 16 in turn, each sum's products apart: drafts over 64 dims 11.2 us one after the other, 10.7)
     f32x4 S[NQ][2];
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int x = 0; x < NQ; ++x) S[x][0] = S[x][1] = f32x4(0.f);
 #pragma unroll
-      for (int x = 0; x < NQ; ++x) S[x][c] = f32x4(0.f);
+    for (int y = 0; y < D / 64; ++y) {
+      const uint4v w0 = key_op(0, y), w1 = key_op(1, y);
 #pragma unroll
-      for (int y = 0; y < D / 64; ++y) {
-        const uint4v w = key_op(c, y);
+      for (int z = 0; z < 2; ++z) {
 #pragma unroll
-        for (int z = 0; z < 2; ++z) {
+        for (int c = 0; c < 2; ++c) {
+          const uint4v w = c ? w1 : w0;
           const bf16x8 kop = kHalf ? from8h(w[2 * z], w[2 * z + 1], 1.f) : from8(w[2 * z], w[2 * z + 1], 1.f);
 #pragma unroll
           for (int x = 0; x < NQ; ++x) {
