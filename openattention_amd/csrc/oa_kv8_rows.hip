@@ -13,6 +13,9 @@
 // largest: values so much smaller are rounded to a multiple of 2^-84 of it.)
 // The loop is a pipeline: iteration i issues the products of S(i + 1) and of O += V(i - 1) P(i - 1) between
 // the steps of the softmax of S(i), puts tile i + 2 into LDS and requests the codes of tile i + 4.
+// Two questions of 64 tokens over 32768 keys (32 heads over 8 of 128) take 95 to 104 us, 660 to 720 TFLOP/s, and the join 9.
+// What bounds it is not one thing: matrix cores are busy 31% of the time, vector units 41%, waves wait 27%.  All
+// workgroups end together with 33 MB of partial sums (by way of LDS in whole lines: 1% less at best).
 #include "oa_kv8_attn.h"
 
 namespace {

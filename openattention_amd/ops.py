@@ -1253,7 +1253,11 @@ def kv8_select(q, ks, kb, table, lens, page: int, n: int, cu_q=None, first: int 
 
 def kv8_chunk(cap: int, units: int, rows: int, listed: bool = False) -> int:
     """Keys per workgroup of kv8_attn, for `units` (sequence or token, KV head, query tile) triples of up to `cap` keys and
-    `rows` query rows."""
+    `rows` query rows: for one workgroup on each of the 256 compute units, two where they are heavier.  Of 1024 / 2048 /
+    4096 keys (8 KV heads of 128; us): one sequence of 131072 keys 53 / 47 / 45, 32 of 32768 365 / 347 / 334, 64 listed
+    blocks of 64 keys for 32 tokens 52 / 49 / 45 and for 128 tokens 94 / 86 / 85; two questions of 64 tokens over 32768
+    keys (256 rows each) 115 / 105 / 122.  Sequences of unlike lengths want smaller pieces, an eighth of the longest and no
+    less than 1024 (61 of 1 to 16001 keys 61 / 60 / 79), which costs batches of one length little."""
     n = max(cap * units // (256 if rows <= 16 else 512), 128)
     if rows <= 64 and not listed:
         n = min(n, max(cap // 8, 1024))
