@@ -94,12 +94,12 @@ __global__ void __launch_bounds__(kThreads, NQ > 1 ? 2 : 3) kv8_attn_kernel(Attn
 
   // a tile's addresses: a scalar base and the lane's place
   const int pmask = (1 << a.lp) - 1;
-  const long headc = ((long)h << a.lp) * D;
+  const unsigned headc = ((unsigned)h << a.lp) * D;
   auto load = [&](Tile<D>& t, int off, int page) {
     const bool bad = (unsigned)page >= (unsigned)a.NP;
     t.bad = bad ? 0x7f800000u : 0u;
-    const long pg = bad ? 0 : page;
-    const long bc = pg * a.c_sp + headc + (long)off * D, bs = pg * a.s_sp + h;
+    const unsigned long pg = bad ? 0u : (unsigned)page;
+    const unsigned long bc = pg * (unsigned long)a.c_sp + (headc + off * D), bs = pg * (unsigned long)a.s_sp + h;
     t.ks = a.ks[bs];
     t.vs = a.vs[bs];
 #pragma unroll
@@ -113,8 +113,8 @@ __global__ void __launch_bounds__(kThreads, NQ > 1 ? 2 : 3) kv8_attn_kernel(Attn
   const int* const list = LISTED ? a.list + ((long)u * a.HKV + h) * a.n : nullptr;
   auto block_at = [&](int i) { return i < nt ? list[(tb + i * kStride) >> a.lp] : -1; };
   auto place_of = [&](int blk, int i) { return (blk << a.lp) + ((tb + i * kStride) & pmask); };
-  auto page_of = [&](int blk) { return trow[min(max(blk, 0), a.width - 1)]; };
-  auto live = [&](int blk, int i) { return blk >= 0 && blk < a.width && place_of(blk, i) < hi; };
+  auto page_of = [&](int blk) { return trow[min((unsigned)blk, (unsigned)(a.width - 1))]; };
+  auto live = [&](int blk, int i) { return (unsigned)blk < (unsigned)a.width && place_of(blk, i) < hi; };
   int b0 = -1, b1 = -1, b2 = -1;
   if (LISTED) {
     b0 = block_at(0);
