@@ -1256,11 +1256,17 @@ def kv8_chunk(cap: int, units: int, rows: int, listed: bool = False) -> int:
     `rows` query rows: for one workgroup on each of the 256 compute units, two where they are heavier.  Of 1024 / 2048 /
     4096 keys (8 KV heads of 128; us): one sequence of 131072 keys 53 / 47 / 45, 32 of 32768 365 / 347 / 334, 64 listed
     blocks of 64 keys for 32 tokens 52 / 49 / 45 and for 128 tokens 94 / 86 / 85; two questions of 64 tokens over 32768
-    keys (256 rows each) 115 / 105 / 122.  Sequences of unlike lengths want smaller pieces, an eighth of the longest and no
-    less than 1024 (61 of 1 to 16001 keys 61 / 60 / 79), which costs batches of one length little."""
+    keys (256 rows each) 115 / 105 / 122.  Sequences of unlike lengths, and those much shorter than their table, want
+    smaller pieces: an eighth of the longest and no less than 1024 (61 of 1 to 16001 keys 61 / 60 / 79), and no more than
+    4096 (of 4096 / 8192 / an eighth of the longest: 16 of 1 to 131072 keys 112 / 131 / 240, 8 of 131072 334 / 340 / 323), or
+    8192 where that gives the card some more workgroups than it holds at once (4 of 131072 182 / 166 / 165).  A table
+    for more than 262144 keys takes 64 pieces of whatever size, or 32: so many hold their sums in the workspace."""
     n = max(cap * units // (256 if rows <= 16 else 512), 128)
     if rows <= 64 and not listed:
         n = min(n, max(cap // 8, 1024))
+        most = max(4096, cap // 64)
+        if n > most:
+            n = min(n, 2 * most) if 512 < units * (cap // most) < 2048 else most
     return min(-(-n // 128), -(-cap // 128)) * 128
 
 

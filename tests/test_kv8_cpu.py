@@ -219,3 +219,15 @@ def test_a_library_of_other_entry_points_is_refused(lacks, want, tmp_path, monke
     with pytest.raises(RuntimeError, match=want) as e:
         lib.load()
     assert "rebuild it" in str(e.value)
+
+
+def test_pieces_of_all_sizes():
+    """Pieces are whole tiles of four waves, cover the keys, and stay within a launch's axes and a workspace's bounds."""
+    for cap in (1, 127, 128, 129, 4096, 16001, 32768, 131072, 262144, 1 << 20, (1 << 30) - 64, 1 << 30):
+        for units in (1, 2, 8, 16, 32, 64, 256, 500, 4096, 1 << 20):
+            for rows in (1, 4, 8, 16, 33, 64, 65, 512):
+                for listed in (False, True):
+                    n = ops.kv8_chunk(cap, units, rows, listed)
+                    pieces = -(-cap // n)
+                    assert n % 128 == 0 and 128 <= n <= -(-cap // 128) * 128
+                    assert pieces <= (256 if rows <= 16 else 512)    # (those of one unit; more units take fewer)
