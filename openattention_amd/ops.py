@@ -1262,7 +1262,9 @@ def kv8_chunk(cap: int, units: int, rows: int, listed: bool = False) -> int:
     8192 where that gives the card some more workgroups than it holds at once (4 of 131072 182 / 166 / 165).  A table
     for more than 262144 keys takes 64 pieces of whatever size, or 32: so many hold their sums in the workspace.  Up to 640
     keys (512 listed ones) one piece, and no join: one sequence of 250 keys 5.8 us, 7.7 in two pieces; 23 of up to 525 7.7
-    for 10.2; but one of 735 9.4 in two and 7.8 in six, 49 tokens of 640 listed keys 9.1 in one and 8.1 in five."""
+    for 10.2; but one of 735 9.4 in two and 7.8 in six, 49 tokens of 640 listed keys 9.1 in one and 8.1 in five.
+    Questions, too, take no more than 4096 keys a piece: 8 of up to 64 tokens over up to 32768 keys 160, in whole sequences
+    280; 8 of 64 over 32768 364 for 356.  Pieces of prompts (one of 2048 tokens 1281 for 1182) keep what fills the card."""
     if cap <= (512 if listed else 640) and rows <= 16:
         return -(-cap // 128) * 128
     n = max(cap * units // (256 if rows <= 16 else 512), 128)
@@ -1271,6 +1273,8 @@ def kv8_chunk(cap: int, units: int, rows: int, listed: bool = False) -> int:
         most = max(4096, cap // 64)
         if n > most:
             n = min(n, 2 * most) if 512 < units * (cap // most) < 2048 else most
+    elif rows <= 1024 and not listed:
+        n = min(n, max(4096, cap // 64))
     return min(-(-n // 128), -(-cap // 128)) * 128
 
 
