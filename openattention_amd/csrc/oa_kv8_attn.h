@@ -7,6 +7,9 @@ namespace kv8 {
 
 using namespace paged;
 
+// query rows of a KV head up to which every workgroup turns its own keys to 16 bits (more: oa_kv8_rows.hip)
+constexpr int kFewRows = 64;
+
 struct AttnArgs {
   const uint16_t* q; long q_st, q_sh;
   const uint8_t* kc; const uint8_t* ks; const uint8_t* vc; const uint8_t* vs;

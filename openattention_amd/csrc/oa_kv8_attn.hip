@@ -1,399 +1,34 @@
 // Causal attention of the newest tokens of every sequence over an 8-bit paged cache (layout and codes: oa_kv8.hip),
 // over all of their keys or over the blocks that a list names for each token and KV head:
 //   out = sum_t p_t v_t / sum_t p_t,  p_t = exp(scale q . k_t - max),
-// in one pass over the keys with a running maximum and sum.
-//
-// One workgroup of four waves takes 16 NQ query rows of a KV head (row = token * G + head, so that any number of
-// query heads fills the tiles; with a list the rows of one token, as each has its own) and a chunk of keys (ops.kv8_chunk
-// says how many and why); each wave walks its own tiles of 32 keys and the waves join at the end.  With several
-// chunks a second kernel joins them.
-// A tile's codes are 4096 (D = 64: 2048) successive bytes of K and of V, loaded as such, 16 bytes to a lane, while the
-// tile before is worked on; the wave puts them into its own part of LDS and takes its operands from there.  (Loaded in
-// the operands' order, where a lane's neighbours take other keys, every access touches half lines: the same loop without
-// any work took 365 us for 32 sequences of 32768 keys, so 327, and 117 us for the blocks of two questions, so 49.)
-//   scores   S^T = K Q^T by v_mfma_f32_16x16x32 of the queries' type, which holds the codes as they are: a lane of the K
-//            operand takes 16 dims of each 64 of a key.  A tile lies in one block, whose scale is a factor of the
-//            scores.  All products are exact.
-//   values   O^T = V^T P^T in bf16, the scale taken in by the conversion: the weights are the B operand as the scores
-//            left them; V^T comes out of LDS by the transpose reads, as codes.
-// The maximum that weights are taken against is raised once a score passes it by 2^8, so that weights are at most that.
-// Weights go into the product as two bf16 terms, so that the sum keeps 16 bits of each: up to 8 rows
-// the second term sits in the tile's other 8 columns, otherwise it takes a second product.
+// in one pass over the keys with a running maximum and sum (oa_kv8_few.h says how).  With several chunks a second
+// kernel joins them.
 // Bound: bytes where they are read once: 32 sequences of 32768 keys (8 KV heads of 128) 320 to 331 us, 6.5 to 6.7 TB/s; one
 // of 131072 40 us and the join's 4.  Where tokens have blocks in common (64 of them for each of two questions' 128 tokens:
 // 1.07 GB, 134 MB of it distinct, 86 us) the instructions: 64 conversions and 8 exponentials among some 145 vector ones a
 // tile of 32 keys, with three waves to a SIMD.  Four waves there spill (204 us); loads two tiles ahead leave two (95).
-#include "oa_kv8_attn.h"
+#include "oa_kv8_few.h"
 
 namespace {
 
 using namespace kv8;
 
-typedef int int2v __attribute__((ext_vector_type(2)));
-typedef __attribute__((address_space(3))) int2v lds_int2v;
-
-constexpr float kLazy = 8.f;              // log2 of how far a weight may pass 1 before the sums are rescaled
-
-// one tile's codes as they lie in memory, lane by lane 16 bytes, and its scales
-template <int D>
-struct Tile {
-  uint4v k[D / 32], v[D / 32];
-  unsigned ks, vs;
-  unsigned bad;                          // the exponent of NaN where the page is outside of the cache
-};
-
-template <bool ONCE>
-__device__ __forceinline__ uint4v load16(const uint8_t* p) {
-  const uint4v* q = reinterpret_cast<const uint4v*>(p);
-  return ONCE ? __builtin_nontemporal_load(q) : *q;
-}
-
-// NQ tiles of 16 query rows; DUP: at most 8 rows, columns 8.. repeat them for the weights' second terms; T: the rows'
-// type; LISTED: over listed blocks, the rows of one token; ONCE: no other workgroup reads these codes, which then pass by
-// the caches (32 sequences of 32768 keys: 365 us through them, 327)
 template <int D, int NQ, bool DUP, typename T, bool LISTED, bool ONCE>
 __global__ void __launch_bounds__(kThreads, NQ > 1 ? 2 : 3) kv8_attn_kernel(AttnArgs a) {
-  constexpr bool kHalf = !std::is_same<T, __bf16>::value;
-  constexpr int kLoads = D / 32;         // 16-byte loads of a lane for a tile of K or V
-  constexpr int kSteps = D / 32;         // products of a 16 x 16 score tile
-  constexpr int kDims = D / 16;          // tiles of 16 dims, 16-byte chunks of a row
-  constexpr int kTileB = kTile * D;      // bytes of a tile
-  constexpr int kStage = 2 * kTileB;
-  constexpr int kCols = DUP ? 8 : 16;
-  constexpr int kStride = kWaves * kTile;
-  // tiles of the waves, K then V; at the end their sums, 16 rows of D floats each
-  __shared__ __align__(16) char s_v[kWaves * (kStage > 64 * D ? kStage : 64 * D)];
+  typedef FewLds<D, NQ> Lds;
+  __shared__ __align__(16) char s_v[Lds::kBytes];
   __shared__ float s_m[kWaves][NQ * 16], s_l[kWaves][NQ * 16];
-
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col = lane & 15, g = lane >> 4;
   // (sequence or token, head) fastest: workgroups go to the XCDs in turn, so that a long sequence's pieces and a
   // batch's short sequences spread over all of them, and the query tiles of a piece meet in one L2
-  const int unit = blockIdx.x, row0 = blockIdx.y * (NQ * kCols), ch = blockIdx.z;
+  const int unit = blockIdx.x, row0 = blockIdx.y * (NQ * (DUP ? 8 : 16)), ch = blockIdx.z;
   const int u = a.by_hkv ? (int)__umulhi((unsigned)unit, a.by_hkv) : unit, h = unit - u * a.HKV;
-  const int b = LISTED && a.cu ? sequence_of(a.B, u, [&](int i) { return a.cu[i]; }) : u;
-  auto token_of = [&](int r) { return LISTED ? 0 : (int)((unsigned)r * a.by_g >> 16); };         // r / G
-  const int k0 = ch * a.chunk, tb = k0 + wave * kTile;
-  const int* const trow = a.table + (long)b * a.t_st;
-  auto page_at = [&](int t0) { return trow[min(t0 >> a.lp, a.width - 1)]; };
-  int page0 = 0, page = 0;
-  if (!LISTED) {                         // (requested beside the length: what lies past it is not used)
-    page0 = page_at(tb);
-    page = page_at(tb + kStride);
-  }
-  const Seq sq = LISTED ? seq_of(a, b, 1L << 32) : seq_of(a, b);
-  const int j0 = LISTED ? u - sq.r0 : 0;                   // the token whose rows these are, or the first
-  if (LISTED && (j0 < 0 || j0 >= min(sq.R, a.max_q))) return;
-  const int rows = LISTED ? a.G : min(sq.R, a.max_q) * a.G;
-  if (row0 >= rows) return;
-  const int first = sq.n - sq.R + j0;    // position of the first token
-  const int hi = sq.bad ? 0 : first + token_of(min(row0 + NQ * kCols, rows) - 1) + 1;    // keys any row sees
-  const int all = first + token_of(row0) + 1;                                              // keys every row sees
-  const int k1 = LISTED ? min(k0 + a.chunk, a.n << a.lp) : min(k0 + a.chunk, hi);
-  if (!LISTED && k0 >= k1 && a.nchunk > 1) return;
-
-  // a tile's addresses: a scalar base and the lane's place
-  const int pmask = (1 << a.lp) - 1;
-  const unsigned headc = ((unsigned)h << a.lp) * D;
-  auto load = [&](Tile<D>& t, int off, int page) {
-    const bool bad = (unsigned)page >= (unsigned)a.NP;
-    t.bad = bad ? 0x7f800000u : 0u;
-    const unsigned long pg = bad ? 0u : (unsigned)page;
-    const unsigned long bc = pg * (unsigned long)a.c_sp + (headc + off * D), bs = pg * (unsigned long)a.s_sp + h;
-    t.ks = a.ks[bs];
-    t.vs = a.vs[bs];
-#pragma unroll
-    for (int n = 0; n < kLoads; ++n) t.k[n] = load16<ONCE>(a.kc + bc + 16 * lane + 1024 * n);
-#pragma unroll
-    for (int n = 0; n < kLoads; ++n) t.v[n] = load16<ONCE>(a.vc + bc + 16 * lane + 1024 * n);
-  };
-  const int nt = max(0, (k1 - tb + kStride - 1) / kStride);                  // this wave's tiles
-  Tile<D> t;
-  // listed blocks: tile i's block, -1 past the last; whether a row sees something of it
-  const int* const list = LISTED ? a.list + ((long)u * a.HKV + h) * a.n : nullptr;
-  auto block_at = [&](int i) { return i < nt ? list[(tb + i * kStride) >> a.lp] : -1; };
-  auto place_of = [&](int blk, int i) { return (blk << a.lp) + ((tb + i * kStride) & pmask); };
-  auto page_of = [&](int blk) { return trow[min((unsigned)blk, (unsigned)(a.width - 1))]; };
-  auto live = [&](int blk, int i) { return (unsigned)blk < (unsigned)a.width && place_of(blk, i) < hi; };
-  int b0 = -1, b1 = -1, b2 = -1;
-  if (LISTED) {
-    b0 = block_at(0);
-    b1 = block_at(1);
-    b2 = block_at(2);
-    page0 = page_of(b0);
-    page = page_of(b1);
-    if (live(b0, 0)) load(t, tb & pmask, page0);
-  } else if (nt > 0) {
-    load(t, tb & pmask, page0);
-  }
-
-  // this lane's columns: rows of q (negated under a negative scale: the maximum is taken before scaling)
-  // and how many keys they see (0: no such row)
-  const float c = fabsf(a.c);
-  const unsigned flip = a.c < 0.f ? 0x80008000u : 0u;
-  bf16x8 Q[NQ][kSteps];
-  int lim[NQ];
-#pragma unroll
-  for (int x = 0; x < NQ; ++x) {
-    const int r = row0 + x * kCols + (DUP ? col & 7 : col);
-    const int rr = min(r, rows - 1), j = token_of(rr), hd = h * a.G + rr - j * a.G;
-    lim[x] = r < rows ? first + j + 1 : 0;
-    const uint16_t* p = a.q + (long)(sq.r0 + j0 + j) * a.q_st + (long)hd * a.q_sh + 16 * g;
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const uint4v w = *reinterpret_cast<const uint4v*>(p + 64 * (s >> 1) + 8 * (s & 1));
-      Q[x][s] = __builtin_bit_cast(bf16x8, w ^ uint4v(flip));
-    }
-  }
-
-  // LDS tiles of 32 rows of D bytes; 16-byte chunk x of row r lies at x ^ f(r), so that rows written as they come (8 or
-  // 16 of them whole), 16 rows read at one chunk and the transpose reads' 16 (keys 8 g' .. and 16 more) spread over all banks
-  char* const sk = s_v + wave * kStage;
-  char* const sv = sk + kTileB;
-  auto f = [](int r) {
-    return D == 128 ? ((r >> 1) & 3) | (((r >> 3) ^ (r >> 4)) & 1) << 2 : ((r >> 2) & 1) | (((r >> 3) ^ (r >> 4)) & 1) << 1;
-  };
-  // the lane's row and chunk of load n, and where it goes
-  const int wrow = lane / kDims, wchunk = lane % kDims;
-  auto put_at = [&](int n) {
-    const int r = wrow + n * (1024 / D);
-    return r * D + ((wchunk ^ f(r)) << 4);
-  };
-  auto key_op = [&](int c, int x) {      // dims 64 x + 16 g .. of key 16 c + col
-    const int r = col + 16 * c;
-    return *reinterpret_cast<const uint4v*>(sk + r * D + (((4 * x + g) ^ f(r)) << 4));
-  };
-  // dims 16 d .. of keys 4 g .. and 16 + 4 g .., the order in which the scores leave the weights
-  const int vrow = 4 * g + ((lane >> 1) & 3) + ((lane & 8) << 1), vat = vrow * D + 8 * (lane & 1);
-  auto val_op = [&](int d) { return __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_int2v*)(sv + vat + ((d ^ f(vrow)) << 4))); };
-
-  f32x4 O[NQ][kDims];
-  float m[NQ], l[NQ];                    // running maximum, scaled, and sum of the lane's keys
-  bool big[NQ];                          // a maximum is past 2^24 (uniform)
-#pragma unroll
-  for (int x = 0; x < NQ; ++x) {
-    m[x] = -FLT_MAX;
-    l[x] = 0.f;
-    big[x] = false;
-#pragma unroll
-    for (int d = 0; d < kDims; ++d) O[x][d] = f32x4(0.f);
-  }
-
-  // the tile in t, whose first key is at position t0; next() requests what comes after it
-  auto body = [&](auto mask_c, int t0, auto next) {
-    const bool MASK = mask_c;            // (known beforehand, or the same for the whole wave)
-    // (the block's scale, a factor of the scores; finite, so that it leaves a product of 0 what it is)
-    const float ck = fminf(c * __uint_as_float(t.ks << 23), FLT_MAX) + __uint_as_float(t.bad) * 0.f;
-    const float fv = __uint_as_float(t.vs << 23);
-    // In a masked tile the values of keys past the last one any row sees count as zeros (their weights are 0, but what
-    // lies there may be anything), and so do chunks with NaN of keys that some rows see
-    unsigned nan = 0;                    // bit n: such a chunk
-#pragma unroll
-    for (int n = 0; n < kLoads; ++n) {
-      uint4v w = t.v[n];
-      if (MASK) {
-        const bool past = t0 + wrow + n * (1024 / D) >= hi;
-        const bool any = (nan_codes(w[0]) | nan_codes(w[1]) | nan_codes(w[2]) | nan_codes(w[3])) != 0;
-        nan |= any && !past ? 1u << n : 0u;
-        w = any || past ? uint4v(0u) : w;
-      }
-      *reinterpret_cast<uint4v*>(sk + put_at(n)) = t.k[n];
-      *reinterpret_cast<uint4v*>(sv + put_at(n)) = w;
-    }
-    lane_order();
-    next();
-    // (16 keys and the other 16 in turn, each sum's products apart: drafts over 64 dims 11.2 us one after the other, 10.7)
-    f32x4 S[NQ][2];
-#pragma unroll
-    for (int x = 0; x < NQ; ++x) S[x][0] = S[x][1] = f32x4(0.f);
-#pragma unroll
-    for (int y = 0; y < D / 64; ++y) {
-      const uint4v w0 = key_op(0, y), w1 = key_op(1, y);
-#pragma unroll
-      for (int z = 0; z < 2; ++z) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const uint4v w = c ? w1 : w0;
-          const bf16x8 kop = kHalf ? from8h(w[2 * z], w[2 * z + 1], 1.f) : from8(w[2 * z], w[2 * z + 1], 1.f);
-#pragma unroll
-          for (int x = 0; x < NQ; ++x) {
-            if constexpr (kHalf)
-              S[x][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, kop),
-                                                               __builtin_bit_cast(f16x8, Q[x][2 * y + z]), S[x][c], 0, 0, 0);
-            else
-              S[x][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop, Q[x][2 * y + z], S[x][c], 0, 0, 0);
-          }
-        }
-      }
-    }
-
-    uint4v P[NQ], Plo[NQ];
-#pragma unroll
-    for (int x = 0; x < NQ; ++x) {
-      float v[8];
-      float mx = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[i] = S[x][i >> 2][i & 3];
-        mx = fmaxf(mx, v[i]);
-      }
-      mx *= ck;
-      if (MASK) {
-        mx = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          v[i] = t0 + 16 * (i >> 2) + 4 * g + (i & 3) < lim[x] ? v[i] * ck : -INFINITY;
-          mx = fmaxf(mx, v[i]);
-        }
-      }
-      // (left behind by up to 2^kLazy, the sums are rescaled in few tiles: the blocks of two questions 82.5 us, 80.1 so)
-      if (__any(mx > m[x] + (big[x] ? 0.f : kLazy))) {
-        const float mn = fmaxf(m[x], max_groups(mx)), alpha = __builtin_amdgcn_exp2f(m[x] - mn);
-        m[x] = mn;
-        l[x] *= alpha;
-#pragma unroll
-        for (int d = 0; d < kDims; ++d) O[x][d] *= alpha;
-        // the maximum rounds S ck, so that the fma below leaves up to half its last place: past 2^24 more than
-        // the exponential should see, and an infinity in time.  There S ck is rounded first, as the maximum is
-        big[x] = __any(fabsf(mn) >= 16777216.f);
-      }
-      if (!MASK && big[x]) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= ck;
-      }
-      const float cc = MASK || big[x] ? 1.f : ck;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[i] = __builtin_amdgcn_exp2f(fmaf(v[i], cc, -m[x]));
-        l[x] += v[i];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t u = pack2(v[2 * i], v[2 * i + 1]);
-        const uint32_t lo = pack2(v[2 * i] - __uint_as_float(u << 16), v[2 * i + 1] - __uint_as_float(u & 0xffff0000u));
-        P[x][i] = DUP && (lane & 8) ? lo : u;
-        Plo[x][i] = lo;
-      }
-    }
-#pragma unroll
-    for (int d = 0; d < kDims; ++d) {
-      const int2v w = val_op(d);
-      const bf16x8 vop = from8((unsigned)w[0], (unsigned)w[1], fv);
-#pragma unroll
-      for (int x = 0; x < NQ; ++x) {
-        O[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vop, __builtin_bit_cast(bf16x8, P[x]), O[x][d], 0, 0, 0);
-        if (!DUP) O[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vop, __builtin_bit_cast(bf16x8, Plo[x]), O[x][d], 0, 0, 0);
-      }
-    }
-    lane_order();
-    if (MASK && __any(nan != 0)) {       // NaN, into the rows that see it (rare)
-#pragma unroll 1
-      for (int n = 0; n < kLoads; ++n) {
-        unsigned long at_nan = __ballot(nan >> n & 1);
-        while (at_nan) {
-          const int at = __builtin_ctzl(at_nan), key = t0 + at / kDims + n * (1024 / D), part = at % kDims;
-          at_nan &= at_nan - 1;
-#pragma unroll
-          for (int x = 0; x < NQ; ++x)
-#pragma unroll
-            for (int d = 0; d < kDims; ++d)
-              if (d == part && key < lim[x]) O[x][d] = f32x4(__builtin_nanf(""));
-        }
-      }
-    }
-  };
-  typedef std::integral_constant<bool, false> whole;
-  typedef std::integral_constant<bool, true> masked;
-  if (LISTED) {
-#pragma unroll 1
-    for (int i = 0; i < nt; ++i) {
-      auto next = [&] {
-        if (live(b1, i + 1)) load(t, (tb + (i + 1) * kStride) & pmask, page);
-      };
-      if (live(b0, i)) {
-        const int t0 = place_of(b0, i);
-        body(t0 + kTile > hi, t0, next);
-      } else {
-        next();
-      }
-      page = page_of(b2);
-      const int b3 = block_at(i + 3);
-      b0 = b1;
-      b1 = b2;
-      b2 = b3;
-    }
-  } else {
-    const int nfull = min(nt, max(0, (all - tb - kTile + kStride) / kStride));    // tiles that every row sees whole
-    int i = 0;
-    auto next = [&] {                    // tile i + 1, and the page of the one after
-      if (i + 1 < nt) {
-        const int t0 = tb + (i + 1) * kStride;
-        load(t, t0 & pmask, page);
-        page = page_at(t0 + kStride);
-      }
-    };
-#pragma unroll 1
-    for (; i < nfull; ++i) body(whole(), tb + i * kStride, next);
-#pragma unroll 1
-    for (; i < nt; ++i) body(masked(), tb + i * kStride, next);
-  }
-
-  // the four waves' sums, with a common maximum
-#pragma unroll
-  for (int x = 0; x < NQ; ++x) {
-    const float lt = sum_groups(l[x]);
-    if (g == 0) {
-      s_m[wave][x * 16 + col] = m[x];
-      s_l[wave][x * 16 + col] = lt;
-    }
-  }
-  float* const so = reinterpret_cast<float*>(s_v);
-#pragma unroll
-  for (int x = 0; x < NQ; ++x) {
-    __syncthreads();                     // (every wave is done with its tile, or with the previous sums)
-    const int sc = x * 16 + col;
-    const float M = fmaxf(fmaxf(s_m[0][sc], s_m[1][sc]), fmaxf(s_m[2][sc], s_m[3][sc]));
-    const float e = __builtin_amdgcn_exp2f(m[x] - M);
-#pragma unroll
-    for (int d = 0; d < kDims; ++d)      // 16-byte chunk y of column col at y ^ col
-      *reinterpret_cast<f32x4*>(so + (wave * 16 + col) * D + (((4 * d + g) ^ col) << 2)) = O[x][d] * e;
-    __syncthreads();
-    constexpr int kChunks = D / 4;
-    for (int i = threadIdx.x; i < kCols * kChunks; i += kThreads) {
-      const int cl = i / kChunks, y = i % kChunks, r = row0 + x * kCols + cl;
-      if (r >= rows) continue;
-      const int c16 = x * 16 + cl;
-      const float Mr = fmaxf(fmaxf(s_m[0][c16], s_m[1][c16]), fmaxf(s_m[2][c16], s_m[3][c16]));
-      float L = 0.f;
-      f32x4 o = f32x4(0.f);
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        L += s_l[w][c16] * __builtin_amdgcn_exp2f(s_m[w][c16] - Mr);
-        o += *reinterpret_cast<const f32x4*>(so + (w * 16 + cl) * D + ((y ^ cl) << 2));
-        if (DUP) o += *reinterpret_cast<const f32x4*>(so + (w * 16 + 8 + cl) * D + ((y ^ (8 + cl)) << 2));
-      }
-      const int j = token_of(r), hd = h * a.G + r - j * a.G;
-      if (a.nchunk == 1) {
-        const bool some = first + j >= 0 && !(LISTED && L == 0.f);
-        o = sq.bad ? f32x4(__builtin_nanf("")) : some ? o / L : f32x4(0.f);
-        *reinterpret_cast<uint2v*>(a.out + (long)(sq.r0 + j0 + j) * a.o_st + (long)hd * a.o_sh + 4 * y) =
-            uint2v{pack_out<T>(o[0], o[1]), pack_out<T>(o[2], o[3])};
-      } else {
-        const long at = ((long)(sq.r0 + j0 + j) * (a.HKV * a.G) + hd) * a.nchunk + ch;
-        *reinterpret_cast<f32x4*>(a.ws_o + at * D + 4 * y) = o;
-        if (y == 0) *reinterpret_cast<f32x2*>(a.ws_ml + at * 2) = f32x2{Mr, L};
-      }
-    }
-  }
+  few_rows<D, NQ, DUP, T, LISTED, ONCE>(a, u, h, row0, ch, Lds{s_v, s_m, s_l});
 }
 
 template <int D, typename T, bool LISTED>
 __global__ void __launch_bounds__(kThreads) kv8_join_kernel(AttnArgs a) {
   join_pieces<D, T, LISTED>(a);
 }
-
-// query rows up to which every workgroup turns its own keys to 16 bits (more: oa_kv8_rows.hip)
-constexpr int kFewRows = 64;
 
 template <int D, typename T, bool LISTED>
 int launch(AttnArgs a, hipStream_t st) {

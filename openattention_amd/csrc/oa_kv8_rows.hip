@@ -16,7 +16,9 @@
 // Two questions of 64 tokens over 32768 keys (32 heads over 8 of 128) take 95 to 104 us, 660 to 720 TFLOP/s, and the join 9.
 // What bounds it is not one thing: matrix cores are busy 31% of the time, vector units 41%, waves wait 27%.  All
 // workgroups end together with 33 MB of partial sums (by way of LDS in whole lines: 1% less at best).
-#include "oa_kv8_attn.h"
+// Sequences of few rows in such a call go the way of oa_kv8_few.h (a question of 64 tokens beside 31 single ones over
+// 32768 keys 466 us, 720 as 128 rows each; calls without such sequences as before).
+#include "oa_kv8_few.h"
 
 namespace {
 
@@ -67,6 +69,24 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_rows_kernel(AttnArgs a) {
   const Seq sq = seq_of(a, b);
   const int rows = min(sq.R, a.max_q) * a.G;
   if (row0 >= rows) return;
+  if (rows <= kFewRows) {                // a short sequence beside long ones
+    static_assert(FewLds<D, 2>::kBytes <= sizeof(s_v) && 2 * FewLds<D, 2>::kFloats * sizeof(float) <= sizeof(s_k), "LDS");
+    auto few = [&](auto nq, auto dup, int r0) {
+      constexpr int kNQ = decltype(nq)::value;
+      float(*const m)[kNQ * 16] = reinterpret_cast<float(*)[kNQ * 16]>(s_k);
+      few_rows<D, kNQ, decltype(dup)::value, T, false, decltype(dup)::value>(a, b, head, r0, ch, FewLds<D, kNQ>{s_v, m, m + kWaves});
+    };
+    if (rows <= 8) {
+      few(std::integral_constant<int, 1>(), std::integral_constant<bool, true>(), 0);
+    } else {
+#pragma unroll 1
+      for (int r0 = 0; r0 < rows; r0 += 32) {
+        few(std::integral_constant<int, 2>(), std::integral_constant<bool, false>(), r0);
+        __syncthreads();
+      }
+    }
+    return;
+  }
   const int first = sq.n - sq.R;         // position of the sequence's first query token
   const int hi = sq.bad ? 0 : first + (min(row0 + kRows, rows) - 1) / a.G + 1;         // keys any row sees
   const int all = first + row0 / a.G + 1;                                              // keys every row sees

@@ -646,3 +646,34 @@ def test_pages_past_32_bits():
         assert torch.equal(x, y)
         assert torch.equal(ops.kv8_attn(q, *near[:4], table, n, cu_q=c, max_q=m, blocks=x),
                            ops.kv8_attn(q, *wide[:4], away, n, cu_q=c, max_q=m, blocks=x))
+
+
+@pytest.mark.parametrize("HQ,HKV,D,page,dtype", [(32, 8, 128, 64, BF), (14, 2, 64, 32, FH), (5, 1, 128, 128, FH)])
+def test_short_sequences_beside_long_ones(HQ, HKV, D, page, dtype, monkeypatch):
+    """Sequences of few rows in a call that holds one of many: what they give on their own, bit by bit."""
+    g = gen(33)
+    rows, lens = [70, 1, 2, 0, 3, 9, 1, 16], [700, 1300, 2, 40, 333, 95, 0, 1100]
+    cache, table = filled(lens, HKV, D, page, g)
+    cu = starts(rows)
+    q = randn(g, cu[-1] + 1, HQ, D, dtype=dtype)
+    for chunk in (1 << 20, 256):
+        monkeypatch.setattr(ops, "kv8_chunk", lambda cap, units, rows, listed: min(chunk, -(-cap // 128) * 128))
+        out = torch.full_like(q, 3.0)
+        got = ops.kv8_attn(q[:-1], *cache[:4], table, i32(lens), cu_q=i32(cu), max_q=70)
+        assert ops.kv8_attn(q[:-1], *cache[:4], table, i32(lens), cu_q=i32(cu), max_q=70, out=out[:-1]).data_ptr() == out.data_ptr()
+        assert torch.equal(out[:-1], got) and (out[-1] == 3).all()
+        check_attn(got, *want_attn(q[:-1], cache, table, lens, cu, D ** -0.5, page))
+        for b, r in enumerate(rows):
+            if 0 < r and r * HQ // HKV <= 64:
+                own = ops.kv8_attn(q[cu[b]:cu[b + 1]], *cache[:4], table[b:b + 1], i32(lens[b:b + 1]), cu_q=i32([0, r]), max_q=r)
+                if r * HQ // HKV <= 8 or r * HQ // HKV > 16:          # (between them the sums of 16 rows, not of 32)
+                    assert torch.equal(got[cu[b]:cu[b + 1]], own)
+    # a page outside of the cache, and a sequence past its table row, beside the others
+    monkeypatch.undo()
+    bad, long = table.clone(), list(lens)
+    bad[1, 0], long[4] = -1, table.shape[1] * page + 1
+    out = ops.kv8_attn(q[:-1], *cache[:4], bad, i32(long), cu_q=i32(cu), max_q=70)
+    good = ops.kv8_attn(q[:-1], *cache[:4], table, i32(lens), cu_q=i32(cu), max_q=70)
+    assert out[cu[1]:cu[2]].isnan().all() and out[cu[4]:cu[5]].isnan().all()
+    rest = [t for t in range(cu[-1]) if not (cu[1] <= t < cu[2] or cu[4] <= t < cu[5])]
+    assert torch.equal(out[rest], good[rest])
