@@ -21,6 +21,8 @@ struct AttnArgs {
   float* ws_o; float* ws_ml;             // partial sums, (maximum, sum) by (row, chunk)
   int B, HKV, G, tokens, max_q, width, NP, lp, chunk, nchunk, ntile, n;
   unsigned by_g, by_hkv;                 // 2^16 / G + 1; 2^32 / HKV, rounded up (0: HKV is 1)
+  int in_turn;                           // workgroups by sequence, piece, tile, head (kv8_attn_kernel)
+  unsigned by_nchunk;                    // 2^32 / nchunk, rounded up
   int clear;                             // the join sets rows of out that no sequence takes to 0
   float c;                               // scale * log2 e
 };

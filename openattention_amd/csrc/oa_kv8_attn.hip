@@ -7,6 +7,8 @@
 // of 131072 40 us and the join's 4.  Where tokens have blocks in common (64 of them for each of two questions' 128 tokens:
 // 1.07 GB, 134 MB of it distinct, 86 us) the instructions: 64 conversions and 8 exponentials among some 145 vector ones a
 // tile of 32 keys, with three waves to a SIMD.  Four waves there spill (204 us); loads two tiles ahead leave two (95).
+#include <algorithm>
+
 #include "oa_kv8_few.h"
 
 namespace {
@@ -18,16 +20,45 @@ __global__ void __launch_bounds__(kThreads, NQ > 1 ? 2 : 3) kv8_attn_kernel(Attn
   typedef FewLds<D, NQ> Lds;
   __shared__ __align__(16) char s_v[Lds::kBytes];
   __shared__ float s_m[kWaves][NQ * 16], s_l[kWaves][NQ * 16];
-  // (sequence or token, head) fastest: workgroups go to the XCDs in turn, so that a long sequence's pieces and a
-  // batch's short sequences spread over all of them, and the query tiles of a piece meet in one L2
-  const int unit = blockIdx.x, row0 = blockIdx.y * (NQ * (DUP ? 8 : 16)), ch = blockIdx.z;
-  const int u = a.by_hkv ? (int)__umulhi((unsigned)unit, a.by_hkv) : unit, h = unit - u * a.HKV;
+  // Workgroups go to the XCDs in turn, and there to the shader engines and their compute units in turn, whatever these
+  // are doing.  So the pieces of a sequence come one after the other, heads fastest, and spread over all of the card
+  // whatever the other sequences hold; the tiles of a piece, which read the same keys, are next to each other.  (With
+  // (sequence, head) fastest all work of one of 4 or 8 sequences is on a quarter of the card: 16 sequences, every fourth
+  // of 131072 keys and the others of 2000, 324 us, 201 so.)  A sequence's first piece is a place further for each
+  // sequence, as the many short ones have no other.
+  int u, h, row0 = blockIdx.y, ch = blockIdx.z;
+  if (!LISTED && a.in_turn) {
+    const int piece = a.by_hkv ? (int)__umulhi(blockIdx.x, a.by_hkv) : blockIdx.x;
+    h = blockIdx.x - piece * a.HKV;
+    row0 = piece & (a.ntile - 1);        // (one tile or two)
+    u = blockIdx.z;
+    ch = (piece >> (a.ntile - 1)) + u - (int)__umulhi((unsigned)u, a.by_nchunk) * a.nchunk;
+    if (ch >= a.nchunk) ch -= a.nchunk;
+  } else {
+    u = a.by_hkv ? (int)__umulhi(blockIdx.x, a.by_hkv) : blockIdx.x;
+    h = blockIdx.x - u * a.HKV;
+  }
+  row0 *= NQ * (DUP ? 8 : 16);
   few_rows<D, NQ, DUP, T, LISTED, ONCE>(a, u, h, row0, ch, Lds{s_v, s_m, s_l});
 }
 
-template <int D, typename T, bool LISTED>
+// TOKENS: a workgroup to every token's head; otherwise to every head of the max_q tokens that each sequence may have,
+// which takes no search
+template <int D, typename T, bool LISTED, bool TOKENS>
 __global__ void __launch_bounds__(kThreads) kv8_join_kernel(AttnArgs a) {
-  join_pieces<D, T, LISTED>(a);
+  if constexpr (TOKENS) {
+    const int heads = a.HKV * a.G, t = blockIdx.x / heads, hd = blockIdx.x - t * heads;
+    const int b = sequence_of(a.B, t, [&](int i) { return a.cu[i]; });
+    const Seq sq = LISTED ? seq_of(a, b, 1L << 32) : seq_of(a, b);
+    const int j = t - sq.r0;
+    if (j >= 0 && j < min(sq.R, a.max_q)) {
+      join_row<D, T, LISTED>(a, sq, hd, j);
+    } else if (a.clear && threadIdx.x < D / 4) {
+      *reinterpret_cast<uint2v*>(a.out + (long)t * a.o_st + (long)hd * a.o_sh + 4 * threadIdx.x) = uint2v(0u);
+    }
+  } else {
+    join_pieces<D, T, LISTED>(a);
+  }
 }
 
 template <int D, typename T, bool LISTED>
@@ -42,10 +73,13 @@ int launch(AttnArgs a, hipStream_t st) {
     return OA_EINVAL;
   // quotients as products with 2^16 / G + 1 and 2^32 / HKV, rounded up: exact while the number times the divisor is
   // less than that power (without a list rows and G are at most 64 here; with one rows are not divided)
-  if (cols < 128 && units * a.HKV > 0xffffffffL) return OA_EINVAL;
+  if (cols < 128 && std::max(units, (long)a.nchunk * a.ntile * a.HKV) * a.HKV > 0xffffffffL) return OA_EINVAL;
   a.by_g = 65536u / a.G + 1;
   a.by_hkv = a.HKV > 1 ? (unsigned)((0x100000000L + a.HKV - 1) / a.HKV) : 0;
-  const dim3 grid((unsigned)units, a.ntile, a.nchunk), blk(kThreads);
+  a.in_turn = !LISTED && cols < 128 && a.nchunk > 1 && a.ntile <= 2;
+  a.by_nchunk = (unsigned)((0x100000000L + a.nchunk - 1) / a.nchunk);        // (of more than one; sequences are at most 65535)
+  const dim3 grid = a.in_turn ? dim3((unsigned)(a.nchunk * a.ntile * a.HKV), 1, a.B) : dim3((unsigned)units, a.ntile, a.nchunk);
+  const dim3 blk(kThreads);
   // (the tokens of a sequence, where it has several, have blocks in common: through the caches)
   if (cols == 8) {
     if (LISTED && a.cu) hipLaunchKernelGGL((kv8_attn_kernel<D, 1, true, T, LISTED, !LISTED>), grid, blk, 0, st, a);
@@ -58,7 +92,15 @@ int launch(AttnArgs a, hipStream_t st) {
   } else {
     launch_rows(a, D, !std::is_same<T, __bf16>::value, dim3((unsigned)(units * a.ntile * a.nchunk)), st);
   }
-  if (a.nchunk > 1) hipLaunchKernelGGL((kv8_join_kernel<D, T, LISTED>), dim3((unsigned)joins, a.B), blk, 0, st, a);
+  if (a.nchunk > 1) {
+    // (512 tokens of one sequence beside 31 single ones: 959 us with the workgroups of 32 times 512 tokens, 707 with those
+    // of 543)
+    const long heads = (long)a.HKV * a.G;
+    if (a.cu && (long)a.max_q * a.B > 4L * a.tokens)
+      hipLaunchKernelGGL((kv8_join_kernel<D, T, LISTED, true>), dim3((unsigned)(a.tokens * heads)), blk, 0, st, a);
+    else
+      hipLaunchKernelGGL((kv8_join_kernel<D, T, LISTED, false>), dim3((unsigned)joins, a.B), blk, 0, st, a);
+  }
   return OA_LAUNCH_STATUS();
 }
 

@@ -17,7 +17,7 @@
 // What bounds it is not one thing: matrix cores are busy 31% of the time, vector units 41%, waves wait 27%.  All
 // workgroups end together with 33 MB of partial sums (by way of LDS in whole lines: 1% less at best).
 // Sequences of few rows in such a call go the way of oa_kv8_few.h (a question of 64 tokens beside 31 single ones over
-// 32768 keys 466 us, 720 as 128 rows each; calls without such sequences as before).
+// 32768 keys 466 us, 720 as 128 rows each).
 #include "oa_kv8_few.h"
 
 namespace {
@@ -62,10 +62,11 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_rows_kernel(AttnArgs a) {
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n32 = lane & 31, h = lane >> 5;
-  const int units = a.B * a.HKV;
-  const int bh = blockIdx.x % units, rest = blockIdx.x / units;
-  const int ch = rest / a.ntile, row0 = (rest - ch * a.ntile) * kRows;
-  const int b = bh / a.HKV, head = bh - b * a.HKV;
+  // by sequence, piece, tile, head, as in oa_kv8_attn.hip, and turned from sequence to sequence, tiles from piece to piece
+  // (8 questions of up to 64 tokens over up to 32768 keys 293 us with (sequence, head) fastest, 162 so)
+  const int tiles = blockIdx.x / a.HKV, head = blockIdx.x - tiles * a.HKV;
+  const int pieces = tiles / a.ntile, row0 = (tiles + pieces) % a.ntile * kRows;
+  const int b = pieces / a.nchunk, ch = (pieces + b) % a.nchunk;
   const Seq sq = seq_of(a, b);
   const int rows = min(sq.R, a.max_q) * a.G;
   if (row0 >= rows) return;

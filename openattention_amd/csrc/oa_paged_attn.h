@@ -106,20 +106,15 @@ __device__ __forceinline__ void clear_rows(const Args& a, int b, int hd, bool ow
   for (int t = t0 + x; t < t1; t += kRows) zero(t, hd);
 }
 
-// joins a row's chunks: weights exp2(m_i - max m), by groups of D / 4 lanes.  T: the rows' type; LISTED: all chunks count
-// (those of a list of blocks, which may hold nothing that the row sees)
+// joins the chunks of head hd of a sequence's token j: weights exp2(m_i - max m), by groups of D / 4 lanes.  T: the rows'
+// type; LISTED: all chunks count (those of a list of blocks, which may hold nothing that the row sees)
 template <int D, typename T, bool LISTED, typename Args>
-__device__ __forceinline__ void join_pieces(const Args& a) {
+__device__ __forceinline__ void join_row(const Args& a, const Seq& sq, int hd, int j) {
   constexpr int kLanes = D / 4, kGroups = kThreads / kLanes;
   __shared__ float s_r[kWaves];
   __shared__ __align__(16) float s_o[kGroups][D];
   __shared__ float s_l[kGroups];
-  const int heads = a.HKV * a.G;
-  const int hd = blockIdx.x % heads, j = blockIdx.x / heads, b = blockIdx.y;
-  const Seq sq = LISTED ? seq_of(a, b, 1L << 32) : seq_of(a, b);
-  if (a.clear) clear_rows<D>(a, b, hd, j == 0);
-  if (j >= sq.R) return;
-  const int seen = sq.n - sq.R + j + 1, tid = threadIdx.x;
+  const int heads = a.HKV * a.G, seen = sq.n - sq.R + j + 1, tid = threadIdx.x;
   const int nv = sq.bad || seen <= 0 ? 0 : LISTED ? a.nchunk : (seen + a.chunk - 1) / a.chunk;
   const long row = ((long)(sq.r0 + j) * heads + hd) * a.nchunk;
   const float* ml = a.ws_ml + row * 2;
@@ -166,6 +161,16 @@ __device__ __forceinline__ void join_pieces(const Args& a) {
   o = sq.bad ? f32x4(__builtin_nanf("")) : nv && !(LISTED && L == 0.f) ? o / L : f32x4(0.f);
   *reinterpret_cast<uint2v*>(a.out + (long)(sq.r0 + j) * a.o_st + (long)hd * a.o_sh + 4 * y) =
       uint2v{pack_out<T>(o[0], o[1]), pack_out<T>(o[2], o[3])};
+}
+
+// joins the chunks of every row, a workgroup to each of max_q tokens' heads (x) of a sequence (y)
+template <int D, typename T, bool LISTED, typename Args>
+__device__ __forceinline__ void join_pieces(const Args& a) {
+  const int heads = a.HKV * a.G, hd = blockIdx.x % heads, j = blockIdx.x / heads, b = blockIdx.y;
+  const Seq sq = LISTED ? seq_of(a, b, 1L << 32) : seq_of(a, b);
+  if (a.clear) clear_rows<D>(a, b, hd, j == 0);
+  if (j >= sq.R) return;
+  join_row<D, T, LISTED>(a, sq, hd, j);
 }
 
 }  // namespace paged

@@ -1257,24 +1257,26 @@ def kv8_chunk(cap: int, units: int, rows: int, listed: bool = False) -> int:
     4096 keys (8 KV heads of 128; us): one sequence of 131072 keys 53 / 47 / 45, 32 of 32768 365 / 347 / 334, 64 listed
     blocks of 64 keys for 32 tokens 52 / 49 / 45 and for 128 tokens 94 / 86 / 85; two questions of 64 tokens over 32768
     keys (256 rows each) 115 / 105 / 122.  Sequences of unlike lengths, and those much shorter than their table, want
-    smaller pieces: an eighth of the longest and no less than 1024 (61 of 1 to 16001 keys 61 / 60 / 79), and no more than
-    4096 (of 4096 / 8192 / an eighth of the longest: 16 of 1 to 131072 keys 112 / 131 / 240, 8 of 131072 334 / 340 / 323), or
-    8192 where that gives the card some more workgroups than it holds at once (4 of 131072 182 / 166 / 165).  A table
-    for more than 262144 keys takes 64 pieces of whatever size, or 32: so many hold their sums in the workspace.  Up to 640
-    keys (512 listed ones) one piece, and no join: one sequence of 250 keys 5.8 us, 7.7 in two pieces; 23 of up to 525 7.7
-    for 10.2; but one of 735 9.4 in two and 7.8 in six, 49 tokens of 640 listed keys 9.1 in one and 8.1 in five.
-    Questions, too, take no more than 4096 keys a piece: 8 of up to 64 tokens over up to 32768 keys 160, in whole sequences
-    280; 8 of 64 over 32768 364 for 356.  Pieces of prompts (one of 2048 tokens 1281 for 1182) keep what fills the card."""
+    smaller pieces: an eighth of the longest, up to 16384 keys a sixteenth, and no less than 1024 (of an eighth / 1024: 61 of
+    1 to 16001 keys 62 / 60, 32 of up to 16384 34 / 28, 8 of 16384 54 / 55), and no more than 4096, or 8192 where that gives
+    the card some more workgroups than it holds at once (of 4096 / 8192 / an eighth of the longest: 16 of 1 to 131072 keys
+    112 / 131 / 240, 8 of 131072 334 / 340 / 323, 4 of 131072 182 / 166 / 165).  A table for more than 262144 keys takes 64
+    pieces of whatever size, or 32: so many hold their sums in the workspace.  Up to 640 keys (512 listed ones) one piece,
+    and no join: one sequence of 250 keys 5.8 us, 7.7 in two pieces; 23 of up to 525 7.7 for 10.2; but one of 735 9.4 in two
+    and 7.8 in six, 49 tokens of 640 listed keys 9.1 in one and 8.1 in five.
+    Many rows, too, take no more than 4096 keys a piece or what makes 64 workgroups of a KV head of one sequence: 8
+    questions of up to 64 tokens over up to 32768 keys 160, in whole sequences 280; 8 of 64 over 32768 364 for 356; 512
+    tokens beside 7 single ones over up to 32768 keys 370 (pieces of 8192) for 812, 4 times 512 over 32768 1237 for 1172."""
     if cap <= (512 if listed else 640) and rows <= 16:
         return -(-cap // 128) * 128
     n = max(cap * units // (256 if rows <= 16 else 512), 128)
     if rows <= 64 and not listed:
-        n = min(n, max(cap // 8, 1024))
+        n = min(n, max(cap // (8 if cap > 16384 else 16), 1024))
         most = max(4096, cap // 64)
         if n > most:
             n = min(n, 2 * most) if 512 < units * (cap // most) < 2048 else most
-    elif rows <= 1024 and not listed:
-        n = min(n, max(4096, cap // 64))
+    elif not listed:
+        n = min(n, max(4096, cap // 64, cap * -(-rows // 128) // 64))
     return min(-(-n // 128), -(-cap // 128)) * 128
 
 

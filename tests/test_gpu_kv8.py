@@ -677,3 +677,32 @@ def test_short_sequences_beside_long_ones(HQ, HKV, D, page, dtype, monkeypatch):
     assert out[cu[1]:cu[2]].isnan().all() and out[cu[4]:cu[5]].isnan().all()
     rest = [t for t in range(cu[-1]) if not (cu[1] <= t < cu[2] or cu[4] <= t < cu[5])]
     assert torch.equal(out[rest], good[rest])
+
+
+@pytest.mark.parametrize("listed", [False, True])
+def test_sparse_calls(listed, monkeypatch):
+    """Few tokens of the many that the sequences may have, in pieces: rows that no sequence takes before, behind and past
+    max_q, left as they were or 0, and starts that do not fit the rows."""
+    monkeypatch.setattr(ops, "kv8_chunk", lambda cap, units, rows, listed: 128)
+    g = gen(34)
+    HQ, HKV, D, page, rows, lens = 8, 2, 64, 32, [40, 1, 2, 0, 1, 1, 3, 1], [300, 170, 90, 0, 1, 0, 260, 64]
+    cache, table = filled(lens, HKV, D, page, g)
+    cu = [2 + c for c in starts(rows)]
+    T = cu[-1] + 3
+    q = randn(g, T, HQ, D, dtype=BF)
+    W = table.shape[1]
+    blocks = lists(T, HKV, 6, W, g) if listed else None
+    want, err = torch.zeros(q.shape, dtype=torch.float64, device=DEV), torch.zeros(q.shape, dtype=torch.float64, device=DEV)
+    own = None if blocks is None else blocks[2:cu[-1]]
+    want[2:cu[-1]], err[2:cu[-1]] = want_attn(q[2:cu[-1]], cache, table, lens, starts(rows), D ** -0.5, page, own)
+    out = ops.kv8_attn(q, *cache[:4], table, i32(lens), cu_q=i32(cu), max_q=40, blocks=blocks)
+    check_attn(out, want, err)
+    kept = torch.full_like(q, 7.0)
+    ops.kv8_attn(q, *cache[:4], table, i32(lens), cu_q=i32(cu), max_q=40, blocks=blocks, out=kept)
+    assert (kept[:2] == 7).all() and (kept[cu[-1]:] == 7).all() and torch.equal(kept[2:cu[-1]], out[2:cu[-1]])
+    # 25 of the first sequence's 40 tokens
+    fewer = ops.kv8_attn(q, *cache[:4], table, i32(lens), cu_q=i32(cu), max_q=25, blocks=blocks)
+    assert (fewer[27:42] == 0).all()
+    check_attn(torch.cat([fewer[2:27], fewer[42:cu[-1]]]), torch.cat([want[2:27], want[42:cu[-1]]]), torch.cat([err[2:27], err[42:cu[-1]]]))
+    for bad in ([-1] + cu[1:], cu[:-1] + [T + 1], [5, 3] + cu[2:], [T + 9] * 9):
+        ops.kv8_attn(q, *cache[:4], table, i32(lens), cu_q=i32(bad), max_q=40, blocks=blocks)
