@@ -5,7 +5,7 @@
 // kernel joins them.
 // Bound: bytes where they are read once: 32 sequences of 32768 keys (8 KV heads of 128) 320 to 331 us, 6.5 to 6.7 TB/s; one
 // of 131072 40 us and the join's 4.  Where tokens have blocks in common (64 of them for each of two questions' 128 tokens:
-// 1.07 GB, 134 MB of it distinct, 86 us) the instructions: 64 conversions and 8 exponentials among some 145 vector ones a
+// 1.07 GB, 134 MB of it distinct, 82 us) the instructions: 64 conversions and 8 exponentials among some 145 vector ones a
 // tile of 32 keys, with three waves to a SIMD.  Four waves there spill (204 us); loads two tiles ahead leave two (95).
 #include <algorithm>
 
